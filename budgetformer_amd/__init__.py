@@ -2,8 +2,9 @@
 
   * budgeted query-centric edge construction (``edges.build_attention_edges``)
   * sparse edge attention forward/backward (``attention``)
+  * operators over packed sequences (``sequences``): dense attention, rotary positions, linear attention
 
-Both run as hand-written HIP kernels behind the C ABI in
+All run as hand-written HIP kernels behind the C ABI in
 ``include/budgetformer_hip.h`` (library ``_lib/libbudgetformer_hip.so``, built
 by ``python -m budgetformer_amd.build``). There is no CPU fallback: every entry
 point raises if the library is missing or a tensor is not on a HIP device.
@@ -14,11 +15,14 @@ from .attention import (CoreAttention, ExphormerCoreAttention, GPSCoreAttention,
 from .edges import EdgeTable, build_attention_edges
 from .graph import CSRGraph
 from .hip_ops import AttentionIndex
+from .sequences import (PackedSequences, RotaryFrequencies, linear_attention, linear_attention_step, packed_attention,
+                        rotary_embedding)
 
 __all__ = [
     "AttentionIndex", "CSRGraph", "CoreAttention", "EdgeTable", "ExphormerCoreAttention", "GPSCoreAttention",
-    "GTCoreAttention",
-    "build_attention_edges", "sparse_edge_attention",
+    "GTCoreAttention", "PackedSequences", "RotaryFrequencies",
+    "build_attention_edges", "linear_attention", "linear_attention_step", "packed_attention", "rotary_embedding",
+    "sparse_edge_attention",
 ]
 
 

@@ -49,6 +49,25 @@ class AttnDropout(C.Structure):
     _fields_ = [("rate", C.c_float), ("seed", u64), ("offset", u64), ("keep", vp)]
 
 
+class PackedAttn(C.Structure):
+    """Mirror of ``struct bf_packed_attn``."""
+    _fields_ = [
+        ("n_q", i64), ("n_k", i64), ("heads_q", i32), ("heads_k", i32), ("head_dim", i32), ("dtype", i32),
+        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
+        ("scale", f32), ("reserved", i32),
+    ]
+
+
+class LinearAttn(C.Structure):
+    """Mirror of ``struct bf_linear_attn``."""
+    _fields_ = [
+        ("n", i64), ("n_seq", i64), ("heads", i32), ("dim_x", i32), ("dim_z", i32), ("dtype", i32),
+        ("x_stride", i64 * 2), ("y_stride", i64 * 2), ("z_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
+        ("offsets", vp), ("log_decay", vp), ("init", vp), ("final_state", vp), ("init_stride", i64 * 2),
+        ("scale", f32), ("reverse", i32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "bf_version": (C.c_int, []),
@@ -146,6 +165,15 @@ _SIGS = {
     "bf_attn_fwd_typed": (C.c_int, [C.POINTER(AttnIndex), i32, i32, i32, vp, vp, vp, P_f32, vp, P_f32, vp]),
     "bf_attn_bwd_typed": (C.c_int, [C.POINTER(AttnIndex), i32, i32, i32, vp, vp, vp, P_f32, P_f32, vp, vp, vp, vp,
                                     P_f32, P_f32, P_f32, vp]),
+    "bf_packed_spans": (C.c_int, [P_i32, P_i32, i64, i64, i64, i32, P_i32, P_i32, P_i32, vp]),
+    "bf_packed_attn_fwd_floats": (i64, [C.POINTER(PackedAttn)]),
+    "bf_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, vp]),
+    "bf_rotary": (C.c_int, [vp, vp, i64, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64), vp, i32, vp, f32, i32,
+                            i32, vp, vp, vp]),
+    "bf_linear_attn_floats": (i64, [C.POINTER(LinearAttn)]),
+    "bf_linear_attn_pass": (C.c_int, [C.POINTER(LinearAttn), vp, vp, vp, vp, P_f32, vp]),
+    "bf_linear_attn_step": (C.c_int, [vp, vp, vp, P_f32, P_f32, i64, i32, i32, i32, i32, f32, vp, P_f32, vp]),
 }
 
 _lib = None

@@ -7,8 +7,9 @@ attn_type=None)`` signatures of
   models/gt_dist_node_level.py:51-522           (sparse path :179-262, dispatch :505-522)
   models/graphgps_dist_node_level.py:135-209    (sparse path :151-177)
   models/exphormer_dist_node_level.py:45-121    (typed-edge modulation)
-and compute the sparse path with the HIP forward/backward kernels. Only
-``attn_type="sparse"`` is on this path; the dense "full"/"flash"/"performer"
+and compute the sparse path with the HIP forward/backward kernels.
+``CoreAttention`` also takes ``attn_type="flash"``, dense attention inside each
+sequence of the batch (``sequences.packed_attention``); the "full"/"performer"
 variants are not part of it and raise.
 
 ``edge_index`` may be the reference's COO LongTensor [2, E] (or [3, E] with a
@@ -32,6 +33,7 @@ import torch.nn as nn
 
 from . import hip_ops
 from .hip_ops import AttentionIndex
+from .sequences import PackedSequences, RotaryFrequencies, packed_attention, rotary_embedding
 
 
 class _SparseEdgeAttention(torch.autograd.Function):
@@ -210,11 +212,35 @@ def _per_head_attention(q, k, v, assign, score_clamp, bias_fn=None, stats=None):
     return pieces[0] if len(pieces) == 1 else torch.cat(pieces, dim=1)
 
 
-class CoreAttention(nn.Module):
-    """Graphormer core attention (models/graphormer_dist_node_level.py:61-613), sparse path on HIP."""
+class _BatchSequences:
+    """The PackedSequences of the last few (batch, length, device) of dense calls."""
 
-    def __init__(self, hidden_size, attention_dropout_rate, num_heads, attn_bias_dim=None):
+    def __init__(self, size: int = 4):
+        self.size = size
+        self._d: "OrderedDict" = OrderedDict()
+
+    def get(self, batch: int, length: int, device: torch.device) -> PackedSequences:
+        key = (batch, length, str(device))
+        hit = self._d.get(key)
+        if hit is None:
+            hit = self._d[key] = PackedSequences.from_lengths([length] * batch, device=device)
+        self._d.move_to_end(key)
+        while len(self._d) > self.size:
+            self._d.popitem(last=False)
+        return hit
+
+
+class CoreAttention(nn.Module):
+    """Graphormer core attention (models/graphormer_dist_node_level.py:61-613), sparse and flash paths on HIP.
+
+    ``rotary`` (a ``RotaryFrequencies``): q and k of the flash path are turned by their place in the sequence
+    first."""
+
+    def __init__(self, hidden_size, attention_dropout_rate, num_heads, attn_bias_dim=None,
+                 rotary: Optional[RotaryFrequencies] = None):
         super().__init__()
+        self.rotary = rotary
+        self._batches = _BatchSequences()
         self.hidden_size_per_attention_head = hidden_size // num_heads
         self.num_attention_heads_per_partition = num_heads
         self.scale = math.sqrt(self.hidden_size_per_attention_head)
@@ -250,10 +276,30 @@ class CoreAttention(nn.Module):
 
     def forward(self, q, k, v, attn_bias=None, edge_index=None, attn_type=None):
         batch_size, s_len = q.size(0), q.size(1)
+        if attn_type == "flash":
+            return self.dense_attention(q, k, v, attn_bias, edge_index)
         if attn_type != "sparse":
             raise NotImplementedError(f"attn_type={attn_type!r} is not on the sparse edge-attention path")
         x = self.sparse_attention_bias(k, q, v, edge_index, attn_bias)
         return x.view(batch_size, s_len, -1)
+
+    def dense_attention(self, q, k, v, attn_bias=None, sequences=None):
+        """softmax(q k^T / sqrt(hn)) v inside each of the batch's sequences
+        (models/graphormer_dist_node_level.py:603-608): q [b, S, H, hn], k and v [b, S, heads, hn]. ``sequences`` (forward's
+        edge_index): a ``PackedSequences`` over the b*S rows instead, for graphs packed along S; an edge set is ignored.
+        No bias and no attention dropout."""
+        if attn_bias is not None:
+            raise NotImplementedError("attn_type='flash' takes no attention bias")
+        if self.training and self.attention_dropout_rate > 0.0:
+            raise NotImplementedError("attn_type='flash' has no attention dropout")
+        batch_size, s_len = q.size(0), q.size(1)
+        q, k, v = (t.reshape(-1, t.size(2), t.size(3)) for t in (q, k, v))
+        seqs = sequences if isinstance(sequences, PackedSequences) else self._batches.get(batch_size, s_len, q.device)
+        if self.rotary is not None:
+            if seqs.n_q != seqs.n_k:
+                raise ValueError("rotary positions of the flash path need as many keys as rows")
+            q, k = rotary_embedding(q, k, self.rotary, seqs=seqs)
+        return packed_attention(q, k, v, seqs).reshape(batch_size, s_len, -1)
 
 
 class GTCoreAttention(nn.Module):

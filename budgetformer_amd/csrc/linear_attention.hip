@@ -1,0 +1,484 @@
+// Linear attention with a decay for each head over packed sequences, on the matrix cores.
+//
+//   out_i = scale sum_{j <= i, same sequence} g^(i - j) (x_i . y_j) z_j
+//
+// One pass in three uses: the forward is (x, y, z) = (q, k, v); the gradients are (dout, v, k) for dq and, with the
+// packed axis read backwards, (v, dout, q) for dk and (k, q, dout) for dv.
+//
+// Chunked form. A workgroup walks a segment of the packed axis in tiles of C tokens, the state M = sum g^(t - j) y_j z_j^T
+// in the accumulators of its waves (wave w owns the columns 32w .. 32w+31 of z, so a column of M is a lane's, its rows
+// are registers). Per tile:
+//   W_ij = (x_i . y_j) g^(i - j) for j <= i of the same sequence          C x C, shared through LDS
+//   out_i = scale (sum_j W_ij z_j + g^(i - t0 + 1) x_i M)                 the second only if the sequence began before t0
+//   M = g^C M + sum_j g^(t1 - 1 - j) y_j z_j^T                            only the last row's sequence
+// M's registers are, packed, the operand of x M in register order (packed_tile.h): the state never moves. Tiles are cut
+// from the packed axis, not from the sequences: a boundary is a comparison of indices, and short sequences fill tiles.
+// Where states come in or go out (init, final) tiles end at the sequences' ends instead.
+//
+// Calls of few heads cut the axis into segments: one launch forms each segment's own contribution to the state, one
+// carries it from segment to segment, and the pass starts from there. States are float32 throughout; as operands M, W and
+// the decayed z are rounded to the activations' type (half a step, as the inputs' own rounding), in float32 not at all.
+#include "packed_tile.h"
+
+namespace bf {
+namespace {
+
+struct LinArgs {
+  const void *x, *y, *z;
+  void* out;
+  int64_t xs_t, xs_h, ys_t, ys_h, zs_t, zs_h;
+  const int2 *row_span, *key_span;
+  const int32_t* offsets;
+  const float *log_decay, *init;
+  float *final_state, *carry;
+  int64_t init_sx, init_sz;
+  int32_t n, n_seq, heads, dx, dz;
+  int32_t seg_len, n_seg;
+  float scale;
+  bool reverse, states;
+};
+
+template <typename T> __device__ __forceinline__ Frag<T> pack8_by(const F32x16& x, int t, float by) {
+  Frag<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = T(x[8 * t + j] * by);
+  return f;
+}
+
+template <typename T> constexpr int lin_tile() { return sizeof(T) == 2 ? 64 : 32; }
+
+// log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
+__device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
+
+// the token at a place of the axis as the pass reads it, and where its sequence starts there
+__device__ __forceinline__ int token_at(const LinArgs& a, int p) { return a.reverse ? a.n - 1 - p : p; }
+__device__ __forceinline__ int start_at(const LinArgs& a, int p) {
+  const int t = token_at(a, p);
+  if (a.reverse) return a.n - a.key_span[t].y;        // behind the last sequence: after p
+  const int2 s = a.row_span[t];
+  return s.y > s.x ? s.x : a.n;                        // a row behind the last sequence sees nothing
+}
+
+// Last s with offsets[s] <= p; n_seq behind the last sequence, -1 before the first.
+__device__ __forceinline__ int sequence_of(const LinArgs& a, int p) {
+  int lo = -1, hi = a.n_seq;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.offsets[mid] <= p)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T, int DX, int DZ, bool OUT>
+__global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
+  constexpr int C = lin_tile<T>(), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
+  using TX = Tile<T, DX>;
+  using TZ = Tile<T, DZ>;
+  using TW = Tile<T, C>;
+  __shared__ __attribute__((aligned(16))) char x_lds[OUT ? TX::bytes(C) : 16];
+  __shared__ __attribute__((aligned(16))) char y_lds[TX::bytes(C)];
+  __shared__ __attribute__((aligned(16))) char z_lds[TZ::bytes(C)];
+  __shared__ __attribute__((aligned(16))) char w_lds[OUT ? TW::bytes(C) : 16];
+  __shared__ int start_lds[C];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
+  const int h = int(slot % a.heads), seg = int(slot / a.heads);     // the heads of a token share its cache lines
+  const int begin = seg * a.seg_len, end = min(begin + a.seg_len, a.n);
+  const float ld = decay_log2(a, h);
+  const T* xp = static_cast<const T*>(a.x) + h * a.xs_h;
+  const T* yp = static_cast<const T*>(a.y) + h * a.ys_h;
+  const T* zp = static_cast<const T*>(a.z) + h * a.zs_h;
+
+  F32x16 m[XB];
+#pragma unroll
+  for (int b = 0; b < XB; ++b) m[b] = zero16();
+  float* carry = a.carry + ((int64_t(seg) * a.heads + h) * XB * NW + wave) * 1024 + lane;       // register r of block b: + (b * NW * 16 + r) * 64
+  if (OUT && seg > 0) {
+#pragma unroll
+    for (int b = 0; b < XB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m[b][r] = carry[(int64_t(b) * NW * 16 + r) * 64];
+  }
+  int seq = a.states ? sequence_of(a, begin) : 0;
+  auto tile_end = [&](int t0) {
+    const int e = min(t0 + C, end);
+    return a.states && seq < a.n_seq ? min(e, seq < 0 ? a.offsets[0] : a.offsets[seq + 1]) : e;
+  };
+
+  Stage<T, DX, C, NT> xs, ys;
+  Stage<T, DZ, C, NT> zs;
+  int start = 0;
+  auto fetch = [&](int t0, int t1) {
+    if constexpr (OUT) xs.load(tid, a.dx, [&](int r) { return t0 + r < t1 ? xp + token_at(a, t0 + r) * a.xs_t : nullptr; });
+    ys.load(tid, a.dx, [&](int r) { return t0 + r < t1 ? yp + token_at(a, t0 + r) * a.ys_t : nullptr; });
+    zs.load(tid, a.dz, [&](int r) { return t0 + r < t1 ? zp + token_at(a, t0 + r) * a.zs_t : nullptr; });
+    if (tid < C) start = start_at(a, min(t0 + tid, t1 - 1));
+  };
+
+  int t1 = begin < end ? tile_end(begin) : begin;
+  if (begin < end) fetch(begin, t1);
+  for (int t0 = begin; t0 < end;) {
+    __syncthreads();
+    if constexpr (OUT) xs.store(tid, x_lds);
+    ys.store(tid, y_lds);
+    zs.store(tid, z_lds);
+    if (tid < C) start_lds[tid] = start;
+    bool odd = false;
+    if constexpr (OUT)
+      odd = __syncthreads_or(zs.tainted());
+    else
+      __syncthreads();
+    const int len = t1 - t0;
+    if (a.states && seq >= 0 && seq < a.n_seq && t0 == a.offsets[seq]) {          // a sequence begins with its tile
+      const float* s0 = a.init ? a.init + (int64_t(seq) * a.heads + h) * a.dx * a.dz : nullptr;
+#pragma unroll
+      for (int b = 0; b < XB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = 32 * b + acc_row(r, half), z = 32 * wave + col;
+          m[b][r] = s0 && x < a.dx && z < a.dz ? s0[x * a.init_sx + z * a.init_sz] : 0.f;
+        }
+    }
+    const bool ends = a.states && seq >= 0 && seq < a.n_seq && t1 == a.offsets[seq + 1];
+    const int this_seq = seq;
+    if (a.states && t1 < end)
+      while (seq < a.n_seq && a.offsets[seq + 1] <= t1) ++seq;
+    const int next = t1 < end ? tile_end(t1) : t1;
+    if (t1 < end) fetch(t1, next);
+
+    const int first_start = start_lds[0], last_start = start_lds[len - 1];
+    if constexpr (OUT) {
+      for (int quad = wave; quad < QB * QB; quad += NW) {
+        const int ib = quad / QB, jb = quad % QB;
+        if (jb > ib) continue;
+        F32x16 acc = zero16();
+#pragma unroll
+        for (int s = 0; s < TX::kSteps; ++s)
+          acc = Mat<T>::mma(TX::row_frag(y_lds, 32 * jb + col, s, half), TX::row_frag(x_lds, 32 * ib + col, s, half), acc);
+        const int i = 32 * ib + col, from = start_lds[i] - t0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = 32 * jb + 8 * g + 4 * half + k;
+            w[k] = j <= i && j >= from ? acc[4 * g + k] * (a.scale * exp2_fast(ld * float(i - j))) : 0.f;
+          }
+          store4<T>(reinterpret_cast<T*>(w_lds + i * TW::kPitch) + 32 * jb + 8 * g + 4 * half, w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncthreads();
+      // with states the tile is one sequence's, whose state came in or was begun above
+      const bool into = a.states || first_start < t0;
+      // float16 ends at 65504 and a sum over a sequence need not: such a state is an operand in units of a power of 2
+      float unit = 1.f;
+      if constexpr (std::is_same<T, _Float16>::value) {
+        float big = 0.f;
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]));
+        if (__any(big > 32768.f)) {
+          for (int o = 32; o; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+          unit = big < INFINITY ? exp2f(ceilf(log2f(big)) - 15.f) : 1.f;
+        }
+      }
+      const float per_unit = 1.f / unit;
+#pragma unroll
+      for (int ib = 0; ib < QB; ++ib) {
+        const int i = 32 * ib + col;
+        F32x16 o = zero16();
+        if (into) {
+#pragma unroll
+          for (int b = 0; b < XB; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              Frag<T> mf;
+              if constexpr (std::is_same<T, _Float16>::value)
+                mf = pack8_by<T>(m[b], t, per_unit);
+              else
+                mf = pack8<T>(m[b], t);
+              o = Mat<T>::mma(mf, TX::row_frag_regs(x_lds, i, 2 * b + t, half), o);
+            }
+          const bool mine = start_lds[i] < t0 + int(a.states);
+          const float f = a.scale * exp2_fast(ld * float(i + 1)) * unit;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] = mine ? o[r] * f : 0.f;
+        }
+        F32x16 bad = zero16();
+#pragma unroll
+        for (int t = 0; t < C / 16; ++t) {
+          if (t >= 2 * (ib + 1)) continue;
+          Frag<T> zf = TZ::template col_frag<false>(z_lds, t, wave, lane);
+          const Frag<T> wf = TW::row_frag(w_lds, i, t, half);
+          if (odd) {
+            Frag<T> clean, up, down, sees;
+            split_finite<T>(zf, clean, up, down);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int j = 16 * t + 8 * half + k;
+              sees[k] = T(j <= i && j >= start_lds[i] - t0 ? 1.f : 0.f);
+              up[k] = T(fmaxf(float(up[k]), float(down[k])));
+            }
+            bad = Mat<T>::mma(up, sees, bad);
+            zf = clean;
+          }
+          o = Mat<T>::mma(zf, wf, o);
+        }
+        if (odd)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (bad[r] > 0.f) o[r] = NAN;
+        if (i < len)
+          store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, 1.f, wave, a.dz,
+                         half);
+      }
+    }
+
+    if (!OUT || t1 < end || ends) {
+      const bool keep = a.states || last_start < t0;
+      const float f = exp2_fast(ld * float(len));
+#pragma unroll
+      for (int b = 0; b < XB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m[b][r] = keep ? m[b][r] * f : 0.f;
+      const int from = a.states ? 0 : last_start - t0;
+      const bool cut = from > 0;
+#pragma unroll
+      for (int t = 0; t < C / 16; ++t) {
+        Frag<T> zf = TZ::template col_frag<true>(z_lds, t, wave, lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = 16 * t + acc_row(k, half);
+          zf[k] = j >= from && j < len ? T(float(zf[k]) * exp2_fast(ld * float(len - 1 - j))) : T(0.f);
+        }
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+          Frag<T> yf = TX::template col_frag<true>(y_lds, t, b, lane);
+          if (cut) {                      // what another sequence holds there may not be finite
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (16 * t + acc_row(k, half) < from) yf[k] = T(0.f);
+          }
+          m[b] = Mat<T>::mma(yf, zf, m[b]);
+        }
+      }
+      if (OUT && ends && a.final_state) {
+        float* fs = a.final_state + (int64_t(this_seq) * a.heads + h) * a.dx * a.dz;
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int x = 32 * b + acc_row(r, half), z = 32 * wave + col;
+            if (x < a.dx && z < a.dz) fs[x * a.dz + z] = m[b][r];
+          }
+      }
+    }
+    t0 = t1;
+    t1 = next;
+  }
+  if constexpr (!OUT) {
+#pragma unroll
+    for (int b = 0; b < XB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) carry[(int64_t(b) * NW * 16 + r) * 64] = m[b][r];
+  }
+}
+
+// Segments' own contributions -> the state each segment starts from, in place: one lane a value of a head's state.
+__global__ __launch_bounds__(256) void linear_carry(const LinArgs a, int64_t values) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= values * a.heads) return;
+  const int h = int(i / values);
+  const float f = exp2_fast(decay_log2(a, h) * float(a.seg_len));
+  float* c = a.carry + i;
+  float into = 0.f;
+  for (int s = 0; s + 1 < a.n_seg; ++s) {
+    const float mine = c[s * values * a.heads];
+    c[s * values * a.heads] = into;
+    const int e = (s + 1) * a.seg_len;
+    const bool began = start_at(a, e - 1) >= e - a.seg_len;         // the segment's last sequence began in it
+    into = began ? mine : fmaf(into, f, mine);
+  }
+  c[(a.n_seg - 1) * values * a.heads] = into;
+}
+
+// The final state of sequences without tokens is their initial one.
+__global__ __launch_bounds__(256) void linear_empty(const LinArgs a) {
+  const int64_t s = blockIdx.x;
+  if (a.offsets[s + 1] > a.offsets[s]) return;
+  const int64_t per = int64_t(a.heads) * a.dx * a.dz;
+  for (int64_t i = threadIdx.x; i < per; i += 256) {
+    const int64_t h = i / (a.dx * a.dz), x = i / a.dz % a.dx, z = i % a.dz;
+    a.final_state[s * per + i] =
+        a.init ? a.init[(s * a.heads + h) * a.dx * a.dz + x * a.init_sx + z * a.init_sz] : 0.f;
+  }
+}
+
+// One token a sequence: a workgroup a state; 256 lanes take 4 columns of 1024 / dz rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_step(const T* q, const T* k, const T* v, const float* log_decay, const float* state,
+                                                   int heads, int dk, int dv, float scale, T* out, float* new_state) {
+  __shared__ float part[256 * 4];
+  const int64_t nh = blockIdx.x;
+  const int h = int(nh % heads), cols = dv / 4, rows = 256 / cols, tid = threadIdx.x;
+  const int c = tid % cols, r0 = tid / cols;
+  const float g = __expf(fmaxf(log_decay[h], -1e4f));
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (r0 < rows) {
+    float vv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = float(v[nh * dv + 4 * c + j]);
+    const float* s = state + nh * dk * dv + 4 * c;
+    float* n = new_state + nh * dk * dv + 4 * c;
+    for (int r = r0; r < dk; r += rows) {
+      const float kr = float(k[nh * dk + r]), qr = float(q[nh * dk + r]);
+      float4 x = *reinterpret_cast<const float4*>(s + int64_t(r) * dv);
+      x.x = fmaf(x.x, g, kr * vv[0]);
+      x.y = fmaf(x.y, g, kr * vv[1]);
+      x.z = fmaf(x.z, g, kr * vv[2]);
+      x.w = fmaf(x.w, g, kr * vv[3]);
+      *reinterpret_cast<float4*>(n + int64_t(r) * dv) = x;
+      o[0] = fmaf(qr, x.x, o[0]);
+      o[1] = fmaf(qr, x.y, o[1]);
+      o[2] = fmaf(qr, x.z, o[2]);
+      o[3] = fmaf(qr, x.w, o[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[r0 * dv + 4 * c + j] = o[j];
+  }
+  __syncthreads();
+  for (int d = tid; d < dv; d += 256) {
+    float sum = 0.f;
+    for (int r = 0; r < rows; ++r) sum += part[r * dv + d];
+    out[nh * dv + d] = T(sum * scale);
+  }
+}
+
+// ---------------------------------------------------------------- launches
+int pad32(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+template <typename F> int with_pad(int d, F&& f) {
+  if (d <= 32) return f(std::integral_constant<int, 32>());
+  if (d <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+
+int check(const bf_linear_attn* p, const char* fn) {
+  BF_CHECK_ARG(p != nullptr, "%s: no arguments", fn);
+  BF_CHECK_ARG(p->dtype == BF_DTYPE_F32 || p->dtype == BF_DTYPE_BF16 || p->dtype == BF_DTYPE_F16, "%s: dtype %d", fn,
+               p->dtype);
+  for (int d : {p->dim_x, p->dim_z})
+    if (d < 8 || d > 128 || d % 8) {
+      set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_x, p->dim_z);
+      return BF_ERR_UNSUPPORTED;
+    }
+  BF_CHECK_ARG(p->n >= 0 && p->n < (int64_t(1) << 31) - 256 && p->n_seq >= 0 && p->n_seq < (int64_t(1) << 31) - 1 &&
+                   p->heads >= 1 && p->heads <= (1 << 20),
+               "%s: bad sizes (%lld rows, %lld sequences, %d heads)", fn, (long long)p->n, (long long)p->n_seq, p->heads);
+  const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;
+  for (const int64_t* s : {p->x_stride, p->y_stride, p->z_stride})
+    BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,
+                 "%s: strides (%lld, %lld) are not whole 16-byte steps", fn, (long long)s[0], (long long)s[1]);
+  BF_CHECK_ARG(p->scale == p->scale && p->scale <= 3e38f && p->scale >= -3e38f, "%s: scale %g", fn, double(p->scale));
+  BF_CHECK_ARG(p->log_decay && (p->n == 0 || (p->reverse ? p->key_span : p->row_span)), "%s: no decays or no spans", fn);
+  BF_CHECK_ARG(!(p->init || p->final_state) || (p->offsets && !p->reverse), "%s: states need the offsets and no reverse", fn);
+  return BF_OK;
+}
+
+// Tokens of a segment: whole tiles, so many that about 512 workgroups share the axis (their own contribution and the
+// carries cost a state each, read and written, which a segment of 256 tokens or more outweighs).
+int64_t segment_of(const bf_linear_attn* p) {
+  const int64_t want = ceil_div(512, p->heads);
+  int64_t len = ceil_div(ceil_div(p->n, want), 64) * 64;
+  return len < 256 ? 256 : len;
+}
+
+}  // namespace
+}  // namespace bf
+
+using namespace bf;
+
+extern "C" int64_t bf_linear_attn_floats(const bf_linear_attn* p) {
+  if (check(p, "linear_attn_floats") != BF_OK) return -1;
+  const int64_t segs = ceil_div(p->n, segment_of(p));
+  return segs <= 1 ? 0 : segs * p->heads * pad32(p->dim_x) * pad32(p->dim_z);
+}
+
+extern "C" int bf_linear_attn_pass(const bf_linear_attn* p, const void* x, const void* y, const void* z, void* out,
+                                   float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "linear_attn_pass"));
+  BF_CHECK_ARG(p->n == 0 || (x && y && z && out), "linear_attn_pass: bad arguments");
+  BF_CHECK_ARG(aligned16({x, y, z, out}), "linear_attn_pass: x, y, z and out must be 16-byte aligned");
+  LinArgs a{};
+  a.x = x, a.y = y, a.z = z, a.out = out;
+  a.xs_t = p->x_stride[0], a.xs_h = p->x_stride[1];
+  a.ys_t = p->y_stride[0], a.ys_h = p->y_stride[1];
+  a.zs_t = p->z_stride[0], a.zs_h = p->z_stride[1];
+  a.row_span = reinterpret_cast<const int2*>(p->row_span);
+  a.key_span = reinterpret_cast<const int2*>(p->key_span);
+  a.offsets = p->offsets, a.log_decay = p->log_decay, a.init = p->init, a.final_state = p->final_state;
+  a.init_sx = p->init_stride[0], a.init_sz = p->init_stride[1];
+  a.n = int32_t(p->n), a.n_seq = int32_t(p->n_seq), a.heads = p->heads, a.dx = p->dim_x, a.dz = p->dim_z;
+  a.scale = p->scale, a.reverse = p->reverse != 0, a.states = (p->init || p->final_state) && p->n_seq > 0;
+  a.seg_len = int32_t(segment_of(p));
+  a.n_seg = int32_t(ceil_div(p->n, a.seg_len));
+  a.carry = scratch;
+  const hipStream_t st = as_stream(stream);
+  if (a.states && a.final_state) {
+    BF_LAUNCH("linear_attn_empty", linear_empty, dim3(unsigned(a.n_seq)), dim3(256), 0, st, a);
+    BF_CHECK_LAUNCH();
+  }
+  if (a.n == 0) return BF_OK;
+  BF_CHECK_ARG(a.n_seg == 1 || scratch, "linear_attn_pass: no scratch (bf_linear_attn_floats)");
+  const int64_t groups = int64_t(a.n_seg) * a.heads;
+  return with_type(p->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_pad(a.dx, [&](auto px) -> int {
+      return with_pad(a.dz, [&](auto pz) -> int {
+        constexpr int DX = decltype(px)::value, DZ = decltype(pz)::value;
+        if (a.n_seg > 1) {
+          auto own = linear_pass<T, DX, DZ, false>;
+          BF_LAUNCH("linear_attn_segments", own, dim3(unsigned(groups)), dim3(2 * DZ), 0, st, a);
+          BF_CHECK_LAUNCH();
+          const int64_t values = DX * DZ;
+          BF_LAUNCH("linear_attn_carry", linear_carry, dim3(unsigned(ceil_div(values * a.heads, 256))), dim3(256), 0, st, a,
+                    values);
+          BF_CHECK_LAUNCH();
+        }
+        auto pass = linear_pass<T, DX, DZ, true>;
+        BF_LAUNCH("linear_attn_pass", pass, dim3(unsigned(groups)), dim3(2 * DZ), 0, st, a);
+        BF_CHECK_LAUNCH();
+        return BF_OK;
+      });
+    });
+  });
+}
+
+extern "C" int bf_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                                   int64_t n, int32_t heads, int32_t dim_k, int32_t dim_v, int32_t dtype, float scale, void* out,
+                                   float* new_state, void* stream) {
+  BF_CHECK_ARG(dtype == BF_DTYPE_F32 || dtype == BF_DTYPE_BF16 || dtype == BF_DTYPE_F16, "linear_attn_step: dtype %d", dtype);
+  for (int d : {dim_k, dim_v})
+    if (d < 8 || d > 128 || d % 8) {
+      set_error("linear_attn_step: head dims (%d, %d) (multiples of 8 up to 128 are supported)", dim_k, dim_v);
+      return BF_ERR_UNSUPPORTED;
+    }
+  BF_CHECK_ARG(n >= 0 && heads >= 1 && n < (int64_t(1) << 24) / heads, "linear_attn_step: %lld sequences of %d heads",
+               (long long)n, heads);
+  if (n == 0) return BF_OK;
+  BF_CHECK_ARG(q && k && v && log_decay && state && out && new_state, "linear_attn_step: bad arguments");
+  BF_CHECK_ARG(aligned16({state, new_state}), "linear_attn_step: states must be 16-byte aligned");
+  const hipStream_t st = as_stream(stream);
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    BF_LAUNCH("linear_attn_step", (linear_step<T>), dim3(unsigned(n * heads)), dim3(256), 0, st, static_cast<const T*>(q),
+              static_cast<const T*>(k), static_cast<const T*>(v), log_decay, state, heads, dim_k, dim_v, scale,
+              static_cast<T*>(out), new_state);
+    BF_CHECK_LAUNCH();
+    return BF_OK;
+  });
+}

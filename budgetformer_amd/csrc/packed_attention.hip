@@ -1,0 +1,742 @@
+// Dense softmax attention inside each sequence of a packed batch, forward and backward, on the matrix cores.
+//
+//   S = scale * q k^T over the keys a row sees, P = exp(S - m) / l, O = P V, lse = m + log l
+//   Delta = sum_d dO O, dV = P^T dO, dP = dO V^T, dS = P (dP - Delta), dQ = scale dS K, dK = scale dS^T Q
+//
+// What a row sees is one interval of keys, [lo, hi), and both ends never fall along the packed axis: own sequence,
+// causal or not, empty sequences and rows behind the last one are all the same to the kernels. Tiles are therefore
+// cut from the packed axis and not from the sequences (a batch of 5-token walks fills its tiles as a long sequence
+// does, and the grid is known without reading a length back): a tile walks the keys from its first row's lo to its
+// last row's hi and compares indices only where a wave's rows do not all see the whole tile. The rows of one key
+// head are (token, head of its group) pairs, token-major, so a group shares its K and V tiles, and dK and dV sum the
+// group in registers. Nothing is added atomically: dQ has a pass of its own (rows own their sums), as dK/dV has (keys
+// own theirs), so results repeat bit for bit; that costs two of seven matrix products and saves the float32
+// dQ buffer with its atomics.
+//
+// Layout. v_mfma 32x32x16 takes 8 values a lane along the contraction (lane l: row or column l % 32, half l / 32) and
+// leaves column l % 32, rows (r % 4) + 8 (r / 4) + 4 (l / 32) of the product in register r. The kernels form S^T
+// (keys by rows) so that a lane owns one row: its maximum and sum are a register loop and one exchange between the
+// halves. Registers 8t .. 8t+7 are then, as they stand, the second operand of the next product over 16 keys, if
+// that product counts its keys as the registers do: value j of half h is key 16t + (j % 4) + 8 (j / 4) + 4 h. The
+// transposed operand (V^T, K^T, Q^T, dO^T) is read from LDS in that order by the transposing LDS reads of 4 x 16
+// blocks. LDS rows are padded by 32 bytes: the 4 rows of such a read, and the 8 rows of a 16-byte read, then
+// fall on different banks. float32 uses the same layout with eight 32x32x2 products for one of 16.
+//
+// Precision: scores, softmax statistics and all sums are float32. P and dS are rounded to the activations' type as
+// operands of the second products (half a step of bf16 is 2^-9 of each term, as the inputs' own rounding); float32
+// rounds nothing.
+//
+// NaN and infinities in places a row does not see: a masked P is 0, but 0 * inf is not. Where a tile is masked its
+// staged operand is checked; one that holds such a value takes a path that multiplies the finite values only, and
+// finds by a second product of indicators which rows do see one.
+#include "packed_tile.h"
+
+namespace bf {
+namespace {
+
+// ---------------------------------------------------------------- arguments
+struct Div {           // n / d for n < 2^31 by a multiplication
+  uint32_t magic, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+};
+
+Div make_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return Div{uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1), s};
+}
+
+struct Args {
+  const void *q, *k, *v, *out, *dout;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta, *part, *stat;
+  const int2 *row_span, *key_span;
+  int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;      // strides in values
+  int32_t rows, n_k, hq, hk, group, dim;           // rows: (token, head of the group) pairs of one key head
+  int32_t tiles, pieces;
+  float scale, c;                                  // c = scale * log2(e)
+  Div by_group;
+  bool head_major;                                 // neighbouring workgroups take the tiles of one head, not the heads of one tile
+};
+
+struct Row {
+  int32_t token, head;     // of the query tensor
+};
+
+__device__ __forceinline__ Row row_of(const Args& a, int h, int rho) {
+  const int32_t t = int32_t(a.by_group(uint32_t(rho)));
+  return Row{t, h * a.group + (rho - t * a.group)};
+}
+
+__device__ __forceinline__ int2 span_at(const int2* s, int i) {
+  const int2 x = s[i];
+  return make_int2(__builtin_amdgcn_readfirstlane(x.x), __builtin_amdgcn_readfirstlane(x.y));
+}
+
+// Which (tile, key head, piece) a workgroup takes. Neighbouring slots share an XCD's L2: by heads (the tiles of a head
+// read the same K and V) or by tiles (the heads of a token share its cache lines). Later tiles first: with a causal
+// mask they see the most keys.
+__device__ __forceinline__ void place(const Args& a, int& tile, int& h, int& piece) {
+  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
+  const int per = a.tiles * a.pieces;
+  int t;
+  if (a.head_major) {
+    h = int(slot / per);
+    t = int(slot % per);
+  } else {
+    t = int(slot / a.hk);
+    h = int(slot % a.hk);
+  }
+  piece = t % a.pieces;
+  tile = a.tiles - 1 - t / a.pieces;
+}
+
+// A row's fragments straight from memory (the operand a wave keeps in registers).
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const T* p, int dim, int half) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int at = 16 * s + 8 * half;
+    if (p && at < dim) {
+      f[s] = *reinterpret_cast<const Frag<T>*>(p + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[s][j] = T(0.f);
+    }
+  }
+}
+
+// A product's columns (one row of the result a lane) to memory, scaled.
+template <int DP, typename O>
+__device__ __forceinline__ void store_cols(O* p, const F32x16 (&acc)[(DP + 31) / 32], float by, int dim, int half) {
+#pragma unroll
+  for (int n = 0; n < (DP + 31) / 32; ++n) store_block<O>(p, acc[n], by, n, dim, half);
+}
+
+// ---------------------------------------------------------------- forward
+template <typename T, int DP, int NW, int BN, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void packed_fwd(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = 64 * NW, BM = 32 * NW;
+  __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
+  __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  int tile, h, piece;
+  place(a, tile, h, piece);
+
+  const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
+  const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
+  int kbeg = max(first_span.x, 0), kend = min(last_span.y, a.n_k);
+  if constexpr (SPLIT) {
+    const int width = (max(kend - kbeg, 0) + a.pieces * BN - 1) / (a.pieces * BN) * BN;
+    kbeg += piece * width;
+    kend = min(kend, kbeg + width);
+  }
+  // this wave's rows, and what they see together
+  const int w_row0 = row0 + 32 * wave, w_last = min(w_row0 + 31, a.rows - 1);
+  const bool w_any = w_row0 < a.rows;
+  const int2 wf = span_at(a.row_span, a.by_group(min(w_row0, a.rows - 1))), wl = span_at(a.row_span, a.by_group(w_last));
+  const int rho = w_row0 + col;
+  const bool valid = rho < a.rows;
+  const Row row = row_of(a, h, valid ? rho : a.rows - 1);
+  const int2 span = a.row_span[row.token];
+  const int lo = span.x, hi = valid ? span.y : span.x;
+
+  Frag<T> qf[TL::kSteps];
+  load_row<T, DP>(qf, valid ? static_cast<const T*>(a.q) + row.token * a.qs_t + row.head * a.qs_h : nullptr, a.dim, half);
+  F32x16 o[TL::kBlocks];
+#pragma unroll
+  for (int n = 0; n < TL::kBlocks; ++n) o[n] = zero16();
+  float mc = -INFINITY, l = 0.f;      // c * maximum, and this half's part of the sum
+
+  const T* kp = static_cast<const T*>(a.k) + h * a.ks_h;
+  const T* vp = static_cast<const T*>(a.v) + h * a.vs_h;
+  Stage<T, DP, BN, NT> ks, vs;
+  auto fetch = [&](int j0) {
+    ks.load(tid, a.dim, [&](int r) { return j0 + r < kend ? kp + (j0 + r) * a.ks_t : nullptr; });
+    vs.load(tid, a.dim, [&](int r) { return j0 + r < kend ? vp + (j0 + r) * a.vs_t : nullptr; });
+  };
+  if (kbeg < kend) fetch(kbeg);
+  for (int j0 = kbeg; j0 < kend; j0 += BN) {
+    __syncthreads();
+    ks.store(tid, k_lds);
+    vs.store(tid, v_lds);
+    bool odd = false;
+    if (j0 < last_span.x || j0 + BN > first_span.y)
+      odd = __syncthreads_or(vs.tainted());
+    else
+      __syncthreads();
+    if (j0 + BN < kend) fetch(j0 + BN);
+    if (!w_any || j0 >= wl.y || j0 + BN <= wf.x) continue;
+
+    float s[BN / 32][16];
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b) {
+      F32x16 acc = zero16();
+#pragma unroll
+      for (int st = 0; st < TL::kSteps; ++st) acc = Mat<T>::mma(TL::row_frag(k_lds, 32 * b + col, st, half), qf[st], acc);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = acc[r];
+    }
+    const bool masked = j0 < wl.x || j0 + BN > wf.y || w_last < w_row0 + 31;
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = j0 + 32 * b + acc_row(r, half);
+          if (key < lo || key >= hi) s[b][r] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float mc_new = fmaxf(mc, top * a.c);
+    if (__any(mc_new > mc)) {
+      const float alpha = mc_new == -INFINITY ? 1.f : exp2_fast(mc - mc_new);
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < TL::kBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+      mc = mc_new;
+    }
+    const float base = mc == -INFINITY ? 0.f : mc;
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = exp2_fast(fmaf(s[b][r], a.c, -base));
+        l += s[b][r];
+      }
+    if (masked && odd) {
+#pragma unroll
+      for (int n = 0; n < TL::kBlocks; ++n) {
+        F32x16 up = zero16(), down = zero16();
+#pragma unroll
+        for (int t = 0; t < BN / 16; ++t) {
+          const Frag<T> p = pack8<T>(s[t / 2], t & 1);
+          Frag<T> clean, fu, fd;
+          split_finite<T>(TL::col_frag(v_lds, t, n, lane), clean, fu, fd);
+          o[n] = Mat<T>::mma(clean, p, o[n]);
+          up = Mat<T>::mma(fu, p, up);
+          down = Mat<T>::mma(fd, p, down);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < BN / 16; ++t) {
+        const Frag<T> p = pack8<T>(s[t / 2], t & 1);
+#pragma unroll
+        for (int n = 0; n < TL::kBlocks; ++n) o[n] = Mat<T>::mma(TL::col_frag(v_lds, t, n, lane), p, o[n]);
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (!valid) return;
+  const int64_t at = int64_t(row.token) * a.hq + row.head;
+  if constexpr (SPLIT) {
+    const int64_t slot = at * a.pieces + piece;
+    if (half == 0) {
+      a.stat[2 * slot] = mc;
+      a.stat[2 * slot + 1] = l;
+    }
+    if (l != 0.f) store_cols<DP>(a.part + slot * a.dim, o, 1.f, a.dim, half);
+  } else {
+    store_cols<DP>(static_cast<T*>(a.o) + at * a.dim, o, l == 0.f ? 0.f : 1.f / l, a.dim, half);
+    if (half == 0) a.lse[at] = l == 0.f ? -INFINITY : mc + __log2f(l);
+  }
+}
+
+// Joins the pieces of a row: one wave a row. out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p.
+template <typename T>
+__global__ __launch_bounds__(256) void packed_join(const float* part, const float* stat, int64_t n_rows, int pieces, int dim,
+                                                   T* out, float* lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= n_rows) return;
+  const float* st = stat + row * pieces * 2;
+  float top = -INFINITY;
+  for (int p = lane; p < pieces; p += 64) top = fmaxf(top, st[2 * p]);
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f, a0 = 0.f, a1 = 0.f;
+  const int d = 2 * lane;
+  for (int p = 0; p < pieces; ++p) {
+    const float m = st[2 * p], lp = st[2 * p + 1];
+    if (lp == 0.f) continue;                              // the piece holds none of the row's keys: nothing was written
+    const float w = exp2_fast(m - base);
+    l = fmaf(w, lp, l);
+    if (d < dim) {
+      const float2 x = *reinterpret_cast<const float2*>(part + (row * pieces + p) * dim + d);
+      a0 = fmaf(w, x.x, a0);
+      a1 = fmaf(w, x.y, a1);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (d < dim) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    const V2 v = {T(a0 * inv), T(a1 * inv)};
+    *reinterpret_cast<V2*>(out + row * dim + d) = v;
+  }
+  if (lane == 0) lse[row] = l == 0.f ? -INFINITY : top + __log2f(l);
+}
+
+// ---------------------------------------------------------------- backward: dQ (and Delta)
+template <typename T, int DP, int NW, int BN>
+__global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = 64 * NW, BM = 32 * NW;
+  __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
+  __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  int tile, h, piece;
+  place(a, tile, h, piece);
+
+  const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
+  const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
+  const int kbeg = max(first_span.x, 0), kend = min(last_span.y, a.n_k);
+  const int w_row0 = row0 + 32 * wave, w_last = min(w_row0 + 31, a.rows - 1);
+  const bool w_any = w_row0 < a.rows;
+  const int2 wf = span_at(a.row_span, a.by_group(min(w_row0, a.rows - 1))), wl = span_at(a.row_span, a.by_group(w_last));
+  const int rho = w_row0 + col;
+  const bool valid = rho < a.rows;
+  const Row row = row_of(a, h, valid ? rho : a.rows - 1);
+  const int2 span = a.row_span[row.token];
+  const int lo = span.x, hi = valid ? span.y : span.x;
+  const int64_t at = int64_t(row.token) * a.hq + row.head;
+
+  Frag<T> qf[TL::kSteps], gf[TL::kSteps];
+  load_row<T, DP>(qf, valid ? static_cast<const T*>(a.q) + row.token * a.qs_t + row.head * a.qs_h : nullptr, a.dim, half);
+  load_row<T, DP>(gf, valid ? static_cast<const T*>(a.dout) + at * a.dim : nullptr, a.dim, half);
+  float delta = 0.f;
+  {
+    Frag<T> of[TL::kSteps];
+    load_row<T, DP>(of, valid ? static_cast<const T*>(a.out) + at * a.dim : nullptr, a.dim, half);
+#pragma unroll
+    for (int s = 0; s < TL::kSteps; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(float(gf[s][j]), float(of[s][j]), delta);
+    delta += __shfl_xor(delta, 32, 64);
+    if (valid && half == 0) a.delta[at] = delta;
+  }
+  // a row without a finite score has lse = -inf and P = 0: +inf in the exponent's place gives that
+  float lse = a.lse[at];
+  if (lse == -INFINITY) lse = INFINITY;
+
+  F32x16 dq[TL::kBlocks];
+#pragma unroll
+  for (int n = 0; n < TL::kBlocks; ++n) dq[n] = zero16();
+  const T* kp = static_cast<const T*>(a.k) + h * a.ks_h;
+  const T* vp = static_cast<const T*>(a.v) + h * a.vs_h;
+  Stage<T, DP, BN, NT> ks, vs;
+  auto fetch = [&](int j0) {
+    ks.load(tid, a.dim, [&](int r) { return j0 + r < kend ? kp + (j0 + r) * a.ks_t : nullptr; });
+    vs.load(tid, a.dim, [&](int r) { return j0 + r < kend ? vp + (j0 + r) * a.vs_t : nullptr; });
+  };
+  if (kbeg < kend) fetch(kbeg);
+  for (int j0 = kbeg; j0 < kend; j0 += BN) {
+    __syncthreads();
+    ks.store(tid, k_lds);
+    vs.store(tid, v_lds);
+    bool odd = false;
+    if (j0 < last_span.x || j0 + BN > first_span.y)
+      odd = __syncthreads_or(ks.tainted());
+    else
+      __syncthreads();
+    if (j0 + BN < kend) fetch(j0 + BN);
+    if (!w_any || j0 >= wl.y || j0 + BN <= wf.x) continue;
+    const bool masked = j0 < wl.x || j0 + BN > wf.y || w_last < w_row0 + 31;
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b) {
+      F32x16 sa = zero16(), pa = zero16();
+#pragma unroll
+      for (int st = 0; st < TL::kSteps; ++st) {
+        sa = Mat<T>::mma(TL::row_frag(k_lds, 32 * b + col, st, half), qf[st], sa);
+        pa = Mat<T>::mma(TL::row_frag(v_lds, 32 * b + col, st, half), gf[st], pa);
+      }
+      float ds[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(fmaf(sa[r], a.c, -lse)) * (pa[r] - delta);
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = j0 + 32 * b + acc_row(r, half);
+          if (key < lo || key >= hi) ds[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag<T> f = pack8<T>(ds, t);
+#pragma unroll
+        for (int n = 0; n < TL::kBlocks; ++n) {
+          Frag<T> kt = TL::col_frag(k_lds, 2 * b + t, n, lane);
+          if (masked && odd) {      // a key with such a value has no finite score: the rows that see it get theirs by dS
+            Frag<T> up, down;
+            split_finite<T>(Frag<T>(kt), kt, up, down);
+          }
+          dq[n] = Mat<T>::mma(kt, f, dq[n]);
+        }
+      }
+    }
+  }
+  if (valid) store_cols<DP>(static_cast<T*>(a.dq) + at * a.dim, dq, a.scale, a.dim, half);
+}
+
+// ---------------------------------------------------------------- backward: dK and dV
+// A wave owns 32 keys (a lane one of them); Q and dO tiles of BR rows pass through LDS with their rows' lse and Delta.
+template <typename T, int DP, int NW, int BR>
+__global__ __launch_bounds__(64 * NW) void packed_bwd_kv(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = 64 * NW, BK = 32 * NW;
+  __shared__ __attribute__((aligned(16))) char q_lds[TL::bytes(BR)];
+  __shared__ __attribute__((aligned(16))) char g_lds[TL::bytes(BR)];
+  __shared__ __attribute__((aligned(16))) float lse_lds[BR], delta_lds[BR];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  int tile, h, piece;
+  place(a, tile, h, piece);
+  tile = a.tiles - 1 - tile;                       // with a causal mask the first keys are seen by the most rows
+
+  const int key0 = tile * BK, last = min(key0 + BK, a.n_k) - 1;
+  const int2 first_span = span_at(a.key_span, key0), last_span = span_at(a.key_span, last);
+  // rows of the group: token * group + head
+  const int rbeg = max(first_span.x, 0) * a.group, rend = min(last_span.y * a.group, a.rows);
+  const int w_key0 = key0 + 32 * wave, w_last = min(w_key0 + 31, a.n_k - 1);
+  const bool w_any = w_key0 < a.n_k;
+  const int2 wf = span_at(a.key_span, min(w_key0, a.n_k - 1)), wl = span_at(a.key_span, w_last);
+  const int w_beg = wf.x * a.group, w_end = wl.y * a.group, w_full_beg = wl.x * a.group, w_full_end = wf.y * a.group;
+  const int key = w_key0 + col;
+  const bool valid = key < a.n_k;
+  const int2 span = a.key_span[valid ? key : a.n_k - 1];
+  const int lo = span.x * a.group, hi = valid ? span.y * a.group : lo;
+
+  Frag<T> kf[TL::kSteps], vf[TL::kSteps];
+  load_row<T, DP>(kf, valid ? static_cast<const T*>(a.k) + key * a.ks_t + h * a.ks_h : nullptr, a.dim, half);
+  load_row<T, DP>(vf, valid ? static_cast<const T*>(a.v) + key * a.vs_t + h * a.vs_h : nullptr, a.dim, half);
+  F32x16 dk[TL::kBlocks], dv[TL::kBlocks];
+#pragma unroll
+  for (int n = 0; n < TL::kBlocks; ++n) dk[n] = zero16(), dv[n] = zero16();
+
+  const T* qp = static_cast<const T*>(a.q);
+  const T* gp = static_cast<const T*>(a.dout);
+  Stage<T, DP, BR, NT> qs, gs;
+  float stat = 0.f;
+  auto fetch = [&](int i0) {
+    qs.load(tid, a.dim, [&](int r) -> const T* {
+      if (i0 + r >= rend) return nullptr;
+      const Row w = row_of(a, h, i0 + r);
+      return qp + w.token * a.qs_t + w.head * a.qs_h;
+    });
+    gs.load(tid, a.dim, [&](int r) -> const T* {
+      if (i0 + r >= rend) return nullptr;
+      const Row w = row_of(a, h, i0 + r);
+      return gp + (int64_t(w.token) * a.hq + w.head) * a.dim;
+    });
+    if (tid < 2 * BR) {
+      const int r = i0 + (tid & (BR - 1));
+      stat = tid < BR ? INFINITY : 0.f;
+      if (r < rend) {
+        const Row w = row_of(a, h, r);
+        const int64_t at = int64_t(w.token) * a.hq + w.head;
+        stat = tid < BR ? a.lse[at] : a.delta[at];
+        if (tid < BR && stat == -INFINITY) stat = INFINITY;
+      }
+    }
+  };
+  static_assert(2 * BR <= NT, "one statistic a lane");
+  if (rbeg < rend) fetch(rbeg);
+  for (int i0 = rbeg; i0 < rend; i0 += BR) {
+    __syncthreads();
+    qs.store(tid, q_lds);
+    gs.store(tid, g_lds);
+    if (tid < BR)
+      lse_lds[tid] = stat;
+    else if (tid < 2 * BR)
+      delta_lds[tid - BR] = stat;
+    bool odd = false;
+    if (i0 < last_span.x * a.group || i0 + BR > first_span.y * a.group) {
+      const bool mine = qs.tainted() || gs.tainted();
+      odd = __syncthreads_or(mine);
+    } else {
+      __syncthreads();
+    }
+    if (i0 + BR < rend) fetch(i0 + BR);
+    if (!w_any || i0 >= w_end || i0 + BR <= w_beg) continue;
+    const bool masked = i0 < w_full_beg || i0 + BR > w_full_end || w_last < w_key0 + 31;
+#pragma unroll
+    for (int b = 0; b < BR / 32; ++b) {
+      F32x16 sa = zero16(), pa = zero16();
+#pragma unroll
+      for (int st = 0; st < TL::kSteps; ++st) {
+        sa = Mat<T>::mma(TL::row_frag(q_lds, 32 * b + col, st, half), kf[st], sa);
+        pa = Mat<T>::mma(TL::row_frag(g_lds, 32 * b + col, st, half), vf[st], pa);
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 ls = *reinterpret_cast<const float4*>(&lse_lds[32 * b + 8 * g + 4 * half]);
+        const float4 de = *reinterpret_cast<const float4*>(&delta_lds[32 * b + 8 * g + 4 * half]);
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[4 * g + j] = exp2_fast(fmaf(sa[4 * g + j], a.c, -lv[j]));
+          ds[4 * g + j] = p[4 * g + j] * (pa[4 * g + j] - dl[j]);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = i0 + 32 * b + acc_row(r, half);
+          if (i < lo || i >= hi) p[r] = 0.f, ds[r] = 0.f;
+        }
+      }
+      if (masked && odd) {
+#pragma unroll
+        for (int n = 0; n < TL::kBlocks; ++n) {
+          F32x16 up = zero16(), down = zero16();
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const Frag<T> pf = pack8<T>(p, t), df = pack8<T>(ds, t);
+            Frag<T> clean, fu, fd;
+            split_finite<T>(TL::col_frag(g_lds, 2 * b + t, n, lane), clean, fu, fd);
+            dv[n] = Mat<T>::mma(clean, pf, dv[n]);
+            up = Mat<T>::mma(fu, pf, up);
+            down = Mat<T>::mma(fd, pf, down);
+            split_finite<T>(TL::col_frag(q_lds, 2 * b + t, n, lane), clean, fu, fd);
+            dk[n] = Mat<T>::mma(clean, df, dk[n]);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dv[n][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const Frag<T> pf = pack8<T>(p, t), df = pack8<T>(ds, t);
+#pragma unroll
+          for (int n = 0; n < TL::kBlocks; ++n) {
+            dv[n] = Mat<T>::mma(TL::col_frag(g_lds, 2 * b + t, n, lane), pf, dv[n]);
+            dk[n] = Mat<T>::mma(TL::col_frag(q_lds, 2 * b + t, n, lane), df, dk[n]);
+          }
+        }
+      }
+    }
+  }
+  if (!valid) return;
+  const int64_t at = (int64_t(key) * a.hk + h) * a.dim;
+  store_cols<DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.dim, half);
+  store_cols<DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.dim, half);
+}
+
+// ---------------------------------------------------------------- spans
+// The keys each query row sees, and the query rows that see each key, from the sequences' offsets (one thread a row:
+// a binary search for its sequence). Rows behind the last sequence see nothing. Offsets are taken as they are and
+// every span is clamped to the tensors, so bad ones give wrong results and no access outside.
+__global__ __launch_bounds__(256) void packed_spans(const int32_t* q_off, const int32_t* k_off, int32_t n_seq, int32_t n_q,
+                                                    int32_t n_k, int causal, int2* row_span, int2* key_span, int32_t* positions) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const bool is_q = i < n_q;
+  if (i >= int64_t(n_q) + n_k) return;
+  const int32_t x = int32_t(is_q ? i : i - n_q);
+  const int32_t* off = is_q ? q_off : k_off;
+  int lo = 0, hi = n_seq;                       // the last s with off[s] <= x
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid + 1] <= x)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  const int32_t lim = is_q ? n_k : n_q;
+  int2 s;
+  if (lo == n_seq || x < off[0]) {
+    const int32_t end = lo == n_seq ? (is_q ? k_off : q_off)[n_seq] : 0;
+    s = make_int2(end, end);
+    if (is_q && positions) positions[x] = 0;
+  } else {
+    const int32_t q0 = q_off[lo], q1 = q_off[lo + 1], k0 = k_off[lo], k1 = k_off[lo + 1];
+    const int32_t past = (k1 - k0) - (q1 - q0);
+    if (is_q && positions) positions[x] = x - q0 + past;
+    if (is_q)
+      s = make_int2(k0, causal ? max(k0, min(k1, k0 + (x - q0) + past + 1)) : k1);
+    else
+      s = make_int2(causal ? max(q0, min(q1, q0 + (x - k0) - past)) : q0, q1);
+  }
+  s.x = min(max(s.x, 0), lim);
+  s.y = min(max(s.y, s.x), lim);
+  (is_q ? row_span : key_span)[x] = s;
+}
+
+// ---------------------------------------------------------------- launches
+constexpr int kWide = 4;          // waves of a workgroup, each 32 rows (or keys)
+constexpr int kMaxPieces = 64;
+
+template <typename T> constexpr int tile_keys() { return sizeof(T) == 2 ? 64 : 32; }
+
+template <typename F> int with_dim(int dim, F&& f) {
+  if (dim <= 16) return f(std::integral_constant<int, 16>());
+  if (dim <= 32) return f(std::integral_constant<int, 32>());
+  if (dim <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+
+int check(const bf_packed_attn* p, const char* fn, bool backward) {
+  BF_CHECK_ARG(p != nullptr, "%s: no arguments", fn);
+  BF_CHECK_ARG(p->dtype == BF_DTYPE_F32 || p->dtype == BF_DTYPE_BF16 || p->dtype == BF_DTYPE_F16, "%s: dtype %d", fn,
+               p->dtype);
+  BF_CHECK_ARG(p->heads_q >= 1 && p->heads_k >= 1 && p->heads_q % p->heads_k == 0,
+               "%s: %d query heads over %d key heads (a multiple expected)", fn, p->heads_q, p->heads_k);
+  if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8) {
+    set_error("%s: head_dim %d (a multiple of 8 up to 128 is supported)", fn, p->head_dim);
+    return BF_ERR_UNSUPPORTED;
+  }
+  BF_CHECK_ARG(p->n_q >= 0 && p->n_k >= 0 && p->n_k < (int64_t(1) << 31) - 256 &&
+                   p->n_q < ((int64_t(1) << 31) - 256) / p->heads_q,
+               "%s: %lld rows of %d heads, %lld keys (below 2^31 each)", fn, (long long)p->n_q, p->heads_q, (long long)p->n_k);
+  BF_CHECK_ARG(p->scale > 0.f && p->scale <= 3e38f, "%s: scale %g (positive and finite expected)", fn, double(p->scale));
+  const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;
+  for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
+    BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,
+                 "%s: strides (%lld, %lld) are not whole 16-byte steps", fn, (long long)s[0], (long long)s[1]);
+  BF_CHECK_ARG(p->n_q == 0 || p->row_span, "%s: no row spans", fn);
+  BF_CHECK_ARG(!backward || p->n_k == 0 || p->key_span, "%s: no key spans", fn);
+  return BF_OK;
+}
+
+Args make_args(const bf_packed_attn* p, const void* q, const void* k, const void* v) {
+  Args a{};
+  a.q = q, a.k = k, a.v = v;
+  a.row_span = reinterpret_cast<const int2*>(p->row_span);
+  a.key_span = reinterpret_cast<const int2*>(p->key_span);
+  a.qs_t = p->q_stride[0], a.qs_h = p->q_stride[1];
+  a.ks_t = p->k_stride[0], a.ks_h = p->k_stride[1];
+  a.vs_t = p->v_stride[0], a.vs_h = p->v_stride[1];
+  a.hq = p->heads_q, a.hk = p->heads_k, a.group = p->heads_q / p->heads_k, a.dim = p->head_dim;
+  a.rows = int32_t(p->n_q * a.group);
+  a.n_k = int32_t(p->n_k);
+  a.scale = p->scale;
+  a.c = p->scale * kLog2e;
+  a.by_group = make_div(uint32_t(a.group));
+  a.pieces = 1;
+  a.head_major = true;
+  return a;
+}
+
+// Pieces a tile's keys are cut into. Workgroups of 4 waves over whole rows fill the chip (256 CUs, two workgroups each)
+// from 512 of them on; below that, one-wave workgroups over pieces of the keys do.
+int pieces_of(const bf_packed_attn* p) {
+  const int64_t rows = p->n_q * (p->heads_q / p->heads_k);
+  if (ceil_div(rows, 32 * kWide) * p->heads_k >= 256) return 1;
+  const int64_t tiles = ceil_div(rows, 32) * p->heads_k;
+  const int64_t want = ceil_div(2048, tiles);
+  const int64_t most = ceil_div(p->n_k, 64);
+  int64_t n = want < most ? want : most;
+  if (n > kMaxPieces) n = kMaxPieces;
+  return n < 1 ? 1 : int(n);
+}
+
+}  // namespace
+}  // namespace bf
+
+using namespace bf;
+
+extern "C" int bf_packed_spans(const int32_t* q_offsets, const int32_t* k_offsets, int64_t n_seq, int64_t n_q, int64_t n_k,
+                               int32_t causal, int32_t* row_span, int32_t* key_span, int32_t* positions,
+                               void* stream) {
+  BF_CHECK_ARG(n_seq >= 0 && n_q >= 0 && n_k >= 0 && n_seq < (int64_t(1) << 31) - 1 && n_q < (int64_t(1) << 31) - 1 &&
+                   n_k < (int64_t(1) << 31) - 1,
+               "packed_spans: sizes must fit 32 bits");
+  if (n_q + n_k == 0) return BF_OK;
+  BF_CHECK_ARG(q_offsets && k_offsets && (n_q == 0 || row_span) && (n_k == 0 || key_span), "packed_spans: bad arguments");
+  BF_LAUNCH("packed_spans", packed_spans, dim3(unsigned(ceil_div(n_q + n_k, 256))), dim3(256), 0, as_stream(stream),
+            q_offsets, k_offsets, int32_t(n_seq), int32_t(n_q), int32_t(n_k), int(causal != 0),
+            reinterpret_cast<int2*>(row_span), reinterpret_cast<int2*>(key_span), positions);
+  BF_CHECK_LAUNCH();
+  return BF_OK;
+}
+
+extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
+  if (check(p, "packed_attn_fwd_floats", false) != BF_OK) return -1;
+  const int n = p->n_q == 0 ? 1 : pieces_of(p);
+  return n == 1 ? 0 : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
+}
+
+extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
+                                  float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "packed_attn_fwd", false));
+  if (p->n_q == 0) return BF_OK;
+  BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
+  Args a = make_args(p, q, k, v);
+  a.o = out, a.lse = lse;
+  a.pieces = pieces_of(p);
+  const hipStream_t st = as_stream(stream);
+  if (a.pieces == 1) {
+    a.tiles = int(ceil_div(a.rows, 32 * kWide));
+    return with_type(p->dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      return with_dim(a.dim, [&](auto dp) -> int {
+        constexpr int DP = decltype(dp)::value, BN = tile_keys<T>();
+        auto kern = packed_fwd<T, DP, kWide, BN, false>;
+        BF_LAUNCH("packed_attn_fwd", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        BF_CHECK_LAUNCH();
+        return BF_OK;
+      });
+    });
+  }
+  BF_CHECK_ARG(scratch != nullptr, "packed_attn_fwd: no scratch (bf_packed_attn_fwd_floats)");
+  const int64_t n_rows = p->n_q * p->heads_q;
+  a.part = scratch;
+  a.stat = scratch + n_rows * a.pieces * a.dim;
+  a.tiles = int(ceil_div(a.rows, 32));
+  return with_type(p->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_dim(a.dim, [&](auto dp) -> int {
+      constexpr int DP = decltype(dp)::value;
+      auto kern = packed_fwd<T, DP, 1, 32, true>;
+      BF_LAUNCH("packed_attn_fwd_pieces", kern, dim3(unsigned(int64_t(a.tiles) * a.hk * a.pieces)), dim3(64), 0, st, a);
+      BF_CHECK_LAUNCH();
+      BF_LAUNCH("packed_attn_join", (packed_join<T>), dim3(unsigned(ceil_div(n_rows, 4))), dim3(256), 0, st, a.part, a.stat,
+                n_rows, a.pieces, a.dim, static_cast<T*>(out), lse);
+      BF_CHECK_LAUNCH();
+      return BF_OK;
+    });
+  });
+}
+
+extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta,
+                                  void* stream) {
+  BF_CHECK_OK(check(p, "packed_attn_bwd", true));
+  BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
+               "packed_attn_bwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
+  Args a = make_args(p, q, k, v);
+  a.out = out, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
+  a.lse = const_cast<float*>(lse);
+  const hipStream_t st = as_stream(stream);
+  return with_type(p->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_dim(a.dim, [&](auto dp) -> int {
+      constexpr int DP = decltype(dp)::value;
+      if (a.rows > 0) {
+        a.tiles = int(ceil_div(a.rows, 32 * kWide));
+        auto kern = packed_bwd_q<T, DP, kWide, 32>;
+        BF_LAUNCH("packed_attn_bwd_q", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        BF_CHECK_LAUNCH();
+      }
+      if (a.n_k > 0) {
+        a.tiles = int(ceil_div(a.n_k, 32 * kWide));
+        auto kern = packed_bwd_kv<T, DP, kWide, 32>;
+        BF_LAUNCH("packed_attn_bwd_kv", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        BF_CHECK_LAUNCH();
+      }
+      return BF_OK;
+    });
+  });
+}

@@ -503,6 +503,227 @@ std::vector<at::Tensor> reverse_index_and_plan(const at::Tensor& keys, const at:
   return out;
 }
 
+// ---------------------------------------------------------------- operators over packed sequences
+// What each row sees (bf_packed_spans): (row_span int32 [n_q, 2], key_span int32 [n_k, 2], positions int32 [n_q]).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_spans(const at::Tensor& q_offsets, const at::Tensor& k_offsets,
+                                                            int64_t n_q, int64_t n_k, bool causal) {
+  const c10::DeviceGuard guard(q_offsets.device());
+  const at::Device dev = q_offsets.device();
+  require(q_offsets, "q_offsets", at::kInt, dev);
+  require(k_offsets, "k_offsets", at::kInt, dev);
+  TORCH_CHECK_VALUE(q_offsets.dim() == 1 && q_offsets.sizes() == k_offsets.sizes() && q_offsets.numel() >= 1,
+                    "offsets must be [n_seq + 1] each (got ", q_offsets.sizes(), " and ", k_offsets.sizes(), ")");
+  TORCH_CHECK_VALUE(n_q >= 0 && n_k >= 0, "packed_spans: bad sizes");
+  at::Tensor row_span = at::empty({n_q, 2}, q_offsets.options()), key_span = at::empty({n_k, 2}, q_offsets.options());
+  at::Tensor positions = at::empty({n_q}, q_offsets.options());
+  check_rc(bf_packed_spans(q_offsets.data_ptr<int32_t>(), k_offsets.data_ptr<int32_t>(), q_offsets.numel() - 1, n_q, n_k,
+                           causal ? 1 : 0, row_span.data_ptr<int32_t>(), key_span.data_ptr<int32_t>(),
+                           positions.data_ptr<int32_t>(), stream_of(q_offsets)),
+           "bf::packed_spans");
+  return {row_span, key_span, positions};
+}
+
+// A [rows, heads, dim] tensor with a contiguous last dimension; its strides of a row and of a head in values. Strides of
+// dimensions of one entry do not matter and are given as 0.
+void require_heads(const at::Tensor& t, const char* name, at::ScalarType st, const at::Device& dev, int64_t (&stride)[2]) {
+  TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), ", expected ", dev);
+  TORCH_CHECK_VALUE(t.scalar_type() == st, name, " must be ", st, " (got ", t.scalar_type(), ")");
+  TORCH_CHECK_VALUE(t.dim() == 3, name, " must be [rows, heads, head_dim] (got ", t.sizes(), ")");
+  TORCH_CHECK_VALUE(t.stride(2) == 1 || t.size(2) <= 1, name, " must be contiguous along the head (strides ", t.strides(),
+                    ")");
+  stride[0] = t.size(0) > 1 ? t.stride(0) : 0;
+  stride[1] = t.size(1) > 1 ? t.stride(1) : 0;
+}
+
+void require_span(const at::Tensor& t, const char* name, int64_t n, const at::Device& dev) {
+  require(t, name, at::kInt, dev);
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == n && t.size(1) == 2, name, " must be [", n, ", 2] (got ", t.sizes(), ")");
+}
+
+bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& row_span,
+                           double scale) {
+  const at::Device dev = q.device();
+  bf_packed_attn p{};
+  p.dtype = dtype_code(q);
+  require_heads(q, "q", q.scalar_type(), dev, p.q_stride);
+  require_heads(k, "k", q.scalar_type(), dev, p.k_stride);
+  require_heads(v, "v", q.scalar_type(), dev, p.v_stride);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && q.size(2) == k.size(2), "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(),
+                    " disagree");
+  TORCH_CHECK_VALUE(q.size(1) < (int64_t(1) << 31) && k.size(1) < (int64_t(1) << 31) && q.size(2) < (int64_t(1) << 31),
+                    "too many heads");
+  p.n_q = q.size(0), p.n_k = k.size(0);
+  p.heads_q = int32_t(q.size(1)), p.heads_k = int32_t(k.size(1)), p.head_dim = int32_t(q.size(2));
+  require_span(row_span, "row_span", p.n_q, dev);
+  p.row_span = row_span.data_ptr<int32_t>();
+  p.scale = float(scale);
+  return p;
+}
+
+// Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2).
+std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                   const at::Tensor& row_span, double scale) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const c10::DeviceGuard guard(q.device());
+  const bf_packed_attn p = packed_args(q, k, v, row_span, scale);
+  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  const int64_t floats = bf_packed_attn_fwd_floats(&p);
+  at::Tensor scratch;
+  if (floats > 0) scratch = at::empty({floats}, lse.options());
+  check_rc(bf_packed_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
+           "bf::packed_attn_fwd");
+  return {out, lse};
+}
+
+// Backward (bf_packed_attn_bwd): (dq, dk, dv), contiguous.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                               const at::Tensor& row_span, const at::Tensor& key_span,
+                                                               const at::Tensor& out, const at::Tensor& lse,
+                                                               const at::Tensor& dout, double scale) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const c10::DeviceGuard guard(q.device());
+  const at::Device dev = q.device();
+  bf_packed_attn p = packed_args(q, k, v, row_span, scale);
+  require_span(key_span, "key_span", p.n_k, dev);
+  p.key_span = key_span.data_ptr<int32_t>();
+  require(out, "out", q.scalar_type(), dev);
+  require(dout, "dout", q.scalar_type(), dev);
+  require(lse, "lse", at::kFloat, dev);
+  TORCH_CHECK_VALUE(out.sizes() == q.sizes() && dout.sizes() == q.sizes() && lse.numel() == q.size(0) * q.size(1), "out ",
+                    out.sizes(), ", dout ", dout.sizes(), " or lse ", lse.sizes(), " do not match q ", q.sizes());
+  const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
+  at::Tensor delta = at::empty_like(lse);
+  check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+                              dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(),
+                              stream_of(q)),
+           "bf::packed_attn_bwd");
+  return {dq, dk, dv};
+}
+
+// Rotary positions (bf_rotary) of x and, if given, y: new contiguous tensors.
+std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& x, const std::optional<at::Tensor>& y, const at::Tensor& positions,
+                                          const at::Tensor& turns, double amplitude, bool interleaved, bool inverse) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a device tensor (got ", x.device(), ")");
+  const c10::DeviceGuard guard(x.device());
+  const at::Device dev = x.device();
+  const bool two = y.has_value() && y->defined();
+  int64_t xs[2], ys[2] = {0, 0};
+  require_heads(x, "x", x.scalar_type(), dev, xs);
+  if (two) {
+    require_heads(*y, "y", x.scalar_type(), dev, ys);
+    TORCH_CHECK_VALUE(y->size(0) == x.size(0) && y->size(2) == x.size(2), "x ", x.sizes(), " and y ", y->sizes(), " disagree");
+  }
+  TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+                    "positions must be int32 or int64 (got ", positions.scalar_type(), ")");
+  require(positions, "positions", positions.scalar_type(), dev);
+  TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == x.size(0), "positions must be [", x.size(0), "] (got ",
+                    positions.sizes(), ")");
+  require(turns, "turns", at::kDouble, dev);
+  TORCH_CHECK_VALUE(turns.dim() == 1, "turns must be [rot / 2]");
+  for (int64_t n : {x.size(1), x.size(2), two ? y->size(1) : 0, turns.size(0)})
+    TORCH_CHECK_VALUE(n < (int64_t(1) << 30), "rotary: bad sizes");
+  const auto plain = x.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor ox = at::empty(x.sizes(), plain), oy = two ? at::empty(y->sizes(), plain) : at::empty({0}, plain);
+  const int32_t code = dtype_code(x);
+  // a y of no heads is no y
+  const bool y_heads = two && y->size(1) > 0;
+  check_rc(bf_rotary(x.data_ptr(), y_heads ? y->data_ptr() : nullptr, x.size(0), int32_t(x.size(1)),
+                     y_heads ? int32_t(y->size(1)) : 0, int32_t(x.size(2)), int32_t(2 * turns.size(0)), code, xs, ys,
+                     positions.data_ptr(), positions.scalar_type() == at::kLong, turns.data_ptr<double>(), float(amplitude),
+                     interleaved ? 1 : 0, inverse ? 1 : 0, ox.data_ptr(), y_heads ? oy.data_ptr() : nullptr, stream_of(x)),
+           "bf::rotary");
+  return {ox, oy};
+}
+
+// One pass of linear attention (bf_linear_attn_pass): (out, final state float32 [n_seq, heads, dim_x, dim_z] or empty).
+// init_state float32 [n_seq, heads, dim_x, dim_z], of any strides over the last two dimensions.
+std::tuple<at::Tensor, at::Tensor> linear_attn_pass(const at::Tensor& x, const at::Tensor& y, const at::Tensor& z,
+                                                    const at::Tensor& log_decay, const at::Tensor& row_span,
+                                                    const at::Tensor& key_span, const at::Tensor& offsets, double scale,
+                                                    bool reverse, const std::optional<at::Tensor>& init_state,
+                                                    bool return_state) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a device tensor (got ", x.device(), ")");
+  const c10::DeviceGuard guard(x.device());
+  const at::Device dev = x.device();
+  bf_linear_attn p{};
+  p.dtype = dtype_code(x);
+  require_heads(x, "x", x.scalar_type(), dev, p.x_stride);
+  require_heads(y, "y", x.scalar_type(), dev, p.y_stride);
+  require_heads(z, "z", x.scalar_type(), dev, p.z_stride);
+  TORCH_CHECK_VALUE(x.sizes() == y.sizes() && z.size(0) == x.size(0) && z.size(1) == x.size(1), "x ", x.sizes(), ", y ",
+                    y.sizes(), ", z ", z.sizes(), " disagree");
+  TORCH_CHECK_VALUE(x.size(1) < (int64_t(1) << 30) && x.size(2) < (int64_t(1) << 30) && z.size(2) < (int64_t(1) << 30),
+                    "linear_attn_pass: bad sizes");
+  const int64_t T = x.size(0), H = x.size(1), dx = x.size(2), dz = z.size(2);
+  require(log_decay, "log_decay", at::kFloat, dev);
+  TORCH_CHECK_VALUE(log_decay.dim() == 1 && log_decay.size(0) == H, "log_decay must be [", H, "] (got ", log_decay.sizes(), ")");
+  require_span(row_span, "row_span", T, dev);
+  require_span(key_span, "key_span", T, dev);
+  require(offsets, "offsets", at::kInt, dev);
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must be [n_seq + 1]");
+  const int64_t n_seq = offsets.numel() - 1;
+  p.n = T, p.n_seq = n_seq, p.heads = int32_t(H), p.dim_x = int32_t(dx), p.dim_z = int32_t(dz);
+  p.row_span = row_span.data_ptr<int32_t>(), p.key_span = key_span.data_ptr<int32_t>();
+  p.offsets = offsets.data_ptr<int32_t>(), p.log_decay = log_decay.data_ptr<float>();
+  p.scale = float(scale), p.reverse = reverse ? 1 : 0;
+  if (init_state.has_value() && init_state->defined()) {
+    const at::Tensor& s = *init_state;
+    TORCH_CHECK_VALUE(s.device() == dev && s.scalar_type() == at::kFloat, "init_state must be float32 on ", dev);
+    TORCH_CHECK_VALUE(s.dim() == 4 && s.size(0) == n_seq && s.size(1) == H && s.size(2) == dx && s.size(3) == dz,
+                      "init_state must be [", n_seq, ", ", H, ", ", dx, ", ", dz, "] (got ", s.sizes(), ")");
+    TORCH_CHECK_VALUE(s.numel() == 0 || ((s.size(0) == 1 || s.stride(0) == H * dx * dz) && (H == 1 || s.stride(1) == dx * dz)),
+                      "init_state must be contiguous over sequences and heads");
+    p.init = s.data_ptr<float>();
+    p.init_stride[0] = s.stride(2), p.init_stride[1] = s.stride(3);
+  }
+  at::Tensor out = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor final_state = return_state ? at::empty({n_seq, H, dx, dz}, log_decay.options()) : at::empty({0}, log_decay.options());
+  if (return_state) p.final_state = final_state.data_ptr<float>();
+  const int64_t floats = bf_linear_attn_floats(&p);
+  at::Tensor scratch;
+  if (floats > 0) scratch = at::empty({floats}, log_decay.options());
+  check_rc(bf_linear_attn_pass(&p, x.data_ptr(), y.data_ptr(), z.data_ptr(), out.data_ptr(),
+                               floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(x)),
+           "bf::linear_attn_pass");
+  return {out, final_state};
+}
+
+// One token of each sequence (bf_linear_attn_step): (out, new state); out_state: where the new state goes (state itself
+// updates it in place), else a new tensor.
+std::tuple<at::Tensor, at::Tensor> linear_attn_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& log_decay, const at::Tensor& state, double scale,
+                                                    const std::optional<at::Tensor>& out_state) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const c10::DeviceGuard guard(q.device());
+  const at::Device dev = q.device();
+  const int32_t code = dtype_code(q);
+  require(q, "q", q.scalar_type(), dev);
+  require(k, "k", q.scalar_type(), dev);
+  require(v, "v", q.scalar_type(), dev);
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.sizes() == q.sizes() && v.dim() == 3 && v.size(0) == q.size(0) && v.size(1) == q.size(1),
+                    "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), " must be [sequences, heads, head_dim]");
+  const int64_t n = q.size(0), H = q.size(1), dk = q.size(2), dv = v.size(2);
+  TORCH_CHECK_VALUE(H < (int64_t(1) << 30) && dk < (int64_t(1) << 30) && dv < (int64_t(1) << 30), "linear_attn_step: bad sizes");
+  require(log_decay, "log_decay", at::kFloat, dev);
+  TORCH_CHECK_VALUE(log_decay.dim() == 1 && log_decay.size(0) == H, "log_decay must be [", H, "] (got ", log_decay.sizes(), ")");
+  const bool given = out_state.has_value() && out_state->defined();
+  for (const at::Tensor* s : {&state, given ? &*out_state : &state}) {
+    require(*s, s == &state ? "state" : "out_state", at::kFloat, dev);
+    TORCH_CHECK_VALUE(s->dim() == 4 && s->size(0) == n && s->size(1) == H && s->size(2) == dk && s->size(3) == dv,
+                      "a state must be [", n, ", ", H, ", ", dk, ", ", dv, "] (got ", s->sizes(), ")");
+  }
+  at::Tensor out = at::empty_like(v), next = given ? *out_state : at::empty_like(state);
+  if (n == 0) return {out, next};
+  check_rc(bf_linear_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr<float>(), state.data_ptr<float>(), n,
+                               int32_t(H), int32_t(dk), int32_t(dv), code, float(scale), out.data_ptr(),
+                               next.data_ptr<float>(), stream_of(q)),
+           "bf::linear_attn_step");
+  return {out, next};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(bf, m) {
@@ -529,6 +750,17 @@ TORCH_LIBRARY(bf, m) {
         "int slot_bits, int plan_items, int chunk, int item, Tensor(a!) counts) -> Tensor[]");
   m.def("reverse_index_and_plan(Tensor keys, Tensor qptr, int nnz, int n_kv, int q_bits, int slot_bits, "
         "bool global_token, int token_row, bool entries, int chunk, int item, Tensor(a!) counts) -> Tensor[]");
+  m.def("packed_spans(Tensor q_offsets, Tensor k_offsets, int n_q, int n_k, bool causal) -> (Tensor, Tensor, Tensor)");
+  m.def("packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor row_span, float scale) -> (Tensor, Tensor)");
+  m.def("packed_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor row_span, Tensor key_span, Tensor out, Tensor lse, "
+        "Tensor dout, float scale) -> (Tensor, Tensor, Tensor)");
+  m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
+        "bool inverse=False) -> (Tensor, Tensor)");
+  m.def("linear_attn_pass(Tensor x, Tensor y, Tensor z, Tensor log_decay, Tensor row_span, Tensor key_span, "
+        "Tensor offsets, float scale, bool reverse=False, Tensor? init_state=None, bool return_state=False) "
+        "-> (Tensor, Tensor)");
+  m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor state, float scale, "
+        "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(bf, CUDA, m) {
@@ -542,4 +774,10 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
   m.impl("transpose_table", &transpose_table);
   m.impl("table_index", &table_index);
   m.impl("reverse_index_and_plan", &reverse_index_and_plan);
+  m.impl("packed_spans", &packed_spans);
+  m.impl("packed_attn_fwd", &packed_attn_fwd);
+  m.impl("packed_attn_bwd", &packed_attn_bwd);
+  m.impl("rotary", &rotary);
+  m.impl("linear_attn_pass", &linear_attn_pass);
+  m.impl("linear_attn_step", &linear_attn_step);
 }

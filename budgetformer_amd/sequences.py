@@ -1,0 +1,354 @@
+"""Operators over packed sequences: softmax attention, rotary positions, linear attention with decay.
+
+Sequences lie one behind the other along the first dimension of [rows, heads, head_dim] tensors: the node
+sequences of a batch of graphs, random walks (a walk is the sequence of its nodes), prompts of different
+lengths. ``PackedSequences`` holds what a batch's layers share: where each sequence starts and what each
+row sees, built on the GPU once per batch as an ``AttentionIndex`` is once per edge set.
+
+  packed_attention       dense softmax attention inside each sequence (grouped heads, causal or not)
+  rotary_embedding       rotary positions of q and k
+  linear_attention       linear attention with a decay for each head, chunked; linear_attention_step: its
+                         recurrent form for single tokens
+
+``CoreAttention`` takes the first (and, with ``rotary``, the second) for ``attn_type="flash"``, the dense
+attention of models/graphormer_dist_node_level.py:603-608. All run as HIP kernels on the current stream;
+there is no CPU fallback. Activations are float32, bfloat16 or float16, sums and statistics float32.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native as N
+
+_MOST_ROWS = 2 ** 31 - 256
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """``t`` as the kernels read it: a contiguous last dimension, rows and heads at whole 16-byte steps (views
+    such as slices of a fused projection are taken as they are; anything else is copied)."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head_dim] (got {tuple(t.shape)})")
+    per = 16 // t.element_size()
+    fits = t.data_ptr() % 16 == 0 and all(t.size(d) <= 1 or (t.stride(d) >= 0 and t.stride(d) % per == 0) for d in (0, 1))
+    return t if fits and (t.stride(2) == 1 or t.size(2) <= 1) else t.contiguous()
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor at a 16-byte aligned address."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class PackedSequences:
+    """Where the sequences of a packed batch start, and what each row sees.
+
+    Query rows of sequence s are ``[q_offsets[s], q_offsets[s + 1])`` and see keys of
+    ``[k_offsets[s], k_offsets[s + 1])``: all of them, or with ``causal`` those up to their own place, the last
+    query at the last key (one query a sequence then sees all its keys). Rows behind the last sequence see
+    nothing: their outputs and gradients are 0.
+    """
+
+    def __init__(self, q_offsets: torch.Tensor, k_offsets: torch.Tensor, n_q: int, n_k: int, causal: bool):
+        self.q_offsets, self.k_offsets = q_offsets, k_offsets
+        self.n_q, self.n_k, self.n_seq, self.causal = int(n_q), int(n_k), q_offsets.numel() - 1, bool(causal)
+        self.self_attention = q_offsets is k_offsets and self.n_q == self.n_k
+        self.row_span, self.key_span, self._positions = N.load_ops().packed_spans(q_offsets, k_offsets, self.n_q, self.n_k,
+                                                                                  self.causal)
+
+    @staticmethod
+    def _sizes(n_q: int, n_k: int) -> None:
+        if not (0 <= n_q < _MOST_ROWS and 0 <= n_k < _MOST_ROWS):
+            raise ValueError(f"{n_q} query rows and {n_k} keys (below 2^31 - 256 each)")
+
+    @classmethod
+    def from_lengths(cls, q_lengths: Sequence[int], k_lengths: Optional[Sequence[int]] = None, *, causal: bool = False,
+                     device="cuda") -> "PackedSequences":
+        """From the sequences' lengths on the host (a list, or a CPU tensor); ``k_lengths``: those of the keys
+        where they differ. Nothing is read back from the device."""
+        device = cls._device(device)
+        lens = [torch.as_tensor(x, dtype=torch.int64, device="cpu") for x in
+                ((q_lengths,) if k_lengths is None else (q_lengths, k_lengths))]
+        for x in lens:
+            if x.dim() != 1 or x.numel() != lens[0].numel():
+                raise ValueError("q_lengths and k_lengths must be one length for each sequence")
+            if x.numel() and int(x.min()) < 0:
+                raise ValueError("a sequence's length is negative")
+        ends = [torch.cat([x.new_zeros(1), x.cumsum(0)]) for x in lens]
+        totals = [int(e[-1]) for e in ends]
+        cls._sizes(totals[0], totals[-1])
+        on = [e.to(torch.int32).to(device) for e in ends]
+        return cls(on[0], on[-1], totals[0], totals[-1], causal)
+
+    @classmethod
+    def from_offsets(cls, q_offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None, *, n_q: Optional[int] = None,
+                     n_k: Optional[int] = None, causal: bool = False, check: bool = True) -> "PackedSequences":
+        """From device offsets ([n_seq + 1], ascending from 0). ``n_q`` and ``n_k``: the rows of the tensors where
+        more lie behind the last sequence. With ``check`` the offsets are read back and refused if they do not
+        ascend from 0 inside the tensors; without it (graph capture) ``n_q`` must be given (``n_k`` too with
+        ``k_offsets``) and bad offsets give wrong results."""
+        for x in (q_offsets,) if k_offsets is None else (q_offsets, k_offsets):
+            if not isinstance(x, torch.Tensor) or x.dtype not in (torch.int32, torch.int64) or x.dim() != 1 or x.numel() < 1:
+                raise ValueError("offsets must be an int32 or int64 tensor [n_seq + 1]")
+            if x.device.type != "cuda":
+                raise ValueError(f"offsets must be on a HIP device (got {x.device}); the HIP path has no CPU fallback")
+            if x.shape != q_offsets.shape or x.device != q_offsets.device:
+                raise ValueError("q_offsets and k_offsets must be of the same sequences, on one device")
+        sizes = [n_q, n_q if k_offsets is None else n_k]
+        if k_offsets is None and n_k is not None and n_k != n_q:
+            raise ValueError("n_k differs from n_q without k_offsets")
+        if check:
+            for i, x in enumerate((q_offsets, q_offsets if k_offsets is None else k_offsets)):
+                host = x.cpu().to(torch.int64)
+                if int(host[0]) != 0 or bool((host[1:] < host[:-1]).any()):
+                    raise ValueError("offsets must ascend from 0")
+                if sizes[i] is None:
+                    sizes[i] = int(host[-1])
+                elif int(host[-1]) > sizes[i]:
+                    raise ValueError(f"the last sequence ends at row {int(host[-1])} of {sizes[i]}")
+        elif sizes[0] is None or sizes[1] is None:
+            raise ValueError("without the check the tensors' rows must be given (n_q, and n_k with k_offsets)")
+        cls._sizes(int(sizes[0]), int(sizes[1]))
+        q = q_offsets.to(torch.int32).contiguous()
+        k = q if k_offsets is None else k_offsets.to(torch.int32).contiguous()
+        return cls(q, k, sizes[0], sizes[1], causal)
+
+    @staticmethod
+    def _device(device) -> torch.device:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"the HIP path takes device tensors (got {device}); it has no CPU fallback")
+        return device
+
+    @property
+    def device(self) -> torch.device:
+        return self.q_offsets.device
+
+    def positions(self) -> torch.Tensor:
+        """int32 [n_q]: each query row's place in its sequence, counted from its first key (0 behind the last
+        sequence)."""
+        return self._positions
+
+
+def _check_seqs(seqs, q: torch.Tensor, k: torch.Tensor) -> None:
+    if not isinstance(seqs, PackedSequences):
+        raise TypeError(f"seqs must be a PackedSequences (got {type(seqs)})")
+    if q.size(0) != seqs.n_q or k.size(0) != seqs.n_k:
+        raise ValueError(f"the sequences cover ({seqs.n_q} rows, {seqs.n_k} keys), the tensors have ({q.size(0)}, {k.size(0)})")
+    if q.device != seqs.device:
+        raise ValueError(f"q is on {q.device}, the sequences on {seqs.device}")
+
+
+# ------------------------------------------------------------------ softmax attention
+class _PackedAttention(torch.autograd.Function):
+    """out, lse (in log2, not differentiable) of packed_attention; HIP forward and backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, seqs, scale):
+        out, lse = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.seqs, ctx.scale = seqs, scale
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, dout, _dlse):
+        if dout is None:
+            return None, None, None, None, None
+        q, k, v, out, lse = ctx.saved_tensors
+        dq, dk, dv = N.load_ops().packed_attn_bwd(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, _dense(dout),
+                                                  ctx.scale)
+        return dq, dk, dv, None, None
+
+
+def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = None, with_lse: bool = False):
+    """softmax(scale q k^T) v inside each sequence of a packed batch.
+
+    q [n_q, heads, hn], k and v [n_k, kv_heads, hn] of one dtype (k and v are cast to q's), heads a multiple of
+    kv_heads (query head h reads key head h // (heads // kv_heads)), hn a multiple of 8 up to 128. Rows and heads
+    may have any strides. ``scale`` (positive): 1 / sqrt(hn) by default. Returns out [n_q, heads, hn], or (out,
+    lse) with ``with_lse``: lse float32 [n_q, heads], the log of the row's sum of exponentials, -inf for a row
+    that sees no key (its out is 0); lse is not differentiable. Gradients repeat bit for bit."""
+    _check_seqs(seqs, q, k)
+    dt = q.dtype
+    q, k, v = _rows(q, "q"), _rows(k.to(dt), "k"), _rows(v.to(dt), "v")
+    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    out, lse = _PackedAttention.apply(q, k, v, seqs, scale)
+    return (out, lse * math.log(2.0)) if with_lse else out
+
+
+# ------------------------------------------------------------------ rotary positions
+class RotaryFrequencies:
+    """The frequencies of rotary positions, formed once on the host in 64 bits.
+
+    Pair i of ``rot`` rotated values turns by theta_i = base^(-2i / rot) radians a position. For contexts longer
+    than a model was trained on, ``scaling``:
+
+      "linear"    theta_i / factor
+      "ntk"       base * factor^(rot / (rot - 2)) in place of base: fast pairs stay, the slowest is divided by factor
+      "by_parts"  pairs that turn at least ``high`` times over ``original`` positions stay, those that turn at
+                  most ``low`` times are divided by factor, those between go over linearly in their turns;
+                  ``amplitude`` (default 1) scales q and k, as such schemes do with the logits' temperature
+    """
+
+    def __init__(self, rot: int, base: float = 10000.0, *, factor: float = 1.0, scaling: str = "linear",
+                 original: Optional[int] = None, low: float = 1.0, high: float = 4.0, amplitude: float = 1.0,
+                 device="cuda"):
+        rot = int(rot)
+        if rot < 2 or rot % 2 or rot > 1024:
+            raise ValueError(f"rot must be an even number of 2 to 1024 (got {rot})")
+        if not (base > 1.0 and math.isfinite(base)) or not (factor > 0.0 and math.isfinite(factor)):
+            raise ValueError(f"base {base} must be above 1 and factor {factor} positive")
+        if not math.isfinite(amplitude):
+            raise ValueError(f"amplitude {amplitude}")
+        exponent = torch.arange(rot // 2, dtype=torch.float64) * 2 / rot
+        if scaling == "linear":
+            theta = base ** -exponent / factor
+        elif scaling == "ntk":
+            if rot < 4:
+                raise ValueError("ntk scaling needs two pairs at least")
+            theta = (base * factor ** (rot / (rot - 2))) ** -exponent
+        elif scaling == "by_parts":
+            if original is None or original < 1 or not 0.0 < low < high:
+                raise ValueError("by_parts scaling needs original positions and 0 < low < high")
+            theta = base ** -exponent
+            keep = ((original * theta / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+            theta = theta * keep + theta / factor * (1.0 - keep)
+        else:
+            raise ValueError(f"scaling {scaling!r} (linear, ntk or by_parts)")
+        self.rot, self.amplitude = rot, float(amplitude)
+        self.turns = (theta / (2 * math.pi)).to(PackedSequences._device(device))
+
+    def to(self, device) -> "RotaryFrequencies":
+        got = object.__new__(RotaryFrequencies)
+        got.rot, got.amplitude, got.turns = self.rot, self.amplitude, self.turns.to(PackedSequences._device(device))
+        return got
+
+
+class _Rotary(torch.autograd.Function):
+    """x and, if given, y turned by their positions; the gradient is turned back."""
+
+    @staticmethod
+    def forward(ctx, x, y, positions, freq, interleaved):
+        ctx.save_for_backward(positions)
+        ctx.freq, ctx.interleaved, ctx.two = freq, interleaved, y is not None
+        ctx.set_materialize_grads(False)
+        ox, oy = N.load_ops().rotary(x, y, positions, freq.turns, freq.amplitude, interleaved, False)
+        return (ox, oy) if ctx.two else ox
+
+    @staticmethod
+    def backward(ctx, dx, dy=None):
+        positions, = ctx.saved_tensors
+        ops, f = N.load_ops(), ctx.freq
+        given = [_rows(g, "gradient") for g in (dx, dy) if g is not None]
+        if not given:
+            return None, None, None, None, None
+        got = ops.rotary(given[0], given[1] if len(given) == 2 else None, positions, f.turns, f.amplitude, ctx.interleaved, True)
+        if len(given) == 2:
+            dx, dy = got
+        elif dx is not None:
+            dx = got[0]
+        else:
+            dy = got[0]
+        return dx, dy, None, None, None
+
+
+def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optional[torch.Tensor] = None,
+                     seqs: Optional[PackedSequences] = None, interleaved: bool = False):
+    """q (and k) [rows, heads, hn] with the first ``freq.rot`` values of every head turned by the row's position.
+
+    ``positions``: int32 or int64 [rows] on the device, of any size and sign (angles are formed in 64 bits);
+    without them each row's place in its sequence (``seqs.positions()``). Pairs are (i, i + rot / 2), or with
+    ``interleaved`` (2i, 2i + 1). Returns new tensors, (q, k) or q alone; gradients are turned back."""
+    if not isinstance(freq, RotaryFrequencies):
+        raise TypeError(f"freq must be a RotaryFrequencies (got {type(freq)})")
+    if positions is None:
+        if seqs is None:
+            raise ValueError("rotary_embedding needs positions or seqs")
+        if seqs.n_q != q.size(0):
+            raise ValueError(f"the sequences cover {seqs.n_q} rows, q has {q.size(0)}")
+        positions = seqs.positions()
+    q = _rows(q, "q")
+    if freq.rot > q.size(2):
+        raise ValueError(f"{freq.rot} rotated values in a head of {q.size(2)}")
+    return _Rotary.apply(q, None if k is None else _rows(k.to(q.dtype), "k"), positions.contiguous(), freq, bool(interleaved))
+
+
+# ------------------------------------------------------------------ linear attention
+class _LinearAttention(torch.autograd.Function):
+    """out and the final state (not differentiable); each gradient is a pass of the same kernel."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, seqs, scale, initial_state, return_state):
+        out, state = N.load_ops().linear_attn_pass(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
+                                                   False, initial_state, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state)
+        ctx.seqs, ctx.scale = seqs, scale
+        ctx.mark_non_differentiable(state)
+        ctx.set_materialize_grads(False)
+        return out, state
+
+    @staticmethod
+    def backward(ctx, dout, _dstate):
+        if dout is None:
+            return (None,) * 8
+        q, k, v, log_decay, init = ctx.saved_tensors
+        s, dout = ctx.seqs, _dense(dout)
+        init = None if init is None else init.transpose(2, 3)
+
+        def one(x, y, z, reverse, state=None):
+            return N.load_ops().linear_attn_pass(x, y, z, log_decay, s.row_span, s.key_span, s.q_offsets, ctx.scale, reverse,
+                                                 state, False)[0]
+
+        need = ctx.needs_input_grad
+        return (one(dout, v, k, False, init) if need[0] else None, one(v, dout, q, True) if need[1] else None,
+                one(k, q, dout, True) if need[2] else None, None, None, None, None, None)
+
+
+def _decays(log_decay, q) -> torch.Tensor:
+    if not isinstance(log_decay, torch.Tensor) or log_decay.dim() != 1 or log_decay.size(0) != q.size(1):
+        raise ValueError(f"log_decay must be [{q.size(1)}]")
+    if log_decay.requires_grad:
+        raise NotImplementedError("the decays are constants: no gradient with respect to log_decay")
+    return log_decay.float().contiguous()
+
+
+def linear_attention(q, k, v, log_decay, seqs: PackedSequences, scale: Optional[float] = None,
+                     initial_state: Optional[torch.Tensor] = None, return_state: bool = False):
+    """out_i = scale sum_{j <= i} exp(log_decay (i - j)) (q_i . k_j) v_j inside each sequence: attention without a
+    softmax, whose state S_i = exp(log_decay) S_{i-1} + k_i v_i^T has a fixed size.
+
+    q and k [rows, heads, dk], v [rows, heads, dv] of one dtype (k and v are cast to q's), dk and dv multiples of 8
+    up to 128; log_decay float32 [heads], at most 0 (0: no decay; -inf: only the row's own token), a constant.
+    ``seqs``: causal, the same sequences for rows and keys. ``scale``: 1 / sqrt(dk) by default.
+    ``initial_state`` float32 [sequences, heads, dk, dv] comes before each sequence's first token; with
+    ``return_state`` (out, state behind the last token) is returned, from which ``linear_attention_step`` or the
+    next chunk go on. Gradients flow to q, k and v; the states are constants."""
+    _check_seqs(seqs, q, k)
+    if not seqs.self_attention or not seqs.causal:
+        raise ValueError("linear attention takes causal sequences of the same rows and keys")
+    dt = q.dtype
+    q, k, v = _rows(q, "q"), _rows(k.to(dt), "k"), _rows(v.to(dt), "v")
+    if initial_state is not None:
+        if initial_state.requires_grad:
+            raise NotImplementedError("the initial state is a constant: no gradient with respect to it")
+        initial_state = initial_state.float().contiguous()
+    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    out, state = _LinearAttention.apply(q, k, v, _decays(log_decay, q), seqs, scale, initial_state, bool(return_state))
+    return (out, state) if return_state else out
+
+
+def linear_attention_step(q, k, v, log_decay, state, scale: Optional[float] = None,
+                          out_state: Optional[torch.Tensor] = None):
+    """One token of each of n sequences: (out [n, heads, dv], new state). q and k [n, heads, dk], v [n, heads, dv],
+    state float32 [n, heads, dk, dv]. ``out_state``: where the new state is written (``state`` itself updates it in
+    place), else a new tensor. For inference: no gradients."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        raise NotImplementedError("linear_attention_step has no gradients (linear_attention has)")
+    dt = q.dtype
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    return N.load_ops().linear_attn_step(q.contiguous(), k.to(dt).contiguous(), v.to(dt).contiguous(), _decays(log_decay, q),
+                                         state, scale, out_state)

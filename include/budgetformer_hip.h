@@ -61,8 +61,10 @@ enum { BF_DTYPE_F32 = 0, BF_DTYPE_BF16 = 1, BF_DTYPE_F16 = 2 };
  *        change to what was there (a caller finds them by name): bf_coo_order,
  *        bf_coo_to_csr_ordered, bf_coo_reverse, bf_coo_reverse_slots,
  *        bf_coalesce_bidirected, bf_table_list_check, bf_table_to_list,
- *        bf_reception_cone, bf_probe_queries, bf_any_nonzero and the
- *        workspace sizes of those that have one.                            */
+ *        bf_reception_cone, bf_probe_queries, bf_any_nonzero, the
+ *        operators over packed sequences (bf_packed_spans, bf_packed_attn_*,
+ *        bf_rotary, bf_linear_attn*) and the workspace sizes of those that
+ *        have one.                                                          */
 #define BF_ABI_VERSION 303
 int bf_version(void);
 /* Message of the last failed call on this thread ("" if none). */
@@ -773,6 +775,112 @@ int bf_gather_probe(const void* t0, int32_t row_bytes0, const void* t1, int32_t 
 int bf_row_stream_probe(const void* r0, const void* r1, void* w0, void* w1, int32_t row_bytes,
                         const int32_t* ids, int64_t n_rows, int32_t nontemporal, uint32_t* sink,
                         void* stream);
+
+/* ======================================================================
+ * Operators over packed sequences
+ *
+ * Sequences lie one behind the other along a tensor's first dimension;
+ * sequence s is the rows [offsets[s], offsets[s + 1]). The node sequences of a
+ * batch of graphs, random walks (a walk is the sequence of its nodes) and
+ * prompts of different lengths are all of this form. They have no counterpart
+ * among the reference's sparse paths; bf_packed_attn_* computes what its dense
+ * attention type does (models/graphormer_dist_node_level.py:603-608).
+ * ====================================================================== */
+
+/* What each row sees, from the offsets (int32 [n_seq + 1], ascending, of the
+ * query rows and of the keys). Query row i of sequence s sees the keys
+ * row_span[i] = [lo, hi): all of the sequence's, or, with `causal`, those up to
+ * its own place with the last query at the last key (row i sees key j of its
+ * sequence when j - k0 <= i - q0 + len_k - len_q). key_span[j] is the rows that
+ * see key j. Rows behind the last sequence see nothing and keys there are seen
+ * by none. positions (int32 [n_q], or NULL): i - q0 + len_k - len_q, 0 behind
+ * the last sequence. row_span int32 [n_q][2], key_span int32 [n_k][2]. Spans are
+ * clamped to the tensors: offsets that do not ascend give wrong results, but no
+ * access outside.                                                           */
+int bf_packed_spans(const int32_t* q_offsets, const int32_t* k_offsets, int64_t n_seq, int64_t n_q, int64_t n_k,
+                    int32_t causal, int32_t* row_span, int32_t* key_span, int32_t* positions, void* stream);
+
+/* Sizes and layout of a packed attention call. q is [n_q, heads_q, head_dim],
+ * k and v [n_k, heads_k, head_dim] with the strides given (in values, of a row
+ * and of a head, whole 16-byte steps; the last dimension is contiguous and the
+ * tensors 16-byte aligned). heads_q is a multiple of heads_k: query head h
+ * reads key head h / (heads_q / heads_k). head_dim: a multiple of 8 up to 128.
+ * row_span and key_span as bf_packed_spans writes them (key_span: backward).  */
+typedef struct bf_packed_attn {
+  int64_t n_q, n_k;
+  int32_t heads_q, heads_k, head_dim, dtype;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  const int32_t* row_span;
+  const int32_t* key_span;
+  float scale;                /* of q.k; positive                            */
+  int32_t reserved;           /* 0                                           */
+} bf_packed_attn;
+
+/* out = softmax(scale q k^T over the row's keys) v, contiguous [n_q, heads_q,
+ * head_dim] in q's dtype; lse float32 [n_q, heads_q]: the log2 of the row's sum
+ * of exp(scale q.k). A row that sees no key has out 0 and lse -inf. scratch:
+ * bf_packed_attn_fwd_floats(p) floats (0: none needed; -1: bad arguments), for
+ * calls of few rows, whose keys are cut into pieces.                        */
+int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p);
+int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
+                       float* scratch, void* stream);
+/* Gradients of it: dq like out, dk and dv contiguous [n_k, heads_k, head_dim]
+ * (summed over the heads of a group). out, dout: contiguous. delta: scratch of
+ * n_q * heads_q floats. No atomics: results repeat bit for bit.             */
+int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
+                       const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, void* stream);
+
+/* Rotary positions: the first `rot` values of every head of x and y (rows of
+ * `dim` values; y may be NULL with heads_y 0) turned pair by pair by the angle
+ * 2 pi positions[row] * turns[pair] and scaled by amplitude; the rest is
+ * copied. Pairs are (2i, 2i + 1) with `interleaved`, else (i, i + rot / 2).
+ * `inverse` turns back (the gradient). turns: float64 [rot / 2] (angles are
+ * formed in 64 bits: far positions keep theirs). positions: int32 or (wide)
+ * int64 [n]. Inputs with strides in values (row, head), last dimension
+ * contiguous; outputs contiguous [n, heads, dim]; out of place.             */
+int bf_rotary(const void* x, const void* y, int64_t n, int32_t heads_x, int32_t heads_y, int32_t dim, int32_t rot,
+              int32_t dtype, const int64_t x_stride[2], const int64_t y_stride[2], const void* positions, int32_t wide,
+              const double* turns, float amplitude, int32_t interleaved, int32_t inverse, void* out_x, void* out_y,
+              void* stream);
+
+/* Linear attention with a decay for each head, over causal packed sequences:
+ *   out_i = scale sum_{j <= i, same sequence} g^(i - j) (x_i . y_j) z_j
+ * with g = exp(log_decay[h]); with `reverse` over j >= i and g^(j - i): the
+ * gradients of out(q, k, v) are dq = (dout, v, k), dk = reverse (v, dout, q)
+ * and dv = reverse (k, q, dout). x, y: [n, heads, dim_x]; z: [n, heads, dim_z];
+ * out contiguous [n, heads, dim_z]; strides as in bf_packed_attn. dims: a
+ * multiple of 8 up to 128. row_span / key_span: bf_packed_spans with causal and
+ * the same offsets for rows and keys.
+ * init (or NULL): float32 [n_seq, heads, ...], each sequence's state before its
+ * first token, value (a, b) of [dim_x][dim_z] at a * init_stride[0] + b *
+ * init_stride[1]; final (or NULL): float32 [n_seq, heads, dim_x, dim_z], the
+ * state sum_j g^(n - 1 - j) y_j z_j^T + g^n init behind its last. Neither with
+ * reverse. offsets (int32 [n_seq + 1]) is read only with one of them.
+ * scratch: bf_linear_attn_floats(p) floats (0: none; -1: bad arguments).    */
+typedef struct bf_linear_attn {
+  int64_t n, n_seq;
+  int32_t heads, dim_x, dim_z, dtype;
+  int64_t x_stride[2], y_stride[2], z_stride[2];
+  const int32_t* row_span;
+  const int32_t* key_span;
+  const int32_t* offsets;
+  const float* log_decay;     /* float32 [heads], <= 0 expected              */
+  const float* init;
+  float* final_state;
+  int64_t init_stride[2];
+  float scale;
+  int32_t reverse;
+} bf_linear_attn;
+int64_t bf_linear_attn_floats(const bf_linear_attn* p);
+int bf_linear_attn_pass(const bf_linear_attn* p, const void* x, const void* y, const void* z, void* out, float* scratch,
+                        void* stream);
+/* One token of each of n sequences: new_state = g state + k v^T, out = scale q
+ * new_state. q, k [n, heads, dim_k], v, out [n, heads, dim_v], states float32
+ * [n, heads, dim_k, dim_v], all contiguous; new_state may be state. dims as
+ * above.                                                                    */
+int bf_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                        int64_t n, int32_t heads, int32_t dim_k, int32_t dim_v, int32_t dtype, float scale,
+                        void* out, float* new_state, void* stream);
 
 #ifdef __cplusplus
 }

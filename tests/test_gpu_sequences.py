@@ -1,0 +1,600 @@
+"""The operators over packed sequences on the GPU against the float64 oracle, each value within the bound that its own
+roundings give (oracle/sequences.py derives them; half a step of the type is torch.finfo(t).eps / 2)."""
+import math
+
+import pytest
+import torch
+
+from oracle import sequences as sq
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _bf():
+    import budgetformer_amd as bf
+    return bf
+
+
+def _randn(seed, *shape, dtype=torch.float32, dev="cuda"):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(dev)
+
+
+def _within(name, got, ref, bound):
+    assert got.shape == ref.shape, (name, got.shape, ref.shape)
+    off = (got.double() - ref).abs()
+    bad = ~(off <= bound)                                 # a NaN is bad too
+    assert not bool(bad.any()), (f"{name}: {int(bad.sum())} of {bad.numel()} values out of bounds, worst "
+                                 f"{float((off / bound.clamp_min(1e-300)).nan_to_num(1e9).max()):.3g} times the bound")
+
+
+def _attention_case(dev, q_lens, k_lens, H, Hk, d, causal, dtype, seed=0, scale=None, train=True):
+    bf = _bf()
+    n_q, n_k = sum(q_lens), sum(k_lens)
+    q, do = (_randn(seed + i, n_q, H, d, dtype=dtype, dev=dev) for i in (0, 3))
+    k, v = (_randn(seed + i, n_k, Hk, d, dtype=dtype, dev=dev) for i in (1, 2))
+    seqs = bf.PackedSequences.from_lengths(q_lens, k_lens, causal=causal, device=dev)
+    leaves = [x.clone().requires_grad_(train) for x in (q, k, v)]
+    out, lse = bf.packed_attention(*leaves, seqs, scale=scale, with_lse=True)
+    ref = sq.attention(q.double(), k.double(), v.double(), q_lens, k_lens, causal, d ** -0.5 if scale is None else scale,
+                       do.double() if train else None, dtype)
+    _within("out", out.detach(), ref["out"], ref["out_bound"])
+    # lse: a sum of exponentials in float32 and its log: the scores' error and a step of the result
+    fin = torch.isfinite(ref["lse"])
+    assert torch.equal(fin, torch.isfinite(lse))
+    if bool(fin.any()):
+        assert float((lse.double() - ref["lse"])[fin].abs().max()) < 2.0 ** -24 * (
+            8 * (d + 8) * (1 + float((q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max()))) + max(k_lens) + 64)
+    if train:
+        grads = torch.autograd.grad(out, leaves, do)
+        for name, got in zip(("dq", "dk", "dv"), grads):
+            _within(name, got, ref[name], ref[f"{name}_bound"])
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", [[1], [5] * 40, [33, 0, 64, 65, 1, 128, 31], [200, 313], [0, 0, 17, 0], [129] * 3],
+                         ids=["one", "walks", "mixed", "long", "empty", "edges"])
+def test_packed_attention_self(hip_device, lens, causal, dtype):
+    _attention_case(hip_device, lens, lens, 4, 2, 32, causal, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d", [(8, 8, 16), (3, 1, 8), (6, 2, 24), (4, 4, 64), (5, 5, 40), (2, 1, 72), (8, 2, 128),
+                                    (7, 1, 128)])
+def test_packed_attention_head_layouts(hip_device, H, Hk, d, dtype):
+    _attention_case(hip_device, [70, 3, 131], [70, 3, 131], H, Hk, d, True, dtype, seed=7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_attention_rows_and_keys_of_different_lengths(hip_device, causal, dtype):
+    """More keys than rows (a chunk behind kept keys), more rows than keys (causal rows that see nothing), sequences
+    without rows or without keys."""
+    _attention_case(hip_device, [1, 40, 100, 0, 9, 64], [300, 200, 37, 12, 0, 64], 4, 2, 64, causal, dtype, seed=11)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d", [(8, 2, 128), (4, 4, 64), (3, 1, 16)])
+def test_single_tokens_against_kept_keys(hip_device, H, Hk, d, dtype):
+    """One row a sequence, few rows in all: the keys are cut into pieces, which are joined."""
+    k_lens = [1, 0, 63, 64, 65, 777, 2050, 5, 128]
+    _attention_case(hip_device, [1] * len(k_lens), k_lens, H, Hk, d, True, dtype, seed=13, train=False)
+    _attention_case(hip_device, [1], [4099], H, Hk, d, True, dtype, seed=17, train=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_train_against_long_keys(hip_device, dtype):
+    _attention_case(hip_device, [7, 3], [1500, 1201], 4, 1, 64, True, dtype, seed=19)
+
+
+def test_whole_rows_of_many_tiles(hip_device):
+    """Enough rows that every key head's tiles take whole rows (no pieces), one long sequence among short ones."""
+    _attention_case(hip_device, [2500, 1, 300, 77], [2500, 1, 300, 77], 32, 16, 64, True, torch.bfloat16, seed=23)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_scores_do_not_overflow(hip_device, dtype):
+    bf = _bf()
+    q = _randn(1, 100, 2, 64, dtype=dtype, dev=hip_device) * 30
+    k, v = _randn(2, 100, 2, 64, dtype=dtype, dev=hip_device) * 30, _randn(3, 100, 2, 64, dtype=dtype, dev=hip_device)
+    seqs = bf.PackedSequences.from_lengths([100], causal=True, device=hip_device)
+    out = bf.packed_attention(q, k, v, seqs)
+    ref = sq.attention(q.double(), k.double(), v.double(), [100], [100], True, 0.125, dtype=dtype)
+    _within("out", out, ref["out"], ref["out_bound"])
+
+
+def _strided(x, kind):
+    """The same values in another layout."""
+    n, h, d = x.shape
+    if kind == "fused":                                   # a slice of a wider projection, 16-byte steps
+        big = x.new_full((n, h + 3, d), float("nan"))
+        big[:, 1:h + 1] = x
+        return big[:, 1:h + 1]
+    if kind == "heads_first":
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+    if kind == "odd":                                     # rows at odd addresses
+        big = x.new_full((n, h * d + 1), float("nan"))
+        big[:, 1:] = x.reshape(n, -1)
+        return big[:, 1:].unflatten(1, (h, d))
+    if kind == "last":                                    # not contiguous along the head
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    raise AssertionError(kind)
+
+
+@pytest.mark.parametrize("kind", ["fused", "heads_first", "odd", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layouts_give_the_same_bits(hip_device, kind, dtype):
+    bf = _bf()
+    lens = [40, 90, 1]
+    q, k, v, do = (_randn(i, 131, 4, 32, dtype=dtype, dev=hip_device) for i in range(4))
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+    ld = torch.full((4,), -0.1, device=hip_device)
+    freq = bf.RotaryFrequencies(32, device=hip_device)
+
+    def every(q, k, v, do):
+        got = []
+        for f in (lambda *x: bf.packed_attention(*x, seqs), lambda *x: bf.linear_attention(*x, ld, seqs)):
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+            out = f(*leaves)
+            got += [out, *torch.autograd.grad(out, leaves, do)]
+        leaves = [x.detach().requires_grad_(True) for x in (q, k)]
+        out = bf.rotary_embedding(*leaves, freq, seqs=seqs)
+        return got + [*out, *torch.autograd.grad(out, leaves, (do, do))]
+
+    for a, b in zip(every(q, k, v, do), every(*(_strided(x, kind) for x in (q, k, v, do)))):
+        assert torch.equal(a, b)
+
+
+def test_a_broadcast_key_head_gets_the_sum_of_its_gradients(hip_device):
+    """k and v expanded over heads and over rows: strides of 0 in, gradients summed by autograd."""
+    bf = _bf()
+    q = _randn(1, 50, 4, 16, dev=hip_device)
+    k, v = (_randn(i, 50, 1, 16, dev=hip_device).requires_grad_(True) for i in (2, 3))
+    do = _randn(4, 50, 4, 16, dev=hip_device)
+    seqs = bf.PackedSequences.from_lengths([30, 20], causal=True, device=hip_device)
+    a = torch.autograd.grad(bf.packed_attention(q, k.expand(50, 4, 16), v.expand(50, 4, 16), seqs), (k, v), do)
+    ref = sq.attention(q.double(), k.detach().double(), v.detach().double(), [30, 20], [30, 20], True, 0.25, do.double(),
+                       torch.float32)
+    for got, name in zip(a, ("dk", "dv")):
+        # the sum of four heads' rounded gradients: four roundings of values no larger than the bound's own terms
+        _within(name, got, ref[name], 5 * ref[f"{name}_bound"])
+    row = _randn(5, 1, 1, 16, dev=hip_device).requires_grad_(True)
+    out = bf.packed_attention(q, row.expand(50, 4, 16), row.expand(50, 4, 16), seqs)
+    assert torch.allclose(out, row.detach().expand(50, 4, 16), atol=1e-5)         # every key the same: its value
+    torch.autograd.grad(out, row, do)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_that_a_row_does_not_see_do_not_reach_it(hip_device, dtype):
+    """NaN and infinities in one sequence, in later tokens and behind the last sequence: every other row, and its
+    gradients, as without them, bit for bit."""
+    bf = _bf()
+    lens, n, bad_seq = [50, 20, 70], 150, slice(50, 70)
+    seqs = bf.PackedSequences.from_offsets(torch.tensor([0, 50, 70, 140], dtype=torch.int32, device=hip_device), n_q=n,
+                                           causal=True)
+    q, k, v, do = (_randn(i, n, 2, 64, dtype=dtype, dev=hip_device) for i in range(4))
+    ld = torch.tensor([-0.05, -0.3], device=hip_device)
+    keep = torch.ones(n, dtype=torch.bool, device=hip_device)
+    keep[bad_seq] = False
+    keep[140:] = False
+
+    def every(q, k, v, do):
+        got = []
+        for f in (lambda *x: bf.packed_attention(*x, seqs), lambda *x: bf.linear_attention(*x, ld, seqs)):
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+            out = f(*leaves)
+            got += [out, *torch.autograd.grad(out, leaves, do)]
+        return got
+
+    clean = every(q, k, v, do)
+    for which in range(4):
+        xs = [x.clone() for x in (q, k, v, do)]
+        for j, value in enumerate((float("nan"), float("inf"), -float("inf"))):
+            xs[which][51 + j:70:3] = value
+            xs[which][140 + j::3] = value
+        for i, (a, b) in enumerate(zip(every(*xs), clean)):
+            assert torch.equal(a[keep], b[keep]), (which, i)
+        for a in clean[0:4] + clean[4:8]:
+            assert bool((a[140:] == 0).all())             # rows behind the last sequence
+    # later tokens of the same sequence: the rows before them
+    for which in (1, 2):
+        xs = [x.clone() for x in (q, k, v, do)]
+        xs[which][30:50] = float("nan")
+        for a, b in zip((f(*xs[:3]) for f in (lambda *x: bf.packed_attention(*x, seqs),
+                                              lambda *x: bf.linear_attention(*x, ld, seqs))), (clean[0], clean[4])):
+            assert torch.equal(a[:30], b[:30])
+            assert bool(a[30:50].isnan().all())           # and the rows that see them are NaN
+    xs = [x.clone() for x in (q, k, v)]
+    xs[2][10] = float("inf")
+    out = bf.packed_attention(*xs, seqs)
+    assert bool((out[10:50] == float("inf")).all()) and torch.equal(out[:10], clean[0][:10])
+
+
+def test_results_repeat_bit_for_bit(hip_device):
+    a = _attention_case(hip_device, [300, 41], [300, 41], 8, 2, 64, True, torch.bfloat16, seed=3, train=False)
+    b = _attention_case(hip_device, [300, 41], [300, 41], 8, 2, 64, True, torch.bfloat16, seed=3, train=False)
+    assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ rotary positions
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("hq,hk,d,rot", [(4, 2, 64, 64), (3, 0, 32, 16), (2, 2, 16, 8), (5, 1, 10, 6), (1, 1, 3, 2),
+                                         (8, 8, 128, 96), (1, 1, 1024, 1024)])
+def test_rotary_values_and_gradients(hip_device, hq, hk, d, rot, interleaved, dtype):
+    bf = _bf()
+    n = 37
+    q = _randn(1, n, hq, d, dtype=dtype, dev=hip_device).requires_grad_(True)
+    k = _randn(2, n, hk, d, dtype=dtype, dev=hip_device).requires_grad_(True) if hk else None
+    pos = torch.randint(-5, 2 ** 20, (n,), generator=torch.Generator().manual_seed(3)).to(hip_device)
+    freq = bf.RotaryFrequencies(rot, base=500.0, factor=2.0, amplitude=1.25, device=hip_device)
+    theta = (500.0 ** -(torch.arange(rot // 2, dtype=torch.float64) * 2 / rot) / 2.0).to(hip_device)
+    xs = [x for x in (q, k) if x is not None]
+    outs = bf.rotary_embedding(q, k, freq, positions=pos, interleaved=interleaved)
+    outs = outs if hk else (outs,)
+    dos = [_randn(5 + i, *x.shape, dtype=dtype, dev=hip_device) for i, x in enumerate(xs)]
+    grads = torch.autograd.grad(outs, xs, dos)
+    u = sq.half_step(dtype)
+    for x, got, inverse in [*zip(xs, outs, [False] * 2), *zip(dos, grads, [True] * 2)]:
+        ref = sq.rotary(x.detach().double(), pos, theta, 1.25, interleaved, inverse)
+        # the result's rounding; a sum of two products whose sin and cos are a few float32 steps off (the angle's rest is
+        # rounded once, 2 pi 2^-25, the functions to 4 steps, amplitude and products to one each)
+        size = torch.full_like(ref, 0.0)
+        size[..., :rot] = x.detach().double()[..., :rot].abs().amax(-1, keepdim=True) * 1.25 * 2
+        _within("turned", got.detach(), ref, u * ref.abs() + 2.0 ** -24 * 16 * size + 2.0 ** -25 * (dtype == torch.float16))
+        assert torch.equal(got[..., rot:], x[..., rot:])
+
+
+def test_rotary_of_one_of_two_gradients(hip_device):
+    bf = _bf()
+    q, k = (_randn(i, 9, 2, 16, dev=hip_device).requires_grad_(True) for i in (1, 2))
+    freq = bf.RotaryFrequencies(16, device=hip_device)
+    pos = torch.arange(9, dtype=torch.int32, device=hip_device)
+    for i in (0, 1):
+        out = bf.rotary_embedding(q, k, freq, positions=pos)
+        g = torch.autograd.grad(out[i].sum(), (q, k), allow_unused=True)
+        assert g[1 - i] is None and g[i] is not None
+        one = bf.rotary_embedding((q, k)[i], None, freq, positions=pos)
+        assert torch.equal(torch.autograd.grad(one.sum(), (q, k)[i])[0], g[i])
+
+
+@pytest.mark.parametrize("scaling", ["linear", "ntk", "by_parts"])
+def test_rotary_frequencies(hip_device, scaling):
+    bf = _bf()
+    f = bf.RotaryFrequencies(64, 10000.0, factor=8.0, scaling=scaling, original=4096, device=hip_device)
+    theta = f.turns.cpu() * 2 * math.pi
+    plain = 10000.0 ** -(torch.arange(32, dtype=torch.float64) / 32)
+    if scaling == "linear":
+        assert torch.allclose(theta, plain / 8, rtol=1e-14, atol=0)
+    if scaling == "ntk":
+        assert theta[0] == 1.0 and abs(float(theta[-1] / plain[-1]) - 1 / 8) < 1e-12
+    if scaling == "by_parts":
+        turns = 4096 * plain / (2 * math.pi)
+        assert torch.equal(theta[turns >= 4], (plain / (2 * math.pi) * (2 * math.pi))[turns >= 4])
+        assert torch.allclose(theta[turns <= 1], plain[turns <= 1] / 8, rtol=1e-14, atol=0)
+        mid = (turns > 1) & (turns < 4)
+        assert bool(mid.any()) and bool(((theta < plain) & (theta > plain / 8))[mid].all())
+
+
+# ------------------------------------------------------------------ linear attention
+def _linear_case(dev, lens, H, dk, dv, dtype, seed=0, decays=None, init=False, tail=0):
+    bf = _bf()
+    n = sum(lens)
+    q, k = (_randn(seed + i, n, H, dk, dtype=dtype, dev=dev) for i in (0, 1))
+    v, do = (_randn(seed + i, n, H, dv, dtype=dtype, dev=dev) for i in (2, 3))
+    ld = torch.tensor(decays if decays is not None else [-0.02 * 3 ** i for i in range(H)], device=dev)
+    s0 = _randn(seed + 4, len(lens), H, dk, dv, dev=dev) if init else None
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=dev)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = bf.linear_attention(*leaves, ld, seqs, initial_state=s0, return_state=init)
+    ref = sq.linear_attention(q.double().cpu(), k.double().cpu(), v.double().cpu(), ld.cpu(), lens, dk ** -0.5,
+                              None if s0 is None else s0.cpu(), do.double().cpu(), dtype)
+    ref = {x: y.to(dev) for x, y in ref.items()}
+    if init:
+        out, state = out
+        _within("state", state, ref["state"], ref["state_bound"])
+    _within("out", out.detach(), ref["out"], ref["out_bound"])
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)):
+        _within(name, got, ref[name], ref[f"{name}_bound"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[1], [5] * 30, [33, 0, 64, 65, 1, 128, 31], [300], [0, 17, 0]],
+                         ids=["one", "walks", "mixed", "long", "empty"])
+@pytest.mark.parametrize("init", [False, True])
+def test_linear_attention(hip_device, lens, init, dtype):
+    _linear_case(hip_device, lens, 3, 32, 32, dtype, seed=31, init=init)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk,dv", [(8, 8), (16, 64), (64, 24), (128, 40), (72, 128), (128, 128)])
+def test_linear_attention_head_sizes(hip_device, dk, dv, dtype):
+    _linear_case(hip_device, [70, 3, 90], 2, dk, dv, dtype, seed=37)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("init", [False, True])
+def test_linear_attention_over_segments(hip_device, init, dtype):
+    """More tokens than a segment (256): the state is carried across, past a sequence's end inside a segment too."""
+    _linear_case(hip_device, [700, 50, 256, 6, 500], 2, 16, 16, dtype, seed=41, init=init)
+
+
+def test_linear_attention_of_extreme_decays(hip_device):
+    """No decay, one that leaves only the row's own token, and one that underflows within a tile."""
+    _linear_case(hip_device, [90, 40], 3, 16, 16, torch.float32, seed=43, decays=[0.0, -math.inf, -40.0])
+
+
+def test_linear_attention_states_past_float16(hip_device):
+    """A state beyond 65504 under small queries: the result fits, so it has to come out."""
+    bf = _bf()
+    n, d = 400, 16
+    seqs = bf.PackedSequences.from_lengths([n], causal=True, device=hip_device)
+    q = torch.full((n, 1, d), 2.0 ** -10, dtype=torch.float16, device=hip_device)
+    k = torch.full((n, 1, d), 32.0, dtype=torch.float16, device=hip_device)
+    out = bf.linear_attention(q, k, k, torch.zeros(1, device=hip_device), seqs, scale=1.0)
+    # out_i = (i + 1) * 16 * 2^-10 * 32 * 32 = 16 (i + 1), each step exact but the state's rounding to 11 bits
+    ref = 16.0 * torch.arange(1, n + 1, device=hip_device).double()[:, None, None].expand(n, 1, d)
+    _within("out", out, ref, 3 * 2.0 ** -11 * ref)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,H,dk,dv", [(1, 1, 8, 8), (3, 5, 128, 128), (7, 2, 24, 72), (2, 3, 64, 16)])
+def test_linear_attention_step_continues_a_prompt(hip_device, n, H, dk, dv, dtype):
+    bf = _bf()
+    q, k = (_randn(i, n, H, dk, dtype=dtype, dev=hip_device) for i in (1, 2))
+    v, s = _randn(3, n, H, dv, dtype=dtype, dev=hip_device), _randn(4, n, H, dk, dv, dev=hip_device)
+    ld = torch.linspace(-2.0, 0.0, H, device=hip_device)
+    before = s.clone()
+    out, new = bf.linear_attention_step(q, k, v, ld, s)
+    assert torch.equal(s, before)
+    ref = sq.linear_attention(q.double().cpu(), k.double().cpu(), v.double().cpu(), ld.cpu(), [1] * n, dk ** -0.5, s.cpu(),
+                              dtype=dtype)
+    # float32 arithmetic of one step, and the result's rounding
+    g = ld.double().exp()[:, None, None]
+    size = g * before.double().abs() + k.double().abs()[..., None] * v.double().abs()[:, :, None]
+    _within("state", new, ref["state"].to(hip_device), 2.0 ** -24 * 8 * size)
+    aq = torch.einsum("nhk,nhkv->nhv", q.double().abs(), size) * dk ** -0.5
+    _within("out", out, ref["out"].to(hip_device),
+            sq.half_step(dtype) * ref["out"].to(hip_device).abs() + 2.0 ** -24 * (dk + 16) * aq + 2.0 ** -25)
+    got, same = bf.linear_attention_step(q, k, v, ld, s, out_state=s)
+    assert same.data_ptr() == s.data_ptr() and torch.equal(s, new) and torch.equal(got, out)
+
+
+# ------------------------------------------------------------------ together, as they are used
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_then_single_tokens_equal_the_whole(hip_device, dtype):
+    """Rotary, softmax attention and linear attention over a prompt and then token by token against what was kept: the
+    rows of one call over everything."""
+    bf = _bf()
+    H, d, n, m = 4, 32, 90, 6
+    q, k, v = (_randn(i, n, H, d, dtype=dtype, dev=hip_device) for i in range(3))
+    freq, ld = bf.RotaryFrequencies(d, device=hip_device), torch.linspace(-0.5, -0.01, H, device=hip_device)
+    whole = bf.PackedSequences.from_lengths([n], causal=True, device=hip_device)
+    qr, kr = bf.rotary_embedding(q, k, freq, seqs=whole)
+    soft, lin = bf.packed_attention(qr, kr, v, whole), bf.linear_attention(q, k, v, ld, whole)
+    head = bf.PackedSequences.from_lengths([n - m], causal=True, device=hip_device)
+    _, state = bf.linear_attention(q[:n - m], k[:n - m], v[:n - m], ld, head, return_state=True)
+    ref = sq.attention(qr.double(), kr.double(), v.double(), [n], [n], True, d ** -0.5, dtype=dtype)
+    lref = sq.linear_attention(q.double().cpu(), k.double().cpu(), v.double().cpu(), ld.cpu(), [n], d ** -0.5, dtype=dtype)
+    for t in range(n - m, n):
+        one = bf.PackedSequences.from_lengths([1], [t + 1], causal=True, device=hip_device)
+        assert int(one.positions()) == t
+        q1 = bf.rotary_embedding(q[t:t + 1], None, freq, seqs=one)
+        assert torch.equal(q1, qr[t:t + 1])
+        got = bf.packed_attention(q1, kr[:t + 1], v[:t + 1], one)
+        for x in (got, soft[t:t + 1]):
+            _within("softmax", x, ref["out"][t:t + 1], ref["out_bound"][t:t + 1])
+        got, state = bf.linear_attention_step(q[t:t + 1], k[t:t + 1], v[t:t + 1], ld, state)
+        for x in (got, lin[t:t + 1]):
+            _within("linear", x, lref["out"][t:t + 1].to(hip_device), lref["out_bound"][t:t + 1].to(hip_device))
+
+
+def test_walks_attend_their_nodes(hip_device):
+    """The framework's own walks as sequences: rotary positions and causal attention over each walk's nodes, trained."""
+    import numpy as np
+    from budgetformer_amd import hip_ops
+    from budgetformer_amd.graph import CSRGraph, chung_lu_csr
+    bf = _bf()
+    n, P, L, H, d = 200, 2, 4, 4, 16
+    rowptr, col = chung_lu_csr(n, 1500, seed=3)
+    g = CSRGraph.from_csr(rowptr, col, n, device=hip_device)
+    u = torch.from_numpy(np.random.default_rng(1).random((n * P, L), dtype=np.float32)).to(hip_device)
+    walks = hip_ops.random_walk(g.rowptr, g.col, 0, n, P, L, u=u)
+    x = _randn(1, n, H * d, dev=hip_device).requires_grad_(True)
+    seqs = bf.PackedSequences.from_lengths([L + 1] * (n * P), causal=True, device=hip_device)
+    freq = bf.RotaryFrequencies(d, device=hip_device)
+    h = x[walks.reshape(-1)].view(-1, H, d)
+    q, k = bf.rotary_embedding(h, h, freq, seqs=seqs)
+    out = bf.packed_attention(q, k, h, seqs)
+    do = _randn(2, *out.shape, dev=hip_device)
+    got, = torch.autograd.grad(out, x, do)
+
+    x64 = x.detach().double().requires_grad_(True)
+    h64 = x64[walks.reshape(-1)].view(n * P, L + 1, H, d)
+    theta = 10000.0 ** -(torch.arange(d // 2, dtype=torch.float64, device=hip_device) * 2 / d)
+    pos = torch.arange(L + 1, device=hip_device).repeat(n * P)
+    r64 = sq.rotary(h64.reshape(-1, H, d), pos, theta, 1.0, False).view(n * P, L + 1, H, d).transpose(1, 2)
+    s = (r64 @ r64.transpose(2, 3) / 4.0).masked_fill(~sq.visible(L + 1, L + 1, True, hip_device), -math.inf)
+    ref = (s.softmax(-1) @ h64.transpose(1, 2)).transpose(1, 2).reshape(-1, H, d)
+    rg, = torch.autograd.grad(ref, x64, do.double())
+    # float32 throughout: sums of at most 5 keys, of 16 values a head, of the rows a node is in
+    assert float((out.detach().double() - ref.detach()).abs().max()) < 2.0 ** -24 * 300 * float(x64.detach().abs().max())
+    scale = float(rg.abs().max())
+    assert float((got.double() - rg).abs().max()) < 2.0 ** -24 * 2000 * scale
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_core_attention_flash(hip_device, dtype):
+    from budgetformer_amd.attention import CoreAttention
+    bf = _bf()
+    b, S, H, d = 3, 45, 4, 16
+    q, k, v = (_randn(i, b, S, H, d, dtype=dtype, dev=hip_device) for i in range(3))
+    ref = sq.attention(*(x.double().reshape(-1, H, d) for x in (q, k, v)), [S] * b, [S] * b, False, 0.25, dtype=dtype)
+    core = CoreAttention(H * d, 0.0, H, 1)
+    for _ in range(2):
+        got = core(q, k, v, attn_type="flash")
+        assert got.shape == (b, S, H * d)
+        _within("flash", got.view(-1, H, d), ref["out"], ref["out_bound"])
+    seqs = bf.PackedSequences.from_lengths([100, 35], device=hip_device)          # graphs packed along the batch's rows
+    ref = sq.attention(*(x.double().reshape(-1, H, d) for x in (q, k, v)), [100, 35], [100, 35], False, 0.25, dtype=dtype)
+    _within("packed", core(q, k, v, edge_index=seqs, attn_type="flash").view(-1, H, d), ref["out"], ref["out_bound"])
+    freq = bf.RotaryFrequencies(d, device=hip_device)
+    turned = CoreAttention(H * d, 0.0, H, 1, rotary=freq)
+    qr, kr = bf.rotary_embedding(q.reshape(-1, H, d), k.reshape(-1, H, d), freq,
+                                 positions=torch.arange(S, device=hip_device).repeat(b))
+    assert torch.equal(turned(q, k, v, attn_type="flash"), core(qr.view_as(q), kr.view_as(k), v, attn_type="flash"))
+    with pytest.raises(NotImplementedError, match="bias"):
+        core(q, k, v, torch.zeros(1, S, S, H, device=hip_device), attn_type="flash")
+    with pytest.raises(NotImplementedError, match="dropout"):
+        CoreAttention(H * d, 0.1, H, 1).train()(q, k, v, attn_type="flash")
+    assert CoreAttention(H * d, 0.1, H, 1).eval()(q, k, v, attn_type="flash").shape == (b, S, H * d)
+
+
+# ------------------------------------------------------------------ streams, graphs, refusals
+def _layer(bf, q, k, v, do, freq, ld, seqs):
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    qr, kr = bf.rotary_embedding(leaves[0], leaves[1], freq, seqs=seqs)
+    a, b = bf.packed_attention(qr, kr, leaves[2], seqs), bf.linear_attention(*leaves, ld, seqs)
+    return [a, b, *torch.autograd.grad((a, b), leaves, (do, do))]
+
+
+def test_a_captured_layer_replays(hip_device):
+    bf = _bf()
+    lens = [300, 1, 64, 400]
+    n, H, d = sum(lens), 4, 64
+    base = [_randn(i, n, H, d, dtype=torch.bfloat16, dev=hip_device) for i in range(4)]
+    q, k, v, do = (x.clone() for x in base)
+    freq, ld = bf.RotaryFrequencies(d, device=hip_device), torch.full((H,), -0.05, device=hip_device)
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+    step = [_randn(9, 3, H, d, dtype=torch.bfloat16, dev=hip_device) for _ in range(3)]
+    state = _randn(10, 3, H, d, d, dev=hip_device)
+
+    def every():
+        return _layer(bf, q, k, v, do, freq, ld, seqs) + list(bf.linear_attention_step(*step, ld, state))
+
+    alive = _layer(bf, q, k, v, do, freq, ld, seqs)            # an eager graph that lives through the capture
+    side = torch.cuda.Stream(device=hip_device)
+    side.wait_stream(torch.cuda.current_stream(hip_device))
+    with torch.cuda.stream(side):
+        every()
+    torch.cuda.current_stream(hip_device).wait_stream(side)
+    torch.cuda.synchronize(hip_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = every()
+    for rep in range(4):
+        for x, y in zip((q, k, v, do), base):
+            x.copy_(y * (0.5 + 0.3 * rep))
+        state.mul_(0.9)
+        graph.replay()
+        torch.cuda.synchronize(hip_device)
+        got = [x.clone() for x in captured]
+        _ = torch.randn(1 << 18, device=hip_device).sum().item()
+        for i, (x, y) in enumerate(zip(got, every())):
+            assert torch.equal(x, y), (rep, i)
+    del alive
+
+
+def test_two_streams_at_once(hip_device):
+    """Calls of different sizes on two streams, with their pieces and carries in flight together."""
+    bf = _bf()
+    freq, ld = bf.RotaryFrequencies(32, device=hip_device), torch.full((4,), -0.05, device=hip_device)
+    jobs = []
+    for i, lens in enumerate(([700, 3], [64] * 9)):
+        args = [_randn(10 * i + j, sum(lens), 4, 32, dtype=torch.bfloat16, dev=hip_device) for j in range(4)]
+        jobs.append((args, bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)))
+    alone = [_layer(bf, *a, freq, ld, s) for a, s in jobs]
+    torch.cuda.synchronize(hip_device)
+    streams = [torch.cuda.Stream(device=hip_device) for _ in jobs]
+    for _ in range(3):
+        got = []
+        for st, (a, s) in zip(streams, jobs):
+            with torch.cuda.stream(st):
+                got.append(_layer(bf, *a, freq, ld, s))
+        torch.cuda.synchronize(hip_device)
+        for x, y in zip(got, alone):
+            assert all(torch.equal(p, r) for p, r in zip(x, y))
+
+
+def test_empty_batches(hip_device):
+    bf = _bf()
+    seqs = bf.PackedSequences.from_lengths([], causal=True, device=hip_device)
+    q = torch.zeros(0, 2, 16, device=hip_device, requires_grad=True)
+    out = bf.packed_attention(q, q, q, seqs)
+    assert out.shape == (0, 2, 16)
+    torch.autograd.grad(out.sum(), q)
+    ld = torch.zeros(2, device=hip_device)
+    out, state = bf.linear_attention(q, q, q, ld, seqs, return_state=True)
+    assert out.shape == (0, 2, 16) and state.shape == (0, 2, 16, 16)
+    freq = bf.RotaryFrequencies(16, device=hip_device)
+    assert bf.rotary_embedding(q, None, freq, seqs=seqs).shape == (0, 2, 16)
+    keys = bf.PackedSequences.from_lengths([0, 0], [3, 4], device=hip_device)     # keys without rows
+    k = torch.ones(7, 2, 16, device=hip_device, requires_grad=True)
+    g, = torch.autograd.grad(bf.packed_attention(q, k, k, keys).sum(), k)
+    assert bool((g == 0).all())
+    empty = bf.PackedSequences.from_lengths([0, 0], causal=True, device=hip_device)
+    s0 = _randn(1, 2, 2, 16, 16, dev=hip_device)
+    _, state = bf.linear_attention(q, q, q, ld, empty, initial_state=s0, return_state=True)
+    assert torch.equal(state, s0)
+
+
+def test_refusals(hip_device):
+    bf = _bf()
+    dev = hip_device
+    seqs = bf.PackedSequences.from_lengths([10, 20], causal=True, device=dev)
+    q = torch.zeros(30, 4, 32, device=dev)
+    with pytest.raises(ValueError, match="cover"):
+        bf.packed_attention(q[:29], q[:29], q[:29], seqs)
+    with pytest.raises(ValueError, match="multiple"):
+        bf.packed_attention(q, q[:, :3], q[:, :3], seqs)
+    with pytest.raises(ValueError, match="disagree"):
+        bf.packed_attention(q, q, q[:, :2], seqs)
+    for d in (4, 12, 136):
+        x = torch.zeros(30, 1, d, device=dev)
+        with pytest.raises(NotImplementedError, match="head_dim"):
+            bf.packed_attention(x, x, x, seqs)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="scale"):
+            bf.packed_attention(q, q, q, seqs, scale=scale)
+    with pytest.raises(ValueError, match="float32, bfloat16"):
+        bf.packed_attention(q.double(), q.double(), q.double(), seqs)
+    with pytest.raises(ValueError, match="rows, heads"):
+        bf.packed_attention(q[0], q, q, bf.PackedSequences.from_lengths([4], [30], device=dev))
+    with pytest.raises(TypeError, match="PackedSequences"):
+        bf.packed_attention(q, q, q, [10, 20])
+    off = torch.tensor([0, 10, 30], device=dev)
+    for bad, n in ((torch.tensor([1, 10, 30], device=dev), None), (torch.tensor([0, 20, 10], device=dev), None), (off, 29)):
+        with pytest.raises(ValueError):
+            bf.PackedSequences.from_offsets(bad, n_q=n)
+    with pytest.raises(ValueError, match="must be given"):
+        bf.PackedSequences.from_offsets(off, check=False)
+    assert bf.PackedSequences.from_offsets(off, check=False, n_q=31).n_q == 31
+    freq = bf.RotaryFrequencies(32, device=dev)
+    pos = torch.zeros(30, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match="positions"):
+        bf.rotary_embedding(q, None, freq)
+    with pytest.raises(ValueError, match="positions"):
+        bf.rotary_embedding(q, None, freq, positions=pos[:29])
+    with pytest.raises(ValueError, match="int32 or int64"):
+        bf.rotary_embedding(q, None, freq, positions=pos.float())
+    with pytest.raises(ValueError, match="rotated values"):
+        bf.rotary_embedding(q[..., :16], None, freq, positions=pos)
+    with pytest.raises(ValueError, match="disagree"):
+        bf.rotary_embedding(q, q[:20], freq, positions=pos)
+    ld = torch.zeros(4, device=dev)
+    with pytest.raises(ValueError, match="causal"):
+        bf.linear_attention(q, q, q, ld, bf.PackedSequences.from_lengths([30], device=dev))
+    with pytest.raises(ValueError, match="log_decay"):
+        bf.linear_attention(q, q, q, ld[:3], seqs)
+    with pytest.raises(NotImplementedError, match="constants"):
+        bf.linear_attention(q, q, q, ld.clone().requires_grad_(True), seqs)
+    with pytest.raises(ValueError, match="init_state"):
+        bf.linear_attention(q, q, q, ld, seqs, initial_state=torch.zeros(1, 4, 32, 32, device=dev))
+    s = torch.zeros(30, 4, 32, 32, device=dev)
+    with pytest.raises(ValueError, match="state must be"):
+        bf.linear_attention_step(q, q, q, ld, s[:29])
+    with pytest.raises(NotImplementedError, match="gradients"):
+        bf.linear_attention_step(q.clone().requires_grad_(True), q, q, ld, s)

@@ -1,0 +1,164 @@
+"""Host-side checks of the operators over packed sequences (CPU): the C ABI's refusals before any launch, the struct
+mirrors, the Python surface's own checks. No kernel runs here."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import budgetformer_amd as bf
+from budgetformer_amd import _native as N
+
+BUF = (C.c_int64 * 64)()
+P = C.c_void_p((C.addressof(BUF) + 15) // 16 * 16)          # 16-byte aligned host memory, never read
+
+
+def _attn(**kw):
+    a = N.PackedAttn(n_q=4, n_k=4, heads_q=2, heads_k=1, head_dim=16, dtype=N.BF_DTYPE_BF16, row_span=P, key_span=P, scale=0.25)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = (32, 16), (16, 16), (16, 16)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def _fwd(a, q=P, k=P, v=P, out=P):
+    N.call("bf_packed_attn_fwd", C.byref(a), q, k, v, out, P, P, None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dtype=7), "dtype"), (dict(heads_q=3, heads_k=2), "multiple"), (dict(heads_k=0), "heads"),
+    (dict(n_q=-1), "rows"), (dict(n_k=2 ** 31), "keys"), (dict(n_q=2 ** 30), "rows"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(row_span=None), "spans")])
+def test_packed_attention_arguments(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _fwd(_attn(**kw))
+    assert N.load().bf_packed_attn_fwd_floats(C.byref(_attn(**kw))) == -1
+
+
+@pytest.mark.parametrize("d", [0, 4, 12, 136])
+def test_packed_attention_head_dims(d):
+    with pytest.raises(NotImplementedError, match="head_dim"):
+        _fwd(_attn(head_dim=d))
+
+
+def test_packed_attention_addresses_and_strides():
+    off = C.c_void_p(P.value + 2)
+    for kw in (dict(q=off), dict(k=off), dict(v=off), dict(out=off)):
+        with pytest.raises(ValueError, match="aligned"):
+            _fwd(_attn(), **kw)
+    a = _attn()
+    a.k_stride[0] = 20
+    with pytest.raises(ValueError, match="16-byte steps"):
+        _fwd(a)
+    with pytest.raises(ValueError, match="bad arguments"):
+        _fwd(_attn(), q=None)
+    with pytest.raises(ValueError, match="no key spans"):
+        N.call("bf_packed_attn_bwd", C.byref(_attn(key_span=None)), P, P, P, P, P, P, P, P, P, P, None)
+    _fwd(_attn(n_q=0))                                       # nothing to do, nothing launched
+
+
+def test_rotary_arguments():
+    s = (C.c_int64 * 2)(16, 16)
+
+    def call(n=4, hx=1, hy=0, dim=16, rot=16, dtype=0, x=P, y=None):
+        N.call("bf_rotary", x, y, n, hx, hy, dim, rot, dtype, s, s, P, 1, P, 1.0, 0, 0, P, P, None)
+
+    for kw in (dict(rot=0), dict(rot=3), dict(rot=18), dict(dim=2000, rot=1026)):
+        with pytest.raises(ValueError, match="even number"):
+            call(**kw)
+    for kw in (dict(n=-1), dict(hx=0), dict(hy=-1), dict(dim=0)):
+        with pytest.raises(ValueError, match="bad sizes"):
+            call(**kw)
+    with pytest.raises(ValueError, match="dtype"):
+        call(dtype=9)
+    for kw in (dict(x=None), dict(hy=2)):
+        with pytest.raises(ValueError, match="bad arguments"):
+            call(**kw)
+    call(n=0)
+
+
+def _lin(**kw):
+    a = N.LinearAttn(n=4, n_seq=1, heads=2, dim_x=16, dim_z=16, dtype=N.BF_DTYPE_F32, row_span=P, key_span=P, offsets=P,
+                     log_decay=P, scale=1.0)
+    a.x_stride[:], a.y_stride[:], a.z_stride[:] = (32, 16), (32, 16), (32, 16)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_linear_attention_arguments():
+    def call(a, x=P):
+        N.call("bf_linear_attn_pass", C.byref(a), x, P, P, P, P, None)
+
+    for kw, match in ((dict(dtype=5), "dtype"), (dict(n=-1), "sizes"), (dict(heads=0), "sizes"), (dict(n=2 ** 31), "sizes"),
+                      (dict(log_decay=None), "decays"), (dict(row_span=None), "spans"), (dict(scale=float("nan")), "scale"),
+                      (dict(init=P, reverse=1), "states"), (dict(final_state=P, offsets=None), "states")):
+        with pytest.raises(ValueError, match=match):
+            call(_lin(**kw))
+        assert N.load().bf_linear_attn_floats(C.byref(_lin(**kw))) == -1
+    for d in (4, 20, 136):
+        with pytest.raises(NotImplementedError, match="head dims"):
+            call(_lin(dim_x=d))
+        with pytest.raises(NotImplementedError, match="head dims"):
+            call(_lin(dim_z=d))
+        with pytest.raises(NotImplementedError, match="head dims"):
+            N.call("bf_linear_attn_step", P, P, P, P, P, 1, 1, d, 16, 0, 1.0, P, P, None)
+    with pytest.raises(ValueError, match="aligned"):
+        call(_lin(), x=C.c_void_p(P.value + 4))
+    with pytest.raises(ValueError, match="sequences"):
+        N.call("bf_linear_attn_step", P, P, P, P, P, 2 ** 24, 1, 16, 16, 0, 1.0, P, P, None)
+    call(_lin(n=0))
+    N.call("bf_linear_attn_step", P, P, P, P, P, 0, 1, 16, 16, 0, 1.0, P, P, None)
+
+
+def test_spans_arguments():
+    with pytest.raises(ValueError, match="32 bits"):
+        N.call("bf_packed_spans", P, P, 1, 2 ** 31, 4, 0, P, P, None, None)
+    with pytest.raises(ValueError, match="bad arguments"):
+        N.call("bf_packed_spans", P, P, 1, 4, 4, 0, None, P, None, None)
+    N.call("bf_packed_spans", None, None, 0, 0, 0, 0, None, None, None, None)
+
+
+def test_host_tensors_and_bad_lengths_are_refused():
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        bf.PackedSequences.from_lengths([1, 2], device="cpu")
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        bf.PackedSequences.from_offsets(torch.tensor([0, 3]))
+    for q, k, match in (([-1, 2], None, "negative"), ([1, 2], [3], "each sequence"), ([2 ** 30, 2 ** 30], None, "2\\^31"),
+                        ([1], [2 ** 31], "2\\^31")):
+        with pytest.raises(ValueError, match=match):
+            bf.PackedSequences.from_lengths(q, k, device="cuda")
+    for kw, match in ((dict(rot=3), "even"), (dict(rot=0), "even"), (dict(rot=8, base=1.0), "base"), (dict(rot=8, factor=0.0), "factor"),
+                      (dict(rot=8, scaling="other"), "scaling"), (dict(rot=2, scaling="ntk"), "two pairs"),
+                      (dict(rot=8, scaling="by_parts"), "original"), (dict(rot=8, amplitude=float("inf")), "amplitude"),
+                      (dict(rot=8, device="cpu"), "no CPU fallback")):
+        with pytest.raises(ValueError, match=match):
+            bf.RotaryFrequencies(**kw)
+    q = torch.zeros(2, 1, 8)
+    with pytest.raises(NotImplementedError):                 # the operators have device kernels only
+        bf.linear_attention_step(q, q, q, torch.zeros(1), torch.zeros(2, 1, 8, 8))
+
+
+def test_operators_are_registered():
+    ops = N.load_ops()
+    for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_pass", "linear_attn_step"):
+        assert str(getattr(ops, name).default._schema).startswith(f"bf::{name}(")
+
+
+@pytest.mark.parametrize("struct,mirror", [("bf_packed_attn", "PackedAttn"), ("bf_linear_attn", "LinearAttn")])
+def test_struct_mirrors_match_the_header(tmp_path, struct, mirror):
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    cls = getattr(N, mirror)
+    names = [f[0] for f in cls._fields_]
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "budgetformer_hip.h"', "int main(void) {",
+             f'  printf("%zu\\n", sizeof({struct}));']
+    lines += [f'  printf("%zu\\n", offsetof({struct}, {f}));' for f in names] + ["  return 0;", "}"]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines) + "\n")
+    subprocess.run([cc, "-I", os.path.dirname(N._HEADER), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(cls)] + [getattr(cls, f).offset for f in names]
