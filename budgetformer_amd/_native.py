@@ -61,10 +61,9 @@ class PackedAttn(C.Structure):
 class LinearAttn(C.Structure):
     """Mirror of ``struct bf_linear_attn``."""
     _fields_ = [
-        ("n", i64), ("n_seq", i64), ("heads", i32), ("dim_x", i32), ("dim_z", i32), ("dtype", i32),
-        ("x_stride", i64 * 2), ("y_stride", i64 * 2), ("z_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
-        ("offsets", vp), ("log_decay", vp), ("init", vp), ("final_state", vp), ("init_stride", i64 * 2),
-        ("scale", f32), ("reverse", i32),
+        ("n", i64), ("n_seq", i64), ("heads", i32), ("dim_k", i32), ("dim_v", i32), ("dtype", i32),
+        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
+        ("offsets", vp), ("log_decay", vp), ("init", vp), ("final_state", vp), ("scale", f32), ("reserved", i32),
     ]
 
 
@@ -168,11 +167,14 @@ _SIGS = {
     "bf_packed_spans": (C.c_int, [P_i32, P_i32, i64, i64, i64, i32, P_i32, P_i32, P_i32, vp]),
     "bf_packed_attn_fwd_floats": (i64, [C.POINTER(PackedAttn)]),
     "bf_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, P_f32, vp]),
-    "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, vp]),
+    "bf_packed_attn_bwd_floats": (i64, [C.POINTER(PackedAttn)]),
+    "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, P_f32, vp]),
     "bf_rotary": (C.c_int, [vp, vp, i64, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64), vp, i32, vp, f32, i32,
                             i32, vp, vp, vp]),
-    "bf_linear_attn_floats": (i64, [C.POINTER(LinearAttn)]),
-    "bf_linear_attn_pass": (C.c_int, [C.POINTER(LinearAttn), vp, vp, vp, vp, P_f32, vp]),
+    "bf_linear_attn_fwd_floats": (i64, [C.POINTER(LinearAttn)]),
+    "bf_linear_attn_fwd": (C.c_int, [C.POINTER(LinearAttn), vp, vp, vp, vp, P_f32, vp]),
+    "bf_linear_attn_bwd_floats": (i64, [C.POINTER(LinearAttn)]),
+    "bf_linear_attn_bwd": (C.c_int, [C.POINTER(LinearAttn), vp, vp, vp, vp, vp, vp, vp, P_f32, vp]),
     "bf_linear_attn_step": (C.c_int, [vp, vp, vp, P_f32, P_f32, i64, i32, i32, i32, i32, f32, vp, P_f32, vp]),
 }
 

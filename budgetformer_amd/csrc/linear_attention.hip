@@ -45,6 +45,10 @@ template <typename T> __device__ __forceinline__ Frag<T> pack8_by(const F32x16& 
   return f;
 }
 
+struct LinRoles {
+  LinArgs role[3];
+};
+
 template <typename T> constexpr int lin_tile() { return sizeof(T) == 2 ? 64 : 32; }
 
 // log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
@@ -72,9 +76,18 @@ __device__ __forceinline__ int sequence_of(const LinArgs& a, int p) {
   return lo;
 }
 
+// The same value, unknown to the compiler: the addresses of a state's 64 values a lane are then formed where a sequence
+// begins or ends, and not kept in registers through the loop.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <typename T, int DX, int DZ, bool OUT>
-__global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
+__global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
+  const LinArgs& a = all.role[blockIdx.y];
   constexpr int C = lin_tile<T>(), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
+  constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, __bf16>::value ? 3 : 2;
   using TX = Tile<T, DX>;
   using TZ = Tile<T, DZ>;
   using TW = Tile<T, C>;
@@ -133,12 +146,13 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
       __syncthreads();
     const int len = t1 - t0;
     if (a.states && seq >= 0 && seq < a.n_seq && t0 == a.offsets[seq]) {          // a sequence begins with its tile
+      const int z = fresh(32 * wave + col), x0 = fresh(4 * half);
       const float* s0 = a.init ? a.init + (int64_t(seq) * a.heads + h) * a.dx * a.dz : nullptr;
 #pragma unroll
       for (int b = 0; b < XB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int x = 32 * b + acc_row(r, half), z = 32 * wave + col;
+          const int x = x0 + 32 * b + acc_row(r, 0);
           m[b][r] = s0 && x < a.dx && z < a.dz ? s0[x * a.init_sx + z * a.init_sz] : 0.f;
         }
     }
@@ -187,7 +201,7 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
         }
       }
       const float per_unit = 1.f / unit;
-#pragma unroll
+#pragma unroll 1
       for (int ib = 0; ib < QB; ++ib) {
         const int i = 32 * ib + col;
         F32x16 o = zero16();
@@ -208,30 +222,30 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r] = mine ? o[r] * f : 0.f;
         }
-        F32x16 bad = zero16();
+        if (!odd) {
 #pragma unroll
-        for (int t = 0; t < C / 16; ++t) {
-          if (t >= 2 * (ib + 1)) continue;
-          Frag<T> zf = TZ::template col_frag<false>(z_lds, t, wave, lane);
-          const Frag<T> wf = TW::row_frag(w_lds, i, t, half);
-          if (odd) {
-            Frag<T> clean, up, down, sees;
-            split_finite<T>(zf, clean, up, down);
+          for (int t = 0; t < C / 16; ++t)
+            if (t < 2 * (ib + 1))
+              o = Mat<T>::mma(TZ::template col_frag<false>(z_lds, t, wave, lane), TW::row_frag(w_lds, i, t, half), o);
+        } else {                          // some z is not finite: NaN for the rows that see it, nothing for the others
+          F32x16 bad = zero16();
+          const int from = start_lds[i] - t0;
+          for (int t = 0; t < 2 * (ib + 1); ++t) {
+            const Frag<T> zf = TZ::template col_frag<false>(z_lds, t, wave, lane);
+            o = Mat<T>::mma(finite<T>(zf), TW::row_frag(w_lds, i, t, half), o);
+            Frag<T> sees;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int j = 16 * t + 8 * half + k;
-              sees[k] = T(j <= i && j >= start_lds[i] - t0 ? 1.f : 0.f);
-              up[k] = T(fmaxf(float(up[k]), float(down[k])));
+              sees[k] = T(j <= i && j >= from ? 1.f : 0.f);
             }
-            bad = Mat<T>::mma(up, sees, bad);
-            zf = clean;
+            bad = Mat<T>::mma(is_infinite<T>(zf, 1.f), sees, bad);
+            bad = Mat<T>::mma(is_infinite<T>(zf, -1.f), sees, bad);
           }
-          o = Mat<T>::mma(zf, wf, o);
-        }
-        if (odd)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (bad[r] > 0.f) o[r] = NAN;
+        }
         if (i < len)
           store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, 1.f, wave, a.dz,
                          half);
@@ -249,11 +263,18 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
       const bool cut = from > 0;
 #pragma unroll
       for (int t = 0; t < C / 16; ++t) {
-        Frag<T> zf = TZ::template col_frag<true>(z_lds, t, wave, lane);
+        // the decayed z in two or three parts of the activations' type, which add up to (nearly) its float32 value
+        const Frag<T> z0 = TZ::template col_frag<true>(z_lds, t, wave, lane);
+        Frag<T> part[3];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int j = 16 * t + acc_row(k, half);
-          zf[k] = j >= from && j < len ? T(float(zf[k]) * exp2_fast(ld * float(len - 1 - j))) : T(0.f);
+          float x = j >= from && j < len ? float(z0[k]) * exp2_fast(ld * float(len - 1 - j)) : 0.f;
+#pragma unroll
+          for (int n = 0; n < kParts; ++n) {
+            part[n][k] = T(x);
+            x -= float(part[n][k]);
+          }
         }
 #pragma unroll
         for (int b = 0; b < XB; ++b) {
@@ -263,16 +284,18 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
             for (int k = 0; k < 8; ++k)
               if (16 * t + acc_row(k, half) < from) yf[k] = T(0.f);
           }
-          m[b] = Mat<T>::mma(yf, zf, m[b]);
+#pragma unroll
+          for (int n = 0; n < kParts; ++n) m[b] = Mat<T>::mma(yf, part[n], m[b]);
         }
       }
       if (OUT && ends && a.final_state) {
+        const int z = fresh(32 * wave + col), x0 = fresh(4 * half);
         float* fs = a.final_state + (int64_t(this_seq) * a.heads + h) * a.dx * a.dz;
 #pragma unroll
         for (int b = 0; b < XB; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int x = 32 * b + acc_row(r, half), z = 32 * wave + col;
+            const int x = x0 + 32 * b + acc_row(r, 0);
             if (x < a.dx && z < a.dz) fs[x * a.dz + z] = m[b][r];
           }
       }
@@ -288,22 +311,31 @@ __global__ __launch_bounds__(2 * DZ) void linear_pass(const LinArgs a) {
   }
 }
 
-// Segments' own contributions -> the state each segment starts from, in place: one lane a value of a head's state.
-__global__ __launch_bounds__(256) void linear_carry(const LinArgs a, int64_t values) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= values * a.heads) return;
+// Segments' own contributions -> the state each segment starts from, in place: one lane a value of a head's state, eight
+// segments' values read before the first of them is replaced.
+__global__ __launch_bounds__(256) void linear_carry(const LinRoles all, int64_t values) {
+  const LinArgs& a = all.role[blockIdx.y];
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, step = values * a.heads;
+  if (i >= step) return;
   const int h = int(i / values);
   const float f = exp2_fast(decay_log2(a, h) * float(a.seg_len));
   float* c = a.carry + i;
   float into = 0.f;
-  for (int s = 0; s + 1 < a.n_seg; ++s) {
-    const float mine = c[s * values * a.heads];
-    c[s * values * a.heads] = into;
-    const int e = (s + 1) * a.seg_len;
-    const bool began = start_at(a, e - 1) >= e - a.seg_len;         // the segment's last sequence began in it
-    into = began ? mine : fmaf(into, f, mine);
+  for (int s0 = 0; s0 < a.n_seg; s0 += 8) {
+    float mine[8];
+    bool began[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k, e = (s + 1) * a.seg_len;
+      mine[k] = s < a.n_seg ? c[s * step] : 0.f;
+      began[k] = s + 1 < a.n_seg && start_at(a, e - 1) >= e - a.seg_len;     // the segment's last sequence began in it
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (s0 + k < a.n_seg) c[(s0 + k) * step] = into;
+      into = began[k] ? mine[k] : fmaf(into, f, mine[k]);
+    }
   }
-  c[(a.n_seg - 1) * values * a.heads] = into;
 }
 
 // The final state of sequences without tokens is their initial one.
@@ -371,21 +403,21 @@ int check(const bf_linear_attn* p, const char* fn) {
   BF_CHECK_ARG(p != nullptr, "%s: no arguments", fn);
   BF_CHECK_ARG(p->dtype == BF_DTYPE_F32 || p->dtype == BF_DTYPE_BF16 || p->dtype == BF_DTYPE_F16, "%s: dtype %d", fn,
                p->dtype);
-  for (int d : {p->dim_x, p->dim_z})
+  for (int d : {p->dim_k, p->dim_v})
     if (d < 8 || d > 128 || d % 8) {
-      set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_x, p->dim_z);
+      set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_k, p->dim_v);
       return BF_ERR_UNSUPPORTED;
     }
   BF_CHECK_ARG(p->n >= 0 && p->n < (int64_t(1) << 31) - 256 && p->n_seq >= 0 && p->n_seq < (int64_t(1) << 31) - 1 &&
                    p->heads >= 1 && p->heads <= (1 << 20),
                "%s: bad sizes (%lld rows, %lld sequences, %d heads)", fn, (long long)p->n, (long long)p->n_seq, p->heads);
   const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;
-  for (const int64_t* s : {p->x_stride, p->y_stride, p->z_stride})
+  for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
     BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,
                  "%s: strides (%lld, %lld) are not whole 16-byte steps", fn, (long long)s[0], (long long)s[1]);
   BF_CHECK_ARG(p->scale == p->scale && p->scale <= 3e38f && p->scale >= -3e38f, "%s: scale %g", fn, double(p->scale));
-  BF_CHECK_ARG(p->log_decay && (p->n == 0 || (p->reverse ? p->key_span : p->row_span)), "%s: no decays or no spans", fn);
-  BF_CHECK_ARG(!(p->init || p->final_state) || (p->offsets && !p->reverse), "%s: states need the offsets and no reverse", fn);
+  BF_CHECK_ARG(p->log_decay && (p->n == 0 || (p->row_span && p->key_span)), "%s: no decays or no spans", fn);
+  BF_CHECK_ARG(!(p->init || p->final_state) || p->offsets, "%s: states need the offsets", fn);
   return BF_OK;
 }
 
@@ -393,69 +425,141 @@ int check(const bf_linear_attn* p, const char* fn) {
 // carries cost a state each, read and written, which a segment of 256 tokens or more outweighs).
 int64_t segment_of(const bf_linear_attn* p) {
   const int64_t want = ceil_div(512, p->heads);
-  int64_t len = ceil_div(ceil_div(p->n, want), 64) * 64;
+  const int64_t len = ceil_div(ceil_div(p->n, want), 64) * 64;
   return len < 256 ? 256 : len;
 }
+
+// Floats that one pass's segments carry.
+int64_t carry_floats(const bf_linear_attn* p) {
+  const int64_t segs = ceil_div(p->n, segment_of(p));
+  return segs <= 1 ? 0 : segs * p->heads * pad32(p->dim_k) * pad32(p->dim_v);
+}
+
+LinArgs make_args(const bf_linear_attn* p) {
+  LinArgs a{};
+  a.row_span = reinterpret_cast<const int2*>(p->row_span);
+  a.key_span = reinterpret_cast<const int2*>(p->key_span);
+  a.offsets = p->offsets, a.log_decay = p->log_decay;
+  a.n = int32_t(p->n), a.n_seq = int32_t(p->n_seq), a.heads = p->heads;
+  a.scale = p->scale;
+  a.seg_len = int32_t(segment_of(p));
+  a.n_seg = int32_t(ceil_div(p->n, a.seg_len));
+  return a;
+}
+
+// One launch (three with segments) for passes of the same head sizes.
+int launch(const LinRoles& roles, int n_roles, int32_t dtype, hipStream_t st) {
+  const LinArgs& a = roles.role[0];
+  const int64_t groups = int64_t(a.n_seg) * a.heads;
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_pad(a.dx, [&](auto px) -> int {
+      return with_pad(a.dz, [&](auto pz) -> int {
+        constexpr int DX = decltype(px)::value, DZ = decltype(pz)::value;
+        const dim3 grid = dim3(unsigned(groups), unsigned(n_roles));
+        if (a.n_seg > 1) {
+          auto own = linear_pass<T, DX, DZ, false>;
+          BF_LAUNCH("linear_attn_segments", own, grid, dim3(2 * DZ), 0, st, roles);
+          BF_CHECK_LAUNCH();
+          const int64_t values = DX * DZ;
+          BF_LAUNCH("linear_attn_carry", linear_carry, dim3(unsigned(ceil_div(values * a.heads, 256)), unsigned(n_roles)),
+                    dim3(256), 0, st, roles, values);
+          BF_CHECK_LAUNCH();
+        }
+        auto pass = linear_pass<T, DX, DZ, true>;
+        BF_LAUNCH("linear_attn_pass", pass, grid, dim3(2 * DZ), 0, st, roles);
+        BF_CHECK_LAUNCH();
+        return BF_OK;
+      });
+    });
+  });
+}
+
+// The passes of a call: those of the same padded head sizes together.
+int run(LinArgs (&pass)[3], int n, int32_t dtype, hipStream_t st) {
+  bool done[3] = {false, false, false};
+  for (int i = 0; i < n; ++i) {
+    if (done[i]) continue;
+    LinRoles r{};
+    int m = 0;
+    for (int j = i; j < n; ++j)
+      if (!done[j] && pad32(pass[j].dx) == pad32(pass[i].dx) && pad32(pass[j].dz) == pad32(pass[i].dz)) {
+        r.role[m++] = pass[j];
+        done[j] = true;
+      }
+    BF_CHECK_OK(launch(r, m, dtype, st));
+  }
+  return BF_OK;
+}
+
+void set_x(LinArgs& a, const void* x, const int64_t (&s)[2], int d) { a.x = x, a.xs_t = s[0], a.xs_h = s[1], a.dx = d; }
+void set_y(LinArgs& a, const void* y, const int64_t (&s)[2]) { a.y = y, a.ys_t = s[0], a.ys_h = s[1]; }
+void set_z(LinArgs& a, const void* z, const int64_t (&s)[2], int d) { a.z = z, a.zs_t = s[0], a.zs_h = s[1], a.dz = d; }
 
 }  // namespace
 }  // namespace bf
 
 using namespace bf;
 
-extern "C" int64_t bf_linear_attn_floats(const bf_linear_attn* p) {
-  if (check(p, "linear_attn_floats") != BF_OK) return -1;
-  const int64_t segs = ceil_div(p->n, segment_of(p));
-  return segs <= 1 ? 0 : segs * p->heads * pad32(p->dim_x) * pad32(p->dim_z);
+extern "C" int64_t bf_linear_attn_fwd_floats(const bf_linear_attn* p) {
+  if (check(p, "linear_attn_fwd_floats") != BF_OK) return -1;
+  return carry_floats(p);
 }
 
-extern "C" int bf_linear_attn_pass(const bf_linear_attn* p, const void* x, const void* y, const void* z, void* out,
-                                   float* scratch, void* stream) {
-  BF_CHECK_OK(check(p, "linear_attn_pass"));
-  BF_CHECK_ARG(p->n == 0 || (x && y && z && out), "linear_attn_pass: bad arguments");
-  BF_CHECK_ARG(aligned16({x, y, z, out}), "linear_attn_pass: x, y, z and out must be 16-byte aligned");
-  LinArgs a{};
-  a.x = x, a.y = y, a.z = z, a.out = out;
-  a.xs_t = p->x_stride[0], a.xs_h = p->x_stride[1];
-  a.ys_t = p->y_stride[0], a.ys_h = p->y_stride[1];
-  a.zs_t = p->z_stride[0], a.zs_h = p->z_stride[1];
-  a.row_span = reinterpret_cast<const int2*>(p->row_span);
-  a.key_span = reinterpret_cast<const int2*>(p->key_span);
-  a.offsets = p->offsets, a.log_decay = p->log_decay, a.init = p->init, a.final_state = p->final_state;
-  a.init_sx = p->init_stride[0], a.init_sz = p->init_stride[1];
-  a.n = int32_t(p->n), a.n_seq = int32_t(p->n_seq), a.heads = p->heads, a.dx = p->dim_x, a.dz = p->dim_z;
-  a.scale = p->scale, a.reverse = p->reverse != 0, a.states = (p->init || p->final_state) && p->n_seq > 0;
-  a.seg_len = int32_t(segment_of(p));
-  a.n_seg = int32_t(ceil_div(p->n, a.seg_len));
-  a.carry = scratch;
+extern "C" int bf_linear_attn_fwd(const bf_linear_attn* p, const void* q, const void* k, const void* v, void* out,
+                                  float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "linear_attn_fwd"));
+  BF_CHECK_ARG(p->n == 0 || (q && k && v && out), "linear_attn_fwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out}), "linear_attn_fwd: q, k, v and out must be 16-byte aligned");
+  LinArgs pass[3] = {make_args(p)};
+  LinArgs& a = pass[0];
+  set_x(a, q, p->q_stride, p->dim_k);
+  set_y(a, k, p->k_stride);
+  set_z(a, v, p->v_stride, p->dim_v);
+  a.out = out, a.carry = scratch;
+  a.init = p->init, a.final_state = p->final_state, a.states = (p->init || p->final_state) && p->n_seq > 0;
+  a.init_sx = p->dim_v, a.init_sz = 1;
   const hipStream_t st = as_stream(stream);
   if (a.states && a.final_state) {
     BF_LAUNCH("linear_attn_empty", linear_empty, dim3(unsigned(a.n_seq)), dim3(256), 0, st, a);
     BF_CHECK_LAUNCH();
   }
   if (a.n == 0) return BF_OK;
-  BF_CHECK_ARG(a.n_seg == 1 || scratch, "linear_attn_pass: no scratch (bf_linear_attn_floats)");
-  const int64_t groups = int64_t(a.n_seg) * a.heads;
-  return with_type(p->dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    return with_pad(a.dx, [&](auto px) -> int {
-      return with_pad(a.dz, [&](auto pz) -> int {
-        constexpr int DX = decltype(px)::value, DZ = decltype(pz)::value;
-        if (a.n_seg > 1) {
-          auto own = linear_pass<T, DX, DZ, false>;
-          BF_LAUNCH("linear_attn_segments", own, dim3(unsigned(groups)), dim3(2 * DZ), 0, st, a);
-          BF_CHECK_LAUNCH();
-          const int64_t values = DX * DZ;
-          BF_LAUNCH("linear_attn_carry", linear_carry, dim3(unsigned(ceil_div(values * a.heads, 256))), dim3(256), 0, st, a,
-                    values);
-          BF_CHECK_LAUNCH();
-        }
-        auto pass = linear_pass<T, DX, DZ, true>;
-        BF_LAUNCH("linear_attn_pass", pass, dim3(unsigned(groups)), dim3(2 * DZ), 0, st, a);
-        BF_CHECK_LAUNCH();
-        return BF_OK;
-      });
-    });
-  });
+  BF_CHECK_ARG(a.n_seg == 1 || scratch, "linear_attn_fwd: no scratch (bf_linear_attn_fwd_floats)");
+  return run(pass, 1, p->dtype, st);
+}
+
+extern "C" int64_t bf_linear_attn_bwd_floats(const bf_linear_attn* p) {
+  if (check(p, "linear_attn_bwd_floats") != BF_OK) return -1;
+  return 3 * carry_floats(p);
+}
+
+extern "C" int bf_linear_attn_bwd(const bf_linear_attn* p, const void* q, const void* k, const void* v, const void* dout,
+                                  void* dq, void* dk, void* dv, float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "linear_attn_bwd"));
+  if (p->n == 0) return BF_OK;
+  BF_CHECK_ARG(q && k && v && dout && dq && dk && dv, "linear_attn_bwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, dout, dq, dk, dv}), "linear_attn_bwd: tensors must be 16-byte aligned");
+  const int64_t ds[2] = {int64_t(p->heads) * p->dim_v, p->dim_v};
+  LinArgs pass[3] = {make_args(p), make_args(p), make_args(p)};
+  const int64_t carry = carry_floats(p);
+  BF_CHECK_ARG(carry == 0 || scratch, "linear_attn_bwd: no scratch (bf_linear_attn_bwd_floats)");
+  for (int i = 0; i < 3; ++i) pass[i].carry = scratch + i * carry, pass[i].reverse = i > 0;
+  set_x(pass[0], dout, ds, p->dim_v);                 // dq = (dout, v, k), from the initial state's transpose
+  set_y(pass[0], v, p->v_stride);
+  set_z(pass[0], k, p->k_stride, p->dim_k);
+  pass[0].out = dq;
+  pass[0].init = p->init, pass[0].states = p->init && p->n_seq > 0;
+  pass[0].init_sx = 1, pass[0].init_sz = p->dim_v;
+  set_x(pass[1], v, p->v_stride, p->dim_v);           // dk = reverse (v, dout, q)
+  set_y(pass[1], dout, ds);
+  set_z(pass[1], q, p->q_stride, p->dim_k);
+  pass[1].out = dk;
+  set_x(pass[2], k, p->k_stride, p->dim_k);           // dv = reverse (k, q, dout)
+  set_y(pass[2], q, p->q_stride);
+  set_z(pass[2], dout, ds, p->dim_v);
+  pass[2].out = dv;
+  return run(pass, 3, p->dtype, as_stream(stream));
 }
 
 extern "C" int bf_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state,

@@ -56,7 +56,7 @@ struct Args {
   int32_t tiles, pieces;
   float scale, c;                                  // c = scale * log2(e)
   Div by_group;
-  bool head_major;                                 // neighbouring workgroups take the tiles of one head, not the heads of one tile
+  int32_t xcd_groups;                              // of heads, dealt to the XCDs (place)
 };
 
 struct Row {
@@ -73,22 +73,21 @@ __device__ __forceinline__ int2 span_at(const int2* s, int i) {
   return make_int2(__builtin_amdgcn_readfirstlane(x.x), __builtin_amdgcn_readfirstlane(x.y));
 }
 
-// Which (tile, key head, piece) a workgroup takes. Neighbouring slots share an XCD's L2: by heads (the tiles of a head
-// read the same K and V) or by tiles (the heads of a token share its cache lines). Later tiles first: with a causal
-// mask they see the most keys.
-__device__ __forceinline__ void place(const Args& a, int& tile, int& h, int& piece) {
-  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
+// Which (tile, key head, piece) a workgroup takes; false: none. Workgroup i runs on XCD i % 8, each with an L2 of its own.
+// The heads are dealt to groups of XCDs (as many groups as divide both), a group's heads follow each other, and its XCDs
+// take their tiles in turn: an XCD reads few heads' keys at a time, and each gets its share of a causal mask's long and
+// short tiles, the long ones (later rows) first. One contiguous run of tiles an XCD instead, which shares its keys as
+// well, leaves the XCDs unevenly loaded: 0.49 instead of 0.36 ms forward on one causal sequence of 8192 (16 heads of 128).
+__device__ __forceinline__ bool place(const Args& a, int& tile, int& h, int& piece) {
   const int per = a.tiles * a.pieces;
-  int t;
-  if (a.head_major) {
-    h = int(slot / per);
-    t = int(slot % per);
-  } else {
-    t = int(slot / a.hk);
-    h = int(slot % a.hk);
-  }
+  const int x = blockIdx.x % kXcds, groups = a.xcd_groups, each = kXcds / groups, heads = a.hk / groups;
+  const int64_t at = int64_t(blockIdx.x / kXcds) * each + x % each;
+  if (at >= int64_t(heads) * per) return false;
+  h = x / each * heads + int(at / per);
+  const int t = int(at % per);
   piece = t % a.pieces;
   tile = a.tiles - 1 - t / a.pieces;
+  return true;
 }
 
 // A row's fragments straight from memory (the operand a wave keeps in registers).
@@ -114,15 +113,19 @@ __device__ __forceinline__ void store_cols(O* p, const F32x16 (&acc)[(DP + 31) /
 }
 
 // ---------------------------------------------------------------- forward
+// A row's terms are taken relative to a maximum that is raised only when a score passes it by 2^kLazy: the sums, then
+// up to 2^kLazy times larger, lose nothing in float32, and most tiles skip the rescaling of the accumulators.
+constexpr float kLazy = 6.f;
+
 template <typename T, int DP, int NW, int BN, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void packed_fwd(const Args a) {
+__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void packed_fwd(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BM = 32 * NW;
   __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
   __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   int tile, h, piece;
-  place(a, tile, h, piece);
+  if (!place(a, tile, h, piece)) return;
 
   const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
   const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
@@ -194,8 +197,8 @@ __global__ __launch_bounds__(64 * NW) void packed_fwd(const Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mc_new = fmaxf(mc, top * a.c);
-    if (__any(mc_new > mc)) {
+    float mc_new = fmaxf(mc, top * a.c);
+    if (__any(mc_new > mc + kLazy)) {
       const float alpha = mc_new == -INFINITY ? 1.f : exp2_fast(mc - mc_new);
       l *= alpha;
 #pragma unroll
@@ -215,18 +218,12 @@ __global__ __launch_bounds__(64 * NW) void packed_fwd(const Args a) {
     if (masked && odd) {
 #pragma unroll
       for (int n = 0; n < TL::kBlocks; ++n) {
-        F32x16 up = zero16(), down = zero16();
 #pragma unroll
-        for (int t = 0; t < BN / 16; ++t) {
-          const Frag<T> p = pack8<T>(s[t / 2], t & 1);
-          Frag<T> clean, fu, fd;
-          split_finite<T>(TL::col_frag(v_lds, t, n, lane), clean, fu, fd);
-          o[n] = Mat<T>::mma(clean, p, o[n]);
-          up = Mat<T>::mma(fu, p, up);
-          down = Mat<T>::mma(fd, p, down);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[n][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+        for (int t = 0; t < BN / 16; ++t)
+          o[n] = Mat<T>::mma(finite<T>(TL::col_frag(v_lds, t, n, lane)), pack8<T>(s[t / 2], t & 1), o[n]);
+        add_infinite<BN / 16>(o[n], [&](int t, F32x16 x, float sign) {
+          return Mat<T>::mma(is_infinite<T>(TL::col_frag(v_lds, t, n, lane), sign), pack8<T>(s[t / 2], t & 1), x);
+        });
       }
     } else {
 #pragma unroll
@@ -254,29 +251,29 @@ __global__ __launch_bounds__(64 * NW) void packed_fwd(const Args a) {
   }
 }
 
-// Joins the pieces of a row: one wave a row. out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p.
+// Joins the pieces of a row: one wave a row. out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p. A lane has a piece's
+// statistics (kMaxPieces is a wave); only pieces that hold keys of the row were written and are read.
 template <typename T>
 __global__ __launch_bounds__(256) void packed_join(const float* part, const float* stat, int64_t n_rows, int pieces, int dim,
                                                    T* out, float* lse) {
   const int lane = threadIdx.x & 63;
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= n_rows) return;
-  const float* st = stat + row * pieces * 2;
-  float top = -INFINITY;
-  for (int p = lane; p < pieces; p += 64) top = fmaxf(top, st[2 * p]);
+  const float2 st = lane < pieces ? *reinterpret_cast<const float2*>(stat + (row * pieces + lane) * 2) : make_float2(-INFINITY, 0.f);
+  float top = st.x;
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f, a0 = 0.f, a1 = 0.f;
+  const float w = exp2_fast(st.x - (top == -INFINITY ? 0.f : top));
+  float l = st.y == 0.f ? 0.f : w * st.y;
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o, 64);
   const int d = 2 * lane;
-  for (int p = 0; p < pieces; ++p) {
-    const float m = st[2 * p], lp = st[2 * p + 1];
-    if (lp == 0.f) continue;                              // the piece holds none of the row's keys: nothing was written
-    const float w = exp2_fast(m - base);
-    l = fmaf(w, lp, l);
+  float a0 = 0.f, a1 = 0.f;
+  for (uint64_t left = __ballot(st.y != 0.f); left; left &= left - 1) {
+    const int p = __ffsll((unsigned long long)left) - 1;
+    const float wp = __shfl(w, p, 64);
     if (d < dim) {
       const float2 x = *reinterpret_cast<const float2*>(part + (row * pieces + p) * dim + d);
-      a0 = fmaf(w, x.x, a0);
-      a1 = fmaf(w, x.y, a1);
+      a0 = fmaf(wp, x.x, a0);
+      a1 = fmaf(wp, x.y, a1);
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -297,7 +294,7 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
   __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   int tile, h, piece;
-  place(a, tile, h, piece);
+  if (!place(a, tile, h, piece)) return;
 
   const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
   const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
@@ -377,10 +374,7 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
 #pragma unroll
         for (int n = 0; n < TL::kBlocks; ++n) {
           Frag<T> kt = TL::col_frag(k_lds, 2 * b + t, n, lane);
-          if (masked && odd) {      // a key with such a value has no finite score: the rows that see it get theirs by dS
-            Frag<T> up, down;
-            split_finite<T>(Frag<T>(kt), kt, up, down);
-          }
+          if (masked && odd) kt = finite<T>(kt);      // a key with such a value has no finite score: the rows that see it get theirs by dS
           dq[n] = Mat<T>::mma(kt, f, dq[n]);
         }
       }
@@ -392,7 +386,7 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
 // ---------------------------------------------------------------- backward: dK and dV
 // A wave owns 32 keys (a lane one of them); Q and dO tiles of BR rows pass through LDS with their rows' lse and Delta.
 template <typename T, int DP, int NW, int BR>
-__global__ __launch_bounds__(64 * NW) void packed_bwd_kv(const Args a) {
+__global__ __launch_bounds__(64 * NW, DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2) void packed_bwd_kv(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BK = 32 * NW;
   __shared__ __attribute__((aligned(16))) char q_lds[TL::bytes(BR)];
@@ -400,13 +394,18 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_kv(const Args a) {
   __shared__ __attribute__((aligned(16))) float lse_lds[BR], delta_lds[BR];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   int tile, h, piece;
-  place(a, tile, h, piece);
+  if (!place(a, tile, h, piece)) return;
   tile = a.tiles - 1 - tile;                       // with a causal mask the first keys are seen by the most rows
 
   const int key0 = tile * BK, last = min(key0 + BK, a.n_k) - 1;
   const int2 first_span = span_at(a.key_span, key0), last_span = span_at(a.key_span, last);
   // rows of the group: token * group + head
-  const int rbeg = max(first_span.x, 0) * a.group, rend = min(last_span.y * a.group, a.rows);
+  int rbeg = max(first_span.x, 0) * a.group, rend = min(last_span.y * a.group, a.rows);
+  if (a.pieces > 1) {
+    const int width = int(ceil_div(max(rend - rbeg, 0), a.pieces * BR)) * BR;
+    rbeg = min(rbeg + piece * width, rend);
+    rend = min(rend, rbeg + width);
+  }
   const int w_key0 = key0 + 32 * wave, w_last = min(w_key0 + 31, a.n_k - 1);
   const bool w_any = w_key0 < a.n_k;
   const int2 wf = span_at(a.key_span, min(w_key0, a.n_k - 1)), wl = span_at(a.key_span, w_last);
@@ -499,20 +498,14 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_kv(const Args a) {
       if (masked && odd) {
 #pragma unroll
         for (int n = 0; n < TL::kBlocks; ++n) {
-          F32x16 up = zero16(), down = zero16();
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const Frag<T> pf = pack8<T>(p, t), df = pack8<T>(ds, t);
-            Frag<T> clean, fu, fd;
-            split_finite<T>(TL::col_frag(g_lds, 2 * b + t, n, lane), clean, fu, fd);
-            dv[n] = Mat<T>::mma(clean, pf, dv[n]);
-            up = Mat<T>::mma(fu, pf, up);
-            down = Mat<T>::mma(fd, pf, down);
-            split_finite<T>(TL::col_frag(q_lds, 2 * b + t, n, lane), clean, fu, fd);
-            dk[n] = Mat<T>::mma(clean, df, dk[n]);
+            dv[n] = Mat<T>::mma(finite<T>(TL::col_frag(g_lds, 2 * b + t, n, lane)), pack8<T>(p, t), dv[n]);
+            dk[n] = Mat<T>::mma(finite<T>(TL::col_frag(q_lds, 2 * b + t, n, lane)), pack8<T>(ds, t), dk[n]);
           }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dv[n][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+          add_infinite<2>(dv[n], [&](int t, F32x16 x, float sign) {
+            return Mat<T>::mma(is_infinite<T>(TL::col_frag(g_lds, 2 * b + t, n, lane), sign), pack8<T>(p, t), x);
+          });
         }
       } else {
 #pragma unroll
@@ -529,8 +522,27 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_kv(const Args a) {
   }
   if (!valid) return;
   const int64_t at = (int64_t(key) * a.hk + h) * a.dim;
+  if (a.pieces > 1) {
+    const int64_t all = int64_t(a.n_k) * a.hk * a.dim;
+    store_cols<DP>(a.part + 2 * piece * all + at, dk, a.scale, a.dim, half);
+    store_cols<DP>(a.part + (2 * piece + 1) * all + at, dv, 1.f, a.dim, half);
+    return;
+  }
   store_cols<DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.dim, half);
   store_cols<DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.dim, half);
+}
+
+// Sums the pieces of dK and dV, in their order: 4 values a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void packed_join_kv(const float* part, int64_t all, int pieces, T* dk, T* dv) {
+  const int64_t i = 4 * (int64_t(blockIdx.x) * 256 + threadIdx.x);
+  if (i >= 2 * all) return;
+  float4 s = *reinterpret_cast<const float4*>(part + i);          // dK's and dV's values lie behind each other, as a piece's do
+  for (int p = 1; p < pieces; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(part + 2 * p * all + i);
+    s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+  }
+  store4<T>(i < all ? dk + i : dv + (i - all), s.x, s.y, s.z, s.w);
 }
 
 // ---------------------------------------------------------------- spans
@@ -574,8 +586,9 @@ __global__ __launch_bounds__(256) void packed_spans(const int32_t* q_off, const 
 
 // ---------------------------------------------------------------- launches
 constexpr int kWide = 4;          // waves of a workgroup, each 32 rows (or keys)
-constexpr int kMaxPieces = 64;
+constexpr int kMaxPieces = 64;    // a wave joins them
 
+template <typename T> constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
 template <typename T> constexpr int tile_keys() { return sizeof(T) == 2 ? 64 : 32; }
 
 template <typename F> int with_dim(int dim, F&& f) {
@@ -623,8 +636,16 @@ Args make_args(const bf_packed_attn* p, const void* q, const void* k, const void
   a.c = p->scale * kLog2e;
   a.by_group = make_div(uint32_t(a.group));
   a.pieces = 1;
-  a.head_major = true;
+  a.xcd_groups = 1;
+  while (a.xcd_groups < kXcds && a.hk % (2 * a.xcd_groups) == 0) a.xcd_groups *= 2;
   return a;
+}
+
+// Workgroups that cover every (tile, key head, piece).
+dim3 grid_of(const Args& a) {
+  const int64_t per = int64_t(a.tiles) * a.pieces;
+  const int64_t each = kXcds / a.xcd_groups;
+  return dim3(unsigned(ceil_div(a.hk / a.xcd_groups * per, each) * kXcds));
 }
 
 // Pieces a tile's keys are cut into. Workgroups of 4 waves over whole rows fill the chip (256 CUs, two workgroups each)
@@ -636,6 +657,18 @@ int pieces_of(const bf_packed_attn* p) {
   const int64_t want = ceil_div(2048, tiles);
   const int64_t most = ceil_div(p->n_k, 64);
   int64_t n = want < most ? want : most;
+  if (n > kMaxPieces) n = kMaxPieces;
+  return n < 1 ? 1 : int(n);
+}
+
+// Pieces a key tile's rows are cut into (float32 partial sums, joined in order): where the key tiles are too few to fill
+// the chip, or too few to even out what a causal mask gives the first and the last of them.
+int kv_pieces_of(const bf_packed_attn* p) {
+  const int64_t rows = p->n_q * (p->heads_q / p->heads_k);
+  const int64_t groups = ceil_div(p->n_k, 32 * kWide) * p->heads_k;
+  if (groups >= 512 || groups == 0) return 1;
+  int64_t n = ceil_div(1024, groups);
+  if (n > rows / 512) n = rows / 512;
   if (n > kMaxPieces) n = kMaxPieces;
   return n < 1 ? 1 : int(n);
 }
@@ -683,7 +716,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
       return with_dim(a.dim, [&](auto dp) -> int {
         constexpr int DP = decltype(dp)::value, BN = tile_keys<T>();
         auto kern = packed_fwd<T, DP, kWide, BN, false>;
-        BF_LAUNCH("packed_attn_fwd", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        BF_LAUNCH("packed_attn_fwd", kern, grid_of(a), dim3(64 * kWide), 0, st, a);
         BF_CHECK_LAUNCH();
         return BF_OK;
       });
@@ -699,7 +732,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
     return with_dim(a.dim, [&](auto dp) -> int {
       constexpr int DP = decltype(dp)::value;
       auto kern = packed_fwd<T, DP, 1, 32, true>;
-      BF_LAUNCH("packed_attn_fwd_pieces", kern, dim3(unsigned(int64_t(a.tiles) * a.hk * a.pieces)), dim3(64), 0, st, a);
+      BF_LAUNCH("packed_attn_fwd_pieces", kern, grid_of(a), dim3(64), 0, st, a);
       BF_CHECK_LAUNCH();
       BF_LAUNCH("packed_attn_join", (packed_join<T>), dim3(unsigned(ceil_div(n_rows, 4))), dim3(256), 0, st, a.part, a.stat,
                 n_rows, a.pieces, a.dim, static_cast<T*>(out), lse);
@@ -709,9 +742,15 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
   });
 }
 
+extern "C" int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p) {
+  if (check(p, "packed_attn_bwd_floats", true) != BF_OK) return -1;
+  const int n = kv_pieces_of(p);
+  return n == 1 ? 0 : 2 * p->n_k * p->heads_k * p->head_dim * n;
+}
+
 extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
                                   const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta,
-                                  void* stream) {
+                                  float* scratch, void* stream) {
   BF_CHECK_OK(check(p, "packed_attn_bwd", true));
   BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
                "packed_attn_bwd: bad arguments");
@@ -727,14 +766,23 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
       if (a.rows > 0) {
         a.tiles = int(ceil_div(a.rows, 32 * kWide));
         auto kern = packed_bwd_q<T, DP, kWide, 32>;
-        BF_LAUNCH("packed_attn_bwd_q", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * kWide), 0, st, a);
         BF_CHECK_LAUNCH();
       }
       if (a.n_k > 0) {
         a.tiles = int(ceil_div(a.n_k, 32 * kWide));
-        auto kern = packed_bwd_kv<T, DP, kWide, 32>;
-        BF_LAUNCH("packed_attn_bwd_kv", kern, dim3(unsigned(int64_t(a.tiles) * a.hk)), dim3(64 * kWide), 0, st, a);
+        a.pieces = kv_pieces_of(p);
+        a.part = scratch;
+        BF_CHECK_ARG(a.pieces == 1 || scratch, "packed_attn_bwd: no scratch (bf_packed_attn_bwd_floats)");
+        auto kern = packed_bwd_kv<T, DP, kWide, tile_rows<T>()>;
+        BF_LAUNCH("packed_attn_bwd_kv", kern, grid_of(a), dim3(64 * kWide), 0, st, a);
         BF_CHECK_LAUNCH();
+        if (a.pieces > 1) {
+          const int64_t all = p->n_k * p->heads_k * p->head_dim;
+          BF_LAUNCH("packed_attn_join_kv", (packed_join_kv<T>), dim3(unsigned(ceil_div(2 * all, 1024))), dim3(256), 0, st,
+                    a.part, all, a.pieces, static_cast<T*>(dk), static_cast<T*>(dv));
+          BF_CHECK_LAUNCH();
+        }
       }
       return BF_OK;
     });

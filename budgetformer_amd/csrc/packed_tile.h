@@ -97,17 +97,36 @@ template <typename T, typename X> __device__ __forceinline__ Frag<T> pack8(const
   return f;
 }
 
-// The finite values of a fragment, and indicators (1 or 0) of +inf or NaN, and of -inf or NaN.
-template <typename T>
-__device__ __forceinline__ void split_finite(const Frag<T>& f, Frag<T>& clean, Frag<T>& up, Frag<T>& down) {
+// A fragment's finite values, the others as 0.
+template <typename T> __device__ __forceinline__ Frag<T> finite(const Frag<T>& f) {
+  Frag<T> o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = fabsf(float(f[j])) < INFINITY ? f[j] : T(0.f);
+  return o;
+}
+
+// 1 where a fragment holds an infinity of this sign or a NaN, else 0.
+template <typename T> __device__ __forceinline__ Frag<T> is_infinite(const Frag<T>& f, float sign) {
+  Frag<T> o;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float x = float(f[j]);
-    const bool nan = x != x;
-    const bool hi = nan || x == INFINITY, lo = nan || x == -INFINITY;
-    clean[j] = hi || lo ? T(0.f) : f[j];
-    up[j] = T(hi ? 1.f : 0.f);
-    down[j] = T(lo ? 1.f : 0.f);
+    const float x = float(f[j]) * sign;
+    o[j] = T(x < INFINITY ? 0.f : 1.f);
+  }
+  return o;
+}
+
+// What infinite values add to a product of weights that are not negative: mma(t, x, sign) multiplies the indicators of
+// that sign in step t; where their sum is positive an infinity of that sign is added (of both: a NaN).
+template <int STEPS, typename F> __device__ __forceinline__ void add_infinite(F32x16& acc, F&& mma) {
+#pragma unroll
+  for (int way = 0; way < 2; ++way) {
+    const float sign = way ? -1.f : 1.f;
+    F32x16 x = zero16();
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) x = mma(t, x, sign);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] += x[r] > 0.f ? sign * INFINITY : 0.f;
   }
 }
 

@@ -595,10 +595,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor&
                     out.sizes(), ", dout ", dout.sizes(), " or lse ", lse.sizes(), " do not match q ", q.sizes());
   const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
   at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
-  at::Tensor delta = at::empty_like(lse);
+  at::Tensor delta = at::empty_like(lse), scratch;
+  const int64_t floats = bf_packed_attn_bwd_floats(&p);
+  if (floats > 0) scratch = at::empty({floats}, lse.options());
   check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
                               dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(),
-                              stream_of(q)),
+                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
            "bf::packed_attn_bwd");
   return {dq, dk, dv};
 }
@@ -638,57 +640,78 @@ std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& x, const std::option
   return {ox, oy};
 }
 
-// One pass of linear attention (bf_linear_attn_pass): (out, final state float32 [n_seq, heads, dim_x, dim_z] or empty).
-// init_state float32 [n_seq, heads, dim_x, dim_z], of any strides over the last two dimensions.
-std::tuple<at::Tensor, at::Tensor> linear_attn_pass(const at::Tensor& x, const at::Tensor& y, const at::Tensor& z,
-                                                    const at::Tensor& log_decay, const at::Tensor& row_span,
-                                                    const at::Tensor& key_span, const at::Tensor& offsets, double scale,
-                                                    bool reverse, const std::optional<at::Tensor>& init_state,
-                                                    bool return_state) {
-  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a device tensor (got ", x.device(), ")");
-  const c10::DeviceGuard guard(x.device());
-  const at::Device dev = x.device();
+bf_linear_attn linear_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                           const at::Tensor& row_span, const at::Tensor& key_span, const at::Tensor& offsets, double scale,
+                           const std::optional<at::Tensor>& init_state) {
+  const at::Device dev = q.device();
   bf_linear_attn p{};
-  p.dtype = dtype_code(x);
-  require_heads(x, "x", x.scalar_type(), dev, p.x_stride);
-  require_heads(y, "y", x.scalar_type(), dev, p.y_stride);
-  require_heads(z, "z", x.scalar_type(), dev, p.z_stride);
-  TORCH_CHECK_VALUE(x.sizes() == y.sizes() && z.size(0) == x.size(0) && z.size(1) == x.size(1), "x ", x.sizes(), ", y ",
-                    y.sizes(), ", z ", z.sizes(), " disagree");
-  TORCH_CHECK_VALUE(x.size(1) < (int64_t(1) << 30) && x.size(2) < (int64_t(1) << 30) && z.size(2) < (int64_t(1) << 30),
-                    "linear_attn_pass: bad sizes");
-  const int64_t T = x.size(0), H = x.size(1), dx = x.size(2), dz = z.size(2);
+  p.dtype = dtype_code(q);
+  require_heads(q, "q", q.scalar_type(), dev, p.q_stride);
+  require_heads(k, "k", q.scalar_type(), dev, p.k_stride);
+  require_heads(v, "v", q.scalar_type(), dev, p.v_stride);
+  TORCH_CHECK_VALUE(q.sizes() == k.sizes() && v.size(0) == q.size(0) && v.size(1) == q.size(1), "q ", q.sizes(), ", k ",
+                    k.sizes(), ", v ", v.sizes(), " disagree");
+  TORCH_CHECK_VALUE(q.size(1) < (int64_t(1) << 30) && q.size(2) < (int64_t(1) << 30) && v.size(2) < (int64_t(1) << 30),
+                    "linear_attn: bad sizes");
+  const int64_t T = q.size(0), H = q.size(1), dk = q.size(2), dv = v.size(2);
   require(log_decay, "log_decay", at::kFloat, dev);
   TORCH_CHECK_VALUE(log_decay.dim() == 1 && log_decay.size(0) == H, "log_decay must be [", H, "] (got ", log_decay.sizes(), ")");
   require_span(row_span, "row_span", T, dev);
   require_span(key_span, "key_span", T, dev);
   require(offsets, "offsets", at::kInt, dev);
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must be [n_seq + 1]");
-  const int64_t n_seq = offsets.numel() - 1;
-  p.n = T, p.n_seq = n_seq, p.heads = int32_t(H), p.dim_x = int32_t(dx), p.dim_z = int32_t(dz);
+  p.n = T, p.n_seq = offsets.numel() - 1, p.heads = int32_t(H), p.dim_k = int32_t(dk), p.dim_v = int32_t(dv);
   p.row_span = row_span.data_ptr<int32_t>(), p.key_span = key_span.data_ptr<int32_t>();
   p.offsets = offsets.data_ptr<int32_t>(), p.log_decay = log_decay.data_ptr<float>();
-  p.scale = float(scale), p.reverse = reverse ? 1 : 0;
+  p.scale = float(scale);
   if (init_state.has_value() && init_state->defined()) {
-    const at::Tensor& s = *init_state;
-    TORCH_CHECK_VALUE(s.device() == dev && s.scalar_type() == at::kFloat, "init_state must be float32 on ", dev);
-    TORCH_CHECK_VALUE(s.dim() == 4 && s.size(0) == n_seq && s.size(1) == H && s.size(2) == dx && s.size(3) == dz,
-                      "init_state must be [", n_seq, ", ", H, ", ", dx, ", ", dz, "] (got ", s.sizes(), ")");
-    TORCH_CHECK_VALUE(s.numel() == 0 || ((s.size(0) == 1 || s.stride(0) == H * dx * dz) && (H == 1 || s.stride(1) == dx * dz)),
-                      "init_state must be contiguous over sequences and heads");
-    p.init = s.data_ptr<float>();
-    p.init_stride[0] = s.stride(2), p.init_stride[1] = s.stride(3);
+    require(*init_state, "init_state", at::kFloat, dev);
+    TORCH_CHECK_VALUE(init_state->sizes() == at::IntArrayRef({p.n_seq, H, dk, dv}), "init_state must be [", p.n_seq, ", ", H,
+                      ", ", dk, ", ", dv, "] (got ", init_state->sizes(), ")");
+    p.init = init_state->data_ptr<float>();
   }
-  at::Tensor out = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
-  at::Tensor final_state = return_state ? at::empty({n_seq, H, dx, dz}, log_decay.options()) : at::empty({0}, log_decay.options());
-  if (return_state) p.final_state = final_state.data_ptr<float>();
-  const int64_t floats = bf_linear_attn_floats(&p);
-  at::Tensor scratch;
+  return p;
+}
+
+// Forward (bf_linear_attn_fwd): (out, final state float32 [n_seq, heads, dim_k, dim_v], or empty without return_state).
+std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                   const at::Tensor& log_decay, const at::Tensor& row_span,
+                                                   const at::Tensor& key_span, const at::Tensor& offsets, double scale,
+                                                   const std::optional<at::Tensor>& init_state, bool return_state) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const c10::DeviceGuard guard(q.device());
+  bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
+  at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), scratch;
+  at::Tensor state = return_state ? at::empty({p.n_seq, p.heads, p.dim_k, p.dim_v}, log_decay.options())
+                                  : at::empty({0}, log_decay.options());
+  if (return_state) p.final_state = state.data_ptr<float>();
+  const int64_t floats = bf_linear_attn_fwd_floats(&p);
   if (floats > 0) scratch = at::empty({floats}, log_decay.options());
-  check_rc(bf_linear_attn_pass(&p, x.data_ptr(), y.data_ptr(), z.data_ptr(), out.data_ptr(),
-                               floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(x)),
-           "bf::linear_attn_pass");
-  return {out, final_state};
+  check_rc(bf_linear_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
+           "bf::linear_attn_fwd");
+  return {out, state};
+}
+
+// Backward (bf_linear_attn_bwd): (dq, dk, dv), contiguous.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                               const at::Tensor& log_decay, const at::Tensor& row_span,
+                                                               const at::Tensor& key_span, const at::Tensor& offsets,
+                                                               const at::Tensor& dout, double scale,
+                                                               const std::optional<at::Tensor>& init_state) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const c10::DeviceGuard guard(q.device());
+  const bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
+  require(dout, "dout", q.scalar_type(), q.device());
+  TORCH_CHECK_VALUE(dout.sizes() == v.sizes(), "dout ", dout.sizes(), " does not match v ", v.sizes());
+  const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain), scratch;
+  const int64_t floats = bf_linear_attn_bwd_floats(&p);
+  if (floats > 0) scratch = at::empty({floats}, log_decay.options());
+  check_rc(bf_linear_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                              dv.data_ptr(), floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
+           "bf::linear_attn_bwd");
+  return {dq, dk, dv};
 }
 
 // One token of each sequence (bf_linear_attn_step): (out, new state); out_state: where the new state goes (state itself
@@ -756,9 +779,10 @@ TORCH_LIBRARY(bf, m) {
         "Tensor dout, float scale) -> (Tensor, Tensor, Tensor)");
   m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
         "bool inverse=False) -> (Tensor, Tensor)");
-  m.def("linear_attn_pass(Tensor x, Tensor y, Tensor z, Tensor log_decay, Tensor row_span, Tensor key_span, "
-        "Tensor offsets, float scale, bool reverse=False, Tensor? init_state=None, bool return_state=False) "
-        "-> (Tensor, Tensor)");
+  m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
+        "float scale, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
+  m.def("linear_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
+        "Tensor dout, float scale, Tensor? init_state=None) -> (Tensor, Tensor, Tensor)");
   m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor state, float scale, "
         "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
 }
@@ -778,6 +802,7 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
   m.impl("packed_attn_fwd", &packed_attn_fwd);
   m.impl("packed_attn_bwd", &packed_attn_bwd);
   m.impl("rotary", &rotary);
-  m.impl("linear_attn_pass", &linear_attn_pass);
+  m.impl("linear_attn_fwd", &linear_attn_fwd);
+  m.impl("linear_attn_bwd", &linear_attn_bwd);
   m.impl("linear_attn_step", &linear_attn_step);
 }

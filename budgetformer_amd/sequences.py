@@ -279,12 +279,12 @@ def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optio
 
 # ------------------------------------------------------------------ linear attention
 class _LinearAttention(torch.autograd.Function):
-    """out and the final state (not differentiable); each gradient is a pass of the same kernel."""
+    """out and the final state (not differentiable); the gradients are passes of the same form."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, seqs, scale, initial_state, return_state):
-        out, state = N.load_ops().linear_attn_pass(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
-                                                   False, initial_state, return_state)
+        out, state = N.load_ops().linear_attn_fwd(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
+                                                  initial_state, return_state)
         ctx.save_for_backward(q, k, v, log_decay, initial_state)
         ctx.seqs, ctx.scale = seqs, scale
         ctx.mark_non_differentiable(state)
@@ -296,16 +296,10 @@ class _LinearAttention(torch.autograd.Function):
         if dout is None:
             return (None,) * 8
         q, k, v, log_decay, init = ctx.saved_tensors
-        s, dout = ctx.seqs, _dense(dout)
-        init = None if init is None else init.transpose(2, 3)
-
-        def one(x, y, z, reverse, state=None):
-            return N.load_ops().linear_attn_pass(x, y, z, log_decay, s.row_span, s.key_span, s.q_offsets, ctx.scale, reverse,
-                                                 state, False)[0]
-
-        need = ctx.needs_input_grad
-        return (one(dout, v, k, False, init) if need[0] else None, one(v, dout, q, True) if need[1] else None,
-                one(k, q, dout, True) if need[2] else None, None, None, None, None, None)
+        s = ctx.seqs
+        dq, dk, dv = N.load_ops().linear_attn_bwd(q, k, v, log_decay, s.row_span, s.key_span, s.q_offsets, _dense(dout),
+                                                  ctx.scale, init)
+        return dq, dk, dv, None, None, None, None, None
 
 
 def _decays(log_decay, q) -> torch.Tensor:

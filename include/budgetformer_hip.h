@@ -826,9 +826,12 @@ int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, co
                        float* scratch, void* stream);
 /* Gradients of it: dq like out, dk and dv contiguous [n_k, heads_k, head_dim]
  * (summed over the heads of a group). out, dout: contiguous. delta: scratch of
- * n_q * heads_q floats. No atomics: results repeat bit for bit.             */
+ * n_q * heads_q floats; scratch: bf_packed_attn_bwd_floats(p) floats (0: none
+ * needed; -1: bad arguments). No atomics: results repeat bit for bit.       */
+int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p);
 int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
-                       const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, void* stream);
+                       const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, float* scratch,
+                       void* stream);
 
 /* Rotary positions: the first `rot` values of every head of x and y (rows of
  * `dim` values; y may be NULL with heads_y 0) turned pair by pair by the angle
@@ -844,36 +847,38 @@ int bf_rotary(const void* x, const void* y, int64_t n, int32_t heads_x, int32_t 
               void* stream);
 
 /* Linear attention with a decay for each head, over causal packed sequences:
- *   out_i = scale sum_{j <= i, same sequence} g^(i - j) (x_i . y_j) z_j
- * with g = exp(log_decay[h]); with `reverse` over j >= i and g^(j - i): the
- * gradients of out(q, k, v) are dq = (dout, v, k), dk = reverse (v, dout, q)
- * and dv = reverse (k, q, dout). x, y: [n, heads, dim_x]; z: [n, heads, dim_z];
- * out contiguous [n, heads, dim_z]; strides as in bf_packed_attn. dims: a
- * multiple of 8 up to 128. row_span / key_span: bf_packed_spans with causal and
+ *   out_i = scale sum_{j <= i, same sequence} g^(i - j) (q_i . k_j) v_j
+ * with g = exp(log_decay[h]). q, k: [n, heads, dim_k]; v: [n, heads, dim_v];
+ * out contiguous [n, heads, dim_v]; strides as in bf_packed_attn. dims: a
+ * multiple of 8 up to 128. row_span, key_span: bf_packed_spans with causal and
  * the same offsets for rows and keys.
- * init (or NULL): float32 [n_seq, heads, ...], each sequence's state before its
- * first token, value (a, b) of [dim_x][dim_z] at a * init_stride[0] + b *
- * init_stride[1]; final (or NULL): float32 [n_seq, heads, dim_x, dim_z], the
- * state sum_j g^(n - 1 - j) y_j z_j^T + g^n init behind its last. Neither with
- * reverse. offsets (int32 [n_seq + 1]) is read only with one of them.
- * scratch: bf_linear_attn_floats(p) floats (0: none; -1: bad arguments).    */
+ * init (or NULL): float32 [n_seq, heads, dim_k, dim_v], each sequence's state
+ * before its first token; final_state (or NULL, forward only): the state
+ * sum_j g^(n - 1 - j) k_j v_j^T + g^n init behind its last. offsets (int32
+ * [n_seq + 1]) is read only with one of them.                               */
 typedef struct bf_linear_attn {
   int64_t n, n_seq;
-  int32_t heads, dim_x, dim_z, dtype;
-  int64_t x_stride[2], y_stride[2], z_stride[2];
+  int32_t heads, dim_k, dim_v, dtype;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
   const int32_t* row_span;
   const int32_t* key_span;
   const int32_t* offsets;
   const float* log_decay;     /* float32 [heads], <= 0 expected              */
   const float* init;
   float* final_state;
-  int64_t init_stride[2];
   float scale;
-  int32_t reverse;
+  int32_t reserved;           /* 0                                           */
 } bf_linear_attn;
-int64_t bf_linear_attn_floats(const bf_linear_attn* p);
-int bf_linear_attn_pass(const bf_linear_attn* p, const void* x, const void* y, const void* z, void* out, float* scratch,
-                        void* stream);
+/* scratch: the *_floats call's floats (0: none needed; -1: bad arguments). The
+ * gradients are passes of the same form, dq = (dout, v, k) and, on the axis
+ * read backwards, dk = (v, dout, q) and dv = (k, q, dout); contiguous, as dout
+ * is. The decays and states are constants.                                  */
+int64_t bf_linear_attn_fwd_floats(const bf_linear_attn* p);
+int bf_linear_attn_fwd(const bf_linear_attn* p, const void* q, const void* k, const void* v, void* out, float* scratch,
+                       void* stream);
+int64_t bf_linear_attn_bwd_floats(const bf_linear_attn* p);
+int bf_linear_attn_bwd(const bf_linear_attn* p, const void* q, const void* k, const void* v, const void* dout, void* dq,
+                       void* dk, void* dv, float* scratch, void* stream);
 /* One token of each of n sequences: new_state = g state + k v^T, out = scale q
  * new_state. q, k [n, heads, dim_k], v, out [n, heads, dim_v], states float32
  * [n, heads, dim_k, dim_v], all contiguous; new_state may be state. dims as

@@ -55,7 +55,7 @@ def test_packed_attention_addresses_and_strides():
     with pytest.raises(ValueError, match="bad arguments"):
         _fwd(_attn(), q=None)
     with pytest.raises(ValueError, match="no key spans"):
-        N.call("bf_packed_attn_bwd", C.byref(_attn(key_span=None)), P, P, P, P, P, P, P, P, P, P, None)
+        N.call("bf_packed_attn_bwd", C.byref(_attn(key_span=None)), P, P, P, P, P, P, P, P, P, P, P, None)
     _fwd(_attn(n_q=0))                                       # nothing to do, nothing launched
 
 
@@ -80,9 +80,9 @@ def test_rotary_arguments():
 
 
 def _lin(**kw):
-    a = N.LinearAttn(n=4, n_seq=1, heads=2, dim_x=16, dim_z=16, dtype=N.BF_DTYPE_F32, row_span=P, key_span=P, offsets=P,
+    a = N.LinearAttn(n=4, n_seq=1, heads=2, dim_k=16, dim_v=16, dtype=N.BF_DTYPE_F32, row_span=P, key_span=P, offsets=P,
                      log_decay=P, scale=1.0)
-    a.x_stride[:], a.y_stride[:], a.z_stride[:] = (32, 16), (32, 16), (32, 16)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = (32, 16), (32, 16), (32, 16)
     for name, value in kw.items():
         setattr(a, name, value)
     return a
@@ -90,19 +90,22 @@ def _lin(**kw):
 
 def test_linear_attention_arguments():
     def call(a, x=P):
-        N.call("bf_linear_attn_pass", C.byref(a), x, P, P, P, P, None)
+        N.call("bf_linear_attn_fwd", C.byref(a), x, P, P, P, P, None)
 
     for kw, match in ((dict(dtype=5), "dtype"), (dict(n=-1), "sizes"), (dict(heads=0), "sizes"), (dict(n=2 ** 31), "sizes"),
                       (dict(log_decay=None), "decays"), (dict(row_span=None), "spans"), (dict(scale=float("nan")), "scale"),
-                      (dict(init=P, reverse=1), "states"), (dict(final_state=P, offsets=None), "states")):
+                      (dict(init=P, offsets=None), "states"), (dict(final_state=P, offsets=None), "states")):
         with pytest.raises(ValueError, match=match):
             call(_lin(**kw))
-        assert N.load().bf_linear_attn_floats(C.byref(_lin(**kw))) == -1
+        assert N.load().bf_linear_attn_fwd_floats(C.byref(_lin(**kw))) == -1
+        assert N.load().bf_linear_attn_bwd_floats(C.byref(_lin(**kw))) == -1
+        with pytest.raises(ValueError, match=match):
+            N.call("bf_linear_attn_bwd", C.byref(_lin(**kw)), P, P, P, P, P, P, P, P, None)
     for d in (4, 20, 136):
         with pytest.raises(NotImplementedError, match="head dims"):
-            call(_lin(dim_x=d))
+            call(_lin(dim_k=d))
         with pytest.raises(NotImplementedError, match="head dims"):
-            call(_lin(dim_z=d))
+            call(_lin(dim_v=d))
         with pytest.raises(NotImplementedError, match="head dims"):
             N.call("bf_linear_attn_step", P, P, P, P, P, 1, 1, d, 16, 0, 1.0, P, P, None)
     with pytest.raises(ValueError, match="aligned"):
@@ -143,7 +146,7 @@ def test_host_tensors_and_bad_lengths_are_refused():
 
 def test_operators_are_registered():
     ops = N.load_ops()
-    for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_pass", "linear_attn_step"):
+    for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_fwd", "linear_attn_bwd", "linear_attn_step"):
         assert str(getattr(ops, name).default._schema).startswith(f"bf::{name}(")
 
 
