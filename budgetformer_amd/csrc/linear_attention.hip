@@ -54,12 +54,11 @@ template <typename T> constexpr int lin_tile() { return sizeof(T) == 2 ? 64 : 32
 // log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
 __device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
 
-// the token at a place of the axis as the pass reads it, and where its sequence starts there
+// the token at a place of the axis as the pass reads it, its span, and where its sequence starts on that axis
 __device__ __forceinline__ int token_at(const LinArgs& a, int p) { return a.reverse ? a.n - 1 - p : p; }
-__device__ __forceinline__ int start_at(const LinArgs& a, int p) {
-  const int t = token_at(a, p);
-  if (a.reverse) return a.n - a.key_span[t].y;        // behind the last sequence: after p
-  const int2 s = a.row_span[t];
+__device__ __forceinline__ int2 span_at(const LinArgs& a, int p) { return (a.reverse ? a.key_span : a.row_span)[token_at(a, p)]; }
+__device__ __forceinline__ int start_of(const LinArgs& a, int2 s) {
+  if (a.reverse) return a.n - s.y;                     // behind the last sequence: after its own place
   return s.y > s.x ? s.x : a.n;                        // a row behind the last sequence sees nothing
 }
 
@@ -85,8 +84,10 @@ __device__ __forceinline__ int fresh(int x) {
 
 template <typename T, int DX, int DZ, bool OUT>
 __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
-  const LinArgs& a = all.role[blockIdx.y];
+  const LinArgs a = all.role[blockIdx.y];
   constexpr int C = lin_tile<T>(), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
+  // parts of the decayed z (see below): the third only for a state that goes out
+  const bool third = a.final_state != nullptr;
   constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, __bf16>::value ? 3 : 2;
   using TX = Tile<T, DX>;
   using TZ = Tile<T, DZ>;
@@ -96,14 +97,19 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   __shared__ __attribute__((aligned(16))) char z_lds[TZ::bytes(C)];
   __shared__ __attribute__((aligned(16))) char w_lds[OUT ? TW::bytes(C) : 16];
   __shared__ int start_lds[C];
+  __shared__ __attribute__((aligned(16))) float power[C];       // g^0 .. g^(C - 1), last first: a tile's weights towards its end
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
   const int h = int(slot % a.heads), seg = int(slot / a.heads);     // the heads of a token share its cache lines
   const int begin = seg * a.seg_len, end = min(begin + a.seg_len, a.n);
   const float ld = decay_log2(a, h);
-  const T* xp = static_cast<const T*>(a.x) + h * a.xs_h;
-  const T* yp = static_cast<const T*>(a.y) + h * a.ys_h;
-  const T* zp = static_cast<const T*>(a.z) + h * a.zs_h;
+  // the axis as the pass reads it: from the last token with steps back, or from the first
+  const int64_t back = a.reverse ? a.n - 1 : 0;
+  const T* xp = static_cast<const T*>(a.x) + h * a.xs_h + back * a.xs_t;
+  const T* yp = static_cast<const T*>(a.y) + h * a.ys_h + back * a.ys_t;
+  const T* zp = static_cast<const T*>(a.z) + h * a.zs_h + back * a.zs_t;
+  const int64_t xs_t = a.reverse ? -a.xs_t : a.xs_t, ys_t = a.reverse ? -a.ys_t : a.ys_t, zs_t = a.reverse ? -a.zs_t : a.zs_t;
+  const int2* spans = a.reverse ? a.key_span : a.row_span;
 
   F32x16 m[XB];
 #pragma unroll
@@ -115,37 +121,45 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) m[b][r] = carry[(int64_t(b) * NW * 16 + r) * 64];
   }
-  int seq = a.states ? sequence_of(a, begin) : 0;
-  auto tile_end = [&](int t0) {
-    const int e = min(t0 + C, end);
-    return a.states && seq < a.n_seq ? min(e, seq < 0 ? a.offsets[0] : a.offsets[seq + 1]) : e;
+  // with states: the sequence of the next tile and its bounds (read again only where one ends)
+  int seq = a.states ? sequence_of(a, begin) : -1, seq_begin = -1, seq_end = a.n;
+  auto bounds = [&]() {
+    const bool in = seq >= 0 && seq < a.n_seq;
+    seq_begin = in ? a.offsets[seq] : -1;
+    seq_end = seq < a.n_seq ? a.offsets[seq + 1] : a.n;
   };
+  if (a.states) bounds();
+  auto tile_end = [&](int t0) { return min(min(t0 + C, end), seq_end); };
 
   Stage<T, DX, C, NT> xs, ys;
   Stage<T, DZ, C, NT> zs;
-  int start = 0;
+  int2 span = make_int2(0, 0);
   auto fetch = [&](int t0, int t1) {
-    if constexpr (OUT) xs.load(tid, a.dx, [&](int r) { return t0 + r < t1 ? xp + token_at(a, t0 + r) * a.xs_t : nullptr; });
-    ys.load(tid, a.dx, [&](int r) { return t0 + r < t1 ? yp + token_at(a, t0 + r) * a.ys_t : nullptr; });
-    zs.load(tid, a.dz, [&](int r) { return t0 + r < t1 ? zp + token_at(a, t0 + r) * a.zs_t : nullptr; });
-    if (tid < C) start = start_at(a, min(t0 + tid, t1 - 1));
+    if constexpr (OUT) xs.load(tid, t1 - t0, a.dx, [&](int r) { return xp + (t0 + r) * xs_t; });
+    ys.load(tid, t1 - t0, a.dx, [&](int r) { return yp + (t0 + r) * ys_t; });
+    zs.load(tid, t1 - t0, a.dz, [&](int r) { return zp + (t0 + r) * zs_t; });
+    if (tid < C) span = spans[token_at(a, min(t0 + tid, t1 - 1))];      // not looked at before the tile is stored: nothing waits here
   };
 
+  if (tid < C) power[tid] = exp2_fast(ld * float(C - 1 - tid));
   int t1 = begin < end ? tile_end(begin) : begin;
   if (begin < end) fetch(begin, t1);
   for (int t0 = begin; t0 < end;) {
+    const int len = t1 - t0;
+    if constexpr (OUT) xs.clip(tid, len, a.dx);
+    ys.clip(tid, len, a.dx);
+    zs.clip(tid, len, a.dz);
     __syncthreads();
     if constexpr (OUT) xs.store(tid, x_lds);
     ys.store(tid, y_lds);
     zs.store(tid, z_lds);
-    if (tid < C) start_lds[tid] = start;
+    if (tid < C) start_lds[tid] = start_of(a, span);
     bool odd = false;
     if constexpr (OUT)
       odd = __syncthreads_or(zs.tainted());
     else
       __syncthreads();
-    const int len = t1 - t0;
-    if (a.states && seq >= 0 && seq < a.n_seq && t0 == a.offsets[seq]) {          // a sequence begins with its tile
+    if (t0 == seq_begin) {                                  // with states: a sequence begins with its tile
       const int z = fresh(32 * wave + col), x0 = fresh(4 * half);
       const float* s0 = a.init ? a.init + (int64_t(seq) * a.heads + h) * a.dx * a.dz : nullptr;
 #pragma unroll
@@ -153,13 +167,16 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int x = x0 + 32 * b + acc_row(r, 0);
-          m[b][r] = s0 && x < a.dx && z < a.dz ? s0[x * a.init_sx + z * a.init_sz] : 0.f;
+          const float v = s0 ? s0[min(x, a.dx - 1) * a.init_sx + min(z, a.dz - 1) * a.init_sz] : 0.f;
+          m[b][r] = x < a.dx && z < a.dz ? v : 0.f;
         }
     }
-    const bool ends = a.states && seq >= 0 && seq < a.n_seq && t1 == a.offsets[seq + 1];
+    const bool ends = seq_begin >= 0 && t1 == seq_end;
     const int this_seq = seq;
-    if (a.states && t1 < end)
+    if (a.states && t1 == seq_end && t1 < end) {
       while (seq < a.n_seq && a.offsets[seq + 1] <= t1) ++seq;
+      bounds();
+    }
     const int next = t1 < end ? tile_end(t1) : t1;
     if (t1 < end) fetch(t1, next);
 
@@ -269,7 +286,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int j = 16 * t + acc_row(k, half);
-          float x = j >= from && j < len ? float(z0[k]) * exp2_fast(ld * float(len - 1 - j)) : 0.f;
+          float x = j >= from && j < len ? float(z0[k]) * power[min(j + C - len, C - 1)] : 0.f;
 #pragma unroll
           for (int n = 0; n < kParts; ++n) {
             part[n][k] = T(x);
@@ -285,7 +302,8 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
               if (16 * t + acc_row(k, half) < from) yf[k] = T(0.f);
           }
 #pragma unroll
-          for (int n = 0; n < kParts; ++n) m[b] = Mat<T>::mma(yf, part[n], m[b]);
+          for (int n = 0; n < kParts; ++n)
+            if (n < 2 || third) m[b] = Mat<T>::mma(yf, part[n], m[b]);
         }
       }
       if (OUT && ends && a.final_state) {
@@ -328,7 +346,7 @@ __global__ __launch_bounds__(256) void linear_carry(const LinRoles all, int64_t 
     for (int k = 0; k < 8; ++k) {
       const int s = s0 + k, e = (s + 1) * a.seg_len;
       mine[k] = s < a.n_seg ? c[s * step] : 0.f;
-      began[k] = s + 1 < a.n_seg && start_at(a, e - 1) >= e - a.seg_len;     // the segment's last sequence began in it
+      began[k] = s + 1 < a.n_seg && start_of(a, span_at(a, e - 1)) >= e - a.seg_len;     // the segment's last sequence began in it
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

@@ -156,11 +156,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
   const T* vp = static_cast<const T*>(a.v) + h * a.vs_h;
   Stage<T, DP, BN, NT> ks, vs;
   auto fetch = [&](int j0) {
-    ks.load(tid, a.dim, [&](int r) { return j0 + r < kend ? kp + (j0 + r) * a.ks_t : nullptr; });
-    vs.load(tid, a.dim, [&](int r) { return j0 + r < kend ? vp + (j0 + r) * a.vs_t : nullptr; });
+    ks.load(tid, kend - j0, a.dim, [&](int r) { return kp + (j0 + r) * a.ks_t; });
+    vs.load(tid, kend - j0, a.dim, [&](int r) { return vp + (j0 + r) * a.vs_t; });
   };
   if (kbeg < kend) fetch(kbeg);
   for (int j0 = kbeg; j0 < kend; j0 += BN) {
+    ks.clip(tid, kend - j0, a.dim);
+    vs.clip(tid, kend - j0, a.dim);
     __syncthreads();
     ks.store(tid, k_lds);
     vs.store(tid, v_lds);
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256) void packed_join(const float* part, const floa
 
 // ---------------------------------------------------------------- backward: dQ (and Delta)
 template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_bwd_q(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BM = 32 * NW;
   __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
@@ -334,11 +336,13 @@ __global__ __launch_bounds__(64 * NW) void packed_bwd_q(const Args a) {
   const T* vp = static_cast<const T*>(a.v) + h * a.vs_h;
   Stage<T, DP, BN, NT> ks, vs;
   auto fetch = [&](int j0) {
-    ks.load(tid, a.dim, [&](int r) { return j0 + r < kend ? kp + (j0 + r) * a.ks_t : nullptr; });
-    vs.load(tid, a.dim, [&](int r) { return j0 + r < kend ? vp + (j0 + r) * a.vs_t : nullptr; });
+    ks.load(tid, kend - j0, a.dim, [&](int r) { return kp + (j0 + r) * a.ks_t; });
+    vs.load(tid, kend - j0, a.dim, [&](int r) { return vp + (j0 + r) * a.vs_t; });
   };
   if (kbeg < kend) fetch(kbeg);
   for (int j0 = kbeg; j0 < kend; j0 += BN) {
+    ks.clip(tid, kend - j0, a.dim);
+    vs.clip(tid, kend - j0, a.dim);
     __syncthreads();
     ks.store(tid, k_lds);
     vs.store(tid, v_lds);
@@ -427,35 +431,29 @@ __global__ __launch_bounds__(64 * NW, DP == 128 || (sizeof(T) == 4 && DP == 64) 
   Stage<T, DP, BR, NT> qs, gs;
   float stat = 0.f;
   auto fetch = [&](int i0) {
-    qs.load(tid, a.dim, [&](int r) -> const T* {
-      if (i0 + r >= rend) return nullptr;
+    qs.load(tid, rend - i0, a.dim, [&](int r) {
       const Row w = row_of(a, h, i0 + r);
       return qp + w.token * a.qs_t + w.head * a.qs_h;
     });
-    gs.load(tid, a.dim, [&](int r) -> const T* {
-      if (i0 + r >= rend) return nullptr;
+    gs.load(tid, rend - i0, a.dim, [&](int r) {
       const Row w = row_of(a, h, i0 + r);
       return gp + (int64_t(w.token) * a.hq + w.head) * a.dim;
     });
-    if (tid < 2 * BR) {
-      const int r = i0 + (tid & (BR - 1));
-      stat = tid < BR ? INFINITY : 0.f;
-      if (r < rend) {
-        const Row w = row_of(a, h, r);
-        const int64_t at = int64_t(w.token) * a.hq + w.head;
-        stat = tid < BR ? a.lse[at] : a.delta[at];
-        if (tid < BR && stat == -INFINITY) stat = INFINITY;
-      }
+    if (tid < 2 * BR) {          // rows behind rend read the last one's: their P and dS are masked
+      const Row w = row_of(a, h, min(i0 + (tid & (BR - 1)), rend - 1));
+      stat = (tid < BR ? a.lse : a.delta)[int64_t(w.token) * a.hq + w.head];
     }
   };
   static_assert(2 * BR <= NT, "one statistic a lane");
   if (rbeg < rend) fetch(rbeg);
   for (int i0 = rbeg; i0 < rend; i0 += BR) {
+    qs.clip(tid, rend - i0, a.dim);
+    gs.clip(tid, rend - i0, a.dim);
     __syncthreads();
     qs.store(tid, q_lds);
     gs.store(tid, g_lds);
     if (tid < BR)
-      lse_lds[tid] = stat;
+      lse_lds[tid] = stat == -INFINITY ? INFINITY : stat;       // as in the dQ pass; not looked at before: nothing waits in fetch
     else if (tid < 2 * BR)
       delta_lds[tid - BR] = stat;
     bool odd = false;

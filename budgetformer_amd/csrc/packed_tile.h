@@ -176,25 +176,34 @@ template <typename T, int DP> struct Tile {
   }
 };
 
-// A tile on its way from memory to LDS, in registers: 16 bytes a lane and step, a row's chunks side by side.
+// A tile on its way from memory to LDS, in registers: 16 bytes a lane and step, a row's chunks side by side. Nothing in
+// load depends on a value it reads and nothing branches, so that all of a tile's loads are on their way at once.
 template <typename T, int DP, int ROWS, int NT> struct Stage {
-  static constexpr int kChunks = DP * int(sizeof(T)) / 16;
+  static constexpr int kChunks = DP * int(sizeof(T)) / 16, kPer = 16 / int(sizeof(T));
   static constexpr int kN = (ROWS * kChunks + NT - 1) / NT;
   uint4 r[kN];
-  // row_at(row): where the row's values are, or NULL for a row of zeros
-  template <typename F> __device__ __forceinline__ void load(int tid, int dim, F&& row_at) {
+  // rows 0 .. n - 1 of the tile (1 <= n) are at row_at(row); the others read row n - 1 again
+  template <typename F> __device__ __forceinline__ void load(int tid, int n, int dim, F&& row_at) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int c = i * NT + tid, row = c / kChunks, at = (c % kChunks) * (16 / int(sizeof(T)));
-      const T* p = row < ROWS ? row_at(row) : nullptr;
-      r[i] = p && at < dim ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0u, 0u, 0u, 0u);
+      const int c = i * NT + tid, row = c / kChunks, at = (c % kChunks) * kPer;
+      r[i] = *reinterpret_cast<const uint4*>(row_at(min(row, n - 1)) + (at < dim ? at : 0));
+    }
+  }
+  // zeros in the place of rows n and on and of values dim and on
+  __device__ __forceinline__ void clip(int tid, int n, int dim) {
+    if (n >= ROWS && dim == DP) return;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = i * NT + tid, row = c / kChunks, at = (c % kChunks) * kPer;
+      if (row >= n || at >= dim) r[i] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
   __device__ __forceinline__ void store(int tid, char* lds) const {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int c = i * NT + tid, row = c / kChunks;
-      if (row < ROWS) *reinterpret_cast<uint4*>(lds + row * Tile<T, DP>::kPitch + (c % kChunks) * 16) = r[i];
+      if (ROWS * kChunks % NT == 0 || row < ROWS) *reinterpret_cast<uint4*>(lds + row * Tile<T, DP>::kPitch + (c % kChunks) * 16) = r[i];
     }
   }
   // whether the lane's part holds an infinity or a NaN
