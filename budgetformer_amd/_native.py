@@ -54,7 +54,7 @@ class PackedAttn(C.Structure):
     _fields_ = [
         ("n_q", i64), ("n_k", i64), ("heads_q", i32), ("heads_k", i32), ("head_dim", i32), ("dtype", i32),
         ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
-        ("scale", f32), ("reserved", i32),
+        ("scale", f32), ("longest", i32),
     ]
 
 

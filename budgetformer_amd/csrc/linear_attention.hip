@@ -278,7 +278,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
         for (int r = 0; r < 16; ++r) m[b][r] = keep ? m[b][r] * f : 0.f;
       const int from = a.states ? 0 : last_start - t0;
       const bool cut = from > 0;
-#pragma unroll
+#pragma unroll 1
       for (int t = 0; t < C / 16; ++t) {
         // the decayed z in two or three parts of the activations' type, which add up to (nearly) its float32 value
         const Frag<T> z0 = TZ::template col_frag<true>(z_lds, t, wave, lane);

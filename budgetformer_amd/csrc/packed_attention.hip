@@ -29,23 +29,13 @@
 // NaN and infinities in places a row does not see: a masked P is 0, but 0 * inf is not. Where a tile is masked its
 // staged operand is checked; one that holds such a value takes a path that multiplies the finite values only, and
 // finds by a second product of indicators which rows do see one.
+#include "packed_short.h"
 #include "packed_tile.h"
 
 namespace bf {
 namespace {
 
 // ---------------------------------------------------------------- arguments
-struct Div {           // n / d for n < 2^31 by a multiplication
-  uint32_t magic, shift;
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
-};
-
-Div make_div(uint32_t d) {
-  uint32_t s = 0;
-  while ((uint64_t(1) << s) < d) ++s;
-  return Div{uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1), s};
-}
-
 struct Args {
   const void *q, *k, *v, *out, *dout;
   void *o, *dq, *dk, *dv;
@@ -609,6 +599,7 @@ int check(const bf_packed_attn* p, const char* fn, bool backward) {
   BF_CHECK_ARG(p->n_q >= 0 && p->n_k >= 0 && p->n_k < (int64_t(1) << 31) - 256 &&
                    p->n_q < ((int64_t(1) << 31) - 256) / p->heads_q,
                "%s: %lld rows of %d heads, %lld keys (below 2^31 each)", fn, (long long)p->n_q, p->heads_q, (long long)p->n_k);
+  BF_CHECK_ARG(p->longest >= 0, "%s: longest sequence %d", fn, p->longest);
   BF_CHECK_ARG(p->scale > 0.f && p->scale <= 3e38f, "%s: scale %g (positive and finite expected)", fn, double(p->scale));
   const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;
   for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
@@ -693,7 +684,7 @@ extern "C" int bf_packed_spans(const int32_t* q_offsets, const int32_t* k_offset
 
 extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
   if (check(p, "packed_attn_fwd_floats", false) != BF_OK) return -1;
-  const int n = p->n_q == 0 ? 1 : pieces_of(p);
+  const int n = p->n_q == 0 || packed_is_short(p) ? 1 : pieces_of(p);
   return n == 1 ? 0 : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
 }
 
@@ -703,6 +694,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
   if (p->n_q == 0) return BF_OK;
   BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
+  if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
   Args a = make_args(p, q, k, v);
   a.o = out, a.lse = lse;
   a.pieces = pieces_of(p);
@@ -742,7 +734,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
 
 extern "C" int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p) {
   if (check(p, "packed_attn_bwd_floats", true) != BF_OK) return -1;
-  const int n = kv_pieces_of(p);
+  const int n = packed_is_short(p) ? 1 : kv_pieces_of(p);
   return n == 1 ? 0 : 2 * p->n_k * p->heads_k * p->head_dim * n;
 }
 
@@ -753,6 +745,7 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
   BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
                "packed_attn_bwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
+  if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, as_stream(stream));
   Args a = make_args(p, q, k, v);
   a.out = out, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   a.lse = const_cast<float*>(lse);

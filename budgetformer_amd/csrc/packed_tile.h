@@ -231,7 +231,18 @@ template <typename T> __device__ __forceinline__ void store_block(T* p, const F3
   }
 }
 
-// f(T()) for a dtype code; f(std::integral_constant<int, DP>()) for a row of `dim` values.
+struct Div {           // n / d for n < 2^31 by a multiplication
+  uint32_t magic, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+};
+
+inline Div make_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return Div{uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1), s};
+}
+
+// f(T()) for a dtype code.
 template <typename F> int with_type(int32_t dtype, F&& f) {
   switch (dtype) {
     case BF_DTYPE_F32: return f(float());

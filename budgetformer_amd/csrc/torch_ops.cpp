@@ -541,7 +541,7 @@ void require_span(const at::Tensor& t, const char* name, int64_t n, const at::De
 }
 
 bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& row_span,
-                           double scale) {
+                           double scale, int64_t longest) {
   const at::Device dev = q.device();
   bf_packed_attn p{};
   p.dtype = dtype_code(q);
@@ -557,15 +557,16 @@ bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::T
   require_span(row_span, "row_span", p.n_q, dev);
   p.row_span = row_span.data_ptr<int32_t>();
   p.scale = float(scale);
+  p.longest = int32_t(std::min<int64_t>(std::max<int64_t>(longest, 0), INT32_MAX));
   return p;
 }
 
 // Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2).
 std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                   const at::Tensor& row_span, double scale) {
+                                                   const at::Tensor& row_span, double scale, int64_t longest) {
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
   const c10::DeviceGuard guard(q.device());
-  const bf_packed_attn p = packed_args(q, k, v, row_span, scale);
+  const bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   const int64_t floats = bf_packed_attn_fwd_floats(&p);
@@ -581,11 +582,11 @@ std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at
 std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                                const at::Tensor& row_span, const at::Tensor& key_span,
                                                                const at::Tensor& out, const at::Tensor& lse,
-                                                               const at::Tensor& dout, double scale) {
+                                                               const at::Tensor& dout, double scale, int64_t longest) {
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
   const c10::DeviceGuard guard(q.device());
   const at::Device dev = q.device();
-  bf_packed_attn p = packed_args(q, k, v, row_span, scale);
+  bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   require_span(key_span, "key_span", p.n_k, dev);
   p.key_span = key_span.data_ptr<int32_t>();
   require(out, "out", q.scalar_type(), dev);
@@ -774,9 +775,9 @@ TORCH_LIBRARY(bf, m) {
   m.def("reverse_index_and_plan(Tensor keys, Tensor qptr, int nnz, int n_kv, int q_bits, int slot_bits, "
         "bool global_token, int token_row, bool entries, int chunk, int item, Tensor(a!) counts) -> Tensor[]");
   m.def("packed_spans(Tensor q_offsets, Tensor k_offsets, int n_q, int n_k, bool causal) -> (Tensor, Tensor, Tensor)");
-  m.def("packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor row_span, float scale) -> (Tensor, Tensor)");
+  m.def("packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor row_span, float scale, int longest=0) -> (Tensor, Tensor)");
   m.def("packed_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor row_span, Tensor key_span, Tensor out, Tensor lse, "
-        "Tensor dout, float scale) -> (Tensor, Tensor, Tensor)");
+        "Tensor dout, float scale, int longest=0) -> (Tensor, Tensor, Tensor)");
   m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
         "bool inverse=False) -> (Tensor, Tensor)");
   m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "

@@ -51,7 +51,8 @@ class PackedSequences:
     nothing: their outputs and gradients are 0.
     """
 
-    def __init__(self, q_offsets: torch.Tensor, k_offsets: torch.Tensor, n_q: int, n_k: int, causal: bool):
+    def __init__(self, q_offsets: torch.Tensor, k_offsets: torch.Tensor, n_q: int, n_k: int, causal: bool, longest: int = 0):
+        self.longest = int(longest)          # no sequence has more rows or keys; 0: unknown
         self.q_offsets, self.k_offsets = q_offsets, k_offsets
         self.n_q, self.n_k, self.n_seq, self.causal = int(n_q), int(n_k), q_offsets.numel() - 1, bool(causal)
         self.self_attention = q_offsets is k_offsets and self.n_q == self.n_k
@@ -80,7 +81,7 @@ class PackedSequences:
         totals = [int(e[-1]) for e in ends]
         cls._sizes(totals[0], totals[-1])
         on = [e.to(torch.int32).to(device) for e in ends]
-        return cls(on[0], on[-1], totals[0], totals[-1], causal)
+        return cls(on[0], on[-1], totals[0], totals[-1], causal, max([int(x.max()) for x in lens if x.numel()], default=0))
 
     @classmethod
     def from_offsets(cls, q_offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None, *, n_q: Optional[int] = None,
@@ -96,7 +97,7 @@ class PackedSequences:
                 raise ValueError(f"offsets must be on a HIP device (got {x.device}); the HIP path has no CPU fallback")
             if x.shape != q_offsets.shape or x.device != q_offsets.device:
                 raise ValueError("q_offsets and k_offsets must be of the same sequences, on one device")
-        sizes = [n_q, n_q if k_offsets is None else n_k]
+        sizes, longest = [n_q, n_q if k_offsets is None else n_k], 0
         if k_offsets is None and n_k is not None and n_k != n_q:
             raise ValueError("n_k differs from n_q without k_offsets")
         if check:
@@ -104,6 +105,7 @@ class PackedSequences:
                 host = x.cpu().to(torch.int64)
                 if int(host[0]) != 0 or bool((host[1:] < host[:-1]).any()):
                     raise ValueError("offsets must ascend from 0")
+                longest = max(longest, int((host[1:] - host[:-1]).max())) if host.numel() > 1 else 0
                 if sizes[i] is None:
                     sizes[i] = int(host[-1])
                 elif int(host[-1]) > sizes[i]:
@@ -113,7 +115,7 @@ class PackedSequences:
         cls._sizes(int(sizes[0]), int(sizes[1]))
         q = q_offsets.to(torch.int32).contiguous()
         k = q if k_offsets is None else k_offsets.to(torch.int32).contiguous()
-        return cls(q, k, sizes[0], sizes[1], causal)
+        return cls(q, k, sizes[0], sizes[1], causal, longest)
 
     @staticmethod
     def _device(device) -> torch.device:
@@ -147,7 +149,7 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seqs, scale):
-        out, lse = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale)
+        out, lse = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.seqs, ctx.scale = seqs, scale
         ctx.mark_non_differentiable(lse)
@@ -160,7 +162,7 @@ class _PackedAttention(torch.autograd.Function):
             return None, None, None, None, None
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv = N.load_ops().packed_attn_bwd(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, _dense(dout),
-                                                  ctx.scale)
+                                                  ctx.scale, ctx.seqs.longest)
         return dq, dk, dv, None, None
 
 

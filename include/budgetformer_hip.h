@@ -813,7 +813,8 @@ typedef struct bf_packed_attn {
   const int32_t* row_span;
   const int32_t* key_span;
   float scale;                /* of q.k; positive                            */
-  int32_t reserved;           /* 0                                           */
+  int32_t longest;            /* no sequence has more rows or keys; 0: unknown
+                                 (chooses how the work is cut, not results)  */
 } bf_packed_attn;
 
 /* out = softmax(scale q k^T over the row's keys) v, contiguous [n_q, heads_q,

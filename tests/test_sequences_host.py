@@ -30,7 +30,8 @@ def _fwd(a, q=P, k=P, v=P, out=P):
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=7), "dtype"), (dict(heads_q=3, heads_k=2), "multiple"), (dict(heads_k=0), "heads"),
     (dict(n_q=-1), "rows"), (dict(n_k=2 ** 31), "keys"), (dict(n_q=2 ** 30), "rows"), (dict(scale=0.0), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(row_span=None), "spans")])
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(row_span=None), "spans"),
+    (dict(longest=-1), "longest")])
 def test_packed_attention_arguments(kw, match):
     with pytest.raises(ValueError, match=match):
         _fwd(_attn(**kw))
