@@ -166,9 +166,10 @@ _SIGS = {
                                     P_f32, P_f32, P_f32, vp]),
     "bf_packed_spans": (C.c_int, [P_i32, P_i32, i64, i64, i64, i32, P_i32, P_i32, P_i32, vp]),
     "bf_packed_attn_fwd_floats": (i64, [C.POINTER(PackedAttn)]),
-    "bf_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_packed_attn_rest": (C.c_int, [C.POINTER(PackedAttn)]),
+    "bf_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, vp, P_f32, P_f32, vp]),
     "bf_packed_attn_bwd_floats": (i64, [C.POINTER(PackedAttn)]),
-    "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, P_f32, vp]),
     "bf_rotary": (C.c_int, [vp, vp, i64, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64), vp, i32, vp, f32, i32,
                             i32, vp, vp, vp]),
     "bf_linear_attn_fwd_floats": (i64, [C.POINTER(LinearAttn)]),

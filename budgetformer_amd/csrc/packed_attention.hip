@@ -23,8 +23,8 @@
 // fall on different banks. float32 uses the same layout with eight 32x32x2 products for one of 16.
 //
 // Precision: scores, softmax statistics and all sums are float32. P and dS are rounded to the activations' type as
-// operands of the second products (half a step of bf16 is 2^-9 of each term, as the inputs' own rounding); float32
-// rounds nothing.
+// operands of the second products (half a step of each term, as the inputs' own rounding); float32 rounds nothing. Delta
+// is a difference's second part: a forward that trains keeps what the rounding of out left (`rest`), for it.
 //
 // NaN and infinities in places a row does not see: a masked P is 0, but 0 * inf is not. Where a tile is masked its
 // staged operand is checked; one that holds such a value takes a path that multiplies the finite values only, and
@@ -38,7 +38,7 @@ namespace {
 // ---------------------------------------------------------------- arguments
 struct Args {
   const void *q, *k, *v, *out, *dout;
-  void *o, *dq, *dk, *dv;
+  void *o, *rest, *dq, *dk, *dv;                   // rest: what the rounding of out left, or NULL
   float *lse, *delta, *part, *stat;
   const int2 *row_span, *key_span;
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;      // strides in values
@@ -239,7 +239,21 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
     }
     if (l != 0.f) store_cols<DP>(a.part + slot * a.dim, o, 1.f, a.dim, half);
   } else {
-    store_cols<DP>(static_cast<T*>(a.o) + at * a.dim, o, l == 0.f ? 0.f : 1.f / l, a.dim, half);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (a.rest) {
+#pragma unroll
+      for (int n = 0; n < TL::kBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] *= inv;
+      store_cols<DP>(static_cast<T*>(a.o) + at * a.dim, o, 1.f, a.dim, half);
+#pragma unroll
+      for (int n = 0; n < TL::kBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] -= float(T(o[n][r]));
+      store_cols<DP>(static_cast<T*>(a.rest) + at * a.dim, o, 1.f, a.dim, half);
+    } else {
+      store_cols<DP>(static_cast<T*>(a.o) + at * a.dim, o, inv, a.dim, half);
+    }
     if (half == 0) a.lse[at] = l == 0.f ? -INFINITY : mc + __log2f(l);
   }
 }
@@ -248,7 +262,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
 // statistics (kMaxPieces is a wave); only pieces that hold keys of the row were written and are read.
 template <typename T>
 __global__ __launch_bounds__(256) void packed_join(const float* part, const float* stat, int64_t n_rows, int pieces, int dim,
-                                                   T* out, float* lse) {
+                                                   T* out, T* rest, float* lse) {
   const int lane = threadIdx.x & 63;
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= n_rows) return;
@@ -274,6 +288,10 @@ __global__ __launch_bounds__(256) void packed_join(const float* part, const floa
     typedef T V2 __attribute__((ext_vector_type(2)));
     const V2 v = {T(a0 * inv), T(a1 * inv)};
     *reinterpret_cast<V2*>(out + row * dim + d) = v;
+    if (rest) {
+      const V2 w = {T(a0 * inv - float(v[0])), T(a1 * inv - float(v[1]))};
+      *reinterpret_cast<V2*>(rest + row * dim + d) = w;
+    }
   }
   if (lane == 0) lse[row] = l == 0.f ? -INFINITY : top + __log2f(l);
 }
@@ -313,6 +331,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     for (int s = 0; s < TL::kSteps; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf(float(gf[s][j]), float(of[s][j]), delta);
+    if (a.rest) {
+      load_row<T, DP>(of, valid ? static_cast<const T*>(a.rest) + at * a.dim : nullptr, a.dim, half);
+#pragma unroll
+      for (int s = 0; s < TL::kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = fmaf(float(gf[s][j]), float(of[s][j]), delta);
+    }
     delta += __shfl_xor(delta, 32, 64);
     if (valid && half == 0) a.delta[at] = delta;
   }
@@ -778,15 +803,20 @@ extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
   return n == 1 ? order_ints(p) : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
 }
 
-extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
-                                  float* scratch, void* stream) {
+extern "C" int bf_packed_attn_rest(const bf_packed_attn* p) {
+  return check(p, "packed_attn_rest", false) == BF_OK && p->dtype != BF_DTYPE_F32 && !packed_is_short(p);
+}
+
+extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
+                                  float* lse, float* scratch, void* stream) {
   BF_CHECK_OK(check(p, "packed_attn_fwd", false));
   if (p->n_q == 0) return BF_OK;
   BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
   if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
   Args a = make_args(p, q, k, v);
-  a.o = out, a.lse = lse;
+  BF_CHECK_ARG(aligned16({rest}), "packed_attn_fwd: rest must be 16-byte aligned");
+  a.o = out, a.rest = rest, a.lse = lse;
   a.pieces = pieces_of(p);
   const hipStream_t st = as_stream(stream);
   if (a.pieces == 1) {
@@ -816,7 +846,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
       BF_LAUNCH("packed_attn_fwd_pieces", kern, grid_of(a), dim3(64), 0, st, a);
       BF_CHECK_LAUNCH();
       BF_LAUNCH("packed_attn_join", (packed_join<T>), dim3(unsigned(ceil_div(n_rows, 4))), dim3(256), 0, st, a.part, a.stat,
-                n_rows, a.pieces, a.dim, static_cast<T*>(out), lse);
+                n_rows, a.pieces, a.dim, static_cast<T*>(out), static_cast<T*>(rest), lse);
       BF_CHECK_LAUNCH();
       return BF_OK;
     });
@@ -831,7 +861,7 @@ extern "C" int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p) {
 }
 
 extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
-                                  const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta,
+                                  const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta,
                                   float* scratch, void* stream) {
   BF_CHECK_OK(check(p, "packed_attn_bwd", true));
   BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
@@ -839,7 +869,8 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
   BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
   if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, as_stream(stream));
   Args a = make_args(p, q, k, v);
-  a.out = out, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
+  BF_CHECK_ARG(aligned16({rest}), "packed_attn_bwd: rest must be 16-byte aligned");
+  a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   a.lse = const_cast<float*>(lse);
   const hipStream_t st = as_stream(stream);
   return with_type(p->dtype, [&](auto t) -> int {

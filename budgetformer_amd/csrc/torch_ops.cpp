@@ -561,28 +561,32 @@ bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::T
   return p;
 }
 
-// Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2).
-std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                   const at::Tensor& row_span, double scale, int64_t longest) {
+// Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2, rest). With `train`,
+// rest is what the backward reads beside out (empty where it needs nothing).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                   const at::Tensor& row_span, double scale, int64_t longest, bool train) {
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
   const c10::DeviceGuard guard(q.device());
   const bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   const int64_t floats = bf_packed_attn_fwd_floats(&p);
-  at::Tensor scratch;
+  const bool keeps = train && bf_packed_attn_rest(&p);
+  at::Tensor scratch, rest = keeps ? at::empty_like(out) : at::empty({0}, out.options());
   if (floats > 0) scratch = at::empty({floats}, lse.options());
-  check_rc(bf_packed_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+  check_rc(bf_packed_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                              keeps ? rest.data_ptr() : nullptr, lse.data_ptr<float>(),
                               floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
            "bf::packed_attn_fwd");
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 // Backward (bf_packed_attn_bwd): (dq, dk, dv), contiguous.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                                const at::Tensor& row_span, const at::Tensor& key_span,
                                                                const at::Tensor& out, const at::Tensor& lse,
-                                                               const at::Tensor& dout, double scale, int64_t longest) {
+                                                               const at::Tensor& dout, double scale, int64_t longest,
+                                                               const std::optional<at::Tensor>& rest) {
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
   const c10::DeviceGuard guard(q.device());
   const at::Device dev = q.device();
@@ -594,12 +598,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor&
   require(lse, "lse", at::kFloat, dev);
   TORCH_CHECK_VALUE(out.sizes() == q.sizes() && dout.sizes() == q.sizes() && lse.numel() == q.size(0) * q.size(1), "out ",
                     out.sizes(), ", dout ", dout.sizes(), " or lse ", lse.sizes(), " do not match q ", q.sizes());
+  const void* rp = nullptr;
+  if (rest.has_value() && rest->defined() && rest->numel() > 0) {
+    require(*rest, "rest", q.scalar_type(), dev);
+    TORCH_CHECK_VALUE(rest->sizes() == q.sizes(), "rest ", rest->sizes(), " does not match q ", q.sizes());
+    rp = rest->data_ptr();
+  }
   const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
   at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
   at::Tensor delta = at::empty_like(lse), scratch;
   const int64_t floats = bf_packed_attn_bwd_floats(&p);
   if (floats > 0) scratch = at::empty({floats}, lse.options());
-  check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+  check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(),
                               dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(),
                               floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
            "bf::packed_attn_bwd");
@@ -775,9 +785,10 @@ TORCH_LIBRARY(bf, m) {
   m.def("reverse_index_and_plan(Tensor keys, Tensor qptr, int nnz, int n_kv, int q_bits, int slot_bits, "
         "bool global_token, int token_row, bool entries, int chunk, int item, Tensor(a!) counts) -> Tensor[]");
   m.def("packed_spans(Tensor q_offsets, Tensor k_offsets, int n_q, int n_k, bool causal) -> (Tensor, Tensor, Tensor)");
-  m.def("packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor row_span, float scale, int longest=0) -> (Tensor, Tensor)");
+  m.def("packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor row_span, float scale, int longest=0, "
+        "bool train=False) -> (Tensor, Tensor, Tensor)");
   m.def("packed_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor row_span, Tensor key_span, Tensor out, Tensor lse, "
-        "Tensor dout, float scale, int longest=0) -> (Tensor, Tensor, Tensor)");
+        "Tensor dout, float scale, int longest=0, Tensor? rest=None) -> (Tensor, Tensor, Tensor)");
   m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
         "bool inverse=False) -> (Tensor, Tensor)");
   m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "

@@ -149,8 +149,8 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seqs, scale):
-        out, lse = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, rest = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest, True)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.seqs, ctx.scale = seqs, scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -160,9 +160,9 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return None, None, None, None, None
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, rest = ctx.saved_tensors
         dq, dk, dv = N.load_ops().packed_attn_bwd(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, _dense(dout),
-                                                  ctx.scale, ctx.seqs.longest)
+                                                  ctx.scale, ctx.seqs.longest, rest)
         return dq, dk, dv, None, None
 
 
@@ -178,7 +178,10 @@ def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = No
     dt = q.dtype
     q, k, v = _rows(q, "q"), _rows(k.to(dt), "k"), _rows(v.to(dt), "v")
     scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
-    out, lse = _PackedAttention.apply(q, k, v, seqs, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _PackedAttention.apply(q, k, v, seqs, scale)
+    else:
+        out, lse, _ = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest, False)
     return (out, lse * math.log(2.0)) if with_lse else out
 
 

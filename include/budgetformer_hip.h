@@ -821,17 +821,22 @@ typedef struct bf_packed_attn {
  * head_dim] in q's dtype; lse float32 [n_q, heads_q]: the log2 of the row's sum
  * of exp(scale q.k). A row that sees no key has out 0 and lse -inf. scratch:
  * bf_packed_attn_fwd_floats(p) floats (0: none needed; -1: bad arguments), for
- * calls of few rows, whose keys are cut into pieces.                        */
+ * calls of few rows, whose keys are cut into pieces, and of sequences of very
+ * different lengths, whose tiles are put in order. rest (or NULL): like out,
+ * what out's rounding left, for the backward; bf_packed_attn_rest(p) says
+ * whether the backward reads it.                                            */
 int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p);
-int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
-                       float* scratch, void* stream);
+int bf_packed_attn_rest(const bf_packed_attn* p);
+int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
+                       float* lse, float* scratch, void* stream);
 /* Gradients of it: dq like out, dk and dv contiguous [n_k, heads_k, head_dim]
- * (summed over the heads of a group). out, dout: contiguous. delta: scratch of
+ * (summed over the heads of a group). out, dout: contiguous. rest: the
+ * forward's, or NULL (Delta then comes from the rounded out). delta: scratch of
  * n_q * heads_q floats; scratch: bf_packed_attn_bwd_floats(p) floats (0: none
  * needed; -1: bad arguments). No atomics: results repeat bit for bit.       */
 int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p);
 int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
-                       const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, float* scratch,
+                       const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, float* scratch,
                        void* stream);
 
 /* Rotary positions: the first `rot` values of every head of x and y (rows of

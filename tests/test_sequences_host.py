@@ -24,7 +24,7 @@ def _attn(**kw):
 
 
 def _fwd(a, q=P, k=P, v=P, out=P):
-    N.call("bf_packed_attn_fwd", C.byref(a), q, k, v, out, P, P, None)
+    N.call("bf_packed_attn_fwd", C.byref(a), q, k, v, out, None, P, P, None)
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -56,7 +56,7 @@ def test_packed_attention_addresses_and_strides():
     with pytest.raises(ValueError, match="bad arguments"):
         _fwd(_attn(), q=None)
     with pytest.raises(ValueError, match="no key spans"):
-        N.call("bf_packed_attn_bwd", C.byref(_attn(key_span=None)), P, P, P, P, P, P, P, P, P, P, P, None)
+        N.call("bf_packed_attn_bwd", C.byref(_attn(key_span=None)), P, P, P, P, None, P, P, P, P, P, P, P, None)
     _fwd(_attn(n_q=0))                                       # nothing to do, nothing launched
 
 
