@@ -177,12 +177,11 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
     const bool masked = j0 < wl.x || j0 + BN > wf.y || w_last < w_row0 + 31;
     if (masked) {
 #pragma unroll
-      for (int b = 0; b < BN / 32; ++b)
+      for (int b = 0; b < BN / 32; ++b) {
+        const uint32_t seen = seen_bits(lo - j0 - 32 * b, hi - j0 - 32 * b, half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = j0 + 32 * b + acc_row(r, half);
-          if (key < lo || key >= hi) s[b][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r) s[b][r] = where_seen(seen, r, s[b][r], -INFINITY);
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -382,11 +381,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(fmaf(sa[r], a.c, -lse)) * (pa[r] - delta);
       if (masked) {
+        const uint32_t seen = seen_bits(lo - j0 - 32 * b, hi - j0 - 32 * b, half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = j0 + 32 * b + acc_row(r, half);
-          if (key < lo || key >= hi) ds[r] = 0.f;
-        }
+        for (int r = 0; r < 16; ++r) ds[r] = where_seen(seen, r, ds[r], 0.f);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -511,11 +508,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
         }
       }
       if (masked) {
+        const uint32_t seen = seen_bits(lo - i0 - 32 * b, hi - i0 - 32 * b, half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = i0 + 32 * b + acc_row(r, half);
-          if (i < lo || i >= hi) p[r] = 0.f, ds[r] = 0.f;
-        }
+        for (int r = 0; r < 16; ++r) p[r] = where_seen(seen, r, p[r], 0.f), ds[r] = where_seen(seen, r, ds[r], 0.f);
       }
       if (masked && odd) {
 #pragma unroll

@@ -87,6 +87,20 @@ template <typename T> __device__ __forceinline__ Frag<T> zero_frag() {
 // Row (of 32) that register r of a product holds, for the lane's half; also value r's row in register order.
 __device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 
+// The places of a 32 block that lie in [lo, hi), a bit each, as the lane's half sees them: register r's place is bit
+// acc_row(r, 0).
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int half) {
+  const uint32_t below_hi = hi >= 32 ? ~0u : hi <= 0 ? 0u : (1u << hi) - 1u;
+  const uint32_t below_lo = lo >= 32 ? ~0u : lo <= 0 ? 0u : (1u << lo) - 1u;
+  return (below_hi & ~below_lo) >> (4 * half);
+}
+
+// x where register r's bit is set, else `other` (two instructions: the bit spread over a word, and a bitwise choice).
+__device__ __forceinline__ float where_seen(uint32_t bits, int r, float x, float other) {
+  const uint32_t all = uint32_t(__builtin_amdgcn_sbfe(int(bits), uint32_t(acc_row(r, 0)), 1u));
+  return __uint_as_float((__float_as_uint(x) & all) | (__float_as_uint(other) & ~all));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Registers 8t .. 8t+7 as an operand of the next product.

@@ -25,6 +25,7 @@ struct RotaryArgs {
 };
 
 constexpr int kRotaryThreads = 256;
+constexpr int kAhead = 4;
 constexpr int kRotaryAngles = 512;     // angles of a workgroup at most (4 KB of LDS)
 
 // V: values a lane moves at a time (16 bytes, or 1 where the sizes or addresses do not allow that).
@@ -49,55 +50,66 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary(const RotaryArgs a) {
   // a head's work: its turned pairs V values at a time, then the values that are copied
   const int turned = (PAIRS ? a.rot : half) / V, rest = (a.dim - a.rot) / V, per = turned + rest;
   const int h0 = blockIdx.y * a.heads, nh = min(a.heads, a.hx + a.hy - h0);
-  for (int i = threadIdx.x; i < nt * nh * per; i += kRotaryThreads) {
-    const int u = i % per, th = i / per, t = th / nh;
-    int h = h0 + th - t * nh;
-    const T* src;
-    T* dst;
-    if (h < a.hx) {
-      src = static_cast<const T*>(a.x) + (t0 + t) * a.xs_t + h * a.xs_h;
-      dst = static_cast<T*>(a.ox) + ((t0 + t) * a.hx + h) * a.dim;
-    } else {
-      h -= a.hx;
-      src = static_cast<const T*>(a.y) + (t0 + t) * a.ys_t + h * a.ys_h;
-      dst = static_cast<T*>(a.oy) + ((t0 + t) * a.hy + h) * a.dim;
-    }
-    const float2* tn = turn + t * half;
-    if (u >= turned) {
-      const int at = a.rot + (u - turned) * V;
-      *reinterpret_cast<Vec*>(dst + at) = *reinterpret_cast<const Vec*>(src + at);
-    } else if constexpr (PAIRS) {
-      const int at = u * V;
-      if constexpr (V == 1) {              // the other value of the pair too: read, not written
-        const bool second = at & 1;
-        const float x = float(src[at]), other = float(src[at ^ 1]);
-        const float2 w = tn[at >> 1];
-        dst[at] = T(second ? fmaf(other, w.y, x * w.x) : fmaf(x, w.x, -other * w.y));
+  // kAhead pieces of work a lane at a time, their loads on their way together
+  const int all = nt * nh * per;
+  for (int i0 = threadIdx.x; i0 < all; i0 += kRotaryThreads * kAhead) {
+    const T* src[kAhead];
+    T* dst[kAhead];
+    const float2* tn[kAhead];
+    int at[kAhead];
+    Vec x[kAhead], y[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = min(i0 + k * kRotaryThreads, all - 1), u = i % per, th = i / per, t = th / nh;
+      int h = h0 + th - t * nh;
+      if (h < a.hx) {
+        src[k] = static_cast<const T*>(a.x) + (t0 + t) * a.xs_t + h * a.xs_h;
+        dst[k] = static_cast<T*>(a.ox) + ((t0 + t) * a.hx + h) * a.dim;
       } else {
-        const Vec x = *reinterpret_cast<const Vec*>(src + at);
-        Vec o;
+        h -= a.hx;
+        src[k] = static_cast<const T*>(a.y) + (t0 + t) * a.ys_t + h * a.ys_h;
+        dst[k] = static_cast<T*>(a.oy) + ((t0 + t) * a.hy + h) * a.dim;
+      }
+      const bool turns = u < turned;
+      at[k] = turns ? u * V : a.rot + (u - turned) * V;
+      tn[k] = turns ? turn + t * half : nullptr;
+      x[k] = *reinterpret_cast<const Vec*>(src[k] + at[k]);
+      // the other value of each pair: elsewhere in the head, or (single values of neighbouring pairs) next to it
+      if constexpr (!PAIRS)
+        y[k] = *reinterpret_cast<const Vec*>(src[k] + at[k] + (turns ? half : 0));
+      else if constexpr (V == 1)
+        y[k] = *reinterpret_cast<const Vec*>(src[k] + (turns ? at[k] ^ 1 : at[k]));
+    }
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const float2 w = tn[(at + j) >> 1];
-          const float p = float(x[j]), q = float(x[j + 1]);
-          o[j] = T(fmaf(p, w.x, -q * w.y));
-          o[j + 1] = T(fmaf(p, w.y, q * w.x));
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 + k * kRotaryThreads >= all) break;
+      Vec o = x[k];
+      if (tn[k]) {
+        if constexpr (!PAIRS) {
+          Vec r;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float2 w = tn[k][at[k] + j];
+            const float p = float(x[k][j]), q = float(y[k][j]);
+            o[j] = T(fmaf(p, w.x, -q * w.y));
+            r[j] = T(fmaf(p, w.y, q * w.x));
+          }
+          *reinterpret_cast<Vec*>(dst[k] + half + at[k]) = r;
+        } else if constexpr (V == 1) {
+          const float2 w = tn[k][at[k] >> 1];
+          const float p = float(x[k][0]), q = float(y[k][0]);
+          o[0] = T(at[k] & 1 ? fmaf(q, w.y, p * w.x) : fmaf(p, w.x, -q * w.y));
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; j += 2) {
+            const float2 w = tn[k][(at[k] + j) >> 1];
+            const float p = float(x[k][j]), q = float(x[k][j + 1]);
+            o[j] = T(fmaf(p, w.x, -q * w.y));
+            o[j + 1] = T(fmaf(p, w.y, q * w.x));
+          }
         }
-        *reinterpret_cast<Vec*>(dst + at) = o;
       }
-    } else {
-      const int at = u * V;
-      const Vec x = *reinterpret_cast<const Vec*>(src + at), y = *reinterpret_cast<const Vec*>(src + half + at);
-      Vec o, r;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float2 w = tn[at + j];
-        const float p = float(x[j]), q = float(y[j]);
-        o[j] = T(fmaf(p, w.x, -q * w.y));
-        r[j] = T(fmaf(p, w.y, q * w.x));
-      }
-      *reinterpret_cast<Vec*>(dst + at) = o;
-      *reinterpret_cast<Vec*>(dst + half + at) = r;
+      *reinterpret_cast<Vec*>(dst[k] + at[k]) = o;
     }
   }
 }

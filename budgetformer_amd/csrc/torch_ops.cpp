@@ -523,6 +523,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_spans(const at::Tensor& q_
   return {row_span, key_span, positions};
 }
 
+// A [rows, heads, dim] tensor as the kernels read it: a contiguous last dimension, rows and heads at whole 16-byte steps.
+// Views that are so (slices of a fused projection, heads expanded) are taken as they are, others are copied.
+at::Tensor as_rows(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 3, name, " must be [rows, heads, head_dim] (got ", t.sizes(), ")");
+  const int64_t per = 16 / t.element_size();
+  bool fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(2) <= 1 || t.stride(2) == 1);
+  for (int d = 0; d < 2; ++d) fits = fits && (t.size(d) <= 1 || t.stride(d) % per == 0);
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// A contiguous tensor at a 16-byte aligned address.
+at::Tensor as_dense(const at::Tensor& t) {
+  return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // A [rows, heads, dim] tensor with a contiguous last dimension; its strides of a row and of a head in values. Strides of
 // dimensions of one entry do not matter and are given as 0.
 void require_heads(const at::Tensor& t, const char* name, at::ScalarType st, const at::Device& dev, int64_t (&stride)[2]) {
@@ -563,10 +578,13 @@ bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::T
 
 // Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2, rest). With `train`,
 // rest is what the backward reads beside out (empty where it needs nothing).
-std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                    const at::Tensor& row_span, double scale, int64_t longest, bool train) {
-  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
-  const c10::DeviceGuard guard(q.device());
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
   const bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
@@ -582,13 +600,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor&
 }
 
 // Backward (bf_packed_attn_bwd): (dq, dk, dv), contiguous.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                                const at::Tensor& row_span, const at::Tensor& key_span,
                                                                const at::Tensor& out, const at::Tensor& lse,
-                                                               const at::Tensor& dout, double scale, int64_t longest,
+                                                               const at::Tensor& dout_in, double scale, int64_t longest,
                                                                const std::optional<at::Tensor>& rest) {
-  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
-  const c10::DeviceGuard guard(q.device());
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
+  const at::Tensor dout = as_dense(dout_in);
   const at::Device dev = q.device();
   bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   require_span(key_span, "key_span", p.n_k, dev);
@@ -617,10 +639,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor&
 }
 
 // Rotary positions (bf_rotary) of x and, if given, y: new contiguous tensors.
-std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& x, const std::optional<at::Tensor>& y, const at::Tensor& positions,
+std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& x_in, const std::optional<at::Tensor>& y_in, const at::Tensor& positions,
                                           const at::Tensor& turns, double amplitude, bool interleaved, bool inverse) {
-  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a device tensor (got ", x.device(), ")");
-  const c10::DeviceGuard guard(x.device());
+  TORCH_CHECK_VALUE(x_in.is_cuda(), "x must be a device tensor (got ", x_in.device(), ")");
+  const c10::DeviceGuard guard(x_in.device());
+  const auto along = [](const at::Tensor& t) {       // contiguous along the head; other strides are taken as they are
+    return t.dim() != 3 || t.size(2) <= 1 || t.stride(2) == 1 ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const at::Tensor x = along(x_in);
+  std::optional<at::Tensor> y;
+  if (y_in.has_value() && y_in->defined()) y = along(*y_in);
   const at::Device dev = x.device();
   const bool two = y.has_value() && y->defined();
   int64_t xs[2], ys[2] = {0, 0};
@@ -685,12 +713,15 @@ bf_linear_attn linear_args(const at::Tensor& q, const at::Tensor& k, const at::T
 }
 
 // Forward (bf_linear_attn_fwd): (out, final state float32 [n_seq, heads, dim_k, dim_v], or empty without return_state).
-std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                    const at::Tensor& log_decay, const at::Tensor& row_span,
                                                    const at::Tensor& key_span, const at::Tensor& offsets, double scale,
                                                    const std::optional<at::Tensor>& init_state, bool return_state) {
-  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
-  const c10::DeviceGuard guard(q.device());
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
   bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
   at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), scratch;
   at::Tensor state = return_state ? at::empty({p.n_seq, p.heads, p.dim_k, p.dim_v}, log_decay.options())
@@ -705,13 +736,17 @@ std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q, const at
 }
 
 // Backward (bf_linear_attn_bwd): (dq, dk, dv), contiguous.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                                const at::Tensor& log_decay, const at::Tensor& row_span,
                                                                const at::Tensor& key_span, const at::Tensor& offsets,
-                                                               const at::Tensor& dout, double scale,
+                                                               const at::Tensor& dout_in, double scale,
                                                                const std::optional<at::Tensor>& init_state) {
-  TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
-  const c10::DeviceGuard guard(q.device());
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
+  const at::Tensor dout = as_dense(dout_in);
   const bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
   require(dout, "dout", q.scalar_type(), q.device());
   TORCH_CHECK_VALUE(dout.sizes() == v.sizes(), "dout ", dout.sizes(), " does not match v ", v.sizes());

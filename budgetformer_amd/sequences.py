@@ -26,20 +26,23 @@ from . import _native as N
 _MOST_ROWS = 2 ** 31 - 256
 
 
-def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """``t`` as the kernels read it: a contiguous last dimension, rows and heads at whole 16-byte steps (views
-    such as slices of a fused projection are taken as they are; anything else is copied)."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [rows, heads, head_dim] (got {tuple(t.shape)})")
-    per = 16 // t.element_size()
-    fits = t.data_ptr() % 16 == 0 and all(t.size(d) <= 1 or (t.stride(d) >= 0 and t.stride(d) % per == 0) for d in (0, 1))
-    return t if fits and (t.stride(2) == 1 or t.size(2) <= 1) else t.contiguous()
+def _op(name: str):
+    """The overload of a ``bf`` operator, resolved once (an operator's own lookup costs a call some 2 us)."""
+    got = _OPS.get(name)
+    if got is None:
+        got = _OPS[name] = getattr(N.load_ops(), name).default
+    return got
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor at a 16-byte aligned address."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+_OPS: dict = {}
+
+
+def _as(q: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == q.dtype else t.to(q.dtype)
+
+
+def _trains(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class PackedSequences:
@@ -56,7 +59,7 @@ class PackedSequences:
         self.q_offsets, self.k_offsets = q_offsets, k_offsets
         self.n_q, self.n_k, self.n_seq, self.causal = int(n_q), int(n_k), q_offsets.numel() - 1, bool(causal)
         self.self_attention = q_offsets is k_offsets and self.n_q == self.n_k
-        self.row_span, self.key_span, self._positions = N.load_ops().packed_spans(q_offsets, k_offsets, self.n_q, self.n_k,
+        self.row_span, self.key_span, self._positions = _op("packed_spans")(q_offsets, k_offsets, self.n_q, self.n_k,
                                                                                   self.causal)
 
     @staticmethod
@@ -149,7 +152,7 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seqs, scale):
-        out, lse, rest = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest, True)
+        out, lse, rest = _op("packed_attn_fwd")(q, k, v, seqs.row_span, scale, seqs.longest, True)
         ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.seqs, ctx.scale = seqs, scale
         ctx.mark_non_differentiable(lse)
@@ -161,7 +164,7 @@ class _PackedAttention(torch.autograd.Function):
         if dout is None:
             return None, None, None, None, None
         q, k, v, out, lse, rest = ctx.saved_tensors
-        dq, dk, dv = N.load_ops().packed_attn_bwd(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, _dense(dout),
+        dq, dk, dv = _op("packed_attn_bwd")(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, dout,
                                                   ctx.scale, ctx.seqs.longest, rest)
         return dq, dk, dv, None, None
 
@@ -175,13 +178,12 @@ def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = No
     lse) with ``with_lse``: lse float32 [n_q, heads], the log of the row's sum of exponentials, -inf for a row
     that sees no key (its out is 0); lse is not differentiable. Gradients repeat bit for bit."""
     _check_seqs(seqs, q, k)
-    dt = q.dtype
-    q, k, v = _rows(q, "q"), _rows(k.to(dt), "k"), _rows(v.to(dt), "v")
-    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    k, v = _as(q, k), _as(q, v)
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    if _trains(q, k, v):
         out, lse = _PackedAttention.apply(q, k, v, seqs, scale)
     else:
-        out, lse, _ = N.load_ops().packed_attn_fwd(q, k, v, seqs.row_span, scale, seqs.longest, False)
+        out, lse, _ = _op("packed_attn_fwd")(q, k, v, seqs.row_span, scale, seqs.longest, False)
     return (out, lse * math.log(2.0)) if with_lse else out
 
 
@@ -241,17 +243,18 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.freq, ctx.interleaved, ctx.two = freq, interleaved, y is not None
         ctx.set_materialize_grads(False)
-        ox, oy = N.load_ops().rotary(x, y, positions, freq.turns, freq.amplitude, interleaved, False)
+        ox, oy = _op("rotary")(x, y, positions, freq.turns, freq.amplitude, interleaved, False)
         return (ox, oy) if ctx.two else ox
 
     @staticmethod
     def backward(ctx, dx, dy=None):
         positions, = ctx.saved_tensors
-        ops, f = N.load_ops(), ctx.freq
-        given = [_rows(g, "gradient") for g in (dx, dy) if g is not None]
+        f = ctx.freq
+        given = [g for g in (dx, dy) if g is not None]
         if not given:
             return None, None, None, None, None
-        got = ops.rotary(given[0], given[1] if len(given) == 2 else None, positions, f.turns, f.amplitude, ctx.interleaved, True)
+        got = _op("rotary")(given[0], given[1] if len(given) == 2 else None, positions, f.turns, f.amplitude, ctx.interleaved,
+                            True)
         if len(given) == 2:
             dx, dy = got
         elif dx is not None:
@@ -276,10 +279,15 @@ def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optio
         if seqs.n_q != q.size(0):
             raise ValueError(f"the sequences cover {seqs.n_q} rows, q has {q.size(0)}")
         positions = seqs.positions()
-    q = _rows(q, "q")
-    if freq.rot > q.size(2):
-        raise ValueError(f"{freq.rot} rotated values in a head of {q.size(2)}")
-    return _Rotary.apply(q, None if k is None else _rows(k.to(q.dtype), "k"), positions.contiguous(), freq, bool(interleaved))
+    if freq.rot > q.size(-1):
+        raise ValueError(f"{freq.rot} rotated values in a head of {q.size(-1)}")
+    k = None if k is None else _as(q, k)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if _trains(q, k):
+        return _Rotary.apply(q, k, positions, freq, bool(interleaved))
+    got = _op("rotary")(q, k, positions, freq.turns, freq.amplitude, bool(interleaved), False)
+    return got[0] if k is None else got
 
 
 # ------------------------------------------------------------------ linear attention
@@ -288,7 +296,7 @@ class _LinearAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, seqs, scale, initial_state, return_state):
-        out, state = N.load_ops().linear_attn_fwd(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
+        out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
                                                   initial_state, return_state)
         ctx.save_for_backward(q, k, v, log_decay, initial_state)
         ctx.seqs, ctx.scale = seqs, scale
@@ -302,7 +310,7 @@ class _LinearAttention(torch.autograd.Function):
             return (None,) * 8
         q, k, v, log_decay, init = ctx.saved_tensors
         s = ctx.seqs
-        dq, dk, dv = N.load_ops().linear_attn_bwd(q, k, v, log_decay, s.row_span, s.key_span, s.q_offsets, _dense(dout),
+        dq, dk, dv = _op("linear_attn_bwd")(q, k, v, log_decay, s.row_span, s.key_span, s.q_offsets, dout,
                                                   ctx.scale, init)
         return dq, dk, dv, None, None, None, None, None
 
@@ -329,14 +337,18 @@ def linear_attention(q, k, v, log_decay, seqs: PackedSequences, scale: Optional[
     _check_seqs(seqs, q, k)
     if not seqs.self_attention or not seqs.causal:
         raise ValueError("linear attention takes causal sequences of the same rows and keys")
-    dt = q.dtype
-    q, k, v = _rows(q, "q"), _rows(k.to(dt), "k"), _rows(v.to(dt), "v")
+    k, v = _as(q, k), _as(q, v)
     if initial_state is not None:
         if initial_state.requires_grad:
             raise NotImplementedError("the initial state is a constant: no gradient with respect to it")
         initial_state = initial_state.float().contiguous()
-    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
-    out, state = _LinearAttention.apply(q, k, v, _decays(log_decay, q), seqs, scale, initial_state, bool(return_state))
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    log_decay = _decays(log_decay, q)
+    if _trains(q, k, v):
+        out, state = _LinearAttention.apply(q, k, v, log_decay, seqs, scale, initial_state, bool(return_state))
+    else:
+        out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
+                                            initial_state, bool(return_state))
     return (out, state) if return_state else out
 
 
@@ -345,9 +357,8 @@ def linear_attention_step(q, k, v, log_decay, state, scale: Optional[float] = No
     """One token of each of n sequences: (out [n, heads, dv], new state). q and k [n, heads, dk], v [n, heads, dv],
     state float32 [n, heads, dk, dv]. ``out_state``: where the new state is written (``state`` itself updates it in
     place), else a new tensor. For inference: no gradients."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if _trains(q, k, v, state):
         raise NotImplementedError("linear_attention_step has no gradients (linear_attention has)")
-    dt = q.dtype
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
-    return N.load_ops().linear_attn_step(q.contiguous(), k.to(dt).contiguous(), v.to(dt).contiguous(), _decays(log_decay, q),
-                                         state, scale, out_state)
+    return _op("linear_attn_step")(q.contiguous(), _as(q, k).contiguous(), _as(q, v).contiguous(), _decays(log_decay, q), state,
+                                   scale, out_state)
