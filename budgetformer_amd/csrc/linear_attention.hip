@@ -49,7 +49,7 @@ struct LinRoles {
   LinArgs role[3];
 };
 
-template <typename T> constexpr int lin_tile() { return sizeof(T) == 2 ? 64 : 32; }
+template <typename T> constexpr int lin_tile(int dx) { return sizeof(T) == 2 && dx < 64 ? 64 : 32; }
 
 // log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
 __device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
@@ -82,12 +82,12 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
-template <typename T, int DX, int DZ, bool OUT>
+template <typename T, int DX, int DZ, bool OUT, bool STATES>
 __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   const LinArgs a = all.role[blockIdx.y];
-  constexpr int C = lin_tile<T>(), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
+  constexpr int C = lin_tile<T>(DX), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
   // parts of the decayed z (see below): the third only for a state that goes out
-  const bool third = a.final_state != nullptr;
+  const bool third = STATES && a.final_state != nullptr;
   constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, __bf16>::value ? 3 : 2;
   using TX = Tile<T, DX>;
   using TZ = Tile<T, DZ>;
@@ -122,13 +122,13 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
       for (int r = 0; r < 16; ++r) m[b][r] = carry[(int64_t(b) * NW * 16 + r) * 64];
   }
   // with states: the sequence of the next tile and its bounds (read again only where one ends)
-  int seq = a.states ? sequence_of(a, begin) : -1, seq_begin = -1, seq_end = a.n;
+  int seq = STATES ? sequence_of(a, begin) : -1, seq_begin = -1, seq_end = a.n;
   auto bounds = [&]() {
     const bool in = seq >= 0 && seq < a.n_seq;
     seq_begin = in ? a.offsets[seq] : -1;
     seq_end = seq < a.n_seq ? a.offsets[seq + 1] : a.n;
   };
-  if (a.states) bounds();
+  if (STATES) bounds();
   auto tile_end = [&](int t0) { return min(min(t0 + C, end), seq_end); };
 
   Stage<T, DX, C, NT> xs, ys;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
       odd = __syncthreads_or(zs.tainted());
     else
       __syncthreads();
-    if (t0 == seq_begin) {                                  // with states: a sequence begins with its tile
+    if (STATES && t0 == seq_begin) {                                  // with states: a sequence begins with its tile
       const int z = fresh(32 * wave + col), x0 = fresh(4 * half);
       const float* s0 = a.init ? a.init + (int64_t(seq) * a.heads + h) * a.dx * a.dz : nullptr;
 #pragma unroll
@@ -171,9 +171,9 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
           m[b][r] = x < a.dx && z < a.dz ? v : 0.f;
         }
     }
-    const bool ends = seq_begin >= 0 && t1 == seq_end;
+    const bool ends = STATES && seq_begin >= 0 && t1 == seq_end;
     const int this_seq = seq;
-    if (a.states && t1 == seq_end && t1 < end) {
+    if (STATES && t1 == seq_end && t1 < end) {
       while (seq < a.n_seq && a.offsets[seq + 1] <= t1) ++seq;
       bounds();
     }
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
       }
       __syncthreads();
       // with states the tile is one sequence's, whose state came in or was begun above
-      const bool into = a.states || first_start < t0;
+      const bool into = STATES || first_start < t0;
       // float16 ends at 65504 and a sum over a sequence need not: such a state is an operand in units of a power of 2
       float unit = 1.f;
       if constexpr (std::is_same<T, _Float16>::value) {
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
                 mf = pack8<T>(m[b], t);
               o = Mat<T>::mma(mf, TX::row_frag_regs(x_lds, i, 2 * b + t, half), o);
             }
-          const bool mine = start_lds[i] < t0 + int(a.states);
+          const bool mine = start_lds[i] < t0 + int(STATES);
           const float f = a.scale * exp2_fast(ld * float(i + 1)) * unit;
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r] = mine ? o[r] * f : 0.f;
@@ -270,13 +270,13 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
     }
 
     if (!OUT || t1 < end || ends) {
-      const bool keep = a.states || last_start < t0;
+      const bool keep = STATES || last_start < t0;
       const float f = exp2_fast(ld * float(len));
 #pragma unroll
       for (int b = 0; b < XB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) m[b][r] = keep ? m[b][r] * f : 0.f;
-      const int from = a.states ? 0 : last_start - t0;
+      const int from = STATES ? 0 : last_start - t0;
       const bool cut = from > 0;
 #pragma unroll 1
       for (int t = 0; t < C / 16; ++t) {
@@ -329,27 +329,37 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   }
 }
 
-// Segments' own contributions -> the state each segment starts from, in place: one lane a value of a head's state, eight
-// segments' values read before the first of them is replaced.
+// Segments' own contributions -> the state each segment starts from, in place: one lane a value of a head's state, the
+// next kCarry segments' values on their way while the last are replaced.
 __global__ __launch_bounds__(256) void linear_carry(const LinRoles all, int64_t values) {
-  const LinArgs& a = all.role[blockIdx.y];
+  constexpr int kCarry = 16;
+  const LinArgs a = all.role[blockIdx.y];
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, step = values * a.heads;
   if (i >= step) return;
   const int h = int(i / values);
   const float f = exp2_fast(decay_log2(a, h) * float(a.seg_len));
   float* c = a.carry + i;
-  float into = 0.f;
-  for (int s0 = 0; s0 < a.n_seg; s0 += 8) {
-    float mine[8];
-    bool began[8];
+  float into = 0.f, mine[kCarry], next[kCarry];
+  int2 span[kCarry];
+  auto fetch = [&](int s0) {             // segments behind the last read it again
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int s = s0 + k, e = (s + 1) * a.seg_len;
-      mine[k] = s < a.n_seg ? c[s * step] : 0.f;
-      began[k] = s + 1 < a.n_seg && start_of(a, span_at(a, e - 1)) >= e - a.seg_len;     // the segment's last sequence began in it
+    for (int k = 0; k < kCarry; ++k) {
+      const int s = min(s0 + k, a.n_seg - 1);
+      next[k] = c[s * step];
+      span[k] = span_at(a, min((s + 1) * a.seg_len, a.n) - 1);
     }
+  };
+  fetch(0);
+  for (int s0 = 0; s0 < a.n_seg; s0 += kCarry) {
+    bool began[kCarry];                  // the segment's last sequence began in it
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < kCarry; ++k) {
+      mine[k] = next[k];
+      began[k] = start_of(a, span[k]) >= (s0 + k) * a.seg_len;
+    }
+    if (s0 + kCarry < a.n_seg) fetch(s0 + kCarry);
+#pragma unroll
+    for (int k = 0; k < kCarry; ++k) {
       if (s0 + k < a.n_seg) c[(s0 + k) * step] = into;
       into = began[k] ? mine[k] : fmaf(into, f, mine[k]);
     }
@@ -476,7 +486,7 @@ int launch(const LinRoles& roles, int n_roles, int32_t dtype, hipStream_t st) {
         constexpr int DX = decltype(px)::value, DZ = decltype(pz)::value;
         const dim3 grid = dim3(unsigned(groups), unsigned(n_roles));
         if (a.n_seg > 1) {
-          auto own = linear_pass<T, DX, DZ, false>;
+          auto own = a.states ? linear_pass<T, DX, DZ, false, true> : linear_pass<T, DX, DZ, false, false>;
           BF_LAUNCH("linear_attn_segments", own, grid, dim3(2 * DZ), 0, st, roles);
           BF_CHECK_LAUNCH();
           const int64_t values = DX * DZ;
@@ -484,7 +494,7 @@ int launch(const LinRoles& roles, int n_roles, int32_t dtype, hipStream_t st) {
                     dim3(256), 0, st, roles, values);
           BF_CHECK_LAUNCH();
         }
-        auto pass = linear_pass<T, DX, DZ, true>;
+        auto pass = a.states ? linear_pass<T, DX, DZ, true, true> : linear_pass<T, DX, DZ, true, false>;
         BF_LAUNCH("linear_attn_pass", pass, grid, dim3(2 * DZ), 0, st, roles);
         BF_CHECK_LAUNCH();
         return BF_OK;
@@ -501,7 +511,8 @@ int run(LinArgs (&pass)[3], int n, int32_t dtype, hipStream_t st) {
     LinRoles r{};
     int m = 0;
     for (int j = i; j < n; ++j)
-      if (!done[j] && pad32(pass[j].dx) == pad32(pass[i].dx) && pad32(pass[j].dz) == pad32(pass[i].dz)) {
+      if (!done[j] && pad32(pass[j].dx) == pad32(pass[i].dx) && pad32(pass[j].dz) == pad32(pass[i].dz) &&
+          pass[j].states == pass[i].states) {
         r.role[m++] = pass[j];
         done[j] = true;
       }
