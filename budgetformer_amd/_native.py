@@ -63,7 +63,7 @@ class LinearAttn(C.Structure):
     _fields_ = [
         ("n", i64), ("n_seq", i64), ("heads", i32), ("dim_k", i32), ("dim_v", i32), ("dtype", i32),
         ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("row_span", vp), ("key_span", vp),
-        ("offsets", vp), ("log_decay", vp), ("init", vp), ("final_state", vp), ("scale", f32), ("reserved", i32),
+        ("offsets", vp), ("log_decay", vp), ("init", vp), ("final_state", vp), ("scale", f32), ("longest", i32),
     ]
 
 

@@ -5,19 +5,23 @@
 // One pass in three uses: the forward is (x, y, z) = (q, k, v); the gradients are (dout, v, k) for dq and, with the
 // packed axis read backwards, (v, dout, q) for dk and (k, q, dout) for dv.
 //
-// Chunked form. A workgroup walks a segment of the packed axis in tiles of C tokens, the state M = sum g^(t - j) y_j z_j^T
+// Chunked form. A workgroup walks a segment of the packed axis in tiles of 32 tokens, the state M = sum g^(t - j) y_j z_j^T
 // in the accumulators of its waves (wave w owns the columns 32w .. 32w+31 of z, so a column of M is a lane's, its rows
-// are registers). Per tile:
-//   W_ij = (x_i . y_j) g^(i - j) for j <= i of the same sequence          C x C, shared through LDS
-//   out_i = scale (sum_j W_ij z_j + g^(i - t0 + 1) x_i M)                 the second only if the sequence began before t0
-//   M = g^C M + sum_j g^(t1 - 1 - j) y_j z_j^T                            only the last row's sequence
-// M's registers are, packed, the operand of x M in register order (packed_tile.h): the state never moves. Tiles are cut
-// from the packed axis, not from the sequences: a boundary is a comparison of indices, and short sequences fill tiles.
-// Where states come in or go out (init, final) tiles end at the sequences' ends instead.
+// are registers). Per tile [t0, t1):
+//   W_ij = scale (x_i . y_j) g^(i - j) for j <= i of the same sequence
+//   out_i = sum_j W_ij z_j + scale g^(i - t0 + 1) x_i M                   the second only if the sequence began before t0
+//   M = g^(t1 - t0) M + sum_j g^(t1 - 1 - j) y_j z_j^T                    only the last row's sequence
+// The registers of W and of M are, packed, operands of the next product as they stand (packed_tile.h): every wave forms
+// W for itself, and the state never moves. (Tiles of 64 tokens share W's four blocks through LDS; their loads on the way
+// leave fewer waves and two barriers more: 90 instead of 57 us for the pass over 8192 tokens, 16 heads of 128, and 110
+// instead of 64 us over 40,000, 8 heads of 16.) Tiles are cut from the packed axis, not from the sequences: a boundary is
+// a comparison of indices, and short sequences fill tiles. Where states come in or go out (init, final) tiles end at the
+// sequences' ends instead.
 //
 // Calls of few heads cut the axis into segments: one launch forms each segment's own contribution to the state, one
-// carries it from segment to segment, and the pass starts from there. States are float32 throughout; as operands M, W and
-// the decayed z are rounded to the activations' type (half a step, as the inputs' own rounding), in float32 not at all.
+// carries it from segment to segment, and the pass starts from there. States are float32 throughout; as operands of x M
+// and W z, M and W are rounded to the activations' type (half a step, as the inputs' own rounding; in float32 not at all);
+// the decayed z that enters the state is given in parts that keep its float32 value.
 #include "packed_tile.h"
 
 namespace bf {
@@ -36,6 +40,7 @@ struct LinArgs {
   int32_t seg_len, n_seg;
   float scale;
   bool reverse, states;
+  bool warm;                       // segments begin with the sequence that their first token is in: nothing is carried
 };
 
 template <typename T> __device__ __forceinline__ Frag<T> pack8_by(const F32x16& x, int t, float by) {
@@ -49,7 +54,7 @@ struct LinRoles {
   LinArgs role[3];
 };
 
-template <typename T> constexpr int lin_tile(int dx) { return sizeof(T) == 2 && dx < 64 ? 64 : 32; }
+constexpr int kTile = 32;        // tokens of a tile
 
 // log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
 __device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
@@ -85,23 +90,22 @@ __device__ __forceinline__ int fresh(int x) {
 template <typename T, int DX, int DZ, bool OUT, bool STATES>
 __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   const LinArgs a = all.role[blockIdx.y];
-  constexpr int C = lin_tile<T>(DX), NW = DZ / 32, NT = 64 * NW, QB = C / 32, XB = DX / 32;
+  constexpr int C = kTile, NW = DZ / 32, NT = 64 * NW, XB = DX / 32;
   // parts of the decayed z (see below): the third only for a state that goes out
   const bool third = STATES && a.final_state != nullptr;
   constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, __bf16>::value ? 3 : 2;
   using TX = Tile<T, DX>;
   using TZ = Tile<T, DZ>;
-  using TW = Tile<T, C>;
   __shared__ __attribute__((aligned(16))) char x_lds[OUT ? TX::bytes(C) : 16];
   __shared__ __attribute__((aligned(16))) char y_lds[TX::bytes(C)];
   __shared__ __attribute__((aligned(16))) char z_lds[TZ::bytes(C)];
-  __shared__ __attribute__((aligned(16))) char w_lds[OUT ? TW::bytes(C) : 16];
   __shared__ int start_lds[C];
   __shared__ __attribute__((aligned(16))) float power[C];       // g^0 .. g^(C - 1), last first: a tile's weights towards its end
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
   const int h = int(slot % a.heads), seg = int(slot / a.heads);     // the heads of a token share its cache lines
-  const int begin = seg * a.seg_len, end = min(begin + a.seg_len, a.n);
+  const int own = seg * a.seg_len, end = min(own + a.seg_len, a.n);
+  const int begin = a.warm && seg > 0 ? min(own, start_of(a, span_at(a, own))) : own;      // rows before `own` are another's
   const float ld = decay_log2(a, h);
   // the axis as the pass reads it: from the last token with steps back, or from the first
   const int64_t back = a.reverse ? a.n - 1 : 0;
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
   for (int b = 0; b < XB; ++b) m[b] = zero16();
   float* carry = a.carry + ((int64_t(seg) * a.heads + h) * XB * NW + wave) * 1024 + lane;       // register r of block b: + (b * NW * 16 + r) * 64
-  if (OUT && seg > 0) {
+  if (OUT && seg > 0 && !a.warm) {
 #pragma unroll
     for (int b = 0; b < XB; ++b)
 #pragma unroll
@@ -181,92 +185,77 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
     if (t1 < end) fetch(t1, next);
 
     const int first_start = start_lds[0], last_start = start_lds[len - 1];
+    // z towards the wave's columns, for out and for the state
+    Frag<T> zf[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) zf[t] = TZ::template col_frag<true>(z_lds, t, wave, lane);
     if constexpr (OUT) {
-      for (int quad = wave; quad < QB * QB; quad += NW) {
-        const int ib = quad / QB, jb = quad % QB;
-        if (jb > ib) continue;
-        F32x16 acc = zero16();
+      const int i = col, from = start_lds[i] - t0;
+      F32x16 acc = zero16(), o = zero16();
 #pragma unroll
-        for (int s = 0; s < TX::kSteps; ++s)
-          acc = Mat<T>::mma(TX::row_frag(y_lds, 32 * jb + col, s, half), TX::row_frag(x_lds, 32 * ib + col, s, half), acc);
-        const int i = 32 * ib + col, from = start_lds[i] - t0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int j = 32 * jb + 8 * g + 4 * half + k;
-            w[k] = j <= i && j >= from ? acc[4 * g + k] * (a.scale * exp2_fast(ld * float(i - j))) : 0.f;
-          }
-          store4<T>(reinterpret_cast<T*>(w_lds + i * TW::kPitch) + 32 * jb + 8 * g + 4 * half, w[0], w[1], w[2], w[3]);
-        }
-      }
-      __syncthreads();
+      for (int s = 0; s < TX::kSteps; ++s)
+        acc = Mat<T>::mma(TX::row_frag(y_lds, col, s, half), TX::row_frag(x_lds, col, s, half), acc);
       // with states the tile is one sequence's, whose state came in or was begun above
-      const bool into = STATES || first_start < t0;
-      // float16 ends at 65504 and a sum over a sequence need not: such a state is an operand in units of a power of 2
-      float unit = 1.f;
-      if constexpr (std::is_same<T, _Float16>::value) {
-        float big = 0.f;
-#pragma unroll
-        for (int b = 0; b < XB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]));
-        if (__any(big > 32768.f)) {
-          for (int o = 32; o; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-          unit = big < INFINITY ? exp2f(ceilf(log2f(big)) - 15.f) : 1.f;
-        }
-      }
-      const float per_unit = 1.f / unit;
-#pragma unroll 1
-      for (int ib = 0; ib < QB; ++ib) {
-        const int i = 32 * ib + col;
-        F32x16 o = zero16();
-        if (into) {
+      if (STATES || first_start < t0) {
+        // float16 ends at 65504 and a sum over a sequence need not: such a state is an operand in units of a power of 2
+        float unit = 1.f;
+        if constexpr (std::is_same<T, _Float16>::value) {
+          float big = 0.f;
 #pragma unroll
           for (int b = 0; b < XB; ++b)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              Frag<T> mf;
-              if constexpr (std::is_same<T, _Float16>::value)
-                mf = pack8_by<T>(m[b], t, per_unit);
-              else
-                mf = pack8<T>(m[b], t);
-              o = Mat<T>::mma(mf, TX::row_frag_regs(x_lds, i, 2 * b + t, half), o);
-            }
-          const bool mine = start_lds[i] < t0 + int(STATES);
-          const float f = a.scale * exp2_fast(ld * float(i + 1)) * unit;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[r] = mine ? o[r] * f : 0.f;
-        }
-        if (!odd) {
-#pragma unroll
-          for (int t = 0; t < C / 16; ++t)
-            if (t < 2 * (ib + 1))
-              o = Mat<T>::mma(TZ::template col_frag<false>(z_lds, t, wave, lane), TW::row_frag(w_lds, i, t, half), o);
-        } else {                          // some z is not finite: NaN for the rows that see it, nothing for the others
-          F32x16 bad = zero16();
-          const int from = start_lds[i] - t0;
-          for (int t = 0; t < 2 * (ib + 1); ++t) {
-            const Frag<T> zf = TZ::template col_frag<false>(z_lds, t, wave, lane);
-            o = Mat<T>::mma(finite<T>(zf), TW::row_frag(w_lds, i, t, half), o);
-            Frag<T> sees;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int j = 16 * t + 8 * half + k;
-              sees[k] = T(j <= i && j >= from ? 1.f : 0.f);
-            }
-            bad = Mat<T>::mma(is_infinite<T>(zf, 1.f), sees, bad);
-            bad = Mat<T>::mma(is_infinite<T>(zf, -1.f), sees, bad);
+            for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]));
+          if (__any(big > 32768.f)) {
+            for (int n = 32; n; n >>= 1) big = fmaxf(big, __shfl_xor(big, n, 64));
+            unit = big < INFINITY ? exp2f(ceilf(log2f(big)) - 15.f) : 1.f;
           }
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (bad[r] > 0.f) o[r] = NAN;
         }
-        if (i < len)
-          store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, 1.f, wave, a.dz,
-                         half);
+        const float per_unit = 1.f / unit;
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            Frag<T> mf;
+            if constexpr (std::is_same<T, _Float16>::value)
+              mf = pack8_by<T>(m[b], t, per_unit);
+            else
+              mf = pack8<T>(m[b], t);
+            o = Mat<T>::mma(mf, TX::row_frag_regs(x_lds, i, 2 * b + t, half), o);
+          }
+        const bool mine = from < int(STATES);
+        const float f = a.scale * exp2_fast(ld * float(i + 1)) * unit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[r] = mine ? o[r] * f : 0.f;
       }
+      float w[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = acc_row(r, half);
+        w[r] = j <= i && j >= from ? acc[r] * (a.scale * exp2_fast(ld * float(i - j))) : 0.f;
+      }
+      if (!odd) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) o = Mat<T>::mma(zf[t], pack8<T>(w, t), o);
+      } else {                            // some z is not finite: NaN for the rows that see it, nothing for the others
+        F32x16 bad = zero16();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          o = Mat<T>::mma(finite<T>(zf[t]), pack8<T>(w, t), o);
+          Frag<T> sees;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int j = 16 * t + acc_row(k, half);
+            sees[k] = T(j <= i && j >= from ? 1.f : 0.f);
+          }
+          bad = Mat<T>::mma(is_infinite<T>(zf[t], 1.f), sees, bad);
+          bad = Mat<T>::mma(is_infinite<T>(zf[t], -1.f), sees, bad);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bad[r] > 0.f) o[r] = NAN;
+      }
+      if (i < len && t0 + i >= own)
+        store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, 1.f, wave, a.dz, half);
     }
 
     if (!OUT || t1 < end || ends) {
@@ -278,15 +267,14 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
         for (int r = 0; r < 16; ++r) m[b][r] = keep ? m[b][r] * f : 0.f;
       const int from = STATES ? 0 : last_start - t0;
       const bool cut = from > 0;
-#pragma unroll 1
-      for (int t = 0; t < C / 16; ++t) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         // the decayed z in two or three parts of the activations' type, which add up to (nearly) its float32 value
-        const Frag<T> z0 = TZ::template col_frag<true>(z_lds, t, wave, lane);
         Frag<T> part[3];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int j = 16 * t + acc_row(k, half);
-          float x = j >= from && j < len ? float(z0[k]) * power[min(j + C - len, C - 1)] : 0.f;
+          float x = j >= from && j < len ? float(zf[t][k]) * power[min(j + C - len, C - 1)] : 0.f;
 #pragma unroll
           for (int n = 0; n < kParts; ++n) {
             part[n][k] = T(x);
@@ -444,23 +432,30 @@ int check(const bf_linear_attn* p, const char* fn) {
     BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,
                  "%s: strides (%lld, %lld) are not whole 16-byte steps", fn, (long long)s[0], (long long)s[1]);
   BF_CHECK_ARG(p->scale == p->scale && p->scale <= 3e38f && p->scale >= -3e38f, "%s: scale %g", fn, double(p->scale));
+  BF_CHECK_ARG(p->longest >= 0, "%s: longest sequence %d", fn, p->longest);
   BF_CHECK_ARG(p->log_decay && (p->n == 0 || (p->row_span && p->key_span)), "%s: no decays or no spans", fn);
   BF_CHECK_ARG(!(p->init || p->final_state) || p->offsets, "%s: states need the offsets", fn);
   return BF_OK;
 }
 
-// Tokens of a segment: whole tiles, so many that about 512 workgroups share the axis (their own contribution and the
-// carries cost a state each, read and written, which a segment of 256 tokens or more outweighs).
+// Tokens of a segment: whole tiles, so many that some 2048 waves share the axis, but at least twice as many as a state
+// has columns (a segment's own contribution and its carry are a state each, written and read, against its tokens' rows).
 int64_t segment_of(const bf_linear_attn* p) {
-  const int64_t want = ceil_div(512, p->heads);
-  const int64_t len = ceil_div(ceil_div(p->n, want), 64) * 64;
-  return len < 256 ? 256 : len;
+  const int64_t columns = pad32(p->dim_k > p->dim_v ? p->dim_k : p->dim_v);
+  const int64_t want = ceil_div(int64_t(2048), p->heads * (columns / 32));
+  const int64_t len = ceil_div(ceil_div(p->n, want), kTile) * kTile;
+  return len < 2 * columns ? 2 * columns : len;
 }
+
+// Whether a segment begins with the whole sequence that its first token is in, instead of being handed that one's state:
+// where no sequence is longer than half a segment (it then walks a quarter more tokens on average, and less when they
+// are shorter; the two launches for the states go).
+bool warms(const bf_linear_attn* p) { return p->longest > 0 && 2 * int64_t(p->longest) <= segment_of(p); }
 
 // Floats that one pass's segments carry.
 int64_t carry_floats(const bf_linear_attn* p) {
   const int64_t segs = ceil_div(p->n, segment_of(p));
-  return segs <= 1 ? 0 : segs * p->heads * pad32(p->dim_k) * pad32(p->dim_v);
+  return segs <= 1 || warms(p) ? 0 : segs * p->heads * pad32(p->dim_k) * pad32(p->dim_v);
 }
 
 LinArgs make_args(const bf_linear_attn* p) {
@@ -472,6 +467,7 @@ LinArgs make_args(const bf_linear_attn* p) {
   a.scale = p->scale;
   a.seg_len = int32_t(segment_of(p));
   a.n_seg = int32_t(ceil_div(p->n, a.seg_len));
+  a.warm = warms(p);
   return a;
 }
 
@@ -485,7 +481,7 @@ int launch(const LinRoles& roles, int n_roles, int32_t dtype, hipStream_t st) {
       return with_pad(a.dz, [&](auto pz) -> int {
         constexpr int DX = decltype(px)::value, DZ = decltype(pz)::value;
         const dim3 grid = dim3(unsigned(groups), unsigned(n_roles));
-        if (a.n_seg > 1) {
+        if (a.n_seg > 1 && !a.warm) {
           auto own = a.states ? linear_pass<T, DX, DZ, false, true> : linear_pass<T, DX, DZ, false, false>;
           BF_LAUNCH("linear_attn_segments", own, grid, dim3(2 * DZ), 0, st, roles);
           BF_CHECK_LAUNCH();
@@ -554,7 +550,7 @@ extern "C" int bf_linear_attn_fwd(const bf_linear_attn* p, const void* q, const 
     BF_CHECK_LAUNCH();
   }
   if (a.n == 0) return BF_OK;
-  BF_CHECK_ARG(a.n_seg == 1 || scratch, "linear_attn_fwd: no scratch (bf_linear_attn_fwd_floats)");
+  BF_CHECK_ARG(a.n_seg == 1 || a.warm || scratch, "linear_attn_fwd: no scratch (bf_linear_attn_fwd_floats)");
   return run(pass, 1, p->dtype, st);
 }
 

@@ -681,7 +681,7 @@ std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& x_in, const std::opt
 
 bf_linear_attn linear_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                            const at::Tensor& row_span, const at::Tensor& key_span, const at::Tensor& offsets, double scale,
-                           const std::optional<at::Tensor>& init_state) {
+                           int64_t longest, const std::optional<at::Tensor>& init_state) {
   const at::Device dev = q.device();
   bf_linear_attn p{};
   p.dtype = dtype_code(q);
@@ -703,6 +703,7 @@ bf_linear_attn linear_args(const at::Tensor& q, const at::Tensor& k, const at::T
   p.row_span = row_span.data_ptr<int32_t>(), p.key_span = key_span.data_ptr<int32_t>();
   p.offsets = offsets.data_ptr<int32_t>(), p.log_decay = log_decay.data_ptr<float>();
   p.scale = float(scale);
+  p.longest = int32_t(std::min<int64_t>(std::max<int64_t>(longest, 0), INT32_MAX));
   if (init_state.has_value() && init_state->defined()) {
     require(*init_state, "init_state", at::kFloat, dev);
     TORCH_CHECK_VALUE(init_state->sizes() == at::IntArrayRef({p.n_seq, H, dk, dv}), "init_state must be [", p.n_seq, ", ", H,
@@ -716,13 +717,14 @@ bf_linear_attn linear_args(const at::Tensor& q, const at::Tensor& k, const at::T
 std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                    const at::Tensor& log_decay, const at::Tensor& row_span,
                                                    const at::Tensor& key_span, const at::Tensor& offsets, double scale,
-                                                   const std::optional<at::Tensor>& init_state, bool return_state) {
+                                                   int64_t longest, const std::optional<at::Tensor>& init_state,
+                                                   bool return_state) {
   TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = as_rows(q_in, "q");
   const at::Tensor k = as_rows(k_in, "k");
   const at::Tensor v = as_rows(v_in, "v");
-  bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
+  bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state);
   at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), scratch;
   at::Tensor state = return_state ? at::empty({p.n_seq, p.heads, p.dim_k, p.dim_v}, log_decay.options())
                                   : at::empty({0}, log_decay.options());
@@ -739,7 +741,7 @@ std::tuple<at::Tensor, at::Tensor> linear_attn_fwd(const at::Tensor& q_in, const
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                                const at::Tensor& log_decay, const at::Tensor& row_span,
                                                                const at::Tensor& key_span, const at::Tensor& offsets,
-                                                               const at::Tensor& dout_in, double scale,
+                                                               const at::Tensor& dout_in, double scale, int64_t longest,
                                                                const std::optional<at::Tensor>& init_state) {
   TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
   const c10::DeviceGuard guard(q_in.device());
@@ -747,7 +749,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor&
   const at::Tensor k = as_rows(k_in, "k");
   const at::Tensor v = as_rows(v_in, "v");
   const at::Tensor dout = as_dense(dout_in);
-  const bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, init_state);
+  const bf_linear_attn p = linear_args(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state);
   require(dout, "dout", q.scalar_type(), q.device());
   TORCH_CHECK_VALUE(dout.sizes() == v.sizes(), "dout ", dout.sizes(), " does not match v ", v.sizes());
   const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
@@ -827,9 +829,9 @@ TORCH_LIBRARY(bf, m) {
   m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
         "bool inverse=False) -> (Tensor, Tensor)");
   m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
-        "float scale, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
+        "float scale, int longest=0, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
   m.def("linear_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
-        "Tensor dout, float scale, Tensor? init_state=None) -> (Tensor, Tensor, Tensor)");
+        "Tensor dout, float scale, int longest=0, Tensor? init_state=None) -> (Tensor, Tensor, Tensor)");
   m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor state, float scale, "
         "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
 }

@@ -297,7 +297,7 @@ class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, seqs, scale, initial_state, return_state):
         out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
-                                                  initial_state, return_state)
+                                          seqs.longest, initial_state, return_state)
         ctx.save_for_backward(q, k, v, log_decay, initial_state)
         ctx.seqs, ctx.scale = seqs, scale
         ctx.mark_non_differentiable(state)
@@ -311,7 +311,7 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, log_decay, init = ctx.saved_tensors
         s = ctx.seqs
         dq, dk, dv = _op("linear_attn_bwd")(q, k, v, log_decay, s.row_span, s.key_span, s.q_offsets, dout,
-                                                  ctx.scale, init)
+                                          ctx.scale, s.longest, init)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -348,7 +348,7 @@ def linear_attention(q, k, v, log_decay, seqs: PackedSequences, scale: Optional[
         out, state = _LinearAttention.apply(q, k, v, log_decay, seqs, scale, initial_state, bool(return_state))
     else:
         out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
-                                            initial_state, bool(return_state))
+                                            seqs.longest, initial_state, bool(return_state))
     return (out, state) if return_state else out
 
 

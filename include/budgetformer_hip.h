@@ -873,7 +873,7 @@ typedef struct bf_linear_attn {
   const float* init;
   float* final_state;
   float scale;
-  int32_t reserved;           /* 0                                           */
+  int32_t longest;            /* no sequence has more rows; 0: unknown       */
 } bf_linear_attn;
 /* scratch: the *_floats call's floats (0: none needed; -1: bad arguments). The
  * gradients are passes of the same form, dq = (dout, v, k) and, on the axis

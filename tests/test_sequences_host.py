@@ -95,7 +95,7 @@ def test_linear_attention_arguments():
 
     for kw, match in ((dict(dtype=5), "dtype"), (dict(n=-1), "sizes"), (dict(heads=0), "sizes"), (dict(n=2 ** 31), "sizes"),
                       (dict(log_decay=None), "decays"), (dict(row_span=None), "spans"), (dict(scale=float("nan")), "scale"),
-                      (dict(init=P, offsets=None), "states"), (dict(final_state=P, offsets=None), "states")):
+                      (dict(init=P, offsets=None), "states"), (dict(longest=-1), "longest"), (dict(final_state=P, offsets=None), "states")):
         with pytest.raises(ValueError, match=match):
             call(_lin(**kw))
         assert N.load().bf_linear_attn_fwd_floats(C.byref(_lin(**kw))) == -1
