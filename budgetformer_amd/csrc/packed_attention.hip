@@ -613,7 +613,18 @@ __global__ __launch_bounds__(256) void packed_spans(const int32_t* q_off, const 
 }
 
 // ---------------------------------------------------------------- launches
-constexpr int kWide = 4;          // waves of a workgroup, each 32 rows (or keys)
+// Waves of a workgroup, of 32 rows (or keys) each. Two walk fewer keys that only a neighbour's rows see and start sooner;
+// more share a tile's loads, which pays where the products of wide 16-bit heads leave time for little else. Forward, dQ,
+// dK and dV with four : two waves, 32,768 rows, 8 heads, not causal, in us: float32 heads of 16, length 50: 60, 80, 103 : 45,
+// 61, 75, length 500: 193, 252, 352 : 180, 238, 311; bfloat16 heads of 64, length 500: 123, 127, 165 : 104, 114, 144, length
+// 2000: 233, 250, 350 : 239, 265, 373; bfloat16 heads of 128 (over 2), length 500: 156, 202, 318 : 198, 198, 318; float16
+// heads of 32, length 130: 47, 59, 57 : 50, 56, 56; float32 heads of 128 (over 2), length 500: 828, 1164, 2039 : 767, 1071, 2704.
+constexpr int fwd_waves(int elem, int dp) { return elem == 2 && (dp == 128 || dp == 32) ? 4 : 2; }
+constexpr int dq_waves(int elem, int dp) { return elem == 2 && dp == 128 ? 4 : 2; }
+// dK and dV of 32 keys of 128 16-bit values fill a wave's registers: eight waves a workgroup stage little enough each that
+// two of them fit a SIMD (with four, some of it leaves the registers, or one wave a SIMD runs: 0.75 and 0.87 instead
+// of 0.61 ms on one causal sequence of 8192, 16 heads over 4).
+constexpr int kv_waves(int elem, int dp) { return dp == 128 ? (elem == 2 ? 8 : 4) : 2; }
 constexpr int kMaxPieces = 64;    // a wave joins them
 
 template <typename T> constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
@@ -681,7 +692,7 @@ dim3 grid_of(const Args& a) {
 // from 512 of them on; below that, one-wave workgroups over pieces of the keys do.
 int pieces_of(const bf_packed_attn* p) {
   const int64_t rows = p->n_q * (p->heads_q / p->heads_k);
-  if (ceil_div(rows, 32 * kWide) * p->heads_k >= 256) return 1;
+  if (ceil_div(rows, 128) * p->heads_k >= 256) return 1;
   const int64_t tiles = ceil_div(rows, 32) * p->heads_k;
   const int64_t want = ceil_div(2048, tiles);
   const int64_t most = ceil_div(p->n_k, 64);
@@ -689,11 +700,6 @@ int pieces_of(const bf_packed_attn* p) {
   if (n > kMaxPieces) n = kMaxPieces;
   return n < 1 ? 1 : int(n);
 }
-
-// Waves of a workgroup of the dK/dV pass: eight where the accumulators of 32 keys (two of 32 x 128) leave no room for a
-// second workgroup's waves otherwise. (With four, V's rows or some accumulators leave the registers, or one wave a
-// SIMD runs: 0.75 and 0.87 instead of 0.61 ms on one causal sequence of 8192, 16 heads of 128 over 4.)
-constexpr int kv_waves(int elem, int dp) { return elem == 2 && dp == 128 ? 8 : kWide; }
 
 // Pieces a key tile's rows are cut into (float32 partial sums, joined in order), where the key tiles are too few to fill
 // the chip and to even out what a causal mask gives them. Equal parts of each tile's own rows, the longest tiles first:
@@ -826,14 +832,14 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
   a.pieces = pieces_of(p);
   const hipStream_t st = as_stream(stream);
   if (a.pieces == 1) {
-    a.tiles = int(ceil_div(a.rows, 32 * kWide));
     return with_type(p->dtype, [&](auto t) -> int {
       using T = decltype(t);
       return with_dim(a.dim, [&](auto dp) -> int {
-        constexpr int DP = decltype(dp)::value, BN = tile_keys<T>();
-        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * kWide, a.rows, scratch, st));
-        auto kern = packed_fwd<T, DP, kWide, BN, false>;
-        BF_LAUNCH("packed_attn_fwd", kern, grid_of(a), dim3(64 * kWide), 0, st, a);
+        constexpr int DP = decltype(dp)::value, BN = tile_keys<T>(), NW = fwd_waves(sizeof(T), DP);
+        a.tiles = int(ceil_div(a.rows, 32 * NW));
+        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
+        auto kern = packed_fwd<T, DP, NW, BN, false>;
+        BF_LAUNCH("packed_attn_fwd", kern, grid_of(a), dim3(64 * NW), 0, st, a);
         BF_CHECK_LAUNCH();
         return BF_OK;
       });
@@ -884,10 +890,11 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
     return with_dim(a.dim, [&](auto dp) -> int {
       constexpr int DP = decltype(dp)::value;
       if (a.rows > 0) {
-        a.tiles = int(ceil_div(a.rows, 32 * kWide));
-        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * kWide, a.rows, scratch, st));
-        auto kern = packed_bwd_q<T, DP, kWide, 32>;
-        BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * kWide), 0, st, a);
+        constexpr int NW = dq_waves(sizeof(T), DP);
+        a.tiles = int(ceil_div(a.rows, 32 * NW));
+        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
+        auto kern = packed_bwd_q<T, DP, NW, 32>;
+        BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * NW), 0, st, a);
         BF_CHECK_LAUNCH();
       }
       if (a.n_k > 0) {
