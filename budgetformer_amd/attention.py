@@ -213,11 +213,15 @@ def _per_head_attention(q, k, v, assign, score_clamp, bias_fn=None, stats=None):
 
 
 class _BatchSequences:
-    """The PackedSequences of the last few (batch, length, device) of dense calls."""
+    """The PackedSequences of the last few (batch, length, device) of dense calls. A copied or pickled module starts
+    with none."""
 
     def __init__(self, size: int = 4):
         self.size = size
         self._d: "OrderedDict" = OrderedDict()
+
+    def __reduce__(self):
+        return _BatchSequences, (self.size,)
 
     def get(self, batch: int, length: int, device: torch.device) -> PackedSequences:
         key = (batch, length, str(device))

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
     seq_end = seq < a.n_seq ? a.offsets[seq + 1] : a.n;
   };
   if (STATES) bounds();
-  auto tile_end = [&](int t0) { return min(min(t0 + C, end), seq_end); };
+  // at least one token on, whatever the offsets hold
+  auto tile_end = [&](int t0) { return max(min(min(t0 + C, end), seq_end), t0 + 1); };
 
   Stage<T, DX, C, NT> xs, ys;
   Stage<T, DZ, C, NT> zs;

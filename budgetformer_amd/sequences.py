@@ -20,6 +20,7 @@ import math
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -35,6 +36,10 @@ def _op(name: str):
 
 
 _OPS: dict = {}
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _as(q: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
@@ -60,7 +65,25 @@ class PackedSequences:
         self.n_q, self.n_k, self.n_seq, self.causal = int(n_q), int(n_k), q_offsets.numel() - 1, bool(causal)
         self.self_attention = q_offsets is k_offsets and self.n_q == self.n_k
         self.row_span, self.key_span, self._positions = _op("packed_spans")(q_offsets, k_offsets, self.n_q, self.n_k,
-                                                                                  self.causal)
+                                                                            self.causal)
+        # the stream that fills them; others wait for it once (see used)
+        self._streams = {_raw_stream(self.device)}
+        self._ready = None
+        if not torch.cuda.is_current_stream_capturing():
+            self._ready = torch.cuda.Event()
+            self._ready.record(torch.cuda.current_stream(self.device))
+
+    def used(self) -> None:
+        """Before a call on the current stream: if another stream filled the spans, this one waits for them, and
+        their memory is not handed out while it may read them."""
+        raw = _raw_stream(self.device)
+        if raw in self._streams or self._ready is None or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(self.device)
+        stream.wait_event(self._ready)
+        for t in (self.q_offsets, self.k_offsets, self.row_span, self.key_span, self._positions):
+            t.record_stream(stream)
+        self._streams.add(raw)
 
     @staticmethod
     def _sizes(n_q: int, n_k: int) -> None:
@@ -116,8 +139,8 @@ class PackedSequences:
         elif sizes[0] is None or sizes[1] is None:
             raise ValueError("without the check the tensors' rows must be given (n_q, and n_k with k_offsets)")
         cls._sizes(int(sizes[0]), int(sizes[1]))
-        q = q_offsets.to(torch.int32).contiguous()
-        k = q if k_offsets is None else k_offsets.to(torch.int32).contiguous()
+        q = q_offsets.to(torch.int32, copy=True).contiguous()          # a copy: the caller's may change
+        k = q if k_offsets is None else k_offsets.to(torch.int32, copy=True).contiguous()
         return cls(q, k, sizes[0], sizes[1], causal, longest)
 
     @staticmethod
@@ -134,6 +157,7 @@ class PackedSequences:
     def positions(self) -> torch.Tensor:
         """int32 [n_q]: each query row's place in its sequence, counted from its first key (0 behind the last
         sequence)."""
+        self.used()
         return self._positions
 
 
@@ -144,6 +168,7 @@ def _check_seqs(seqs, q: torch.Tensor, k: torch.Tensor) -> None:
         raise ValueError(f"the sequences cover ({seqs.n_q} rows, {seqs.n_k} keys), the tensors have ({q.size(0)}, {k.size(0)})")
     if q.device != seqs.device:
         raise ValueError(f"q is on {q.device}, the sequences on {seqs.device}")
+    seqs.used()
 
 
 # ------------------------------------------------------------------ softmax attention
@@ -160,6 +185,7 @@ class _PackedAttention(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, _dlse):
         if dout is None:
             return None, None, None, None, None
@@ -247,6 +273,7 @@ class _Rotary(torch.autograd.Function):
         return (ox, oy) if ctx.two else ox
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx, dy=None):
         positions, = ctx.saved_tensors
         f = ctx.freq
@@ -305,6 +332,7 @@ class _LinearAttention(torch.autograd.Function):
         return out, state
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, _dstate):
         if dout is None:
             return (None,) * 8

@@ -96,6 +96,43 @@ def test_whole_rows_of_many_tiles(hip_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_few_key_tiles_seen_by_many_rows(hip_device, d, dtype):
+    """A group of four heads over one: the key tiles' rows are cut into pieces, whose sums are joined."""
+    _attention_case(hip_device, [1603], [1603], 4, 1, d, True, dtype, seed=29)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d", [(8, 8, 16), (6, 2, 24), (4, 1, 8), (2, 2, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_short_sequences(hip_device, H, Hk, d, causal, dtype):
+    """Sequences of a few tokens take a few lanes a row: rows without keys, keys without rows, a row of one key."""
+    q_lens = [1, 5, 0, 9, 3, 2, 11, 1] * 9
+    k_lens = [1, 5, 4, 2, 3, 7, 11, 0] * 9
+    _attention_case(hip_device, q_lens, k_lens, H, Hk, d, causal, dtype, seed=31)
+
+
+def test_keys_past_32_bit_offsets(hip_device):
+    """A cache of more than 2^31 values: the last sequence's keys lie behind them."""
+    bf = _bf()
+    H, d, far, n = 8, 128, 2 ** 21 - 1000, 6000              # rows of 1024 values
+    k = torch.zeros(far + n, H, d, dtype=torch.bfloat16, device=hip_device)
+    v = torch.zeros_like(k)
+    assert k.numel() > 2 ** 31 + 2 ** 20
+    k[far:], v[far:] = _randn(1, n, H, d, dtype=torch.bfloat16, dev=hip_device), _randn(2, n, H, d, dtype=torch.bfloat16, dev=hip_device)
+    for rows in (1, 300):
+        q = _randn(3, 1 + rows, H, d, dtype=torch.bfloat16, dev=hip_device)
+        seqs = bf.PackedSequences.from_lengths([1, rows], [far, n], causal=True, device=hip_device)
+        out = bf.packed_attention(q, k, v, seqs)
+        ref = sq.attention(q[1:].double(), k[far:].double(), v[far:].double(), [rows], [n], True, d ** -0.5, dtype=torch.bfloat16)
+        _within("out", out[1:], ref["out"], ref["out_bound"])
+        assert bool((out[0] == 0).all())
+    freq = bf.RotaryFrequencies(d, device=hip_device)
+    pos = torch.zeros(far + n, dtype=torch.int32, device=hip_device)
+    assert torch.equal(bf.rotary_embedding(k, None, freq, positions=pos)[far:], k[far:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_large_scores_do_not_overflow(hip_device, dtype):
     bf = _bf()
     q = _randn(1, 100, 2, 64, dtype=dtype, dev=hip_device) * 30
@@ -211,6 +248,43 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(hip_device, dtype):
     xs[2][10] = float("inf")
     out = bf.packed_attention(*xs, seqs)
     assert bool((out[10:50] == float("inf")).all()) and torch.equal(out[:10], clean[0][:10])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_short_sequences_keep_what_they_do_not_see_out(hip_device, dtype):
+    bf = _bf()
+    lens = [5, 3, 6] * 4
+    n = sum(lens) + 7
+    off = torch.tensor([0] + lens).cumsum(0).to(hip_device)
+    seqs = bf.PackedSequences.from_offsets(off, n_q=n, causal=True)
+    assert seqs.longest == 6
+    ld = torch.tensor([-0.05, -0.3], device=hip_device)
+    base = [_randn(i, n, 2, 16, dtype=dtype, dev=hip_device) for i in range(4)]
+    keep = torch.ones(n, dtype=torch.bool, device=hip_device)
+    keep[5:8] = False
+    keep[sum(lens):] = False
+
+    def every(q, k, v, do):
+        got = []
+        for f in (lambda *x: bf.packed_attention(*x, seqs), lambda *x: bf.linear_attention(*x, ld, seqs)):
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+            out = f(*leaves)
+            got += [out, *torch.autograd.grad(out, leaves, do)]
+        return got
+
+    clean = every(*base)
+    for which in range(4):
+        for value in (float("nan"), float("inf")):
+            xs = [x.clone() for x in base]
+            xs[which][5:8] = value
+            xs[which][sum(lens):] = value
+            for i, (a, b) in enumerate(zip(every(*xs), clean)):
+                assert torch.equal(a[keep], b[keep]), (which, value, i)
+                assert bool((a[sum(lens):] == 0).all())
+    xs = [x.clone() for x in base]
+    xs[2][2] = float("inf")
+    out = bf.packed_attention(*xs[:3], seqs)
+    assert bool((out[2:5] == float("inf")).all()) and torch.equal(out[:2], clean[0][:2])
 
 
 def test_results_repeat_bit_for_bit(hip_device):
@@ -450,6 +524,9 @@ def test_core_attention_flash(hip_device, dtype):
         core(q, k, v, torch.zeros(1, S, S, H, device=hip_device), attn_type="flash")
     with pytest.raises(NotImplementedError, match="dropout"):
         CoreAttention(H * d, 0.1, H, 1).train()(q, k, v, attn_type="flash")
+    import copy
+    again = copy.deepcopy(core)
+    assert torch.equal(again(q, k, v, attn_type="flash"), core(q, k, v, attn_type="flash"))
     assert CoreAttention(H * d, 0.1, H, 1).eval()(q, k, v, attn_type="flash").shape == (b, S, H * d)
 
 
@@ -517,6 +594,51 @@ def test_two_streams_at_once(hip_device):
         torch.cuda.synchronize(hip_device)
         for x, y in zip(got, alone):
             assert all(torch.equal(p, r) for p, r in zip(x, y))
+
+
+def test_sequences_built_on_another_stream(hip_device):
+    """A stream that uses sequences another one still builds waits for them; they may be dropped while it reads."""
+    bf = _bf()
+    lens = [300, 40]
+    q = _randn(1, 340, 2, 32, dev=hip_device)
+    ref = bf.packed_attention(q, q, q, bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device))
+    build, use = torch.cuda.Stream(device=hip_device), torch.cuda.Stream(device=hip_device)
+    torch.cuda.synchronize(hip_device)
+    big = torch.randn(4096, 4096, device=hip_device)
+    for _ in range(3):
+        with torch.cuda.stream(build):
+            x = big
+            for _ in range(4):
+                x = x @ big                                    # work before the spans on their stream
+            seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+        with torch.cuda.stream(use):
+            got = bf.packed_attention(q, q, q, seqs)
+        del seqs
+        torch.cuda.synchronize(hip_device)
+        assert torch.equal(got, ref)
+
+
+def test_second_derivatives_are_refused(hip_device):
+    bf = _bf()
+    seqs = bf.PackedSequences.from_lengths([20], causal=True, device=hip_device)
+    q = _randn(1, 20, 2, 16, dev=hip_device).requires_grad_(True)
+    freq, ld = bf.RotaryFrequencies(16, device=hip_device), torch.zeros(2, device=hip_device)
+    for f in (lambda: bf.packed_attention(q, q, q, seqs), lambda: bf.linear_attention(q, q, q, ld, seqs),
+              lambda: bf.rotary_embedding(q, None, freq, seqs=seqs)):
+        g, = torch.autograd.grad(f().square().sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_offsets_that_change_afterwards_do_not_matter(hip_device):
+    bf = _bf()
+    off = torch.tensor([0, 5, 40], dtype=torch.int32, device=hip_device)
+    seqs = bf.PackedSequences.from_offsets(off, causal=True)
+    q, ld = _randn(1, 40, 2, 16, dev=hip_device), torch.full((2,), -0.1, device=hip_device)
+    a = bf.linear_attention(q, q, q, ld, seqs, return_state=True)
+    off.zero_()
+    for x, y in zip(a, bf.linear_attention(q, q, q, ld, seqs, return_state=True)):
+        assert torch.equal(x, y)
 
 
 def test_empty_batches(hip_device):
