@@ -12,6 +12,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -795,6 +797,158 @@ std::tuple<at::Tensor, at::Tensor> linear_attn_step(const at::Tensor& q, const a
   return {out, next};
 }
 
+// ---------------------------------------------------------------- gradients of the operators over packed sequences
+// Formed here and not in Python: a small call's time is its host work (forward and backward of 64 tokens: 48, 42 and 43 us
+// with Python functions, 41, 35 and 36 us so, for the three operators).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool trains(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that raise if they are differentiated again.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list given;
+  for (at::Tensor& g : grads)
+    if (g.defined()) given.push_back(g.detach().set_requires_grad(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with once_differentiable", int64_t(given.size()));
+  variable_list out = (*error)(std::move(given));
+  size_t at = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = out[at++];
+  return grads;
+}
+
+struct PackedAttention : torch::autograd::Function<PackedAttention> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& row_span, const at::Tensor& key_span, double scale, int64_t longest) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, lse, rest] = packed_attn_fwd(q, k, v, row_span, scale, longest, true);
+    ctx->save_for_backward({q, k, v, out, lse, rest, row_span, key_span});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["longest"] = longest;
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    return {out, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(7);
+    if (!grads[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1], out[2]) =
+          packed_attn_bwd(s[0], s[1], s[2], s[6], s[7], s[3], s[4], grads[0], ctx->saved_data["scale"].toDouble(),
+                          ctx->saved_data["longest"].toInt(), s[5]);
+    }
+    return once(std::move(out));
+  }
+};
+
+// packed_attn_fwd's out and lse, with gradients.
+std::tuple<at::Tensor, at::Tensor> packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& row_span, const at::Tensor& key_span, double scale,
+                                                    int64_t longest) {
+  if (trains({&q, &k, &v})) {
+    variable_list r = PackedAttention::apply(q, k, v, row_span, key_span, scale, longest);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [out, lse, rest] = packed_attn_fwd(q, k, v, row_span, scale, longest, false);
+  return {out, lse};
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& y,
+                               const at::Tensor& positions, const at::Tensor& turns, double amplitude, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [ox, oy] = rotary(x, y, positions, turns, amplitude, interleaved, false);
+    ctx->save_for_backward({positions, turns});
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->set_materialize_grads(false);
+    if (!y.has_value()) ctx->mark_non_differentiable({oy});
+    return {ox, oy};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    const at::Tensor &dx = grads[0], &dy = grads[1];
+    if (!dx.defined() && !dy.defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const bool both = dx.defined() && dy.defined();
+      auto [a, b] = rotary(dx.defined() ? dx : dy, both ? std::optional<at::Tensor>(dy) : std::nullopt, s[0], s[1],
+                           ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["interleaved"].toBool(), true);
+      if (dx.defined()) out[0] = a;
+      if (dy.defined()) out[1] = both ? b : a;
+    }
+    return once(std::move(out));
+  }
+};
+
+// rotary of x and y (undefined: none), with gradients.
+std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& x, const std::optional<at::Tensor>& y,
+                                                    const at::Tensor& positions, const at::Tensor& turns, double amplitude,
+                                                    bool interleaved) {
+  const at::Tensor second = y.has_value() ? *y : at::Tensor();
+  if (trains({&x, &second})) {
+    variable_list r = Rotary::apply(x, second.defined() ? std::optional<at::Tensor>(second) : std::nullopt, positions, turns, amplitude, interleaved);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rotary(x, y, positions, turns, amplitude, interleaved, false);
+}
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& log_decay, const at::Tensor& row_span, const at::Tensor& key_span,
+                               const at::Tensor& offsets, double scale, int64_t longest,
+                               const std::optional<at::Tensor>& init_state, bool return_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, state] = linear_attn_fwd(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state, return_state);
+    ctx->save_for_backward({q, k, v, log_decay, row_span, key_span, offsets, init_state.value_or(at::Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["longest"] = longest;
+    ctx->mark_non_differentiable({state});
+    ctx->set_materialize_grads(false);
+    return {out, state};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(11);
+    if (!grads[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1], out[2]) =
+          linear_attn_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], grads[0], ctx->saved_data["scale"].toDouble(),
+                          ctx->saved_data["longest"].toInt(), s[7].defined() ? std::optional<at::Tensor>(s[7]) : std::nullopt);
+    }
+    return once(std::move(out));
+  }
+};
+
+// linear_attn_fwd, with gradients for q, k and v.
+std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& log_decay, const at::Tensor& row_span,
+                                                    const at::Tensor& key_span, const at::Tensor& offsets, double scale,
+                                                    int64_t longest, const std::optional<at::Tensor>& init_state,
+                                                    bool return_state) {
+  if (trains({&q, &k, &v})) {
+    variable_list r =
+        LinearAttention::apply(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state, return_state);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return linear_attn_fwd(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state, return_state);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(bf, m) {
@@ -832,6 +986,13 @@ TORCH_LIBRARY(bf, m) {
         "float scale, int longest=0, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
   m.def("linear_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
         "Tensor dout, float scale, int longest=0, Tensor? init_state=None) -> (Tensor, Tensor, Tensor)");
+  // the same with gradients (packed_attn_bwd, rotary with inverse, linear_attn_bwd)
+  m.def("packed_attention(Tensor q, Tensor k, Tensor v, Tensor row_span, Tensor key_span, float scale, int longest=0) "
+        "-> (Tensor, Tensor)");
+  m.def("rotary_embedding(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False) "
+        "-> (Tensor, Tensor)");
+  m.def("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
+        "float scale, int longest=0, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
   m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor state, float scale, "
         "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
 }
@@ -854,4 +1015,13 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
   m.impl("linear_attn_fwd", &linear_attn_fwd);
   m.impl("linear_attn_bwd", &linear_attn_bwd);
   m.impl("linear_attn_step", &linear_attn_step);
+  m.impl("packed_attention", &packed_attention);
+  m.impl("rotary_embedding", &rotary_embedding);
+  m.impl("linear_attention", &linear_attention);
+}
+
+TORCH_LIBRARY_IMPL(bf, AutogradCUDA, m) {
+  m.impl("packed_attention", &packed_attention);
+  m.impl("rotary_embedding", &rotary_embedding);
+  m.impl("linear_attention", &linear_attention);
 }

@@ -20,7 +20,6 @@ import math
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -172,29 +171,6 @@ def _check_seqs(seqs, q: torch.Tensor, k: torch.Tensor) -> None:
 
 
 # ------------------------------------------------------------------ softmax attention
-class _PackedAttention(torch.autograd.Function):
-    """out, lse (in log2, not differentiable) of packed_attention; HIP forward and backward."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, seqs, scale):
-        out, lse, rest = _op("packed_attn_fwd")(q, k, v, seqs.row_span, scale, seqs.longest, True)
-        ctx.save_for_backward(q, k, v, out, lse, rest)
-        ctx.seqs, ctx.scale = seqs, scale
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, _dlse):
-        if dout is None:
-            return None, None, None, None, None
-        q, k, v, out, lse, rest = ctx.saved_tensors
-        dq, dk, dv = _op("packed_attn_bwd")(q, k, v, ctx.seqs.row_span, ctx.seqs.key_span, out, lse, dout,
-                                                  ctx.scale, ctx.seqs.longest, rest)
-        return dq, dk, dv, None, None
-
-
 def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = None, with_lse: bool = False):
     """softmax(scale q k^T) v inside each sequence of a packed batch.
 
@@ -206,10 +182,7 @@ def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = No
     _check_seqs(seqs, q, k)
     k, v = _as(q, k), _as(q, v)
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
-    if _trains(q, k, v):
-        out, lse = _PackedAttention.apply(q, k, v, seqs, scale)
-    else:
-        out, lse, _ = _op("packed_attn_fwd")(q, k, v, seqs.row_span, scale, seqs.longest, False)
+    out, lse = _op("packed_attention")(q, k, v, seqs.row_span, seqs.key_span, scale, seqs.longest)
     return (out, lse * math.log(2.0)) if with_lse else out
 
 
@@ -261,36 +234,6 @@ class RotaryFrequencies:
         return got
 
 
-class _Rotary(torch.autograd.Function):
-    """x and, if given, y turned by their positions; the gradient is turned back."""
-
-    @staticmethod
-    def forward(ctx, x, y, positions, freq, interleaved):
-        ctx.save_for_backward(positions)
-        ctx.freq, ctx.interleaved, ctx.two = freq, interleaved, y is not None
-        ctx.set_materialize_grads(False)
-        ox, oy = _op("rotary")(x, y, positions, freq.turns, freq.amplitude, interleaved, False)
-        return (ox, oy) if ctx.two else ox
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dx, dy=None):
-        positions, = ctx.saved_tensors
-        f = ctx.freq
-        given = [g for g in (dx, dy) if g is not None]
-        if not given:
-            return None, None, None, None, None
-        got = _op("rotary")(given[0], given[1] if len(given) == 2 else None, positions, f.turns, f.amplitude, ctx.interleaved,
-                            True)
-        if len(given) == 2:
-            dx, dy = got
-        elif dx is not None:
-            dx = got[0]
-        else:
-            dy = got[0]
-        return dx, dy, None, None, None
-
-
 def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optional[torch.Tensor] = None,
                      seqs: Optional[PackedSequences] = None, interleaved: bool = False):
     """q (and k) [rows, heads, hn] with the first ``freq.rot`` values of every head turned by the row's position.
@@ -311,38 +254,11 @@ def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optio
     k = None if k is None else _as(q, k)
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    if _trains(q, k):
-        return _Rotary.apply(q, k, positions, freq, bool(interleaved))
-    got = _op("rotary")(q, k, positions, freq.turns, freq.amplitude, bool(interleaved), False)
+    got = _op("rotary_embedding")(q, k, positions, freq.turns, freq.amplitude, bool(interleaved))
     return got[0] if k is None else got
 
 
 # ------------------------------------------------------------------ linear attention
-class _LinearAttention(torch.autograd.Function):
-    """out and the final state (not differentiable); the gradients are passes of the same form."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, seqs, scale, initial_state, return_state):
-        out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
-                                          seqs.longest, initial_state, return_state)
-        ctx.save_for_backward(q, k, v, log_decay, initial_state)
-        ctx.seqs, ctx.scale = seqs, scale
-        ctx.mark_non_differentiable(state)
-        ctx.set_materialize_grads(False)
-        return out, state
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, _dstate):
-        if dout is None:
-            return (None,) * 8
-        q, k, v, log_decay, init = ctx.saved_tensors
-        s = ctx.seqs
-        dq, dk, dv = _op("linear_attn_bwd")(q, k, v, log_decay, s.row_span, s.key_span, s.q_offsets, dout,
-                                          ctx.scale, s.longest, init)
-        return dq, dk, dv, None, None, None, None, None
-
-
 def _decays(log_decay, q) -> torch.Tensor:
     if not isinstance(log_decay, torch.Tensor) or log_decay.dim() != 1 or log_decay.size(0) != q.size(1):
         raise ValueError(f"log_decay must be [{q.size(1)}]")
@@ -372,11 +288,8 @@ def linear_attention(q, k, v, log_decay, seqs: PackedSequences, scale: Optional[
         initial_state = initial_state.float().contiguous()
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     log_decay = _decays(log_decay, q)
-    if _trains(q, k, v):
-        out, state = _LinearAttention.apply(q, k, v, log_decay, seqs, scale, initial_state, bool(return_state))
-    else:
-        out, state = _op("linear_attn_fwd")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
-                                            seqs.longest, initial_state, bool(return_state))
+    out, state = _op("linear_attention")(q, k, v, log_decay, seqs.row_span, seqs.key_span, seqs.q_offsets, scale,
+                                         seqs.longest, initial_state, bool(return_state))
     return (out, state) if return_state else out
 
 
