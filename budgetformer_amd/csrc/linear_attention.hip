@@ -425,7 +425,7 @@ int check(const bf_linear_attn* p, const char* fn) {
       set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_k, p->dim_v);
       return BF_ERR_UNSUPPORTED;
     }
-  BF_CHECK_ARG(p->n >= 0 && p->n < (int64_t(1) << 31) - 256 && p->n_seq >= 0 && p->n_seq < (int64_t(1) << 31) - 1 &&
+  BF_CHECK_ARG(p->n >= 0 && p->n < kMaxRows && p->n_seq >= 0 && p->n_seq < (int64_t(1) << 31) - 1 &&
                    p->heads >= 1 && p->heads <= (1 << 20),
                "%s: bad sizes (%lld rows, %lld sequences, %d heads)", fn, (long long)p->n, (long long)p->n_seq, p->heads);
   const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;

@@ -21,7 +21,7 @@ struct ShortArgs {
   const int2 *row_span, *key_span;
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;
   int32_t n_rows, n_keys;          // (token, head) pairs of the queries, of the keys
-  int32_t n_k, hq, hk, group, dim;
+  int32_t n_q, n_k, hq, hk, group, dim;
   Div by_hq, by_hk, by_group;
   float scale, c;
 };
@@ -169,6 +169,7 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
   if (item < a.n_keys) {                             // dK and dV of a key, over its rows and their heads of the group
     const int key = int(a.by_hk(uint32_t(item))), h = int(item) - key * a.hk;
     const int2 span = a.key_span[key];
+    const int lo = max(span.x, 0), hi = min(span.y, a.n_q);
     Ch k, v, dk, dv;
     k.set(Ch::raw(static_cast<const T*>(a.k) + key * a.ks_t + h * a.ks_h + d));
     v.set(Ch::raw(static_cast<const T*>(a.v) + key * a.vs_t + h * a.vs_h + d));
@@ -176,12 +177,12 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
     dk.zero(), dv.zero();
     constexpr int U = 2;
     for (int head = h * a.group; head < (h + 1) * a.group; ++head) {
-      for (int i = span.x; i < span.y; i += U) {
+      for (int i = lo; i < hi; i += U) {
         uint4 qr[U], gr[U], orr[U];
         float stat[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int row = min(i + u, span.y - 1);
+          const int row = min(i + u, hi - 1);
           const int64_t r = int64_t(row) * a.hq + head;
           qr[u] = Ch::raw(qp + row * a.qs_t + head * a.qs_h);
           gr[u] = Ch::raw(gp + r * a.dim);
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
           if (!mine) q.zero(), g.zero(), o.zero();
           const float s = row_sum<LPR>(q.dot(k)), dp = row_sum<LPR>(g.dot(v)), delta = row_sum<LPR>(g.dot(o));
           const float p = exp2_fast(fmaf(s, a.c, stat[u] == -INFINITY ? -INFINITY : -stat[u]));
-          if (i + u < span.y) {
+          if (i + u < hi) {
             dv.add(p, g);
             dk.add(p * (dp - delta), q);
           }
@@ -220,7 +221,7 @@ ShortArgs make_args(const bf_packed_attn* p, const void* q, const void* k, const
   a.hq = p->heads_q, a.hk = p->heads_k, a.group = p->heads_q / p->heads_k, a.dim = p->head_dim;
   a.n_rows = int32_t(p->n_q * a.hq);
   a.n_keys = int32_t(p->n_k * a.hk);
-  a.n_k = int32_t(p->n_k);
+  a.n_q = int32_t(p->n_q), a.n_k = int32_t(p->n_k);
   a.by_hq = make_div(uint32_t(a.hq)), a.by_hk = make_div(uint32_t(a.hk)), a.by_group = make_div(uint32_t(a.group));
   a.scale = p->scale, a.c = p->scale * kLog2e;
   return a;
@@ -252,7 +253,7 @@ template <typename F> int with_lanes(const bf_packed_attn* p, F&& f) {
 bool packed_is_short(const bf_packed_attn* p) {
   const int64_t row = int64_t(p->head_dim) * (p->dtype == BF_DTYPE_F32 ? 4 : 2);
   return p->longest > 0 && p->longest <= 24 && p->longest * row <= (p->dtype == BF_DTYPE_F32 ? 2048 : 1024) &&
-         p->n_k < ((int64_t(1) << 31) - 256) / p->heads_k;
+         p->n_k < kMaxRows / p->heads_k;
 }
 
 int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,

@@ -17,6 +17,9 @@ typedef float F32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Rows of an axis at most: the end of a tile, of a piece of one or of a segment may lie behind the last row, in 32 bits.
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - (1 << 17);
+
 template <typename T> struct Mat;
 
 template <> struct Mat<__bf16> {

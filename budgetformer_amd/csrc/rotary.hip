@@ -169,7 +169,7 @@ extern "C" int bf_rotary(const void* x, const void* y, int64_t n, int32_t heads_
   BF_CHECK_ARG(x && out_x && x_stride && (heads_y == 0 || (y && out_y && y_stride)) && positions && turns,
                "rotary: bad arguments");
   // one workgroup's items are counted in 32 bits
-  BF_CHECK_ARG(int64_t(16) * (int64_t(heads_x) + heads_y) * dim < (int64_t(1) << 31), "rotary: a token of %d heads of %d",
+  BF_CHECK_ARG(int64_t(16) * (int64_t(heads_x) + heads_y) * dim <= (int64_t(1) << 30), "rotary: a token of %d heads of %d",
                heads_x + heads_y, dim);
   RotaryArgs a{};
   a.x = x, a.y = y, a.ox = out_x, a.oy = out_y;

@@ -23,7 +23,7 @@ import torch
 
 from . import _native as N
 
-_MOST_ROWS = 2 ** 31 - 256
+_MOST_ROWS = 2 ** 31 - 2 ** 17
 
 
 def _op(name: str):
@@ -87,7 +87,7 @@ class PackedSequences:
     @staticmethod
     def _sizes(n_q: int, n_k: int) -> None:
         if not (0 <= n_q < _MOST_ROWS and 0 <= n_k < _MOST_ROWS):
-            raise ValueError(f"{n_q} query rows and {n_k} keys (below 2^31 - 256 each)")
+            raise ValueError(f"{n_q} query rows and {n_k} keys (below 2^31 - 2^17 each)")
 
     @classmethod
     def from_lengths(cls, q_lengths: Sequence[int], k_lengths: Optional[Sequence[int]] = None, *, causal: bool = False,

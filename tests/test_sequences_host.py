@@ -23,6 +23,9 @@ def _attn(**kw):
     return a
 
 
+_TWO = (C.c_int64 * 2)(8, 8)
+
+
 def _fwd(a, q=P, k=P, v=P, out=P):
     N.call("bf_packed_attn_fwd", C.byref(a), q, k, v, out, None, P, P, None)
 
@@ -42,6 +45,20 @@ def test_packed_attention_arguments(kw, match):
 def test_packed_attention_head_dims(d):
     with pytest.raises(NotImplementedError, match="head_dim"):
         _fwd(_attn(head_dim=d))
+
+
+def test_rows_leave_room_for_a_tile_behind_the_last():
+    """Ends of tiles, pieces and segments are formed in 32 bits, behind the last row too."""
+    most = 2 ** 31 - 2 ** 17
+    lib = N.load()
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(n_k=most - 1))) >= 0
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(n_k=most))) == -1
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(n_q=most // 2 - 1))) >= 0
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(n_q=most // 2))) == -1
+    assert lib.bf_linear_attn_fwd_floats(C.byref(_lin(n=most - 1))) >= 0
+    assert lib.bf_linear_attn_fwd_floats(C.byref(_lin(n=most))) == -1
+    with pytest.raises(ValueError, match="a token of"):
+        N.call("bf_rotary", P, None, 1, 2 ** 20, 0, 65, 2, 0, _TWO, _TWO, P, 1, P, 1.0, 0, 0, P, None, None)
 
 
 def test_packed_attention_addresses_and_strides():
@@ -147,7 +164,8 @@ def test_host_tensors_and_bad_lengths_are_refused():
 
 def test_operators_are_registered():
     ops = N.load_ops()
-    for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_fwd", "linear_attn_bwd", "linear_attn_step"):
+    for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_fwd", "linear_attn_bwd", "linear_attn_step",
+                 "packed_attention", "rotary_embedding", "linear_attention"):
         assert str(getattr(ops, name).default._schema).startswith(f"bf::{name}(")
 
 
