@@ -10,6 +10,7 @@
 // integers, in the order of kIndexTensors and make_index below
 // (budgetformer_amd.hip_ops.AttentionIndex.op_args builds them).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -790,6 +791,13 @@ std::tuple<at::Tensor, at::Tensor> linear_attn_step(const at::Tensor& q, const a
   }
   at::Tensor out = at::empty_like(v), next = given ? *out_state : at::empty_like(state);
   if (n == 0) return {out, next};
+  if (given) {
+    const auto apart = at::MemOverlapStatus::No, same = at::MemOverlapStatus::Full, states = at::get_overlap_status(next, state);
+    TORCH_CHECK_VALUE(states == apart || states == same, "out_state overlaps state and is not state itself");
+    for (const at::Tensor* t : {&q, &k, &v, &log_decay})
+      TORCH_CHECK_VALUE(at::get_overlap_status(next, *t) == apart, "out_state overlaps an input");
+    next.unsafeGetTensorImpl()->bump_version();          // a gradient that kept the old state is refused, not wrong
+  }
   check_rc(bf_linear_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr<float>(), state.data_ptr<float>(), n,
                                int32_t(H), int32_t(dk), int32_t(dv), code, float(scale), out.data_ptr(),
                                next.data_ptr<float>(), stream_of(q)),

@@ -297,8 +297,8 @@ def linear_attention_step(q, k, v, log_decay, state, scale: Optional[float] = No
                           out_state: Optional[torch.Tensor] = None):
     """One token of each of n sequences: (out [n, heads, dv], new state). q and k [n, heads, dk], v [n, heads, dv],
     state float32 [n, heads, dk, dv]. ``out_state``: where the new state is written (``state`` itself updates it in
-    place), else a new tensor. For inference: no gradients."""
-    if _trains(q, k, v, state):
+    place; anything else must not overlap it), else a new tensor. For inference: no gradients."""
+    if _trains(q, k, v, state, out_state):
         raise NotImplementedError("linear_attention_step has no gradients (linear_attention has)")
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     return _op("linear_attn_step")(q.contiguous(), _as(q, k).contiguous(), _as(q, v).contiguous(), _decays(log_decay, q), state,

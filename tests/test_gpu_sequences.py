@@ -437,6 +437,35 @@ def test_linear_attention_step_continues_a_prompt(hip_device, n, H, dk, dv, dtyp
     assert same.data_ptr() == s.data_ptr() and torch.equal(s, new) and torch.equal(got, out)
 
 
+def test_linear_attention_step_states_that_overlap(hip_device):
+    bf = _bf()
+    n, H, d = 4, 2, 16
+    store = _randn(1, n + 1, H, d, d, dev=hip_device)
+    q, ld = _randn(2, n, H, d, dev=hip_device), torch.full((H,), -0.5, device=hip_device)
+    for state, into in ((store[:n], store[1:]), (store[1:], store[:n])):
+        with pytest.raises(ValueError, match="overlaps state"):
+            bf.linear_attention_step(q, q, q, ld, state, out_state=into)
+    room = torch.zeros(n * H * d * d, device=hip_device)
+    inside = room[:n * H * d].view(n, H, d)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        bf.linear_attention_step(q, inside, q, ld, store[:n], out_state=room.view(n, H, d, d))
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        bf.linear_attention_step(q, q, q, ld, store[:n], out_state=room.view(n, H, d, d).requires_grad_(True))
+
+
+def test_a_state_updated_in_place_does_not_change_a_gradient_that_kept_it(hip_device):
+    bf = _bf()
+    seqs = bf.PackedSequences.from_lengths([5, 7], causal=True, device=hip_device)
+    x, ld = _randn(1, 12, 2, 16, dev=hip_device).requires_grad_(True), torch.full((2,), -0.5, device=hip_device)
+    state, one = _randn(2, 2, 2, 16, 16, dev=hip_device), _randn(3, 2, 2, 16, dev=hip_device)
+    out = bf.linear_attention(x, x, x, ld, seqs, initial_state=state)
+    bf.linear_attention_step(one, one, one, ld, state)              # into a new tensor: nothing changes
+    torch.autograd.grad(out.sum(), x, retain_graph=True)
+    bf.linear_attention_step(one, one, one, ld, state, out_state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.sum(), x)
+
+
 # ------------------------------------------------------------------ together, as they are used
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_prompt_then_single_tokens_equal_the_whole(hip_device, dtype):
