@@ -687,11 +687,19 @@ dim3 grid_of(const Args& a) {
   return dim3(unsigned(ceil_div(a.hk / a.xcd_groups * per, each) * kXcds));
 }
 
-// Pieces a tile's keys are cut into. Workgroups of 4 waves over whole rows fill the chip (256 CUs, two workgroups each)
-// from 512 of them on; below that, one-wave workgroups over pieces of the keys do.
+// Pieces a tile's keys are cut into. From some number of rows on, workgroups over whole rows fill the chip (256 CUs); below
+// that, one-wave workgroups over pieces of the keys do. Whole : pieces in us, one causal sequence of keys with the last
+// (workgroups of 128 rows) of them as rows:
+//   16 bits, heads of 128 (16 over 4): 2000 keys (64) 58 : 49, (96) 57 : 67, (136) 60 : 82; 8192 keys (72) 204 : 167, (96) 203 :
+//     211, (136) 208 : 298, (248) 209 : 383
+//   16 bits, heads of 64: 2000 keys (136) 42 : 38, (248) 43 : 43, (264) 43 : 52; 8192 keys (136) 158 : 141, (264) 160 : 177;
+//     heads of 32: 2000 keys (136) 34 : 31, (264) 35 : 42; 8192 keys (136) 125 : 83, (264) 127 : 125, (504) 129 : 136
+//   float32, heads of 16: 2000 keys (264) 81 : 67, (504) 82 : 72; 8192 keys (264) 427 : 311; heads of 128 (16 over 2): 2000
+//     keys (264) 307 : 194, (504) 309 : 201; 8192 keys (264) 1902 : 1666, (504) 1898 : 2049
 int pieces_of(const bf_packed_attn* p) {
   const int64_t rows = p->n_q * (p->heads_q / p->heads_k);
-  if (ceil_div(rows, 128) * p->heads_k >= 256) return 1;
+  const int64_t enough = p->dtype == BF_DTYPE_F32 ? 512 : p->head_dim > 64 ? 96 : 256;
+  if (ceil_div(rows, 128) * p->heads_k >= enough) return 1;
   const int64_t tiles = ceil_div(rows, 32) * p->heads_k;
   const int64_t want = ceil_div(2048, tiles);
   const int64_t most = ceil_div(p->n_k, 64);
