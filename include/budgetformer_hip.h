@@ -820,8 +820,8 @@ typedef struct bf_packed_attn {
 /* out = softmax(scale q k^T over the row's keys) v, contiguous [n_q, heads_q,
  * head_dim] in q's dtype; lse float32 [n_q, heads_q]: the log2 of the row's sum
  * of exp(scale q.k). A row that sees no key has out 0 and lse -inf. scratch:
- * bf_packed_attn_fwd_floats(p) floats (0: none needed; -1: bad arguments), for
- * calls of few rows, whose keys are cut into pieces, and of sequences of very
+ * bf_packed_attn_fwd_floats(p) floats, 16-byte aligned (0: none needed; -1: bad
+ * arguments), for calls of few rows, whose keys are cut into pieces, and of sequences of very
  * different lengths, whose tiles are put in order. rest (or NULL): like out,
  * what out's rounding left, for the backward; bf_packed_attn_rest(p) says
  * whether the backward reads it.                                            */
@@ -832,8 +832,9 @@ int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, co
 /* Gradients of it: dq like out, dk and dv contiguous [n_k, heads_k, head_dim]
  * (summed over the heads of a group). out, dout: contiguous. rest: the
  * forward's, or NULL (Delta then comes from the rounded out). delta: scratch of
- * n_q * heads_q floats; scratch: bf_packed_attn_bwd_floats(p) floats (0: none
- * needed; -1: bad arguments). No atomics: results repeat bit for bit.       */
+ * n_q * heads_q floats; scratch: bf_packed_attn_bwd_floats(p) floats, 16-byte
+ * aligned (0: none needed; -1: bad arguments). No atomics: results repeat bit
+ * for bit.                                                                  */
 int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p);
 int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
                        const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, float* scratch,
@@ -875,10 +876,10 @@ typedef struct bf_linear_attn {
   float scale;
   int32_t longest;            /* no sequence has more rows; 0: unknown       */
 } bf_linear_attn;
-/* scratch: the *_floats call's floats (0: none needed; -1: bad arguments). The
- * gradients are passes of the same form, dq = (dout, v, k) and, on the axis
- * read backwards, dk = (v, dout, q) and dv = (k, q, dout); contiguous, as dout
- * is. The decays and states are constants.                                  */
+/* scratch: the *_floats call's floats, 16-byte aligned (0: none needed; -1: bad
+ * arguments). The gradients are passes of the same form, dq = (dout, v, k) and,
+ * on the axis read backwards, dk = (v, dout, q) and dv = (k, q, dout);
+ * contiguous, as dout is. The decays and states are constants.              */
 int64_t bf_linear_attn_fwd_floats(const bf_linear_attn* p);
 int bf_linear_attn_fwd(const bf_linear_attn* p, const void* q, const void* k, const void* v, void* out, float* scratch,
                        void* stream);

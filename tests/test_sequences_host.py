@@ -134,6 +134,18 @@ def test_linear_attention_arguments():
     N.call("bf_linear_attn_step", P, P, P, P, P, 0, 1, 16, 16, 0, 1.0, P, P, None)
 
 
+def test_scratch_addresses():
+    off = C.c_void_p(P.value + 4)
+    with pytest.raises(ValueError, match="scratch must be 16-byte aligned"):
+        N.call("bf_packed_attn_fwd", C.byref(_attn()), P, P, P, P, None, P, off, None)
+    with pytest.raises(ValueError, match="scratch must be 16-byte aligned"):
+        N.call("bf_packed_attn_bwd", C.byref(_attn()), P, P, P, P, None, P, P, P, P, P, P, off, None)
+    with pytest.raises(ValueError, match="scratch must be 16-byte aligned"):
+        N.call("bf_linear_attn_fwd", C.byref(_lin()), P, P, P, P, off, None)
+    with pytest.raises(ValueError, match="aligned"):
+        N.call("bf_linear_attn_bwd", C.byref(_lin()), P, P, P, P, P, P, P, off, None)
+
+
 def test_spans_arguments():
     with pytest.raises(ValueError, match="32 bits"):
         N.call("bf_packed_spans", P, P, 1, 2 ** 31, 4, 0, P, P, None, None)
