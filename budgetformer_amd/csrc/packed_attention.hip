@@ -626,6 +626,10 @@ __global__ __launch_bounds__(256) void packed_spans(const int32_t* q_off, const 
 // heads of 32, length 130: 47, 59, 57 : 50, 56, 56; float32 heads of 128 (over 2), length 500: 828, 1164, 2039 : 767, 1071, 2704.
 constexpr int fwd_waves(int elem, int dp) { return elem == 2 && (dp == 128 || dp == 32) ? 4 : 2; }
 constexpr int dq_waves(int elem, int dp) { return elem == 2 && dp == 128 ? 4 : 2; }
+// Keys of a tile of the dQ pass: more where their products are short (32 : 64 keys in us; 8 heads of 16, bfloat16, 256
+// graphs of 9 to 250 nodes 55 : 49, two causal sequences of 8000 181 : 159; heads of 32, float16: 63 : 61, 192 : 188; heads of 64:
+// 72 : 75, 264 : 260).
+constexpr int dq_keys(int elem, int dp) { return elem == 2 && dp <= 32 ? 64 : 32; }
 // dK and dV of 32 keys of 128 16-bit values fill a wave's registers: eight waves a workgroup stage little enough each that
 // two of them fit a SIMD (with four, some of it leaves the registers, or one wave a SIMD runs: 0.75 and 0.87 instead
 // of 0.61 ms on one causal sequence of 8192, 16 heads over 4).
@@ -839,7 +843,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
   BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
   if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
   Args a = make_args(p, q, k, v);
-  BF_CHECK_ARG(aligned16({rest}), "packed_attn_fwd: rest must be 16-byte aligned");
+  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_fwd: rest and scratch must be 16-byte aligned");
   a.o = out, a.rest = rest, a.lse = lse;
   a.pieces = pieces_of(p);
   const hipStream_t st = as_stream(stream);
@@ -893,7 +897,7 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
   BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
   if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, as_stream(stream));
   Args a = make_args(p, q, k, v);
-  BF_CHECK_ARG(aligned16({rest}), "packed_attn_bwd: rest must be 16-byte aligned");
+  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_bwd: rest and scratch must be 16-byte aligned");
   a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   a.lse = const_cast<float*>(lse);
   const hipStream_t st = as_stream(stream);
@@ -905,7 +909,7 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
         constexpr int NW = dq_waves(sizeof(T), DP);
         a.tiles = int(ceil_div(a.rows, 32 * NW));
         BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
-        auto kern = packed_bwd_q<T, DP, NW, 32>;
+        auto kern = packed_bwd_q<T, DP, NW, dq_keys(sizeof(T), DP)>;
         BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * NW), 0, st, a);
         BF_CHECK_LAUNCH();
       }
