@@ -252,10 +252,19 @@ template <typename F> int with_lanes(const bf_packed_attn* p, F&& f) {
 //   bfloat16, heads of 64: 4 keys 138..146 : 227, 8 keys 178..217 : 229, 16 keys 270..367 : 233
 //   bfloat16, heads of 128: 4 keys 200..265 : 254, 8 keys 318..473 : 253
 //   float32, heads of 64:  4 keys 285..329 : 665, 8 keys 403..509 : 669, 16 keys 663..916 : 668
+// Heads that share keys fill a tile with fewer tokens, which masks less of it (100,000 rows, 5, 12 and 24 tokens):
+//   float16, 32 heads of 16 over 8: 392, 524, 880 : 442, 441, 447; bfloat16, 32 of 32 over 4: 642, 906, 1562 : 559, 560, 573
+//   float32, 16 heads of 16 over 1: 271, 365, 601 : 399, 413, 462; 16 of 64 over 2: 1123, 1657, 2899 : 1284, 1296, 1359
+// A call of few rows leaves most of the chip idle either way and is as long as its longest chain, for lanes the rows of a
+// key's group (2000 rows, 12 and 24 tokens; float16, 8 heads of 128 over 4: 39, 60 : 78, 80; bfloat16, 16 of 64 over 8: 37, 56 : 37, 37):
+//   bfloat16, 8 of 64: 27, 38 : 45, 45; float32, 8 of 128: 87, 103 : 123, 123
 bool packed_is_short(const bf_packed_attn* p) {
-  const int64_t row = int64_t(p->head_dim) * (p->dtype == BF_DTYPE_F32 ? 4 : 2);
-  return p->longest > 0 && p->longest <= 24 && p->longest * row <= (p->dtype == BF_DTYPE_F32 ? 2048 : 1024) &&
-         p->n_k < kMaxRows / p->heads_k;
+  const bool wide = p->dtype == BF_DTYPE_F32;
+  const int64_t row = int64_t(p->head_dim) * (wide ? 4 : 2), group = p->heads_q / p->heads_k;
+  if (p->longest <= 0 || p->longest > 24 || p->n_k >= kMaxRows / p->heads_k) return false;
+  const int64_t most = group > 2 ? (wide ? 1280 : 256) : (wide ? 2048 : 1024);
+  const bool few = p->longest * group <= 40 && p->n_q * p->heads_q * row <= (int64_t(wide ? 8 : 4) << 20);
+  return few || p->longest * row <= most;
 }
 
 int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
