@@ -103,6 +103,20 @@ def test_few_key_tiles_seen_by_many_rows(hip_device, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d,lens", [(32, 2, 128, [5] * 60), (16, 1, 64, [100] * 4 + [37]), (8, 1, 16, [12, 24, 3] * 20)])
+def test_key_tiles_of_several_sequences_in_pieces(hip_device, H, Hk, d, lens, dtype):
+    """Few key tiles, each of several sequences whose rows are cut into pieces."""
+    _attention_case(hip_device, lens, lens, H, Hk, d, True, dtype, seed=30)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d", [(2, 2, 128), (4, 2, 72)])
+def test_few_rows_of_wide_heads(hip_device, H, Hk, d, dtype):
+    """Short sequences of few rows take a few lanes a row at any head size."""
+    _attention_case(hip_device, [20, 1, 7, 16], [20, 4, 0, 16], H, Hk, d, False, dtype, seed=32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,Hk,d", [(8, 8, 16), (6, 2, 24), (4, 1, 8), (2, 2, 40)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_short_sequences(hip_device, H, Hk, d, causal, dtype):
@@ -394,6 +408,17 @@ def test_linear_attention_head_sizes(hip_device, dk, dv, dtype):
 def test_linear_attention_over_segments(hip_device, init, dtype):
     """More tokens than a segment (256): the state is carried across, past a sequence's end inside a segment too."""
     _linear_case(hip_device, [700, 50, 256, 6, 500], 2, 16, 16, dtype, seed=41, init=init)
+
+
+@pytest.mark.parametrize("lens", [[20000], [9000, 3, 64, 10900]])
+def test_linear_attention_over_hundreds_of_segments(hip_device, lens):
+    """313 segments of 64 tokens: more than a workgroup of the carry holds at a time."""
+    _linear_case(hip_device, lens, 1, 8, 8, torch.float32, seed=43, decays=[-0.003])
+
+
+def test_linear_attention_states_of_many_empty_sequences(hip_device):
+    """Sequences without tokens, more than a wave looks at together: their final state is their initial one."""
+    _linear_case(hip_device, ([0, 3, 0] * 30 + [0] * 70 + [40]) * 2, 2, 16, 24, torch.float32, seed=47, init=True)
 
 
 def test_linear_attention_of_extreme_decays(hip_device):
