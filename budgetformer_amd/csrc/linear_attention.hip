@@ -24,7 +24,7 @@
 // the decayed z that enters the state is given in parts that keep its float32 value.
 //
 // What bounds it is the wait for a tile's loads with two waves a SIMD: 8192 tokens, 16 heads of 128, bfloat16 with a final
-// state take 29 (segments) + 13 (carry) + 52 us (pass), where the tensors' bytes are 26 us of a copy.
+// state take 29 (segments) + 12 (carry) + 52 us (pass), where the tensors' bytes are 26 us of a copy.
 #include "packed_tile.h"
 
 namespace bf {

@@ -723,7 +723,8 @@ int pieces_of(const bf_packed_attn* p) {
 // one causal sequence of 8192 (16 heads of 128 over 4). Whole : pieces in us, forward and backward: 500 rows in sequences
 // of 5, 32 heads of 128 over 2, bfloat16 289 : 72; in sequences of 100, 16 heads of 64 over 2, float32 319 : 123. Tiles that fill
 // the chip once gain by pieces only what a long mask leaves uneven: 20,000 rows in sequences of 500, 8 heads of 128 over 4,
-// float16 456 : 520.
+// float16 456 : 520. Short walks of narrow 16-bit heads do not earn the second launch: 640 rows of one causal sequence, 8 heads
+// of 64, float16, dK and dV 24 : 25, 900 rows 33 : 29 (float32 heads of 16: 43 : 32, 60 : 36).
 int kv_pieces_of(const bf_packed_attn* p) {
   const int elem = p->dtype == BF_DTYPE_F32 ? 4 : 2;
   const int64_t keys = 32 * kv_waves(elem, p->head_dim > 64 ? 128 : 64), groups = ceil_div(p->n_k, keys) * p->heads_k;
@@ -732,6 +733,7 @@ int kv_pieces_of(const bf_packed_attn* p) {
   // what a tile of several sequences walks: its keys' sequences
   const int64_t walks = p->longest > 0 && p->longest + keys < p->n_q ? p->longest + keys : p->n_q;
   const int64_t rows = walks * (p->heads_q / p->heads_k);
+  if (elem == 2 && p->head_dim <= 64 && rows < 768) return 1;
   int64_t n = ceil_div(512, groups);
   if (n > rows / 256) n = rows / 256;
   if (n > kMaxPieces) n = kMaxPieces;
