@@ -21,7 +21,8 @@
 // Calls of few heads cut the axis into segments: one launch forms each segment's own contribution to the state, one
 // carries it from segment to segment, and the pass starts from there. States are float32 throughout; as operands of x M
 // and W z, M and W are rounded to the activations' type (half a step, as the inputs' own rounding; in float32 not at all);
-// the decayed z that enters the state is given in parts that keep its float32 value.
+// the decayed z that enters the state is given in parts that keep its float32 value. float16 ends at 65504 and loses bits
+// below 2^-14, where a score or a state need not: there both are operands in units of a power of 2 (kScoreUnit, kStateUnit).
 //
 // What bounds it is the wait for a tile's loads with two waves a SIMD: 8192 tokens, 16 heads of 128, bfloat16 with a final
 // state take 29 (segments) + 12 (carry) + 52 us (pass), where the tensors' bytes are 26 us of a copy.
@@ -58,6 +59,16 @@ struct LinRoles {
 };
 
 constexpr int kTile = 32;        // tokens of a tile
+
+// float16's units of scores and of states as operands: what is 64 times (512 times) a score or state of ordinary size still
+// fits, and the gradients' small ones keep their bits (a state's rounding is then 2^-31 at most, a score's 2^-34, where the
+// result's own is 2^-25). Larger ones take a unit of their own, that brings the largest to 2^15.
+constexpr float kScoreUnit = 1.f / 512.f, kStateUnit = 1.f / 64.f, kUnitMost = 32768.f;
+
+// The unit, a power of 2, in which `big` is at most 2^15; `usual` where it is not finite.
+__device__ __forceinline__ float unit_of(float big, float usual) {
+  return big < INFINITY ? ldexpf(1.f, __builtin_amdgcn_frexp_expf(big) - 15) : usual;
+}
 
 // log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
 __device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
@@ -112,6 +123,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   constexpr int C = kTile, NW = DZ / 32, NT = 64 * NW, XB = DX / 32;
   // parts of the decayed z (see below): the third only for a state that goes out
   const bool third = STATES && a.final_state != nullptr;
+  constexpr bool kUnits = std::is_same<T, _Float16>::value;
   constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, __bf16>::value ? 3 : 2;
   using TX = Tile<T, DX>;
   using TZ = Tile<T, DZ>;
@@ -217,17 +229,17 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
         acc = Mat<T>::mma(TX::row_frag(y_lds, col, s, half), TX::row_frag(x_lds, col, s, half), acc);
       // with states the tile is one sequence's, whose state came in or was begun above
       if (STATES || first_start < t0) {
-        // float16 ends at 65504 and a sum over a sequence need not: such a state is an operand in units of a power of 2
         float unit = 1.f;
-        if constexpr (std::is_same<T, _Float16>::value) {
+        if constexpr (kUnits) {                // one for the wave: the state's rows are other lanes' contractions
+          unit = kStateUnit;
           float big = 0.f;
 #pragma unroll
           for (int b = 0; b < XB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]));
-          if (__any(big > 32768.f)) {
+          if (__any(big > kUnitMost * kStateUnit)) {
             for (int n = 32; n; n >>= 1) big = fmaxf(big, __shfl_xor(big, n, 64));
-            unit = big < INFINITY ? exp2f(ceilf(log2f(big)) - 15.f) : 1.f;
+            unit = unit_of(big, kStateUnit);
           }
         }
         const float per_unit = 1.f / unit;
@@ -236,7 +248,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             Frag<T> mf;
-            if constexpr (std::is_same<T, _Float16>::value)
+            if constexpr (kUnits)
               mf = pack8_by<T>(m[b], t, per_unit);
             else
               mf = pack8<T>(m[b], t);
@@ -252,6 +264,20 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
       for (int r = 0; r < 16; ++r) {
         const int j = acc_row(r, half);
         w[r] = j <= i && j >= from ? acc[r] * (a.scale * exp2_fast(ld * float(i - j))) : 0.f;
+      }
+      float unit = 1.f;
+      if constexpr (kUnits) {                  // a row's own: it is the lane's (and its other half's)
+        unit = kScoreUnit;
+        float big = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(w[r]));
+        if (__any(big > kUnitMost * kScoreUnit)) {
+          big = fmaxf(big, __shfl_xor(big, 32, 64));
+          if (big > kUnitMost * kScoreUnit) unit = unit_of(big, kScoreUnit);
+        }
+        const float per_unit = 1.f / unit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] *= per_unit, o[r] *= per_unit;
       }
       if (!odd) {
 #pragma unroll
@@ -275,7 +301,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
           if (bad[r] > 0.f) o[r] = NAN;
       }
       if (i < len && t0 + i >= own)
-        store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, 1.f, wave, a.dz, half);
+        store_block<T>(static_cast<T*>(a.out) + (int64_t(token_at(a, t0 + i)) * a.heads + h) * a.dz, o, unit, wave, a.dz, half);
     }
 
     if (!OUT || t1 < end || ends) {

@@ -99,10 +99,11 @@ def rotary(x, positions, theta, amplitude, interleaved, inverse=False):
     return torch.cat([got.flatten(-2), rest], -1)
 
 
-def linear_attention(q, k, v, log_decay, lens, scale, initial_state=None, dout=None, dtype=None):
+def linear_attention(q, k, v, log_decay, lens, scale, initial_state=None, dout=None, dtype=None, operand_tiny=None):
     """The recurrence S_i = g S_{i-1} + k_i v_i^T, out_i = scale q_i S_i, a token at a time; q, k [n, H, dk], v [n, H, dv]
     float64. Returns a dict: out, state [sequences, H, dk, dv], with dout dq, dk, dv (the same recurrence on the way
-    back), and with dtype the bounds, from the recurrence over absolute values."""
+    back), and with dtype the bounds, from the recurrence over absolute values. operand_tiny: half a step of a subnormal
+    operand (the scores, the state), where that is finer than the type's own."""
     H, dk, dv = q.shape[1], q.shape[2], v.shape[2]
     g = log_decay.double().exp()[:, None, None]
     res = {"out": torch.zeros_like(v), "state": q.new_zeros(len(lens), H, dk, dv)}
@@ -145,6 +146,7 @@ def linear_attention(q, k, v, log_decay, lens, scale, initial_state=None, dout=N
         up = 0.0 if dtype == torch.float32 else 3 * u
         c32 = 2.0 ** -24 * (max(list(lens) + [1]) + 2 * (dk + dv) + 256)
         for x in list(seen):
-            res[f"{x}_bound"] = u * res[x].abs() + (up + c32) * size[x] + _tiny(dtype) * (seen[x] + 1)
+            small = _tiny(dtype) if operand_tiny is None else operand_tiny
+            res[f"{x}_bound"] = u * res[x].abs() + (up + c32) * size[x] + small * seen[x] + _tiny(dtype)
         res["state_bound"] = (up / 3 + c32) * size["state"] + _tiny(dtype) * max(list(lens) + [1]) * 8
     return res

@@ -439,6 +439,45 @@ def test_linear_attention_states_past_float16(hip_device):
     _within("out", out, ref, 3 * 2.0 ** -11 * ref)
 
 
+def _linear_of_sizes(dev, sizes, lens, operand_tiny=None, names=("out", "dq", "dk", "dv"), H=2, d=64):
+    """float16, q, k, v and the output's gradient of the given sizes."""
+    bf = _bf()
+    n = sum(lens)
+    q, k, v, do = (_randn(i, n, H, d, dev=dev).mul(size).half() for i, size in enumerate(sizes))
+    v[::7] = 0.0
+    ld = torch.tensor([-0.02, -0.3], device=dev)
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=dev)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = bf.linear_attention(*leaves, ld, seqs)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))))
+    ref = sq.linear_attention(q.double().cpu(), k.double().cpu(), v.double().cpu(), ld.cpu(), lens, d ** -0.5, None,
+                              do.double().cpu(), torch.float16, operand_tiny)
+    for x in names:
+        assert float(ref[x].abs().max()) < 65504
+        _within(x, got[x], ref[x].to(dev), ref[f"{x}_bound"].to(dev))
+
+
+@pytest.mark.parametrize("lens", [[1, 5], [90, 33]])
+def test_linear_attention_scores_past_float16(hip_device, lens):
+    """Scores of some 80,000 under small values: the result fits, so it has to come out, values of 0 among them."""
+    bf = _bf()
+    _linear_of_sizes(hip_device, (100.0, 100.0, 0.01, 0.01), lens)
+    _linear_of_sizes(hip_device, (0.01, 0.01, 100.0, 100.0), lens)         # the gradients' scores, v and dout
+    seqs = bf.PackedSequences.from_lengths([3], causal=True, device=hip_device)
+    q = torch.full((3, 1, 64), 100.0, dtype=torch.float16, device=hip_device)
+    v = torch.full((3, 1, 64), 0.01, dtype=torch.float16, device=hip_device)
+    v[:, :, 1::2] = 0.0
+    out = bf.linear_attention(q, q, v, torch.full((1,), -math.inf, device=hip_device), seqs)
+    ref = (80000.0 * v.double())                                           # only the row's own token
+    _within("out", out, ref, 2 * 2.0 ** -11 * ref)
+
+
+def test_linear_attention_small_gradients_keep_their_bits_in_float16(hip_device):
+    """Gradients of 1e-6 under queries and keys of 100: the scores they form lie below float16's normal numbers, the
+    results do not. A score is rounded in units of 2^-9 (half a step of 2^-34), a state in units of 2^-6."""
+    _linear_of_sizes(hip_device, (100.0, 100.0, 1.0, 1e-6), [300, 33], 2.0 ** -31, ("dq", "dk"))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,H,dk,dv", [(1, 1, 8, 8), (3, 5, 128, 128), (7, 2, 24, 72), (2, 3, 64, 16)])
 def test_linear_attention_step_continues_a_prompt(hip_device, n, H, dk, dv, dtype):
