@@ -29,9 +29,10 @@ def visible(m: int, n: int, causal: bool, device=None):
     return j <= i + (n - m) if causal else torch.ones(m, n, dtype=torch.bool, device=device)
 
 
-def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None):
+def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, operand_tiny=None):
     """q [n_q, H, d], k, v [n_k, Hk, d] float64 packed. Returns a dict: out, lse (natural log) and with dout dq, dk, dv;
-    with dtype also each one's bound (``out_bound``, ...). Rows that see no key: out 0, lse -inf."""
+    with dtype also each one's bound (``out_bound``, ...). Rows that see no key: out 0, lse -inf. operand_tiny: half a step
+    of a subnormal P or dS, where that is finer than the type's own."""
     H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
     g = H // Hk
     names = ["out"] + (["dq", "dk", "dv"] if dout is not None else [])
@@ -41,6 +42,7 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None):
     u = half_step(dtype) if dtype is not None else 0.0
     up = 0.0 if dtype == torch.float32 else u                    # P and dS as operands: rounded to the type
     tiny = _tiny(dtype)
+    small = tiny if operand_tiny is None else operand_tiny
     q0 = k0 = 0
     for m, n in zip(q_lens, k_lens):
         rows, keys = slice(q0, q0 + m), slice(k0, k0 + n)
@@ -64,7 +66,7 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None):
             big = scale * (a.abs() @ b.abs().T).masked_fill(~see, 0).amax() if see.any() else 0.0
             # scores: sums of d products, each step off by 2^-24, scaled; their exponentials' relative error, the sums over n
             c32 = 2.0 ** -24 * (2 * (d + 8) * (1 + float(big)) + n + m * g + 32)
-            ob = u * out.abs() + (up + c32) * (p @ w.abs()) + tiny * (see.double() @ w.abs() + 1)
+            ob = u * out.abs() + (up + c32) * (p @ w.abs()) + small * (see.double() @ w.abs()) + tiny
             bnd["out"][rows, h] = ob
             if dout is None:
                 continue
@@ -75,10 +77,10 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None):
             res["dk"][keys, h // g] += scale * ds.T @ a
             res["dv"][keys, h // g] += p.T @ do
             mean_off = (do.abs() * ob).sum(1, keepdim=True)       # Delta comes from the rounded out
-            e = (up + c32) * ds.abs() + p * (mean_off + 2 * c32 * (do.abs() @ w.abs().T)) + tiny * see
+            e = (up + c32) * ds.abs() + p * (mean_off + 2 * c32 * (do.abs() @ w.abs().T)) + small * see
             bnd["dq"][rows, h] = scale * (e + c32 * ds.abs()) @ b.abs()
             bnd["dk"][keys, h // g] += scale * (e + c32 * ds.abs()).T @ a.abs()
-            bnd["dv"][keys, h // g] += ((up + 2 * c32) * p + tiny * see).T @ do.abs()
+            bnd["dv"][keys, h // g] += ((up + 2 * c32) * p + small * see).T @ do.abs()
     for x in ("dq", "dk", "dv"):
         bnd[x] += u * res[x].abs() + tiny
     got = {x: res[x] for x in names + ["lse"]}

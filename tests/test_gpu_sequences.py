@@ -157,6 +157,67 @@ def test_large_scores_do_not_overflow(hip_device, dtype):
     _within("out", out, ref["out"], ref["out_bound"])
 
 
+def _float16_gradients(dev, sizes, lens, H, Hk, d, causal, operand_tiny=None, seed=0):
+    """float16 training with q, k, v and the output's gradient of the given sizes."""
+    bf = _bf()
+    n = sum(lens)
+    q, k, v, do = (_randn(seed + i, n, h, d, dev=dev).mul(size).half() for i, (h, size) in
+                   enumerate(zip((H, Hk, Hk, H), sizes)))
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = bf.packed_attention(*leaves, bf.PackedSequences.from_lengths(lens, causal=causal, device=dev))
+    ref = sq.attention(q.double(), k.double(), v.double(), lens, lens, causal, d ** -0.5, do.double(), torch.float16, operand_tiny)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))):
+        assert float(ref[name].abs().max()) < 65504
+        _within(name, got, ref[name], ref[f"{name}_bound"])
+
+
+@pytest.mark.parametrize("H,Hk,d", [(2, 2, 64), (2, 1, 128), (4, 4, 16)])
+def test_small_gradients_keep_their_bits_in_float16(hip_device, H, Hk, d):
+    """Gradients of 1e-4 over up to 2048 keys, keys and queries of 8: dS lies below float16's normal numbers, the results
+    do not. Operands are times 2^12 (forward 2^9): half a step of a subnormal one is 2^-34 at most."""
+    _float16_gradients(hip_device, (0.1, 8.0, 1.0, 1e-4), [2048, 3], H, Hk, d, True, 2.0 ** -34)
+    _float16_gradients(hip_device, (8.0, 0.1, 1.0, 1e-4), [700, 1200], H, Hk, d, False, 2.0 ** -34)
+
+
+@pytest.mark.parametrize("H,Hk,d", [(2, 2, 64), (4, 1, 128), (4, 4, 16), (2, 2, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_large_gradients_do_not_overflow_in_float16(hip_device, H, Hk, d, causal):
+    """dS of several 100,000, in some rows and later tiles only, under small queries and keys: the results fit."""
+    _float16_gradients(hip_device, (0.01, 0.01, 50.0, 1000.0), [100, 1, 513, 40], H, Hk, d, causal, seed=5)
+    bf = _bf()
+    n = 400                                       # values grow along the axis: each tile's dS pass the ones before
+    q, k = (_randn(i, n, 1, d, dev=hip_device).mul(0.01).half() for i in (1, 2))
+    up = torch.logspace(-2, 2, n, device=hip_device)[:, None, None]
+    v, do = (_randn(3, n, 1, d, dev=hip_device) * up).half(), (_randn(4, n, 1, d, dev=hip_device) * up).mul(20).half()
+    for flip in (False, True):
+        xs = [x.flip(0) if flip else x for x in (q, k, v, do)]
+        leaves = [x.clone().requires_grad_(True) for x in xs[:3]]
+        out = bf.packed_attention(*leaves, bf.PackedSequences.from_lengths([n], causal=causal, device=hip_device))
+        ref = sq.attention(*(x.double() for x in xs[:3]), [n], [n], causal, d ** -0.5, xs[3].double(), torch.float16)
+        for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, xs[3]))):
+            _within(name, got, ref[name], ref[f"{name}_bound"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,H,d", [(2, 1, 64), (2048, 16, 64), (4099, 8, 16), (2048, 8, 128)])
+def test_many_small_terms_count(hip_device, rows, H, d, dtype):
+    """One key at score 0 and 200,000 at -16.5, whose weights are each below float16's last bit and together 1.3%."""
+    bf = _bf()
+    n = 200001
+    q = torch.zeros(rows, H, d, dtype=dtype, device=hip_device)
+    q[:, :, 0] = 1.0
+    k, v = torch.zeros(n, H, d, dtype=dtype, device=hip_device), torch.ones(n, H, d, dtype=dtype, device=hip_device)
+    k[1:, :, 0] = -16.5
+    v[0] = 0.0
+    out = bf.packed_attention(q, k, v, bf.PackedSequences.from_lengths([rows], [n], device=hip_device), scale=1.0)
+    w = (n - 1) * math.exp(-16.5)
+    # each term's rounding, the same for all (half a step), and the result's; two running float32 sums (of the terms, of
+    # their products) of n terms, n roundings of 2^-24 of the sum each: equal terms are all rounded the same way, so these
+    # add up (6.8e-8 onto 1 becomes 1.2e-7); exponentials at 16.5
+    off = (2 * sq.half_step(dtype) + 2.0 ** -24 * (2 * n + 200)) * w / (1 + w)
+    assert float((out.double() - w / (1 + w)).abs().max()) < off
+
+
 def _strided(x, kind):
     """The same values in another layout."""
     n, h, d = x.shape
