@@ -29,10 +29,12 @@ def visible(m: int, n: int, causal: bool, device=None):
     return j <= i + (n - m) if causal else torch.ones(m, n, dtype=torch.bool, device=device)
 
 
-def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, operand_tiny=None):
+def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, operand_tiny=None,
+              rounds=True):
     """q [n_q, H, d], k, v [n_k, Hk, d] float64 packed. Returns a dict: out, lse (natural log) and with dout dq, dk, dv;
     with dtype also each one's bound (``out_bound``, ...). Rows that see no key: out 0, lse -inf. operand_tiny: half a step
-    of a subnormal P or dS, where that is finer than the type's own."""
+    of a subnormal P or dS, where that is finer than the type's own. rounds: whether P and dS are operands of the type and
+    Delta comes from the rounded out (False: neither; Delta from out and its rounding's rest, rounded itself)."""
     H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
     g = H // Hk
     names = ["out"] + (["dq", "dk", "dv"] if dout is not None else [])
@@ -40,9 +42,9 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
            "lse": q.new_full(q.shape[:2], -math.inf)}
     bnd = {x: torch.zeros_like(res[x]) for x in ("out", "dq", "dk", "dv")}
     u = half_step(dtype) if dtype is not None else 0.0
-    up = 0.0 if dtype == torch.float32 else u                    # P and dS as operands: rounded to the type
+    up = 0.0 if dtype == torch.float32 or not rounds else u      # P and dS as operands: rounded to the type
     tiny = _tiny(dtype)
-    small = tiny if operand_tiny is None else operand_tiny
+    small = 0.0 if not rounds else tiny if operand_tiny is None else operand_tiny
     q0 = k0 = 0
     for m, n in zip(q_lens, k_lens):
         rows, keys = slice(q0, q0 + m), slice(k0, k0 + n)
@@ -76,6 +78,8 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
             res["dq"][rows, h] = scale * ds @ b
             res["dk"][keys, h // g] += scale * ds.T @ a
             res["dv"][keys, h // g] += p.T @ do
+            if not rounds:
+                ob = u * u * out.abs() + c32 * (p @ w.abs()) + tiny
             mean_off = (do.abs() * ob).sum(1, keepdim=True)       # Delta comes from the rounded out
             e = (up + c32) * ds.abs() + p * (mean_off + 2 * c32 * (do.abs() @ w.abs().T)) + small * see
             bnd["dq"][rows, h] = scale * (e + c32 * ds.abs()) @ b.abs()

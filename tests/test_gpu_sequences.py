@@ -126,6 +126,23 @@ def test_short_sequences(hip_device, H, Hk, d, causal, dtype):
     _attention_case(hip_device, q_lens, k_lens, H, Hk, d, causal, dtype, seed=31)
 
 
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("H,Hk,d,lens", [(8, 8, 16, [5] * 40), (4, 2, 64, [2, 7, 1, 4] * 5), (2, 1, 128, [6, 3])])
+def test_short_sequences_form_delta_from_the_unrounded_out(hip_device, H, Hk, d, lens, dtype):
+    """Values of 8 and a little: out's rounding is as large as what the scores' gradients are made of. The lanes round
+    neither P nor dS, so that the bound is float32's and the results' own rounding."""
+    bf = _bf()
+    n = sum(lens)
+    q, do = (_randn(i, n, H, d, dtype=dtype, dev=hip_device) for i in (0, 3))
+    k = _randn(1, n, Hk, d, dtype=dtype, dev=hip_device)
+    v = (8 + 0.25 * _randn(2, n, Hk, d, dev=hip_device)).to(dtype)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = bf.packed_attention(*leaves, bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device))
+    ref = sq.attention(q.double(), k.double(), v.double(), lens, lens, True, d ** -0.5, do.double(), dtype, rounds=False)
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)):
+        _within(name, got, ref[name], ref[f"{name}_bound"])
+
+
 def test_keys_past_32_bit_offsets(hip_device):
     """A cache of more than 2^31 values: the last sequence's keys lie behind them."""
     bf = _bf()
