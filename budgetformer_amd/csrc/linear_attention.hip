@@ -70,8 +70,9 @@ __device__ __forceinline__ float unit_of(float big, float usual) {
   return big < INFINITY ? ldexpf(1.f, __builtin_amdgcn_frexp_expf(big) - 15) : usual;
 }
 
-// log2 of a head's decay; a decay of 0 (log -inf) stays finite, so that its power 0 is 1
-__device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return fmaxf(a.log_decay[h], -1e4f) * kLog2e; }
+// A head's log decay; one of 0 (log -inf) stays finite, so that its power 0 is 1; a NaN stays one
+__device__ __forceinline__ float finite_decay(float x) { return x < -1e4f ? -1e4f : x; }
+__device__ __forceinline__ float decay_log2(const LinArgs& a, int h) { return finite_decay(a.log_decay[h]) * kLog2e; }
 
 // the token at a place of the axis as the pass reads it, its span, and where its sequence starts on that axis
 __device__ __forceinline__ int token_at(const LinArgs& a, int p) { return a.reverse ? a.n - 1 - p : p; }
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(256) void linear_step(const T* q, const T* k, const
   const int64_t nh = blockIdx.x;
   const int h = int(nh % heads), cols = dv / 4, rows = 256 / cols, tid = threadIdx.x;
   const int c = tid % cols, r0 = tid / cols;
-  const float g = __expf(fmaxf(log_decay[h], -1e4f));
+  const float g = __expf(finite_decay(log_decay[h]));
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   if (r0 < rows) {
     float vv[4];

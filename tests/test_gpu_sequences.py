@@ -517,6 +517,29 @@ def test_linear_attention_states_past_float16(hip_device):
     _within("out", out, ref, 3 * 2.0 ** -11 * ref)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[5, 40], [700, 3]], ids=["tiles", "segments"])
+def test_linear_attention_of_a_decay_that_is_nan(hip_device, lens, dtype):
+    """Its head's results are NaN, gradients and states too; the others' are as without it."""
+    bf = _bf()
+    n, H, d = sum(lens), 3, 32
+    base = [_randn(i, n, H, d, dtype=dtype, dev=hip_device) for i in range(4)]
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+    fine = torch.tensor([-0.1, -0.2, -math.inf], device=hip_device)
+    bad = fine.clone()
+    bad[1] = math.nan
+
+    def every(ld):
+        leaves = [x.clone().requires_grad_(True) for x in base[:3]]
+        out, state = bf.linear_attention(*leaves, ld, seqs, return_state=True)
+        one = bf.linear_attention_step(*(x[:2] for x in base[:3]), ld, state)
+        return [x.detach() for x in (out, state, *one, *torch.autograd.grad(out, leaves, base[3]))]
+
+    for a, b in zip(every(bad), every(fine)):
+        assert torch.equal(a[:, ::2], b[:, ::2])
+        assert bool(a[:, 1].isnan().all())
+
+
 def _linear_of_sizes(dev, sizes, lens, operand_tiny=None, names=("out", "dq", "dk", "dv"), H=2, d=64):
     """float16, q, k, v and the output's gradient of the given sizes."""
     bf = _bf()
