@@ -159,6 +159,14 @@ class PackedSequences:
         self.used()
         return self._positions
 
+    def key_positions(self) -> torch.Tensor:
+        """int32 [n_k]: each key's place in its sequence (0 behind the last sequence). Formed anew in each call where the
+        keys' sequences are not the rows'."""
+        if self.self_attention:
+            return self.positions()
+        self.used()
+        return _op("packed_spans")(self.k_offsets, self.k_offsets, self.n_k, self.n_k, False)[2]
+
 
 def _check_seqs(seqs, q: torch.Tensor, k: torch.Tensor) -> None:
     if not isinstance(seqs, PackedSequences):
@@ -239,7 +247,9 @@ def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optio
     """q (and k) [rows, heads, hn] with the first ``freq.rot`` values of every head turned by the row's position.
 
     ``positions``: int32 or int64 [rows] on the device, of any size and sign (angles are formed in 64 bits);
-    without them each row's place in its sequence (``seqs.positions()``). Pairs are (i, i + rot / 2), or with
+    without them each row's place in its sequence: q by ``seqs.positions()``, k by ``seqs.key_positions()`` where it
+    has a row for each of the sequences' keys, or as q where it has one for each of their rows (the new tokens' keys,
+    before they are put behind the kept ones). Pairs are (i, i + rot / 2), or with
     ``interleaved`` (2i, 2i + 1). Returns new tensors, (q, k) or q alone; gradients are turned back."""
     if not isinstance(freq, RotaryFrequencies):
         raise TypeError(f"freq must be a RotaryFrequencies (got {type(freq)})")
@@ -249,6 +259,9 @@ def rotary_embedding(q, k=None, freq: RotaryFrequencies = None, positions: Optio
         if seqs.n_q != q.size(0):
             raise ValueError(f"the sequences cover {seqs.n_q} rows, q has {q.size(0)}")
         positions = seqs.positions()
+        if k is not None and k.size(0) == seqs.n_k and not seqs.self_attention:      # keys of sequences of their own
+            return (rotary_embedding(q, None, freq, positions, interleaved=interleaved),
+                    rotary_embedding(_as(q, k), None, freq, seqs.key_positions(), interleaved=interleaved))
     if freq.rot > q.size(-1):
         raise ValueError(f"{freq.rot} rotated values in a head of {q.size(-1)}")
     k = None if k is None else _as(q, k)

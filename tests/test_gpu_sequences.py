@@ -427,6 +427,34 @@ def test_rotary_of_one_of_two_gradients(hip_device):
         assert torch.equal(torch.autograd.grad(one.sum(), (q, k)[i])[0], g[i])
 
 
+@pytest.mark.parametrize("q_lens,k_lens", [([3, 5, 0, 4], [5, 3, 4, 0]), ([2, 6], [2, 6]), ([1, 2, 1], [7, 2, 3])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rotary_of_keys_with_sequences_of_their_own(hip_device, causal, q_lens, k_lens):
+    """Rows stand behind their sequence's earlier keys, keys at their own place, also where as many rows as keys are
+    there in all; keys of the new rows stand where the rows do."""
+    from budgetformer_amd.attention import CoreAttention
+    bf = _bf()
+    n_q, n_k, H, d = sum(q_lens), sum(k_lens), 2, 16
+    q, k = _randn(1, n_q, H, d, dev=hip_device).requires_grad_(True), _randn(2, n_k, H, d, dev=hip_device).requires_grad_(True)
+    freq = bf.RotaryFrequencies(d, device=hip_device)
+    seqs = bf.PackedSequences.from_lengths(q_lens, k_lens, causal=causal, device=hip_device)
+    q_pos = torch.cat([torch.arange(m) + n - m for m, n in zip(q_lens, k_lens)]).to(hip_device)
+    k_pos = torch.cat([torch.arange(n) for n in k_lens]).to(hip_device)
+    assert torch.equal(seqs.positions().long(), q_pos) and torch.equal(seqs.key_positions().long(), k_pos)
+    want = (bf.rotary_embedding(q, None, freq, positions=q_pos), bf.rotary_embedding(k, None, freq, positions=k_pos))
+    got = bf.rotary_embedding(q, k, freq, seqs=seqs)
+    dos = [_randn(3 + i, *x.shape, dev=hip_device) for i, x in enumerate(want)]
+    for a, b in zip((*got, *torch.autograd.grad(got, (q, k), dos)), (*want, *torch.autograd.grad(want, (q, k), dos))):
+        assert torch.equal(a, b)
+    if n_q != n_k:
+        for a, b in zip(bf.rotary_embedding(q, q, freq, seqs=seqs), (want[0], want[0])):
+            assert torch.equal(a, b)
+    else:
+        core = CoreAttention(H * d, 0.0, H, 1, rotary=freq)
+        got = core(q[None], k[None], k[None], edge_index=seqs, attn_type="flash")
+        assert torch.equal(got.view(n_q, H, d), bf.packed_attention(*want, k, seqs))
+
+
 @pytest.mark.parametrize("scaling", ["linear", "ntk", "by_parts"])
 def test_rotary_frequencies(hip_device, scaling):
     bf = _bf()
