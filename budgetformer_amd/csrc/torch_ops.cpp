@@ -765,12 +765,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attn_bwd(const at::Tensor&
   return {dq, dk, dv};
 }
 
+// The kernels know no forward-mode derivatives: a dual tensor is refused, not taken as a plain one.
+void refuse_tangents(std::initializer_list<const at::Tensor*> ts, const char* name) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), name,
+                                " has no forward-mode derivatives (an input is a dual tensor)");
+}
+
 // One token of each sequence (bf_linear_attn_step): (out, new state); out_state: where the new state goes (state itself
 // updates it in place), else a new tensor.
 std::tuple<at::Tensor, at::Tensor> linear_attn_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                     const at::Tensor& log_decay, const at::Tensor& state, double scale,
                                                     const std::optional<at::Tensor>& out_state) {
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a device tensor (got ", q.device(), ")");
+  const at::Tensor into = out_state.value_or(at::Tensor());
+  refuse_tangents({&q, &k, &v, &log_decay, &state, &into}, "linear_attention_step");
   const c10::DeviceGuard guard(q.device());
   const at::Device dev = q.device();
   const int32_t code = dtype_code(q);
@@ -863,6 +872,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
 std::tuple<at::Tensor, at::Tensor> packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                     const at::Tensor& row_span, const at::Tensor& key_span, double scale,
                                                     int64_t longest) {
+  refuse_tangents({&q, &k, &v}, "packed_attention");
   if (trains({&q, &k, &v})) {
     variable_list r = PackedAttention::apply(q, k, v, row_span, key_span, scale, longest);
     return {r[0], r[1]};
@@ -906,6 +916,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& x, const s
                                                     const at::Tensor& positions, const at::Tensor& turns, double amplitude,
                                                     bool interleaved) {
   const at::Tensor second = y.has_value() ? *y : at::Tensor();
+  refuse_tangents({&x, &second}, "rotary_embedding");
   if (trains({&x, &second})) {
     variable_list r = Rotary::apply(x, second.defined() ? std::optional<at::Tensor>(second) : std::nullopt, positions, turns, amplitude, interleaved);
     return {r[0], r[1]};
@@ -948,6 +959,8 @@ std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor& q, const a
                                                     const at::Tensor& key_span, const at::Tensor& offsets, double scale,
                                                     int64_t longest, const std::optional<at::Tensor>& init_state,
                                                     bool return_state) {
+  const at::Tensor init = init_state.value_or(at::Tensor());
+  refuse_tangents({&q, &k, &v, &log_decay, &init}, "linear_attention");
   if (trains({&q, &k, &v})) {
     variable_list r =
         LinearAttention::apply(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state, return_state);

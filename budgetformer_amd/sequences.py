@@ -12,7 +12,8 @@ row sees, built on the GPU once per batch as an ``AttentionIndex`` is once per e
 
 ``CoreAttention`` takes the first (and, with ``rotary``, the second) for ``attn_type="flash"``, the dense
 attention of models/graphormer_dist_node_level.py:603-608. All run as HIP kernels on the current stream;
-there is no CPU fallback. Activations are float32, bfloat16 or float16, sums and statistics float32.
+there is no CPU fallback. Activations are float32, bfloat16 or float16, sums and statistics float32. Gradients
+are backward-mode and once differentiable; dual tensors (forward mode) are refused.
 """
 from __future__ import annotations
 

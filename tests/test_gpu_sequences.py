@@ -852,6 +852,37 @@ def test_second_derivatives_are_refused(hip_device):
             g.sum().backward()
 
 
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(hip_device, grad):
+    """A dual tensor, with or without a gradient wanted, in any place and also under no_grad: no result without its tangent."""
+    import torch.autograd.forward_ad as fwd
+    bf = _bf()
+    seqs = bf.PackedSequences.from_lengths([20], causal=True, device=hip_device)
+    x, ld, s = _randn(1, 20, 2, 16, dev=hip_device).requires_grad_(grad), torch.zeros(2, device=hip_device), torch.zeros(20, 2, 16, 16, device=hip_device)
+    freq = bf.RotaryFrequencies(16, device=hip_device)
+    p = x.detach()
+    with fwd.dual_level():
+        d, dl, ds = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, ld, s))
+        calls = [lambda: bf.packed_attention(d, p, p, seqs), lambda: bf.packed_attention(p, p, d, seqs),
+                 lambda: bf.packed_attention(x, d, p, seqs, with_lse=True),
+                 lambda: bf.rotary_embedding(d, None, freq, seqs=seqs), lambda: bf.rotary_embedding(x, d, freq, seqs=seqs),
+                 lambda: bf.linear_attention(d, p, p, ld, seqs), lambda: bf.linear_attention(x, p, d, ld, seqs),
+                 lambda: bf.linear_attention(p, p, p, dl, seqs),
+                 lambda: bf.linear_attention(p, p, p, ld, seqs, initial_state=fwd.make_dual(torch.zeros(1, 2, 16, 16, device=hip_device),
+                                                                                           torch.ones(1, 2, 16, 16, device=hip_device)))]
+        if not grad:
+            calls += [lambda: bf.linear_attention_step(d, p, p, ld, s), lambda: bf.linear_attention_step(p, p, p, dl, s),
+                      lambda: bf.linear_attention_step(p, p, p, ld, ds)]
+        for f in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+    assert bf.packed_attention(p, p, p, seqs).shape == p.shape
+    with pytest.raises(Exception):                         # as a transform does it
+        torch.func.jvp(lambda t: bf.packed_attention(t, t, t, seqs), (p,), (torch.ones_like(p),))
+
+
 def test_offsets_that_change_afterwards_do_not_matter(hip_device):
     bf = _bf()
     off = torch.tensor([0, 5, 40], dtype=torch.int32, device=hip_device)
