@@ -59,7 +59,13 @@ class PackedSequences:
     nothing: their outputs and gradients are 0.
     """
 
+    # Plain tensors also where a batch is built in inference mode: training later saves them.
+    @torch.inference_mode(False)
     def __init__(self, q_offsets: torch.Tensor, k_offsets: torch.Tensor, n_q: int, n_k: int, causal: bool, longest: int = 0):
+        if q_offsets.is_inference() or k_offsets.is_inference():
+            same = q_offsets is k_offsets
+            q_offsets = q_offsets.clone()
+            k_offsets = q_offsets if same else k_offsets.clone()
         self.longest = int(longest)          # no sequence has more rows or keys; 0: unknown
         self.q_offsets, self.k_offsets = q_offsets, k_offsets
         self.n_q, self.n_k, self.n_seq, self.causal = int(n_q), int(n_k), q_offsets.numel() - 1, bool(causal)
@@ -106,7 +112,8 @@ class PackedSequences:
         ends = [torch.cat([x.new_zeros(1), x.cumsum(0)]) for x in lens]
         totals = [int(e[-1]) for e in ends]
         cls._sizes(totals[0], totals[-1])
-        on = [e.to(torch.int32).to(device) for e in ends]
+        with torch.inference_mode(False):
+            on = [e.to(torch.int32).to(device) for e in ends]
         return cls(on[0], on[-1], totals[0], totals[-1], causal, max([int(x.max()) for x in lens if x.numel()], default=0))
 
     @classmethod
@@ -139,8 +146,9 @@ class PackedSequences:
         elif sizes[0] is None or sizes[1] is None:
             raise ValueError("without the check the tensors' rows must be given (n_q, and n_k with k_offsets)")
         cls._sizes(int(sizes[0]), int(sizes[1]))
-        q = q_offsets.to(torch.int32, copy=True).contiguous()          # a copy: the caller's may change
-        k = q if k_offsets is None else k_offsets.to(torch.int32, copy=True).contiguous()
+        with torch.inference_mode(False):
+            q = q_offsets.to(torch.int32, copy=True).contiguous()      # a copy: the caller's may change
+            k = q if k_offsets is None else k_offsets.to(torch.int32, copy=True).contiguous()
         return cls(q, k, sizes[0], sizes[1], causal, longest)
 
     @staticmethod
@@ -212,6 +220,7 @@ class RotaryFrequencies:
     def __init__(self, rot: int, base: float = 10000.0, *, factor: float = 1.0, scaling: str = "linear",
                  original: Optional[int] = None, low: float = 1.0, high: float = 4.0, amplitude: float = 1.0,
                  device="cuda"):
+        device = PackedSequences._device(device)
         rot = int(rot)
         if rot < 2 or rot % 2 or rot > 1024:
             raise ValueError(f"rot must be an even number of 2 to 1024 (got {rot})")
@@ -219,6 +228,12 @@ class RotaryFrequencies:
             raise ValueError(f"base {base} must be above 1 and factor {factor} positive")
         if not math.isfinite(amplitude):
             raise ValueError(f"amplitude {amplitude}")
+        with torch.inference_mode(False):           # a plain tensor: training saves it
+            self.turns = (self._theta(rot, base, factor, scaling, original, low, high) / (2 * math.pi)).to(device)
+        self.rot, self.amplitude = rot, float(amplitude)
+
+    @staticmethod
+    def _theta(rot, base, factor, scaling, original, low, high) -> torch.Tensor:
         exponent = torch.arange(rot // 2, dtype=torch.float64) * 2 / rot
         if scaling == "linear":
             theta = base ** -exponent / factor
@@ -234,9 +249,9 @@ class RotaryFrequencies:
             theta = theta * keep + theta / factor * (1.0 - keep)
         else:
             raise ValueError(f"scaling {scaling!r} (linear, ntk or by_parts)")
-        self.rot, self.amplitude = rot, float(amplitude)
-        self.turns = (theta / (2 * math.pi)).to(PackedSequences._device(device))
+        return theta
 
+    @torch.inference_mode(False)
     def to(self, device) -> "RotaryFrequencies":
         got = object.__new__(RotaryFrequencies)
         got.rot, got.amplitude, got.turns = self.rot, self.amplitude, self.turns.to(PackedSequences._device(device))

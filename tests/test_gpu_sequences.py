@@ -752,6 +752,39 @@ def test_core_attention_flash(hip_device, dtype):
     assert CoreAttention(H * d, 0.1, H, 1).eval()(q, k, v, attn_type="flash").shape == (b, S, H * d)
 
 
+def test_what_inference_mode_builds_serves_training(hip_device):
+    """Validation before training: sequences and frequencies built in inference mode, by the flash path or by hand."""
+    from budgetformer_amd.attention import CoreAttention
+    bf = _bf()
+    b, S, H, d = 2, 40, 2, 16
+    x = _randn(1, b, S, H, d, dev=hip_device)
+    ld = torch.full((H,), -0.1, device=hip_device)
+
+    def train(core, seqs, freq):
+        t = x.clone().requires_grad_(True)
+        flash = core(t, t, t, attn_type="flash")
+        r = t.view(-1, H, d)
+        q, k = bf.rotary_embedding(r, r, freq, seqs=seqs)
+        outs = [flash, bf.packed_attention(q, k, r, seqs), bf.linear_attention(r, r, r, ld, seqs)]
+        return outs + [g for o in outs for g in torch.autograd.grad(o.sum(), t, retain_graph=True)]
+
+    def build():
+        off = torch.arange(0, b * S + 1, S, device=hip_device)
+        return (bf.RotaryFrequencies(d, device=hip_device), [bf.PackedSequences.from_lengths([S] * b, causal=True, device=hip_device),
+                bf.PackedSequences.from_offsets(off, causal=True), bf.PackedSequences.from_offsets(off, n_q=b * S, causal=True, check=False)])
+
+    freq, seqs = build()
+    ref = train(CoreAttention(H * d, 0.0, H, 1, rotary=freq), seqs[0], freq)
+    with torch.inference_mode():
+        freq, seqs = build()
+        core = CoreAttention(H * d, 0.0, H, 1, rotary=freq.to(hip_device))
+        y = core(x, x, x, attn_type="flash")
+        assert torch.equal(y, ref[0])
+    for s in seqs:
+        for a, r in zip(train(core, s, freq), ref):
+            assert torch.equal(a, r)
+
+
 # ------------------------------------------------------------------ streams, graphs, refusals
 def _layer(bf, q, k, v, do, freq, ld, seqs):
     leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
