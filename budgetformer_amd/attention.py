@@ -25,6 +25,7 @@ call on their slice of q, k and v.
 from __future__ import annotations
 
 import math
+import threading
 from collections import OrderedDict
 from typing import Optional
 
@@ -213,25 +214,36 @@ def _per_head_attention(q, k, v, assign, score_clamp, bias_fn=None, stats=None):
 
 
 class _BatchSequences:
-    """The PackedSequences of the last few (batch, length, device) of dense calls. A copied or pickled module starts
-    with none."""
+    """The PackedSequences of the last few (batch, length, device) of dense calls, and all that a capturing stream used:
+    a captured graph reads them as long as it is replayed. A copied or pickled module starts with none."""
 
     def __init__(self, size: int = 4):
         self.size = size
         self._d: "OrderedDict" = OrderedDict()
+        self._captured: dict = {}
+        self._lock = threading.Lock()
 
     def __reduce__(self):
         return _BatchSequences, (self.size,)
 
     def get(self, batch: int, length: int, device: torch.device) -> PackedSequences:
         key = (batch, length, str(device))
-        hit = self._d.get(key)
-        if hit is None:
-            hit = self._d[key] = PackedSequences.from_lengths([length] * batch, device=device)
-        self._d.move_to_end(key)
-        while len(self._d) > self.size:
-            self._d.popitem(last=False)
-        return hit
+        with self._lock:
+            hit = self._captured.get(key)
+            if hit is not None:
+                return hit
+            hit = self._d.get(key)
+            if hit is None:
+                hit = PackedSequences.from_lengths([length] * batch, device=device)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                self._captured[key] = hit
+                self._d.pop(key, None)
+                return hit
+            self._d[key] = hit
+            self._d.move_to_end(key)
+            while len(self._d) > self.size:
+                self._d.popitem(last=False)
+            return hit
 
 
 class CoreAttention(nn.Module):

@@ -830,6 +830,41 @@ def test_a_captured_layer_replays(hip_device):
     del alive
 
 
+def test_a_captured_flash_layer_replays_after_other_shapes(hip_device):
+    from budgetformer_amd.attention import CoreAttention
+    H, d = 2, 32
+    core = CoreAttention(H * d, 0.0, H, 1)
+    x, do = _randn(1, 3, 90, H, d, dtype=torch.bfloat16, dev=hip_device), _randn(2, 3, 90, H * d, dtype=torch.bfloat16, dev=hip_device)
+    base = x.clone()
+
+    def every(t):
+        leaf = t.detach().requires_grad_(True)
+        out = core(leaf, leaf, leaf, attn_type="flash")
+        return [out, *torch.autograd.grad(out, leaf, do)]
+
+    side = torch.cuda.Stream(device=hip_device)
+    side.wait_stream(torch.cuda.current_stream(hip_device))
+    with torch.cuda.stream(side):
+        every(x)
+    torch.cuda.current_stream(hip_device).wait_stream(side)
+    torch.cuda.synchronize(hip_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = every(x)
+    for rep in range(3):
+        for b in range(1, 9):                              # more shapes than the layer keeps
+            y = _randn(b, b, 70 + rep, H, d, dtype=torch.bfloat16, dev=hip_device)
+            core(y, y, y, attn_type="flash")
+        junk = [torch.full((n,), 2 ** 30, dtype=torch.int32, device=hip_device) for n in (4, 270, 540, 128, 1024) * 20]
+        x.copy_(base * (0.5 + rep))
+        graph.replay()
+        torch.cuda.synchronize(hip_device)
+        got = [t.clone() for t in captured]
+        for a, r in zip(got, every(x)):
+            assert torch.equal(a, r)
+        del junk
+
+
 def test_two_streams_at_once(hip_device):
     """Calls of different sizes on two streams, with their pieces and carries in flight together."""
     bf = _bf()

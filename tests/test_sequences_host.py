@@ -174,6 +174,57 @@ def test_host_tensors_and_bad_lengths_are_refused():
         bf.linear_attention_step(q, q, q, torch.zeros(1), torch.zeros(2, 1, 8, 8))
 
 
+def test_sequences_that_a_capture_used_are_kept(monkeypatch):
+    """The flash path's own sequences: the last four shapes, and every one that a capturing stream used."""
+    from budgetformer_amd import attention
+    built, capturing = [], [False]
+
+    def from_lengths(lens, device=None):
+        built.append(len(lens))
+        return object()
+
+    monkeypatch.setattr(attention.PackedSequences, "from_lengths", from_lengths)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    cache, dev = attention._BatchSequences(), torch.device("cuda:0")
+    first = cache.get(1, 10, dev)
+    capturing[0] = True
+    assert cache.get(1, 10, dev) is first and built == [1]
+    capturing[0] = False
+    others = [cache.get(b, 10, dev) for b in range(2, 12)]
+    assert cache.get(1, 10, dev) is first and built == list(range(1, 12))
+    assert all(cache.get(b, 10, dev) is others[b - 2] for b in range(8, 12)) and len(built) == 11
+    cache.get(2, 10, dev)                                    # one of the first is built again
+    assert built[-1] == 2 and len(built) == 12
+
+
+def test_sequences_of_calls_from_several_threads(monkeypatch):
+    import sys
+    import threading
+    from budgetformer_amd import attention
+    monkeypatch.setattr(attention.PackedSequences, "from_lengths", lambda lens, device=None: len(lens))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    cache, dev, wrong = attention._BatchSequences(), torch.device("cuda:0"), []
+
+    def work(seed):
+        try:
+            for i in range(20000):
+                b = (i * seed) % 7 + 1
+                if cache.get(b, 3, dev) != b:
+                    wrong.append(b)
+        except Exception as e:                               # an entry gone between two steps
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2, 3, 5)]
+    often = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)                              # a thread gives way between any two steps
+    try:
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        sys.setswitchinterval(often)
+    assert not wrong
+
+
 def test_operators_are_registered():
     ops = N.load_ops()
     for name in ("packed_spans", "packed_attn_fwd", "packed_attn_bwd", "rotary", "linear_attn_fwd", "linear_attn_bwd", "linear_attn_step",
