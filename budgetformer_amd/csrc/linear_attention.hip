@@ -137,7 +137,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
   const int64_t slot = xcd_slot(blockIdx.x, gridDim.x);
   const int h = int(slot % a.heads), seg = int(slot / a.heads);     // the heads of a token share its cache lines
   const int own = seg * a.seg_len, end = min(own + a.seg_len, a.n);
-  const int begin = a.warm && seg > 0 ? min(own, start_of(a, span_at(a, own))) : own;      // rows before `own` are another's
+  const int begin = a.warm && seg > 0 ? max(min(own, start_of(a, span_at(a, own))), 0) : own;      // rows before `own` are another's
   const float ld = decay_log2(a, h);
   // the axis as the pass reads it: from the last token with steps back, or from the first
   const int64_t back = a.reverse ? a.n - 1 : 0;

@@ -52,7 +52,7 @@ struct Args {
   float *lse, *delta, *part, *stat;
   const int2 *row_span, *key_span;
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;      // strides in values
-  int32_t rows, n_k, hq, hk, group, dim;           // rows: (token, head of the group) pairs of one key head
+  int32_t rows, n_q, n_k, hq, hk, group, dim;      // rows: (token, head of the group) pairs of one key head
   int32_t tiles, pieces;
   const int32_t* order;                            // of the tiles, or NULL: the last one first
   float scale, c;                                  // c = scale * log2(e)
@@ -72,6 +72,12 @@ __device__ __forceinline__ Row row_of(const Args& a, int h, int rho) {
 __device__ __forceinline__ int2 span_at(const int2* s, int i) {
   const int2 x = s[i];
   return make_int2(__builtin_amdgcn_readfirstlane(x.x), __builtin_amdgcn_readfirstlane(x.y));
+}
+
+// A row's bound among the keys, and the rows of the group that a key's span names: inside the tensors whatever a span holds.
+__device__ __forceinline__ int in_keys(const Args& a, int x) { return min(max(x, 0), a.n_k); }
+__device__ __forceinline__ int2 group_rows(const Args& a, int2 s) {
+  return make_int2(min(max(s.x, 0), a.n_q) * a.group, min(max(s.y, 0), a.n_q) * a.group);
 }
 
 // Which (tile, key head, piece) a workgroup takes; false: none. Workgroup i runs on XCD i % 8, each with an L2 of its own.
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
 
   const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
   const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
-  int kbeg = max(first_span.x, 0), kend = min(last_span.y, a.n_k);
+  int kbeg = in_keys(a, first_span.x), kend = in_keys(a, last_span.y);
   if constexpr (SPLIT) {
     const int width = (max(kend - kbeg, 0) + a.pieces * BN - 1) / (a.pieces * BN) * BN;
     kbeg += piece * width;
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
   const int row0 = tile * BM, last = min(row0 + BM, a.rows) - 1;
   const int2 first_span = span_at(a.row_span, a.by_group(row0)), last_span = span_at(a.row_span, a.by_group(last));
-  const int kbeg = max(first_span.x, 0), kend = min(last_span.y, a.n_k);
+  const int kbeg = in_keys(a, first_span.x), kend = in_keys(a, last_span.y);
   const int w_row0 = row0 + 32 * wave, w_last = min(w_row0 + 31, a.rows - 1);
   const bool w_any = w_row0 < a.rows;
   const int2 wf = span_at(a.row_span, a.by_group(min(w_row0, a.rows - 1))), wl = span_at(a.row_span, a.by_group(w_last));
@@ -476,9 +482,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
   if (!a.order) tile = a.tiles - 1 - tile;         // with a causal mask the first keys are seen by the most rows
 
   const int key0 = tile * BK, last = min(key0 + BK, a.n_k) - 1;
-  const int2 first_span = span_at(a.key_span, key0), last_span = span_at(a.key_span, last);
   // rows of the group: token * group + head
-  int rbeg = max(first_span.x, 0) * a.group, rend = min(last_span.y * a.group, a.rows);
+  const int2 first_span = group_rows(a, span_at(a.key_span, key0)), last_span = group_rows(a, span_at(a.key_span, last));
+  int rbeg = first_span.x, rend = last_span.y;
   if (a.pieces > 1) {                             // equal parts of the tile's own rows
     const int width = int(ceil_div(max(rend - rbeg, 0), a.pieces * BR)) * BR;
     rbeg = min(rbeg + piece * width, rend);
@@ -486,12 +492,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
   }
   const int w_key0 = key0 + 32 * wave, w_last = min(w_key0 + 31, a.n_k - 1);
   const bool w_any = w_key0 < a.n_k;
-  const int2 wf = span_at(a.key_span, min(w_key0, a.n_k - 1)), wl = span_at(a.key_span, w_last);
-  const int w_beg = wf.x * a.group, w_end = wl.y * a.group, w_full_beg = wl.x * a.group, w_full_end = wf.y * a.group;
+  const int2 wf = group_rows(a, span_at(a.key_span, min(w_key0, a.n_k - 1))), wl = group_rows(a, span_at(a.key_span, w_last));
+  const int w_beg = wf.x, w_end = wl.y, w_full_beg = wl.x, w_full_end = wf.y;
   const int key = w_key0 + col;
   const bool valid = key < a.n_k;
-  const int2 span = a.key_span[valid ? key : a.n_k - 1];
-  const int lo = span.x * a.group, hi = valid ? span.y * a.group : lo;
+  const int2 span = group_rows(a, a.key_span[valid ? key : a.n_k - 1]);
+  const int lo = span.x, hi = valid ? span.y : lo;
 
   Frag<T> kf[TL::kSteps], vf[TL::kSteps];
   load_row<T, DP>(kf, valid ? static_cast<const T*>(a.k) + key * a.ks_t + h * a.ks_h : nullptr, a.dim, half);
@@ -538,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
     else if (tid < 2 * BR)
       delta_lds[tid - BR] = stat;
     bool odd = false;
-    if (i0 < last_span.x * a.group || i0 + BR > first_span.y * a.group) {
+    if (i0 < last_span.x || i0 + BR > first_span.y) {
       const bool mine = qs.tainted() || gs.tainted();
       odd = __syncthreads_or(mine);
     } else {
@@ -741,7 +747,7 @@ Args make_args(const bf_packed_attn* p, const void* q, const void* k, const void
   a.vs_t = p->v_stride[0], a.vs_h = p->v_stride[1];
   a.hq = p->heads_q, a.hk = p->heads_k, a.group = p->heads_q / p->heads_k, a.dim = p->head_dim;
   a.rows = int32_t(p->n_q * a.group);
-  a.n_k = int32_t(p->n_k);
+  a.n_q = int32_t(p->n_q), a.n_k = int32_t(p->n_k);
   a.scale = p->scale;
   a.c = p->scale * kLog2e;
   a.by_group = make_div(uint32_t(a.group));

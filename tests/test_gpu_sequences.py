@@ -385,6 +385,30 @@ def test_results_repeat_bit_for_bit(hip_device):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [16, 128])
+@pytest.mark.parametrize("longest", [0, 5, 2100])
+def test_spans_of_any_numbers_stay_inside_the_tensors(hip_device, longest, d, dtype):
+    """The operators below the sequences take spans as they come: any 32-bit numbers give some result, from the tensors'
+    own rows (here a group's row number would pass 32 bits, and differences of two bounds)."""
+    ops, H, Hk, n = torch.ops.bf, 8, 2, 2100
+    q, do = (_randn(i, n, H, d, dtype=dtype, dev=hip_device) for i in (0, 3))
+    k, v = (_randn(i, n, Hk, d, dtype=dtype, dev=hip_device) for i in (1, 2))
+    gen = torch.Generator().manual_seed(5)
+    ld = torch.full((H,), -0.1, device=hip_device)
+    off = torch.tensor([0, 700, n], dtype=torch.int32, device=hip_device)
+    far = torch.tensor([-2 ** 31, -2 ** 29, -7, 0, 5, n, 2 ** 29, 2 ** 29 + 3, 2 ** 31 - 1], dtype=torch.int64)
+    for rep in range(3):
+        row_span, key_span = (far[torch.randint(len(far), (n, 2), generator=gen)].to(torch.int32).to(hip_device) for _ in range(2))
+        out, lse, rest = ops.packed_attn_fwd(q, k, v, row_span, 0.1, longest, True)
+        grads = ops.packed_attn_bwd(q, k, v, row_span, key_span, out, lse, do, 0.1, longest, rest)
+        few = ops.packed_attn_fwd(q[:3], k, v, row_span[:3].contiguous(), 0.1, longest, False)
+        lin = ops.linear_attn_fwd(q, q, q, ld, row_span, key_span, off, 0.1, longest, None, True)
+        back = ops.linear_attn_bwd(q, q, q, ld, row_span, key_span, off, do, 0.1, longest)
+        torch.cuda.synchronize()
+        assert all(t.numel() for t in (*grads, *few[:2], *lin, *back))
+
+
 # ------------------------------------------------------------------ rotary positions
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
