@@ -86,7 +86,7 @@ __device__ __forceinline__ int start_of(const LinArgs& a, int2 s) {
 __device__ __forceinline__ int sequence_of(const LinArgs& a, int p) {
   int lo = -1, hi = a.n_seq;
   while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
+    const int mid = hi - ((hi - lo) >> 1);      // their sum may pass 32 bits; lo + 1 at least
     if (a.offsets[mid] <= p)
       lo = mid;
     else

@@ -659,7 +659,7 @@ __global__ __launch_bounds__(256) void packed_spans(const int32_t* q_off, const 
   const int32_t* off = is_q ? q_off : k_off;
   int lo = 0, hi = n_seq;                       // the last s with off[s] <= x
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
+    const int mid = lo + ((hi - lo) >> 1);      // their sum may pass 32 bits
     if (off[mid + 1] <= x)
       lo = mid + 1;
     else

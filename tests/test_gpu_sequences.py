@@ -379,6 +379,19 @@ def test_short_sequences_keep_what_they_do_not_see_out(hip_device, dtype):
     assert bool((out[2:5] == float("inf")).all()) and torch.equal(out[:2], clean[0][:2])
 
 
+def test_more_than_2_to_the_30_sequences(hip_device):
+    """Sequences without tokens before and behind a few with: their numbers, summed in a search, pass 32 bits."""
+    bf = _bf()
+    n_seq, lens = 2 ** 30 + 100, [5, 40, 3]
+    off = torch.zeros(n_seq + 1, dtype=torch.int32, device=hip_device)
+    off[-3:] = torch.tensor(lens, device=hip_device).cumsum(0)
+    seqs = bf.PackedSequences.from_offsets(off, n_q=48, causal=True, check=False)
+    del off
+    plain = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+    assert torch.equal(seqs.row_span, plain.row_span) and torch.equal(seqs.key_span, plain.key_span)
+    assert torch.equal(seqs.positions(), plain.positions())
+
+
 def test_results_repeat_bit_for_bit(hip_device):
     a = _attention_case(hip_device, [300, 41], [300, 41], 8, 2, 64, True, torch.bfloat16, seed=3, train=False)
     b = _attention_case(hip_device, [300, 41], [300, 41], 8, 2, 64, True, torch.bfloat16, seed=3, train=False)
