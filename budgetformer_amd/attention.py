@@ -308,14 +308,14 @@ class CoreAttention(nn.Module):
             raise NotImplementedError("attn_type='flash' takes no attention bias")
         if self.training and self.attention_dropout_rate > 0.0:
             raise NotImplementedError("attn_type='flash' has no attention dropout")
-        batch_size, s_len = q.size(0), q.size(1)
-        q, k, v = (t.reshape(-1, t.size(2), t.size(3)) for t in (q, k, v))
+        batch_size, s_len, width = q.size(0), q.size(1), q.size(2) * q.size(3)
+        q, k, v = (t.reshape(t.size(0) * t.size(1), t.size(2), t.size(3)) for t in (q, k, v))
         seqs = sequences if isinstance(sequences, PackedSequences) else self._batches.get(batch_size, s_len, q.device)
         if self.rotary is not None:
             if seqs.n_q != seqs.n_k:
                 raise ValueError("rotary positions of the flash path need as many keys as rows")
             q, k = rotary_embedding(q, k, self.rotary, seqs=seqs)
-        return packed_attention(q, k, v, seqs).reshape(batch_size, s_len, -1)
+        return packed_attention(q, k, v, seqs).reshape(batch_size, s_len, width)
 
 
 class GTCoreAttention(nn.Module):

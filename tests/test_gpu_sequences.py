@@ -1021,6 +1021,17 @@ def test_empty_batches(hip_device):
     assert torch.equal(state, s0)
 
 
+@pytest.mark.parametrize("b,S", [(0, 7), (3, 0), (0, 0)])
+def test_flash_of_empty_batches(hip_device, b, S):
+    from budgetformer_amd.attention import CoreAttention
+    bf = _bf()
+    x = torch.zeros(b, S, 2, 16, device=hip_device, requires_grad=True)
+    for core in (CoreAttention(32, 0.0, 2, 1), CoreAttention(32, 0.0, 2, 1, rotary=bf.RotaryFrequencies(16, device=hip_device))):
+        out = core(x, x, x, attn_type="flash")
+        assert out.shape == (b, S, 32)
+        assert torch.autograd.grad(out.sum(), x)[0].shape == x.shape
+
+
 def test_refusals(hip_device):
     bf = _bf()
     dev = hip_device
