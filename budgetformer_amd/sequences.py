@@ -100,7 +100,8 @@ class PackedSequences:
     def from_lengths(cls, q_lengths: Sequence[int], k_lengths: Optional[Sequence[int]] = None, *, causal: bool = False,
                      device="cuda") -> "PackedSequences":
         """From the sequences' lengths on the host (a list, or a CPU tensor); ``k_lengths``: those of the keys
-        where they differ. Nothing is read back from the device."""
+        where they differ. Nothing is read back from the device. Not under graph capture, which would copy from the host's
+        lengths again at each replay (``from_offsets`` without the check)."""
         device = cls._device(device)
         lens = [torch.as_tensor(x, dtype=torch.int64, device="cpu") for x in
                 ((q_lengths,) if k_lengths is None else (q_lengths, k_lengths))]
@@ -112,6 +113,7 @@ class PackedSequences:
         ends = [torch.cat([x.new_zeros(1), x.cumsum(0)]) for x in lens]
         totals = [int(e[-1]) for e in ends]
         cls._sizes(totals[0], totals[-1])
+        cls._not_capturing("from_lengths")
         with torch.inference_mode(False):
             on = [e.to(torch.int32).to(device) for e in ends]
         return cls(on[0], on[-1], totals[0], totals[-1], causal, max([int(x.max()) for x in lens if x.numel()], default=0))
@@ -134,6 +136,7 @@ class PackedSequences:
         if k_offsets is None and n_k is not None and n_k != n_q:
             raise ValueError("n_k differs from n_q without k_offsets")
         if check:
+            cls._not_capturing("from_offsets with the check")
             for i, x in enumerate((q_offsets, q_offsets if k_offsets is None else k_offsets)):
                 host = x.cpu().to(torch.int64)
                 if int(host[0]) != 0 or bool((host[1:] < host[:-1]).any()):
@@ -150,6 +153,12 @@ class PackedSequences:
             q = q_offsets.to(torch.int32, copy=True).contiguous()      # a copy: the caller's may change
             k = q if k_offsets is None else k_offsets.to(torch.int32, copy=True).contiguous()
         return cls(q, k, sizes[0], sizes[1], causal, longest)
+
+    @staticmethod
+    def _not_capturing(what: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} is not for graph capture: build the sequences before it (a flash layer's by a call at "
+                               "the same shape), or from device offsets without the check")
 
     @staticmethod
     def _device(device) -> torch.device:

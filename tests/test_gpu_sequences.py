@@ -902,6 +902,33 @@ def test_a_captured_flash_layer_replays_after_other_shapes(hip_device):
         del junk
 
 
+def test_sequences_built_under_capture(hip_device):
+    """From device offsets without the check, anew at each replay; what would read or copy from the host is refused and
+    leaves the capture as it is."""
+    bf = _bf()
+    off = torch.tensor([0, 20, 50], device=hip_device)
+    x = _randn(1, 60, 2, 16, dev=hip_device)
+
+    def every():
+        return bf.packed_attention(x, x, x, bf.PackedSequences.from_offsets(off, n_q=60, causal=True, check=False))
+
+    every()
+    torch.cuda.synchronize(hip_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="not for graph capture"):
+            bf.PackedSequences.from_lengths([20, 40], device=hip_device)
+        with pytest.raises(RuntimeError, match="not for graph capture"):
+            bf.PackedSequences.from_offsets(off)
+        out = every()
+    for ends in ([20, 50], [1, 60], [0, 33], [25, 25]):
+        off[1:] = torch.tensor(ends, device=hip_device)
+        graph.replay()
+        torch.cuda.synchronize(hip_device)
+        got = out.clone()
+        assert torch.equal(got, every())
+
+
 def test_two_streams_at_once(hip_device):
     """Calls of different sizes on two streams, with their pieces and carries in flight together."""
     bf = _bf()

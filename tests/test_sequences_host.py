@@ -197,6 +197,15 @@ def test_sequences_that_a_capture_used_are_kept(monkeypatch):
     assert built[-1] == 2 and len(built) == 12
 
 
+def test_lengths_from_the_host_are_refused_under_capture(monkeypatch):
+    from budgetformer_amd import attention
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="not for graph capture"):
+        bf.PackedSequences.from_lengths([3, 4])
+    with pytest.raises(RuntimeError, match="not for graph capture"):
+        attention._BatchSequences().get(2, 5, torch.device("cuda:0"))
+
+
 def test_sequences_of_calls_from_several_threads(monkeypatch):
     import sys
     import threading
