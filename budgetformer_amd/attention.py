@@ -312,6 +312,8 @@ class CoreAttention(nn.Module):
         q, k, v = (t.reshape(t.size(0) * t.size(1), t.size(2), t.size(3)) for t in (q, k, v))
         seqs = sequences if isinstance(sequences, PackedSequences) else self._batches.get(batch_size, s_len, q.device)
         if self.rotary is not None:
+            if self.rotary.turns.device != q.device:             # the module has moved
+                self.rotary = self.rotary.to(q.device)
             if seqs.n_q != seqs.n_k:
                 raise ValueError("rotary positions of the flash path need as many keys as rows")
             q, k = rotary_embedding(q, k, self.rotary, seqs=seqs)

@@ -206,6 +206,29 @@ def test_lengths_from_the_host_are_refused_under_capture(monkeypatch):
         attention._BatchSequences().get(2, 5, torch.device("cuda:0"))
 
 
+def test_rotary_frequencies_follow_the_layer_to_another_device(monkeypatch):
+    from budgetformer_amd import attention
+    there = object.__new__(bf.RotaryFrequencies)
+    there.rot, there.amplitude, there.turns = 8, 1.0, torch.zeros(4, device="meta")
+    moved = []
+
+    def to(self, device):
+        got = object.__new__(bf.RotaryFrequencies)
+        got.rot, got.amplitude, got.turns = self.rot, self.amplitude, torch.zeros(4, device=device)
+        moved.append(got)
+        return got
+
+    monkeypatch.setattr(bf.RotaryFrequencies, "to", to)
+    monkeypatch.setattr(attention, "rotary_embedding", lambda q, k, freq, seqs: (q, k) if freq.turns.device == q.device else None)
+    monkeypatch.setattr(attention, "packed_attention", lambda q, k, v, seqs: q)
+    seqs = object.__new__(bf.PackedSequences)
+    seqs.n_q = seqs.n_k = 6
+    core, x = bf.CoreAttention(16, 0.0, 2, 1, rotary=there), torch.zeros(2, 3, 2, 8)
+    for _ in range(2):
+        assert core(x, x, x, edge_index=seqs, attn_type="flash").shape == (2, 3, 16)
+    assert len(moved) == 1 and core.rotary is moved[0]
+
+
 def test_sequences_of_calls_from_several_threads(monkeypatch):
     import sys
     import threading
