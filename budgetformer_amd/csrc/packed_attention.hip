@@ -727,7 +727,8 @@ int check(const bf_packed_attn* p, const char* fn, bool backward) {
   BF_CHECK_ARG(p->n_q >= 0 && p->n_k >= 0 && p->n_k < kMaxRows && p->n_q < kMaxRows / p->heads_q,
                "%s: %lld rows of %d heads, %lld keys (below 2^31 - 2^17 each)", fn, (long long)p->n_q, p->heads_q, (long long)p->n_k);
   BF_CHECK_ARG(p->longest >= 0, "%s: longest sequence %d", fn, p->longest);
-  BF_CHECK_ARG(p->scale > 0.f && p->scale <= 3e38f, "%s: scale %g (positive and finite expected)", fn, double(p->scale));
+  // its product with log2 e has to be finite too
+  BF_CHECK_ARG(p->scale > 0.f && p->scale <= 2e38f, "%s: scale %g (positive, up to 2e38 expected)", fn, double(p->scale));
   const int64_t per16 = p->dtype == BF_DTYPE_F32 ? 4 : 8;
   for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
     BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,

@@ -202,7 +202,7 @@ def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = No
 
     q [n_q, heads, hn], k and v [n_k, kv_heads, hn] of one dtype (k and v are cast to q's), heads a multiple of
     kv_heads (query head h reads key head h // (heads // kv_heads)), hn a multiple of 8 up to 128. Rows and heads
-    may have any strides. ``scale`` (positive): 1 / sqrt(hn) by default. Returns out [n_q, heads, hn], or (out,
+    may have any strides. ``scale`` (positive, up to 2e38): 1 / sqrt(hn) by default. Returns out [n_q, heads, hn], or (out,
     lse) with ``with_lse``: lse float32 [n_q, heads], the log of the row's sum of exponentials, -inf for a row
     that sees no key (its out is 0); lse is not differentiable. Gradients repeat bit for bit."""
     _check_seqs(seqs, q, k)

@@ -812,7 +812,7 @@ typedef struct bf_packed_attn {
   int64_t q_stride[2], k_stride[2], v_stride[2];
   const int32_t* row_span;
   const int32_t* key_span;
-  float scale;                /* of q.k; positive                            */
+  float scale;                /* of q.k; positive, up to 2e38                */
   int32_t longest;            /* no sequence has more rows or keys; 0: unknown
                                  (chooses how the work is cut, not results)  */
 } bf_packed_attn;

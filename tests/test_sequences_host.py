@@ -41,6 +41,13 @@ def test_packed_attention_arguments(kw, match):
     assert N.load().bf_packed_attn_fwd_floats(C.byref(_attn(**kw))) == -1
 
 
+def test_packed_attention_scales_at_the_end_of_float32():
+    """A scale whose product with log2 e is infinite would make a score of 0 a NaN."""
+    lib = N.load()
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(scale=2e38))) >= 0
+    assert lib.bf_packed_attn_fwd_floats(C.byref(_attn(scale=2.5e38))) == -1
+
+
 @pytest.mark.parametrize("d", [0, 4, 12, 136])
 def test_packed_attention_head_dims(d):
     with pytest.raises(NotImplementedError, match="head_dim"):
