@@ -95,6 +95,46 @@ def test_whole_rows_of_many_tiles(hip_device):
     _attention_case(hip_device, [2500, 1, 300, 77], [2500, 1, 300, 77], 32, 16, 64, True, torch.bfloat16, seed=23)
 
 
+def _scratch_floats(lens, H, Hk, d, dtype):
+    """What the forward asks for: 0 for whole rows in the order they lie, 8192 with the tiles put in order, else pieces."""
+    import ctypes as C
+    from budgetformer_amd import _native as N
+    code = {torch.float32: N.BF_DTYPE_F32, torch.bfloat16: N.BF_DTYPE_BF16, torch.float16: N.BF_DTYPE_F16}[dtype]
+    a = N.PackedAttn(n_q=sum(lens), n_k=sum(lens), heads_q=H, heads_k=Hk, head_dim=d, dtype=code, row_span=64, key_span=64,
+                     scale=1.0, longest=max(lens))
+    return N.load().bf_packed_attn_fwd_floats(C.byref(a))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 64, 72, 128])
+@pytest.mark.parametrize("lens,causal,floats", [([1300, 1, 517, 0, 230, 7], True, 8192), ([2051], True, 0), ([300] * 13 + [259], True, 0),
+                                                ([700, 1351], False, 8192)], ids=["mixed", "one", "many", "all"])
+def test_whole_rows_of_every_type_and_head_size(hip_device, lens, causal, floats, d, dtype):
+    """No pieces: the workgroups of two and four waves over whole rows, with tiles that end anywhere, put in order or not."""
+    H, Hk = 32, 16
+    assert _scratch_floats(lens, H, Hk, d, dtype) == floats
+    _attention_case(hip_device, lens, lens, H, Hk, d, causal, dtype, seed=37)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_the_backward_reads_what_rounding_left(hip_device, d, dtype):
+    """Values of 8 and a little: Delta from the rounded out is off by out's rounding, some 2^3 half-steps of the type a
+    value. With `rest` what is left comes from the rounding of P, which is as large a part of each of 400 to 1000 terms
+    and averages out over them: less than a quarter."""
+    ops, bf, n, H = torch.ops.bf, _bf(), 1000, 2
+    q, k, do = (_randn(i, n, H, d, dtype=dtype, dev=hip_device) for i in (0, 1, 3))
+    v = (8 + 0.25 * _randn(2, n, H, d, dev=hip_device)).to(dtype)
+    seqs = bf.PackedSequences.from_lengths([n], device=hip_device)
+    out, lse, rest = ops.packed_attn_fwd(q, k, v, seqs.row_span, d ** -0.5, n, True)
+    ref = sq.attention(q.double(), k.double(), v.double(), [n], [n], False, d ** -0.5, do.double())
+    off = []
+    for r in (rest, None):
+        got = ops.packed_attn_bwd(q, k, v, seqs.row_span, seqs.key_span, out, lse, do, d ** -0.5, n, r)
+        off.append([float((x.double() - ref[name]).norm()) for x, name in zip(got, ("dq", "dk"))])
+    assert rest.shape == out.shape and off[0][0] < off[1][0] / 4 and off[0][1] < off[1][1] / 4, off
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128])
 def test_few_key_tiles_seen_by_many_rows(hip_device, d, dtype):
@@ -451,6 +491,35 @@ def test_rotary_values_and_gradients(hip_device, hq, hk, d, rot, interleaved, dt
         assert torch.equal(got[..., rot:], x[..., rot:])
 
 
+def test_operators_without_gradients_give_the_same_bits(hip_device):
+    """bf::rotary, packed_attn_* and linear_attn_* as a caller takes them beside the differentiable ones."""
+    bf, ops = _bf(), torch.ops.bf
+    lens, H, d = [70, 1, 130], 2, 32
+    q, k, v, do = (_randn(i, sum(lens), H, d, dtype=torch.bfloat16, dev=hip_device) for i in range(4))
+    seqs = bf.PackedSequences.from_lengths(lens, causal=True, device=hip_device)
+    freq, ld = bf.RotaryFrequencies(d, amplitude=1.5, device=hip_device), torch.full((H,), -0.1, device=hip_device)
+    spans = (seqs.row_span, seqs.key_span)
+
+    def gradients(f, *xs):
+        leaves = [x.clone().requires_grad_(True) for x in xs]
+        out = f(*leaves)
+        outs = out if isinstance(out, tuple) else (out,)
+        return [*outs, *torch.autograd.grad(outs, leaves, [do] * len(outs))]
+
+    pos = seqs.positions()
+    got = [*ops.rotary(q, k, pos, freq.turns, 1.5, True), *ops.rotary(do, do, pos, freq.turns, 1.5, True, True)]
+    for a, b in zip(got, gradients(lambda x, y: bf.rotary_embedding(x, y, freq, seqs=seqs, interleaved=True), q, k)):
+        assert torch.equal(a, b)
+    out, lse, rest = ops.packed_attn_fwd(q, k, v, spans[0], 0.2, seqs.longest, True)
+    got = [out, *ops.packed_attn_bwd(q, k, v, *spans, out, lse, do, 0.2, seqs.longest, rest)]
+    for a, b in zip(got, gradients(lambda *x: bf.packed_attention(*x, seqs, scale=0.2), q, k, v)):
+        assert torch.equal(a, b)
+    out, _ = ops.linear_attn_fwd(q, k, v, ld, *spans, seqs.q_offsets, 0.2, seqs.longest)
+    got = [out, *ops.linear_attn_bwd(q, k, v, ld, *spans, seqs.q_offsets, do, 0.2, seqs.longest)]
+    for a, b in zip(got, gradients(lambda *x: bf.linear_attention(*x, ld, seqs, scale=0.2), q, k, v)):
+        assert torch.equal(a, b)
+
+
 def test_rotary_of_one_of_two_gradients(hip_device):
     bf = _bf()
     q, k = (_randn(i, 9, 2, 16, dev=hip_device).requires_grad_(True) for i in (1, 2))
@@ -551,6 +620,15 @@ def test_linear_attention_head_sizes(hip_device, dk, dv, dtype):
 def test_linear_attention_over_segments(hip_device, init, dtype):
     """More tokens than a segment (256): the state is carried across, past a sequence's end inside a segment too."""
     _linear_case(hip_device, [700, 50, 256, 6, 500], 2, 16, 16, dtype, seed=41, init=init)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("init", [False, True])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 128), (128, 72)])
+@pytest.mark.parametrize("lens", [[600, 50, 131], [100] * 7 + [81]], ids=["carried", "warm"])
+def test_linear_attention_of_wide_heads_over_segments(hip_device, lens, dk, dv, init, dtype):
+    """Four waves and four blocks of the state over segments of 256 tokens, carried or (short sequences) begun anew."""
+    _linear_case(hip_device, lens, 2, dk, dv, dtype, seed=42, init=init)
 
 
 @pytest.mark.parametrize("lens", [[20000], [9000, 3, 64, 10900]])
