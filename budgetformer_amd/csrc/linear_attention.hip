@@ -65,10 +65,8 @@ constexpr int kTile = 32;        // tokens of a tile
 // result's own is 2^-25). Larger ones take a unit of their own, that brings the largest to 2^15.
 constexpr float kScoreUnit = 1.f / 512.f, kStateUnit = 1.f / 64.f, kUnitMost = 32768.f;
 
-// The unit, a power of 2, in which `big` is at most 2^15; `usual` where it is not finite.
-__device__ __forceinline__ float unit_of(float big, float usual) {
-  return big < INFINITY ? ldexpf(1.f, __builtin_amdgcn_frexp_expf(big) - 15) : usual;
-}
+// The unit, a power of 2, in which `big` is at most 2^15.
+__device__ __forceinline__ float unit_of(float big) { return ldexpf(1.f, __builtin_amdgcn_frexp_expf(big) - 15); }
 
 // A head's log decay; one of 0 (log -inf) stays finite, so that its power 0 is 1; a NaN stays one
 __device__ __forceinline__ float finite_decay(float x) { return x < -1e4f ? -1e4f : x; }
@@ -239,8 +237,15 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]));
           if (__any(big > kUnitMost * kStateUnit)) {
+            if (!(big < INFINITY)) {           // a column that is not finite is no reason for the others to overflow
+              big = 0.f;
+#pragma unroll
+              for (int b = 0; b < XB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(m[b][r]) < INFINITY ? fabsf(m[b][r]) : 0.f);
+            }
             for (int n = 32; n; n >>= 1) big = fmaxf(big, __shfl_xor(big, n, 64));
-            unit = unit_of(big, kStateUnit);
+            if (big > kUnitMost * kStateUnit) unit = unit_of(big);
           }
         }
         const float per_unit = 1.f / unit;
@@ -274,7 +279,7 @@ __global__ __launch_bounds__(2 * DZ, 2) void linear_pass(const LinRoles all) {
         for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(w[r]));
         if (__any(big > kUnitMost * kScoreUnit)) {
           big = fmaxf(big, __shfl_xor(big, 32, 64));
-          if (big > kUnitMost * kScoreUnit) unit = unit_of(big, kScoreUnit);
+          if (big > kUnitMost * kScoreUnit && big < INFINITY) unit = unit_of(big);
         }
         const float per_unit = 1.f / unit;
 #pragma unroll

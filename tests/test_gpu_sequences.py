@@ -722,6 +722,31 @@ def test_linear_attention_small_gradients_keep_their_bits_in_float16(hip_device)
     _linear_of_sizes(hip_device, (100.0, 100.0, 1.0, 1e-6), [300, 33], 2.0 ** -31, ("dq", "dk"))
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** -10, 32.0), (2.0 ** -6, 2.0)])
+@pytest.mark.parametrize("where", ["v", "state"])
+def test_linear_attention_columns_beside_one_that_is_not_finite(hip_device, where, q_size, k_size, bad):
+    """A value that is not finite, in one column of v or of the initial state: the other columns of its rows' results, whose
+    states are past 1000 and past 65504, come out as without it."""
+    bf = _bf()
+    n, d = 400, 16
+    seqs = bf.PackedSequences.from_lengths([n], causal=True, device=hip_device)
+    q = torch.full((n, 1, d), q_size, dtype=torch.float16, device=hip_device)
+    k = torch.full((n, 1, d), k_size, dtype=torch.float16, device=hip_device)
+    v = torch.full((n, 1, d), 32.0, dtype=torch.float16, device=hip_device)
+    state = torch.zeros(1, 1, d, d, device=hip_device)
+    first = 3
+    if where == "v":
+        v[first, :, 5] = bad
+    else:
+        state[..., 5], first = bad, 0
+    out = bf.linear_attention(q, k, v, torch.zeros(1, device=hip_device), seqs, scale=1.0, initial_state=state)
+    ref = (16 * q_size * k_size * 32) * torch.arange(1, n + 1, device=hip_device).double()[:, None, None].expand(n, 1, d)
+    keep = torch.arange(d, device=hip_device) != 5
+    _within("out", out[..., keep], ref[..., keep], 3 * 2.0 ** -11 * ref[..., keep])      # the state's rounding to 11 bits, the result's
+    assert not bool(torch.isfinite(out[first:, :, 5]).any())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,H,dk,dv", [(1, 1, 8, 8), (3, 5, 128, 128), (7, 2, 24, 72), (2, 3, 64, 16)])
 def test_linear_attention_step_continues_a_prompt(hip_device, n, H, dk, dv, dtype):
