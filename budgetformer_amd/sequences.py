@@ -57,6 +57,8 @@ class PackedSequences:
     ``[k_offsets[s], k_offsets[s + 1])``: all of them, or with ``causal`` those up to their own place, the last
     query at the last key (one query a sequence then sees all its keys). Rows behind the last sequence see
     nothing: their outputs and gradients are 0.
+
+    A captured graph reads these tensors at each replay: keep the object as long as the graph.
     """
 
     # Plain tensors also where a batch is built in inference mode: training later saves them.
@@ -311,7 +313,9 @@ def linear_attention(q, k, v, log_decay, seqs: PackedSequences, scale: Optional[
     softmax, whose state S_i = exp(log_decay) S_{i-1} + k_i v_i^T has a fixed size.
 
     q and k [rows, heads, dk], v [rows, heads, dv] of one dtype (k and v are cast to q's), dk and dv multiples of 8
-    up to 128; log_decay float32 [heads], at most 0 (0: no decay; -inf: only the row's own token), a constant.
+    up to 128; log_decay float32 [heads], at most 0 (0: no decay; -inf: only the row's own token; NaN: the head's results
+    are NaN), a constant. A value of v that is not finite makes its column NaN or infinite in the rows that see it, and
+    leaves the other columns and rows as they are.
     ``seqs``: causal, the same sequences for rows and keys. ``scale``: 1 / sqrt(dk) by default.
     ``initial_state`` float32 [sequences, heads, dk, dv] comes before each sequence's first token; with
     ``return_state`` (out, state behind the last token) is returned, from which ``linear_attention_step`` or the

@@ -824,7 +824,9 @@ typedef struct bf_packed_attn {
  * arguments), for calls of few rows, whose keys are cut into pieces, and of sequences of very
  * different lengths, whose tiles are put in order. rest (or NULL): like out,
  * what out's rounding left, for the backward; bf_packed_attn_rest(p) says
- * whether the backward reads it.                                            */
+ * whether the backward reads it (in 16-bit types). In float16 P and, in the
+ * backward, dS are operands in units of a power of 2: neither small nor large
+ * ones leave the type's range where the results fit it.                     */
 int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p);
 int bf_packed_attn_rest(const bf_packed_attn* p);
 int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
@@ -862,7 +864,11 @@ int bf_rotary(const void* x, const void* y, int64_t n, int32_t heads_x, int32_t 
  * init (or NULL): float32 [n_seq, heads, dim_k, dim_v], each sequence's state
  * before its first token; final_state (or NULL, forward only): the state
  * sum_j g^(n - 1 - j) k_j v_j^T + g^n init behind its last. offsets (int32
- * [n_seq + 1]) is read only with one of them.                               */
+ * [n_seq + 1]) is read only with one of them. A decay that is NaN makes its
+ * head's results NaN. A value of v that is not finite makes its column of the
+ * results that see it NaN or infinite (an infinity's sign is not kept: the
+ * state it enters is multiplied by values of both signs); other columns, and
+ * rows that do not see it, are as without it.                               */
 typedef struct bf_linear_attn {
   int64_t n, n_seq;
   int32_t heads, dim_k, dim_v, dtype;
