@@ -909,7 +909,7 @@ extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
 }
 
 extern "C" int bf_packed_attn_rest(const bf_packed_attn* p) {
-  return check(p, "packed_attn_rest", false) == BF_OK && p->dtype != BF_DTYPE_F32;
+  return check(p, "packed_attn_rest", false) == BF_OK && p->dtype != BF_DTYPE_F32 && !packed_is_short(p);
 }
 
 extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
@@ -919,7 +919,7 @@ extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const 
   BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
   BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_fwd: rest and scratch must be 16-byte aligned");
-  if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, rest, lse, as_stream(stream));
+  if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
   Args a = make_args(p, q, k, v);
   a.o = out, a.rest = rest, a.lse = lse;
   a.pieces = pieces_of(p);
@@ -973,7 +973,7 @@ extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const 
                "packed_attn_bwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
   BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_bwd: rest and scratch must be 16-byte aligned");
-  if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, rest, lse, dout, dq, dk, dv, as_stream(stream));
+  if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, delta, as_stream(stream));
   Args a = make_args(p, q, k, v);
   a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   a.lse = const_cast<float*>(lse);

@@ -9,9 +9,9 @@ namespace bf {
 bool packed_is_short(const bf_packed_attn* p);
 
 // bf_packed_attn_fwd / _bwd of such a call; arguments checked by the caller.
-int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
+int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
                      hipStream_t st);
-int packed_short_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out, const void* rest,
-                     const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st);
+int packed_short_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                     const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t st);
 
 }  // namespace bf

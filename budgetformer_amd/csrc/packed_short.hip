@@ -4,13 +4,17 @@
 // slow besides. Here a row of one head is a group of LPR lanes with 16 bytes of the row each, which walks the few keys
 // that the row sees: dot products by shuffles within the group, the softmax's maximum and sum running in registers.
 // Neighbouring groups are a token's heads, so q, out and every k and v row are read in whole cache lines, and rows of
-// one sequence find its keys in the caches: what is left is one read and one write of each tensor. The backward
-// does rows (dQ) and keys (dK, dV) of one range in one launch, so that the second finds in the caches what the first
-// read; Delta of a row is formed again for each of its keys instead of making a round trip through memory, from out and,
-// in 16-bit types, what its rounding left (`rest`): Delta is a difference's second part.
+// one sequence find its keys in the caches: what is left is one read and one write of each tensor.
+//
+// The backward in float32 does rows (dQ) and keys (dK, dV) of one range in one launch, so that the second finds in the
+// caches what the first read; Delta of a row is formed again from out for each of its keys instead of making a round trip
+// through memory. In 16-bit types out is rounded, and Delta, the second part of a difference, would carry that rounding (dQ
+// of bfloat16 walks of 5 was off by up to 27 times what its own rounding allows). There the rows' launch forms it from
+// the scores, and the keys' launch reads it: fewer rows are read for each pair of row and key, four tensors are read
+// twice. One launch : two in us, forward and backward: 338,686 walks of 5, 8 heads of 16, bfloat16 1447 : 1400; 140,000
+// rows in sequences of 2 to 5, 8 of 64, float16 404 : 422; 100,000 rows of 5, float16, 32 of 16 over 8 378 : 339.
 // 338,686 walks of 5, 8 heads of 16, float32: forward 0.65 ms for 3.5 GB (5.4 TB/s), backward 1.65 ms for 6.9 GB (4.2
-// TB/s); in tiles both took 8.1 ms together. In bfloat16 both take 1.69 ms; from the rounded out alone 1.45, with dQ
-// off by up to 27 times what its own rounding allows.
+// TB/s); in tiles both took 8.1 ms together.
 #include "packed_short.h"
 
 #include "packed_tile.h"
@@ -20,8 +24,8 @@ namespace {
 
 struct ShortArgs {
   const void *q, *k, *v, *out, *dout;
-  void *o, *rest, *dq, *dk, *dv;                   // rest: what the rounding of out left, or NULL
-  float* lse;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta;
   const int2 *row_span, *key_span;
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;
   int32_t n_rows, n_keys;          // (token, head) pairs of the queries, of the keys
@@ -61,14 +65,6 @@ template <typename T> struct Chunk {               // a lane's 16 bytes of a row
     for (int j = 0; j < kN; ++j) v[j] = T(x[j] * by);
     *reinterpret_cast<V*>(p) = v;
   }
-  // what store's rounding leaves
-  __device__ __forceinline__ void store_rest(T* p, float by) const {
-    typedef T V __attribute__((ext_vector_type(kN)));
-    V v;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) v[j] = T(x[j] * by - float(T(x[j] * by)));
-    *reinterpret_cast<V*>(p) = v;
-  }
 };
 
 template <int LPR> __device__ __forceinline__ float row_sum(float x) {
@@ -76,8 +72,6 @@ template <int LPR> __device__ __forceinline__ float row_sum(float x) {
   for (int o = 1; o < LPR; o <<= 1) x += __shfl_xor(x, o, 64);
   return x;
 }
-
-template <typename T> constexpr bool kRest = sizeof(T) == 2;       // float32's out is not rounded again
 
 constexpr int kShortThreads = 256;
 constexpr int kAhead = 4;          // keys whose loads are on their way together
@@ -132,12 +126,11 @@ __global__ __launch_bounds__(kShortThreads) void short_fwd(const ShortArgs a) {
       if (j + u < hi) acc.add(p, v);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (mine) acc.store(static_cast<T*>(a.o) + item * a.dim + at, inv);
-  if (kRest<T> && a.rest && mine) acc.store_rest(static_cast<T*>(a.rest) + item * a.dim + at, inv);
+  if (mine) acc.store(static_cast<T*>(a.o) + item * a.dim + at, l == 0.f ? 0.f : 1.f / l);
   if (part == 0) a.lse[item] = l == 0.f ? -INFINITY : mc + __log2f(l);
 }
 
+// float32: dQ of rows, and dK and dV of keys, of one range.
 template <typename T, int LPR>
 __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
   using Ch = Chunk<T>;
@@ -148,19 +141,6 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
   const T* qp = static_cast<const T*>(a.q) + d;
   const T* gp = static_cast<const T*>(a.dout) + d;
   const T* op = static_cast<const T*>(a.out) + d;
-  const T* rp = kRest<T> && a.rest ? static_cast<const T*>(a.rest) + d : nullptr;
-  const auto mean = [&](const Ch& g, const Ch& o, const uint4& rest) {       // the lane's part of Delta
-    float s = g.dot(o);
-    if constexpr (kRest<T>) {
-      if (rp) {
-        Ch r;
-        r.set(rest);
-        if (!mine) r.zero();
-        s += g.dot(r);
-      }
-    }
-    return s;
-  };
   if (item < a.n_rows) {                             // dQ of a row
     const int token = int(a.by_hq(uint32_t(item))), head = int(item) - token * a.hq, h = int(a.by_group(uint32_t(head)));
     const int2 span = a.row_span[token];
@@ -171,7 +151,7 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
     o.set(Ch::raw(op + item * a.dim));
     if (!mine) q.zero(), g.zero(), o.zero();
     acc.zero();
-    const float delta = row_sum<LPR>(mean(g, o, rp ? Ch::raw(rp + item * a.dim) : make_uint4(0u, 0u, 0u, 0u))), stat = a.lse[item], lse = stat == -INFINITY ? INFINITY : stat;
+    const float delta = row_sum<LPR>(g.dot(o)), stat = a.lse[item], lse = stat == -INFINITY ? INFINITY : stat;
     const T* kp = static_cast<const T*>(a.k) + h * a.ks_h + d;
     const T* vp = static_cast<const T*>(a.v) + h * a.vs_h + d;
     for (int j = lo; j < hi; j += kAhead) {
@@ -207,7 +187,7 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
     constexpr int U = 2;
     for (int head = h * a.group; head < (h + 1) * a.group; ++head) {
       for (int i = lo; i < hi; i += U) {
-        uint4 qr[U], gr[U], orr[U], rr[U];
+        uint4 qr[U], gr[U], orr[U];
         float stat[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -216,7 +196,6 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
           qr[u] = Ch::raw(qp + row * a.qs_t + head * a.qs_h);
           gr[u] = Ch::raw(gp + r * a.dim);
           orr[u] = Ch::raw(op + r * a.dim);
-          if (rp) rr[u] = Ch::raw(rp + r * a.dim);
           stat[u] = a.lse[r];
         }
 #pragma unroll
@@ -224,7 +203,7 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
           Ch q, g, o;
           q.set(qr[u]), g.set(gr[u]), o.set(orr[u]);
           if (!mine) q.zero(), g.zero(), o.zero();
-          const float s = row_sum<LPR>(q.dot(k)), dp = row_sum<LPR>(g.dot(v)), delta = row_sum<LPR>(mean(g, o, rr[u]));
+          const float s = row_sum<LPR>(q.dot(k)), dp = row_sum<LPR>(g.dot(v)), delta = row_sum<LPR>(g.dot(o));
           const float p = exp2_fast(fmaf(s, a.c, stat[u] == -INFINITY ? -INFINITY : -stat[u]));
           if (i + u < hi) {
             dv.add(p, g);
@@ -237,6 +216,110 @@ __global__ __launch_bounds__(kShortThreads) void short_bwd(const ShortArgs a) {
       dk.store(static_cast<T*>(a.dk) + item * a.dim + at, a.scale);
       dv.store(static_cast<T*>(a.dv) + item * a.dim + at, 1.f);
     }
+  }
+}
+
+// 16-bit types: dQ and Delta of a row in one walk of its keys, without the rounded out. With Delta = sum P dP,
+// sum P (dP - Delta) k is sum P dP' k - (sum P dP') (sum P k); dP' is relative to the first key's dP, so that nothing
+// large cancels where the values have a part in common (and a row of one key has dQ = 0).
+template <typename T, int LPR>
+__global__ __launch_bounds__(kShortThreads) void short_bwd_rows(const ShortArgs a) {
+  using Ch = Chunk<T>;
+  const int part = threadIdx.x % LPR, at = part * Ch::kN;
+  const int64_t item = int64_t(blockIdx.x) * (kShortThreads / LPR) + threadIdx.x / LPR;
+  if (item >= a.n_rows) return;
+  const bool mine = at < a.dim;
+  const int d = mine ? at : 0;
+  const int token = int(a.by_hq(uint32_t(item))), head = int(item) - token * a.hq, h = int(a.by_group(uint32_t(head)));
+  const int2 span = a.row_span[token];
+  const int lo = max(span.x, 0), hi = min(span.y, a.n_k);
+  Ch q, g, pdk, pk;
+  q.set(Ch::raw(static_cast<const T*>(a.q) + token * a.qs_t + head * a.qs_h + d));
+  g.set(Ch::raw(static_cast<const T*>(a.dout) + item * a.dim + d));
+  if (!mine) q.zero(), g.zero();
+  pdk.zero(), pk.zero();
+  const float stat = a.lse[item], lse = stat == -INFINITY ? INFINITY : stat;
+  const T* kp = static_cast<const T*>(a.k) + h * a.ks_h + d;
+  const T* vp = static_cast<const T*>(a.v) + h * a.vs_h + d;
+  float first = 0.f, mean = 0.f;
+  for (int j = lo; j < hi; j += kAhead) {
+    uint4 kr[kAhead], vr[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t key = min(j + u, hi - 1);
+      kr[u] = Ch::raw(kp + key * a.ks_t);
+      vr[u] = Ch::raw(vp + key * a.vs_t);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      Ch k, v;
+      k.set(kr[u]);
+      v.set(vr[u]);
+      if (!mine) k.zero(), v.zero();
+      const float s = row_sum<LPR>(q.dot(k)), dp = row_sum<LPR>(g.dot(v));
+      if (u == 0 && j == lo) first = dp;
+      const float p = exp2_fast(fmaf(s, a.c, -lse)), pd = p * (dp - first);
+      if (j + u < hi) {
+        mean += pd;
+        pdk.add(pd, k);
+        pk.add(p, k);
+      }
+    }
+  }
+  pdk.add(-mean, pk);
+  if (mine) pdk.store(static_cast<T*>(a.dq) + item * a.dim + at, a.scale);
+  if (part == 0) a.delta[item] = first + mean;
+}
+
+// dK and dV of a key, over its rows and their heads of the group, with the rows' Delta from memory.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kShortThreads) void short_bwd_keys(const ShortArgs a) {
+  using Ch = Chunk<T>;
+  const int part = threadIdx.x % LPR, at = part * Ch::kN;
+  const int64_t item = int64_t(blockIdx.x) * (kShortThreads / LPR) + threadIdx.x / LPR;
+  if (item >= a.n_keys) return;
+  const bool mine = at < a.dim;
+  const int d = mine ? at : 0;
+  const T* qp = static_cast<const T*>(a.q) + d;
+  const T* gp = static_cast<const T*>(a.dout) + d;
+  const int key = int(a.by_hk(uint32_t(item))), h = int(item) - key * a.hk;
+  const int2 span = a.key_span[key];
+  const int lo = max(span.x, 0), hi = min(span.y, a.n_q);
+  Ch k, v, dk, dv;
+  k.set(Ch::raw(static_cast<const T*>(a.k) + key * a.ks_t + h * a.ks_h + d));
+  v.set(Ch::raw(static_cast<const T*>(a.v) + key * a.vs_t + h * a.vs_h + d));
+  if (!mine) k.zero(), v.zero();
+  dk.zero(), dv.zero();
+  constexpr int U = 4;
+  for (int head = h * a.group; head < (h + 1) * a.group; ++head) {
+    for (int i = lo; i < hi; i += U) {
+      uint4 qr[U], gr[U];
+      float stat[U], delta[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = min(i + u, hi - 1);
+        const int64_t r = int64_t(row) * a.hq + head;
+        qr[u] = Ch::raw(qp + row * a.qs_t + head * a.qs_h);
+        gr[u] = Ch::raw(gp + r * a.dim);
+        stat[u] = a.lse[r], delta[u] = a.delta[r];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        Ch q, g;
+        q.set(qr[u]), g.set(gr[u]);
+        if (!mine) q.zero(), g.zero();
+        const float s = row_sum<LPR>(q.dot(k)), dp = row_sum<LPR>(g.dot(v));
+        const float p = exp2_fast(fmaf(s, a.c, stat[u] == -INFINITY ? -INFINITY : -stat[u]));
+        if (i + u < hi) {
+          dv.add(p, g);
+          dk.add(p * (dp - delta[u]), q);
+        }
+      }
+    }
+  }
+  if (mine) {
+    dk.store(static_cast<T*>(a.dk) + item * a.dim + at, a.scale);
+    dv.store(static_cast<T*>(a.dv) + item * a.dim + at, 1.f);
   }
 }
 
@@ -276,16 +359,16 @@ template <typename F> int with_lanes(const bf_packed_attn* p, F&& f) {
 // A row costs a key's lanes for every key it sees here, and its share of whole tiles otherwise. Forward and backward of
 // 25,000 to 1.6 million rows took, as lanes : tiles in us, causal and not,
 //   float32, heads of 16:  8 keys 299..345 : 743, 16 keys 426..544 : 745, 24 keys 499..727 : 949..1036, 32 keys 692..906 : 698..744
-//   bfloat16, heads of 16: 8 keys 169..194 : 465, 16 keys 226..299 : 465, 24 keys 286..403 : 500..523, 32 keys 359..512 : 465
-//   bfloat16, heads of 64: 4 keys 138..146 : 227, 8 keys 178..217 : 229, 16 keys 270..367 : 233
-//   bfloat16, heads of 128: 4 keys 200..265 : 254, 8 keys 318..473 : 253
+//   bfloat16, heads of 16: 8 keys 170..188 : 488, 16 keys 220..276 : 491, 24 keys 281..372 : 492, 32 keys 359..512 : 465
+//   bfloat16, heads of 64: 4 keys 141..144 : 268, 8 keys 194..209 : 270, 16 keys 270..367 : 233
+//   bfloat16, heads of 128: 4 keys 203..249 : 308, 8 keys 318..473 : 253
 //   float32, heads of 64:  4 keys 285..329 : 665, 8 keys 403..509 : 669, 16 keys 663..916 : 668
 // Heads that share keys fill a tile with fewer tokens, which masks less of it (100,000 rows, 5, 12 and 24 tokens):
-//   float16, 32 heads of 16 over 8: 392, 524, 880 : 442, 441, 447; bfloat16, 32 of 32 over 4: 642, 906, 1562 : 559, 560, 573
+//   float16, 32 heads of 16 over 8: 343, 524, 880 : 461, 441, 447; bfloat16, 32 of 32 over 4: 642, 906, 1562 : 559, 560, 573
 //   float32, 16 heads of 16 over 1: 271, 365, 601 : 399, 413, 462; 16 of 64 over 2: 1123, 1657, 2899 : 1284, 1296, 1359
 // A call of few rows leaves most of the chip idle either way and is as long as its longest chain, for lanes the rows of a
-// key's group (2000 rows, 12 and 24 tokens; float16, 8 heads of 128 over 4: 39, 60 : 78, 80; bfloat16, 16 of 64 over 8: 37, 56 : 37, 37):
-//   bfloat16, 8 of 64: 27, 38 : 45, 45; float32, 8 of 128: 87, 103 : 123, 123
+// key's group (2000 rows, 12 and 24 tokens; float16, 8 heads of 128 over 4: 39, 60 : 78, 80; bfloat16, 16 of 64 over 8: 38, 56 : 36, 37):
+//   bfloat16, 8 of 64: 27, 41 : 44, 46; float32, 8 of 128: 87, 103 : 123, 123
 bool packed_is_short(const bf_packed_attn* p) {
   const bool wide = p->dtype == BF_DTYPE_F32;
   const int64_t row = int64_t(p->head_dim) * (wide ? 4 : 2), group = p->heads_q / p->heads_k;
@@ -295,10 +378,10 @@ bool packed_is_short(const bf_packed_attn* p) {
   return few || p->longest * row <= most;
 }
 
-int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
+int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, float* lse,
                      hipStream_t st) {
   ShortArgs a = make_args(p, q, k, v);
-  a.o = out, a.rest = rest, a.lse = lse;
+  a.o = out, a.lse = lse;
   return with_lanes(p, [&](auto t, auto lanes) -> int {
     using T = decltype(t);
     constexpr int LPR = decltype(lanes)::value;
@@ -310,19 +393,33 @@ int packed_short_fwd(const bf_packed_attn* p, const void* q, const void* k, cons
   });
 }
 
-int packed_short_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out, const void* rest,
-                     const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
+int packed_short_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                     const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t st) {
   ShortArgs a = make_args(p, q, k, v);
-  a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
-  a.lse = const_cast<float*>(lse);
-  const int64_t most = a.n_rows > a.n_keys ? a.n_rows : a.n_keys;
-  if (most == 0) return BF_OK;
+  a.out = out, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.lse = const_cast<float*>(lse), a.delta = delta;
   return with_lanes(p, [&](auto t, auto lanes) -> int {
     using T = decltype(t);
     constexpr int LPR = decltype(lanes)::value;
-    auto kern = short_bwd<T, LPR>;
-    BF_LAUNCH("packed_attn_bwd_short", kern, dim3(unsigned(ceil_div(most, kShortThreads / LPR))), dim3(kShortThreads), 0, st, a);
-    BF_CHECK_LAUNCH();
+    const dim3 block(kShortThreads);
+    if constexpr (sizeof(T) == 2) {
+      if (a.n_rows > 0) {
+        auto rows = short_bwd_rows<T, LPR>;
+        BF_LAUNCH("packed_attn_bwd_short_rows", rows, dim3(unsigned(ceil_div(a.n_rows, kShortThreads / LPR))), block, 0, st, a);
+        BF_CHECK_LAUNCH();
+      }
+      if (a.n_keys > 0) {
+        auto keys = short_bwd_keys<T, LPR>;
+        BF_LAUNCH("packed_attn_bwd_short_keys", keys, dim3(unsigned(ceil_div(a.n_keys, kShortThreads / LPR))), block, 0, st, a);
+        BF_CHECK_LAUNCH();
+      }
+    } else {
+      const int64_t most = a.n_rows > a.n_keys ? a.n_rows : a.n_keys;
+      if (most == 0) return BF_OK;
+      auto kern = short_bwd<T, LPR>;
+      BF_LAUNCH("packed_attn_bwd_short", kern, dim3(unsigned(ceil_div(most, kShortThreads / LPR))), block, 0, st, a);
+      BF_CHECK_LAUNCH();
+    }
     return BF_OK;
   });
 }

@@ -824,9 +824,10 @@ typedef struct bf_packed_attn {
  * arguments), for calls of few rows, whose keys are cut into pieces, and of sequences of very
  * different lengths, whose tiles are put in order. rest (or NULL): like out,
  * what out's rounding left, for the backward; bf_packed_attn_rest(p) says
- * whether the backward reads it (in 16-bit types). In float16 P and, in the
- * backward, dS are operands in units of a power of 2: neither small nor large
- * ones leave the type's range where the results fit it.                     */
+ * whether the backward reads it (in 16-bit types, where the sequences are not
+ * short). In float16 P and, in the backward, dS are operands in units of a
+ * power of 2: neither small nor large ones leave the type's range where the
+ * results fit it.                                                           */
 int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p);
 int bf_packed_attn_rest(const bf_packed_attn* p);
 int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,

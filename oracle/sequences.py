@@ -34,7 +34,7 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
     """q [n_q, H, d], k, v [n_k, Hk, d] float64 packed. Returns a dict: out, lse (natural log) and with dout dq, dk, dv;
     with dtype also each one's bound (``out_bound``, ...). Rows that see no key: out 0, lse -inf. operand_tiny: half a step
     of a subnormal P or dS, where that is finer than the type's own. rounds: whether P and dS are operands of the type and
-    Delta comes from the rounded out (False: neither; Delta from out and its rounding's rest, rounded itself)."""
+    Delta comes from the rounded out (False: neither; Delta as good as from out and its rounding's rest, rounded itself)."""
     H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
     g = H // Hk
     names = ["out"] + (["dq", "dk", "dv"] if dout is not None else [])
