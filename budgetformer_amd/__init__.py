@@ -2,7 +2,8 @@
 
   * budgeted query-centric edge construction (``edges.build_attention_edges``)
   * sparse edge attention forward/backward (``attention``)
-  * operators over packed sequences (``sequences``): dense attention, rotary positions, linear attention
+  * operators over packed sequences (``sequences``): dense attention, rotary positions, linear attention,
+    the gated delta rule
 
 All run as hand-written HIP kernels behind the C ABI in
 ``include/budgetformer_hip.h`` (library ``_lib/libbudgetformer_hip.so``, built
@@ -15,13 +16,13 @@ from .attention import (CoreAttention, ExphormerCoreAttention, GPSCoreAttention,
 from .edges import EdgeTable, build_attention_edges
 from .graph import CSRGraph
 from .hip_ops import AttentionIndex
-from .sequences import (PackedSequences, RotaryFrequencies, linear_attention, linear_attention_step, packed_attention,
-                        rotary_embedding)
+from .sequences import (PackedSequences, RotaryFrequencies, gated_delta_rule, gated_delta_step, linear_attention,
+                        linear_attention_step, packed_attention, rotary_embedding)
 
 __all__ = [
     "AttentionIndex", "CSRGraph", "CoreAttention", "EdgeTable", "ExphormerCoreAttention", "GPSCoreAttention",
     "GTCoreAttention", "PackedSequences", "RotaryFrequencies",
-    "build_attention_edges", "linear_attention", "linear_attention_step", "packed_attention", "rotary_embedding",
+    "build_attention_edges", "gated_delta_rule", "gated_delta_step", "linear_attention", "linear_attention_step", "packed_attention", "rotary_embedding",
     "sparse_edge_attention",
 ]
 

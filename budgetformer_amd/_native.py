@@ -67,6 +67,15 @@ class LinearAttn(C.Structure):
     ]
 
 
+class GatedDelta(C.Structure):
+    """Mirror of ``struct bf_gated_delta``."""
+    _fields_ = [
+        ("n", i64), ("n_seq", i64), ("heads", i32), ("heads_k", i32), ("dim_k", i32), ("dim_v", i32), ("dtype", i32),
+        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("offsets", vp), ("log_gate", vp), ("beta", vp),
+        ("init", vp), ("final_state", vp), ("scale", f32), ("longest", i32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "bf_version": (C.c_int, []),
@@ -177,6 +186,12 @@ _SIGS = {
     "bf_linear_attn_bwd_floats": (i64, [C.POINTER(LinearAttn)]),
     "bf_linear_attn_bwd": (C.c_int, [C.POINTER(LinearAttn), vp, vp, vp, vp, vp, vp, vp, P_f32, vp]),
     "bf_linear_attn_step": (C.c_int, [vp, vp, vp, P_f32, P_f32, i64, i32, i32, i32, i32, f32, vp, P_f32, vp]),
+    "bf_gated_delta_kept_floats": (i64, [C.POINTER(GatedDelta)]),
+    "bf_gated_delta_fwd_floats": (i64, [C.POINTER(GatedDelta), i32]),
+    "bf_gated_delta_fwd": (C.c_int, [C.POINTER(GatedDelta), vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_gated_delta_bwd_floats": (i64, [C.POINTER(GatedDelta)]),
+    "bf_gated_delta_bwd": (C.c_int, [C.POINTER(GatedDelta), vp, vp, vp, vp, P_f32, vp, vp, vp, P_f32, P_f32, P_f32, vp]),
+    "bf_gated_delta_step": (C.c_int, [C.POINTER(GatedDelta), vp, vp, vp, vp, vp]),
 }
 
 _lib = None

@@ -1,0 +1,189 @@
+// The gated delta rule over packed sequences: checks, how a call is cut, workspaces (the kernels: gated_delta.h).
+#include "gated_delta.h"
+
+namespace bf {
+namespace {
+
+int check(const bf_gated_delta* p, const char* fn, bool step) {
+  BF_CHECK_ARG(p != nullptr, "%s: no arguments", fn);
+  BF_CHECK_ARG(p->dtype == BF_DTYPE_F32 || p->dtype == BF_DTYPE_BF16 || p->dtype == BF_DTYPE_F16, "%s: dtype %d", fn,
+               p->dtype);
+  for (int d : {p->dim_k, p->dim_v})
+    if (d < 8 || d > 128 || d % 8) {
+      set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_k, p->dim_v);
+      return BF_ERR_UNSUPPORTED;
+    }
+  BF_CHECK_ARG(p->heads >= 1 && p->heads <= (1 << 20) && p->heads_k >= 1 && p->heads % p->heads_k == 0,
+               "%s: %d value heads over %d key heads (a multiple expected, up to 2^20)", fn, p->heads, p->heads_k);
+  BF_CHECK_ARG(p->n >= 0 && p->n < kMaxRows && p->n_seq >= 0 && p->n_seq < kMaxRows, "%s: bad sizes (%lld rows, %lld sequences)", fn,
+               (long long)p->n, (long long)p->n_seq);
+  BF_CHECK_ARG(p->scale == p->scale && p->scale <= 3e38f && p->scale >= -3e38f, "%s: scale %g", fn, double(p->scale));
+  BF_CHECK_ARG(p->longest >= 0, "%s: longest sequence %d", fn, p->longest);
+  BF_CHECK_ARG(p->n == 0 || (p->log_gate && p->beta), "%s: no gates or strengths", fn);
+  BF_CHECK_ARG(aligned16({p->init, p->final_state}), "%s: states must be 16-byte aligned", fn);
+  const int64_t per16 = step ? 1 : p->dtype == BF_DTYPE_F32 ? 4 : 8;
+  for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
+    BF_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[0] % per16 == 0 && s[1] % per16 == 0,
+                 "%s: strides (%lld, %lld) are not whole 16-byte steps", fn, (long long)s[0], (long long)s[1]);
+  if (step) {
+    BF_CHECK_ARG(p->n < (int64_t(1) << 24) / p->heads, "%s: %lld sequences of %d heads", fn, (long long)p->n, p->heads);
+  } else {
+    BF_CHECK_ARG(p->offsets != nullptr, "%s: no offsets", fn);
+  }
+  return BF_OK;
+}
+
+// Chunks of a segment: so many that some 512 workgroups share a call, at least 4 (a segment's own contribution and its
+// map are as much work as its tokens) and at most 64.
+int seg_chunks(const bf_gated_delta* p) {
+  const int64_t n = ceil_div(p->n * p->heads, int64_t(512) * kDeltaChunk);
+  return int(n < 4 ? 4 : n > 64 ? 64 : n);
+}
+
+bool carries(const bf_gated_delta* p) {
+  const int64_t seg = int64_t(seg_chunks(p)) * kDeltaChunk;
+  return p->n > seg && !(p->longest > 0 && p->longest <= seg);
+}
+
+// A call's workspaces, in floats: what the backward reads (kept), what only the forward needs, what only the backward does.
+struct Sizes {
+  int64_t chunks, segs;            // places
+  int64_t rows, frags, map, state;
+  explicit Sizes(const bf_gated_delta* p) {
+    const int64_t seg = int64_t(seg_chunks(p)) * kDeltaChunk, d = delta_pad(p->dim_k, p->dim_v), parts = delta_mid_parts(p->dtype);
+    chunks = p->n / kDeltaChunk + p->n_seq + 1;
+    segs = p->n / seg + p->n_seq + 1;
+    rows = ceil_div(p->n * p->heads, int64_t(4)) * 4;
+    frags = chunks * p->heads * (2 * parts * 64 * 4);
+    map = carries(p) ? segs * p->heads * (parts * d * d / 2) : 0;
+    state = carries(p) ? segs * p->heads * int64_t(p->dim_k) * p->dim_v : 0;
+  }
+};
+
+int64_t kept_floats(const bf_gated_delta* p) {
+  const Sizes s(p);
+  return 3 * s.rows + 2 * s.frags + s.map + s.state + p->n * p->heads * p->dim_v;
+}
+
+int64_t fwd_floats(const bf_gated_delta* p, bool train) {
+  const Sizes s(p);
+  return 2 * s.frags + s.map + (train ? 0 : 3 * s.rows + s.state);
+}
+
+int64_t bwd_floats(const bf_gated_delta* p) {
+  const Sizes s(p);
+  const int64_t keys = p->n * p->heads * p->dim_k;
+  return s.state + p->n * p->heads * p->dim_v + keys * (p->heads > p->heads_k ? 2 : 1);
+}
+
+DeltaArgs make_args(const bf_gated_delta* p, const void* q, const void* k, const void* v) {
+  const Sizes s(p);
+  DeltaArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.qs_t = p->q_stride[0], a.qs_h = p->q_stride[1];
+  a.ks_t = p->k_stride[0], a.ks_h = p->k_stride[1];
+  a.vs_t = p->v_stride[0], a.vs_h = p->v_stride[1];
+  a.log_gate = p->log_gate, a.beta = p->beta, a.offsets = p->offsets;
+  a.init = p->init, a.final_state = p->final_state;
+  a.n = int32_t(p->n), a.n_seq = int32_t(p->n_seq), a.heads = p->heads, a.heads_k = p->heads_k, a.group = p->heads / p->heads_k;
+  a.dim_k = p->dim_k, a.dim_v = p->dim_v;
+  a.seg_chunks = seg_chunks(p), a.n_chunk = s.chunks, a.n_seg = s.segs;
+  a.scale = p->scale;
+  a.carried = carries(p);
+  return a;
+}
+
+void take_kept(DeltaArgs& a, const bf_gated_delta* p, float* f) {
+  const Sizes s(p);
+  a.inv_t = reinterpret_cast<uint4*>(f), f += s.frags;
+  a.score_t = reinterpret_cast<uint4*>(f), f += s.frags;
+  a.map_b = s.map ? reinterpret_cast<uint4*>(f) : nullptr, f += s.map;
+  a.state = f, f += s.state;
+  a.g2 = f, f += s.rows;
+  a.gin = f, f += s.rows;
+  a.gout = f, f += s.rows;
+  a.e = f;
+}
+
+template <typename F> int with_launch(int32_t dtype, F&& f) {
+  return with_type(dtype, [&](auto t) -> int { return f(DeltaLaunch<decltype(t)>()); });
+}
+
+}  // namespace
+}  // namespace bf
+
+using namespace bf;
+
+extern "C" int64_t bf_gated_delta_kept_floats(const bf_gated_delta* p) {
+  return check(p, "gated_delta_kept_floats", false) == BF_OK ? kept_floats(p) : -1;
+}
+
+extern "C" int64_t bf_gated_delta_fwd_floats(const bf_gated_delta* p, int32_t train) {
+  return check(p, "gated_delta_fwd_floats", false) == BF_OK ? fwd_floats(p, train != 0) : -1;
+}
+
+extern "C" int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, void* out, float* kept,
+                                  float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "gated_delta_fwd", false));
+  BF_CHECK_ARG(p->n == 0 || (q && k && v && out), "gated_delta_fwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out, kept, scratch}), "gated_delta_fwd: tensors and workspaces must be 16-byte aligned");
+  if (p->n == 0 && !(p->final_state && p->n_seq > 0)) return BF_OK;
+  BF_CHECK_ARG(scratch != nullptr, "gated_delta_fwd: no scratch (bf_gated_delta_fwd_floats)");
+  DeltaArgs a = make_args(p, q, k, v);
+  const Sizes s(p);
+  a.out = out;
+  float* f = scratch;
+  a.inv = reinterpret_cast<uint4*>(f), f += s.frags;
+  a.score = reinterpret_cast<uint4*>(f), f += s.frags;
+  a.map_f = reinterpret_cast<__bf16*>(f), f += s.map;
+  if (kept) {
+    take_kept(a, p, kept);
+  } else {
+    a.state = f, f += s.state;
+    a.g2 = f, f += s.rows;
+    a.gin = f, f += s.rows;
+    a.gout = f;
+  }
+  const hipStream_t st = as_stream(stream);
+  return with_launch(p->dtype, [&](auto l) -> int {
+    if (a.n > 0) BF_CHECK_OK(l.prep(a, st));
+    return l.forward(a, st);
+  });
+}
+
+extern "C" int64_t bf_gated_delta_bwd_floats(const bf_gated_delta* p) {
+  return check(p, "gated_delta_bwd_floats", false) == BF_OK ? bwd_floats(p) : -1;
+}
+
+extern "C" int bf_gated_delta_bwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, const void* dout,
+                                  const float* kept, void* dq, void* dk, void* dv, float* dgate, float* dbeta, float* scratch,
+                                  void* stream) {
+  BF_CHECK_OK(check(p, "gated_delta_bwd", false));
+  if (p->n == 0) return BF_OK;
+  BF_CHECK_ARG(q && k && v && dout && kept && dq && dk && dv && dgate && dbeta && scratch, "gated_delta_bwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, dout, kept, dq, dk, dv, scratch}), "gated_delta_bwd: tensors and workspaces must be 16-byte aligned");
+  DeltaArgs a = make_args(p, q, k, v);
+  take_kept(a, p, const_cast<float*>(kept));
+  a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.dgate = dgate, a.dbeta = dbeta;
+  float* f = scratch;
+  a.dstate = f, f += Sizes(p).state;
+  a.z = f, f += p->n * p->heads * p->dim_v;
+  a.dk32 = f, f += p->n * p->heads * p->dim_k;
+  a.dq32 = a.group > 1 ? f : nullptr;
+  return with_launch(p->dtype, [&](auto l) -> int { return l.backward(a, as_stream(stream)); });
+}
+
+extern "C" int bf_gated_delta_step(const bf_gated_delta* p, const void* q, const void* k, const void* v, void* out, void* stream) {
+  BF_CHECK_OK(check(p, "gated_delta_step", true));
+  if (p->n == 0) return BF_OK;
+  BF_CHECK_ARG(q && k && v && out && p->init && p->final_state, "gated_delta_step: bad arguments");
+  DeltaArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.qs_t = p->q_stride[0], a.qs_h = p->q_stride[1];
+  a.ks_t = p->k_stride[0], a.ks_h = p->k_stride[1];
+  a.vs_t = p->v_stride[0], a.vs_h = p->v_stride[1];
+  a.log_gate = p->log_gate, a.beta = p->beta, a.init = p->init, a.final_state = p->final_state;
+  a.heads = p->heads, a.group = p->heads / p->heads_k, a.dim_k = p->dim_k, a.dim_v = p->dim_v;
+  a.scale = p->scale, a.out = out;
+  return with_launch(p->dtype, [&](auto l) -> int { return l.step(a, p->n, as_stream(stream)); });
+}

@@ -814,6 +814,145 @@ std::tuple<at::Tensor, at::Tensor> linear_attn_step(const at::Tensor& q, const a
   return {out, next};
 }
 
+// The gated delta rule's arguments: q, k [n, heads_k, dim_k], v [n, heads, dim_v], log_gate and beta [n, heads].
+bf_gated_delta delta_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_gate,
+                          const at::Tensor& beta, double scale) {
+  const at::Device dev = q.device();
+  bf_gated_delta p{};
+  p.dtype = dtype_code(q);
+  require_heads(q, "q", q.scalar_type(), dev, p.q_stride);
+  require_heads(k, "k", q.scalar_type(), dev, p.k_stride);
+  require_heads(v, "v", q.scalar_type(), dev, p.v_stride);
+  TORCH_CHECK_VALUE(q.sizes() == k.sizes() && v.size(0) == q.size(0), "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), " disagree");
+  TORCH_CHECK_VALUE(q.size(1) < (int64_t(1) << 30) && v.size(1) < (int64_t(1) << 30) && q.size(2) < (int64_t(1) << 30) &&
+                        v.size(2) < (int64_t(1) << 30), "gated_delta: bad sizes");
+  for (const at::Tensor* t : {&log_gate, &beta}) {
+    require(*t, t == &beta ? "beta" : "log_gate", at::kFloat, dev);
+    TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == v.size(0) && t->size(1) == v.size(1), t == &beta ? "beta" : "log_gate", " must be [",
+                      v.size(0), ", ", v.size(1), "] (got ", t->sizes(), ")");
+  }
+  p.n = q.size(0), p.heads_k = int32_t(q.size(1)), p.heads = int32_t(v.size(1)), p.dim_k = int32_t(q.size(2)), p.dim_v = int32_t(v.size(2));
+  p.log_gate = log_gate.data_ptr<float>(), p.beta = beta.data_ptr<float>();
+  p.scale = float(scale);
+  return p;
+}
+
+void delta_sequences(bf_gated_delta& p, const at::Tensor& offsets, int64_t longest, const std::optional<at::Tensor>& init_state,
+                     const at::Device& dev) {
+  require(offsets, "offsets", at::kInt, dev);
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must be [n_seq + 1]");
+  p.offsets = offsets.data_ptr<int32_t>(), p.n_seq = offsets.numel() - 1;
+  p.longest = int32_t(std::min<int64_t>(std::max<int64_t>(longest, 0), INT32_MAX));
+  if (init_state.has_value() && init_state->defined()) {
+    require(*init_state, "init_state", at::kFloat, dev);
+    TORCH_CHECK_VALUE(init_state->sizes() == at::IntArrayRef({p.n_seq, p.heads, p.dim_k, p.dim_v}), "init_state must be [", p.n_seq, ", ",
+                      p.heads, ", ", p.dim_k, ", ", p.dim_v, "] (got ", init_state->sizes(), ")");
+    p.init = init_state->data_ptr<float>();
+  }
+}
+
+// Forward (bf_gated_delta_fwd): (out, final state or empty without return_state, kept or empty without train).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_delta_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                                               const at::Tensor& log_gate, const at::Tensor& beta,
+                                                               const at::Tensor& offsets, double scale, int64_t longest,
+                                                               const std::optional<at::Tensor>& init_in, bool return_state,
+                                                               bool train) {
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
+  std::optional<at::Tensor> init;
+  if (init_in.has_value() && init_in->defined()) init = as_dense(*init_in);
+  bf_gated_delta p = delta_args(q, k, v, log_gate, beta, scale);
+  delta_sequences(p, offsets, longest, init, q.device());
+  at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), scratch;
+  at::Tensor state = return_state ? at::empty({p.n_seq, p.heads, p.dim_k, p.dim_v}, log_gate.options()) : at::empty({0}, log_gate.options());
+  if (return_state) p.final_state = state.data_ptr<float>();
+  const int64_t floats = bf_gated_delta_fwd_floats(&p, train ? 1 : 0), keeps = train ? bf_gated_delta_kept_floats(&p) : 0;
+  at::Tensor kept = at::empty({std::max<int64_t>(keeps, 0)}, log_gate.options());
+  if (floats > 0) scratch = at::empty({floats}, log_gate.options());
+  check_rc(bf_gated_delta_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), keeps > 0 ? kept.data_ptr<float>() : nullptr,
+                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
+           "bf::gated_delta_fwd");
+  return {out, state, kept};
+}
+
+// Backward (bf_gated_delta_bwd): (dq, dk, dv, dlog_gate, dbeta), contiguous.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_delta_bwd(
+    const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& log_gate, const at::Tensor& beta,
+    const at::Tensor& offsets, const at::Tensor& kept, const at::Tensor& dout_in, double scale, int64_t longest,
+    const std::optional<at::Tensor>& init_in) {
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = as_rows(q_in, "q");
+  const at::Tensor k = as_rows(k_in, "k");
+  const at::Tensor v = as_rows(v_in, "v");
+  const at::Tensor dout = as_dense(dout_in);
+  std::optional<at::Tensor> init;
+  if (init_in.has_value() && init_in->defined()) init = as_dense(*init_in);
+  bf_gated_delta p = delta_args(q, k, v, log_gate, beta, scale);
+  delta_sequences(p, offsets, longest, init, q.device());
+  require(dout, "dout", q.scalar_type(), q.device());
+  TORCH_CHECK_VALUE(dout.sizes() == v.sizes(), "dout ", dout.sizes(), " does not match v ", v.sizes());
+  require(kept, "kept", at::kFloat, q.device());
+  TORCH_CHECK_VALUE(kept.numel() == bf_gated_delta_kept_floats(&p), "kept has ", kept.numel(), " values, expected ",
+                    bf_gated_delta_kept_floats(&p));
+  const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain), scratch;
+  at::Tensor dgate = at::empty_like(log_gate), dbeta = at::empty_like(beta);
+  const int64_t floats = bf_gated_delta_bwd_floats(&p);
+  if (floats > 0) scratch = at::empty({floats}, log_gate.options());
+  check_rc(bf_gated_delta_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), kept.data_ptr<float>(), dq.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), dgate.data_ptr<float>(), dbeta.data_ptr<float>(),
+                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
+           "bf::gated_delta_bwd");
+  return {dq, dk, dv, dgate, dbeta};
+}
+
+// Whether the memory between two tensors' first and last values meets (strides are not negative).
+bool ranges_meet(const at::Tensor& x, const at::Tensor& y) {
+  const auto range = [](const at::Tensor& t) {
+    uintptr_t values = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) values += uintptr_t(t.size(d) - 1) * uintptr_t(t.stride(d));
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::make_pair(from, from + values * t.element_size());
+  };
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  const auto a = range(x), b = range(y);
+  return a.first < b.second && b.first < a.second;
+}
+
+// One token of each sequence (bf_gated_delta_step): (out, new state); out_state as in linear_attn_step.
+std::tuple<at::Tensor, at::Tensor> gated_delta_step(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                                    const at::Tensor& log_gate, const at::Tensor& beta, const at::Tensor& state,
+                                                    double scale, const std::optional<at::Tensor>& out_state) {
+  TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
+  const at::Tensor into = out_state.value_or(at::Tensor());
+  refuse_tangents({&q_in, &k_in, &v_in, &log_gate, &beta, &state, &into}, "gated_delta_step");
+  const c10::DeviceGuard guard(q_in.device());
+  const auto along = [](const at::Tensor& t) { return t.dim() != 3 || t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous(); };
+  const at::Tensor q = along(q_in), k = along(k_in), v = along(v_in);
+  bf_gated_delta p = delta_args(q, k, v, log_gate, beta, scale);
+  const bool given = out_state.has_value() && out_state->defined();
+  for (const at::Tensor* s : {&state, given ? &*out_state : &state}) {
+    require(*s, s == &state ? "state" : "out_state", at::kFloat, q.device());
+    TORCH_CHECK_VALUE(s->sizes() == at::IntArrayRef({p.n, p.heads, p.dim_k, p.dim_v}), "a state must be [", p.n, ", ", p.heads, ", ", p.dim_k,
+                      ", ", p.dim_v, "] (got ", s->sizes(), ")");
+  }
+  at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), next = given ? *out_state : at::empty_like(state);
+  if (given) {
+    const auto apart = at::MemOverlapStatus::No, same = at::MemOverlapStatus::Full, states = at::get_overlap_status(next, state);
+    TORCH_CHECK_VALUE(p.n == 0 || states == apart || states == same, "out_state overlaps state and is not state itself");
+    for (const at::Tensor* t : {&q, &k, &v, &log_gate, &beta})
+      TORCH_CHECK_VALUE(!ranges_meet(next, *t), "out_state overlaps an input");
+    next.unsafeGetTensorImpl()->bump_version();          // a gradient that kept the old state is refused, not wrong
+  }
+  p.init = state.data_ptr<float>(), p.final_state = next.data_ptr<float>();
+  check_rc(bf_gated_delta_step(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stream_of(q)), "bf::gated_delta_step");
+  return {out, next};
+}
+
 // ---------------------------------------------------------------- gradients of the operators over packed sequences
 // Formed here and not in Python: a small call's time is its host work (forward and backward of 64 tokens: 48, 42 and 43 us
 // with Python functions, 41, 35 and 36 us so, for the three operators).
@@ -970,6 +1109,49 @@ std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor& q, const a
   return linear_attn_fwd(q, k, v, log_decay, row_span, key_span, offsets, scale, longest, init_state, return_state);
 }
 
+struct GatedDelta : torch::autograd::Function<GatedDelta> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& log_gate, const at::Tensor& beta, const at::Tensor& offsets, double scale,
+                               int64_t longest, const std::optional<at::Tensor>& init_state, bool return_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, state, kept] = gated_delta_fwd(q, k, v, log_gate, beta, offsets, scale, longest, init_state, return_state, true);
+    ctx->save_for_backward({q, k, v, log_gate, beta, offsets, kept, init_state.value_or(at::Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["longest"] = longest;
+    ctx->mark_non_differentiable({state});
+    ctx->set_materialize_grads(false);
+    return {out, state};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(10);
+    if (!grads[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1], out[2], out[3], out[4]) =
+          gated_delta_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], grads[0], ctx->saved_data["scale"].toDouble(),
+                          ctx->saved_data["longest"].toInt(), s[7].defined() ? std::optional<at::Tensor>(s[7]) : std::nullopt);
+    }
+    return once(std::move(out));
+  }
+};
+
+// gated_delta_fwd, with gradients for q, k, v, log_gate and beta.
+std::tuple<at::Tensor, at::Tensor> gated_delta_rule(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& log_gate, const at::Tensor& beta, const at::Tensor& offsets,
+                                                    double scale, int64_t longest, const std::optional<at::Tensor>& init_state,
+                                                    bool return_state) {
+  const at::Tensor init = init_state.value_or(at::Tensor());
+  refuse_tangents({&q, &k, &v, &log_gate, &beta, &init}, "gated_delta_rule");
+  if (trains({&q, &k, &v, &log_gate, &beta})) {
+    variable_list r = GatedDelta::apply(q, k, v, log_gate, beta, offsets, scale, longest, init_state, return_state);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [out, state, kept] = gated_delta_fwd(q, k, v, log_gate, beta, offsets, scale, longest, init_state, return_state, false);
+  return {out, state};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(bf, m) {
@@ -1014,6 +1196,14 @@ TORCH_LIBRARY(bf, m) {
         "-> (Tensor, Tensor)");
   m.def("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
         "float scale, int longest=0, Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
+  m.def("gated_delta_fwd(Tensor q, Tensor k, Tensor v, Tensor log_gate, Tensor beta, Tensor offsets, float scale, int longest=0, "
+        "Tensor? init_state=None, bool return_state=False, bool train=False) -> (Tensor, Tensor, Tensor)");
+  m.def("gated_delta_bwd(Tensor q, Tensor k, Tensor v, Tensor log_gate, Tensor beta, Tensor offsets, Tensor kept, Tensor dout, "
+        "float scale, int longest=0, Tensor? init_state=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("gated_delta_rule(Tensor q, Tensor k, Tensor v, Tensor log_gate, Tensor beta, Tensor offsets, float scale, int longest=0, "
+        "Tensor? init_state=None, bool return_state=False) -> (Tensor, Tensor)");
+  m.def("gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor log_gate, Tensor beta, Tensor state, float scale, "
+        "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
   m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor state, float scale, "
         "Tensor(a!)? out_state=None) -> (Tensor, Tensor)");
 }
@@ -1039,10 +1229,15 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
   m.impl("packed_attention", &packed_attention);
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("linear_attention", &linear_attention);
+  m.impl("gated_delta_fwd", &gated_delta_fwd);
+  m.impl("gated_delta_bwd", &gated_delta_bwd);
+  m.impl("gated_delta_step", &gated_delta_step);
+  m.impl("gated_delta_rule", &gated_delta_rule);
 }
 
 TORCH_LIBRARY_IMPL(bf, AutogradCUDA, m) {
   m.impl("packed_attention", &packed_attention);
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("linear_attention", &linear_attention);
+  m.impl("gated_delta_rule", &gated_delta_rule);
 }

@@ -1,4 +1,4 @@
-"""Operators over packed sequences: softmax attention, rotary positions, linear attention with decay.
+"""Operators over packed sequences: softmax attention, rotary positions, linear attention with decay, the gated delta rule.
 
 Sequences lie one behind the other along the first dimension of [rows, heads, head_dim] tensors: the node
 sequences of a batch of graphs, random walks (a walk is the sequence of its nodes), prompts of different
@@ -9,6 +9,7 @@ row sees, built on the GPU once per batch as an ``AttentionIndex`` is once per e
   rotary_embedding       rotary positions of q and k
   linear_attention       linear attention with a decay for each head, chunked; linear_attention_step: its
                          recurrent form for single tokens
+  gated_delta_rule       a state that each token gates and corrects, chunked; gated_delta_step: its recurrent form
 
 ``CoreAttention`` takes the first (and, with ``rotary``, the second) for ``attn_type="flash"``, the dense
 attention of models/graphormer_dist_node_level.py:603-608. All run as HIP kernels on the current stream;
@@ -345,3 +346,55 @@ def linear_attention_step(q, k, v, log_decay, state, scale: Optional[float] = No
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     return _op("linear_attn_step")(q.contiguous(), _as(q, k).contiguous(), _as(q, v).contiguous(), _decays(log_decay, q), state,
                                    scale, out_state)
+
+
+# ------------------------------------------------------------------ the gated delta rule
+def _gates(log_gate, beta, v):
+    got = []
+    for name, x in (("log_gate", log_gate), ("beta", beta)):
+        if not isinstance(x, torch.Tensor) or x.shape != v.shape[:2]:
+            raise ValueError(f"{name} must be {list(v.shape[:2])}")
+        got.append(x.float().contiguous())
+    return got
+
+
+def gated_delta_rule(q, k, v, log_gate, beta, seqs: PackedSequences, scale: Optional[float] = None,
+                     initial_state: Optional[torch.Tensor] = None, return_state: bool = False):
+    """The gated delta rule inside each sequence: a state of a fixed size that forgets by a gate of each token and is corrected
+    towards v_t at k_t with strength beta_t,
+
+        S' = exp(log_gate_t) S,  S = S' + beta_t k_t (v_t - S'^T k_t)^T,  out_t = scale S^T q_t.
+
+    q and k [rows, key heads, dk], v [rows, heads, dv] of one dtype (k and v are cast to q's), heads a multiple of the key
+    heads (value head h reads key head h // (heads // key heads)), dk and dv multiples of 8 up to 128; log_gate (at most 0; -inf:
+    the state is emptied first) and beta (0: the token writes nothing) [rows, heads], taken in float32. Keys are usually of unit
+    length: with beta of 0 to 1 (2: a reflection) the state then stays bounded.
+    ``seqs``: causal, the same sequences for rows and keys. ``scale``: 1 / sqrt(dk) by default. ``initial_state`` float32
+    [sequences, heads, dk, dv] comes before each sequence's first token; with ``return_state`` (out, state behind the last token)
+    is returned, from which ``gated_delta_step`` or the next chunk go on. Gradients flow to q, k, v, log_gate and beta and repeat
+    bit for bit; the states are constants. A value that is not finite makes the rows of its sequence from its own on NaN (one of v:
+    their column; one of q: its own row)."""
+    _check_seqs(seqs, q, k)
+    if not seqs.self_attention or not seqs.causal:
+        raise ValueError("the gated delta rule takes causal sequences of the same rows and keys")
+    k, v = _as(q, k), _as(q, v)
+    if initial_state is not None:
+        if initial_state.requires_grad:
+            raise NotImplementedError("the initial state is a constant: no gradient with respect to it")
+        initial_state = initial_state.float().contiguous()
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    log_gate, beta = _gates(log_gate, beta, v)
+    out, state = _op("gated_delta_rule")(q, k, v, log_gate, beta, seqs.q_offsets, scale, seqs.longest, initial_state,
+                                         bool(return_state))
+    return (out, state) if return_state else out
+
+
+def gated_delta_step(q, k, v, log_gate, beta, state, scale: Optional[float] = None, out_state: Optional[torch.Tensor] = None):
+    """One token of each of n sequences: (out [n, heads, dv], new state). q and k [n, key heads, dk], v [n, heads, dv],
+    log_gate and beta [n, heads], state float32 [n, heads, dk, dv]. ``out_state``: where the new state is written (``state``
+    itself updates it in place; anything else must not overlap it), else a new tensor. For inference: no gradients."""
+    if _trains(q, k, v, log_gate, beta, state, out_state):
+        raise NotImplementedError("gated_delta_step has no gradients (gated_delta_rule has)")
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    log_gate, beta = _gates(log_gate, beta, v)
+    return _op("gated_delta_step")(q, _as(q, k), _as(q, v), log_gate, beta, state, scale, out_state)

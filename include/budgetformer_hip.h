@@ -901,6 +901,49 @@ int bf_linear_attn_step(const void* q, const void* k, const void* v, const float
                         int64_t n, int32_t heads, int32_t dim_k, int32_t dim_v, int32_t dtype, float scale,
                         void* out, float* new_state, void* stream);
 
+/* The gated delta rule over causal packed sequences, a state of [dim_k, dim_v]
+ * for each value head h (which reads key head h / (heads / heads_k)):
+ *   S'_t = exp(log_gate[t, h]) S_{t-1},  e_t = v_t - S'_t^T k_t
+ *   S_t  = S'_t + beta[t, h] k_t e_t^T,  out_t = scale S_t^T q_t
+ * q, k: [n, heads_k, dim_k], v: [n, heads, dim_v], strides as in
+ * bf_packed_attn; out contiguous [n, heads, dim_v]; dims: a multiple of 8 up to
+ * 128. Sequence s is rows [offsets[s], offsets[s + 1]); rows behind the last one
+ * have out 0. init (or NULL), final_state (or NULL): float32 [n_seq, heads,
+ * dim_k, dim_v], the states before each sequence's first token and behind its
+ * last. Gates below exp(-150) are taken as that. A value that is not finite
+ * makes what follows of its own sequence NaN (one of v: its column), of q its own
+ * row.                                                                      */
+typedef struct bf_gated_delta {
+  int64_t n, n_seq;
+  int32_t heads, heads_k, dim_k, dim_v, dtype;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  const int32_t* offsets;     /* int32 [n_seq + 1], ascending from 0         */
+  const float* log_gate;      /* float32 [n, heads], <= 0 expected           */
+  const float* beta;          /* float32 [n, heads]                          */
+  const float* init;
+  float* final_state;
+  float scale;
+  int32_t longest;            /* no sequence has more rows; 0: unknown       */
+} bf_gated_delta;
+/* kept (NULL: no backward follows): bf_gated_delta_kept_floats(p) floats that
+ * the backward reads; scratch: bf_gated_delta_fwd_floats(p, kept != NULL)
+ * floats; both 16-byte aligned (-1: bad arguments).                         */
+int64_t bf_gated_delta_kept_floats(const bf_gated_delta* p);
+int64_t bf_gated_delta_fwd_floats(const bf_gated_delta* p, int32_t train);
+int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, void* out, float* kept,
+                       float* scratch, void* stream);
+/* Gradients of it, contiguous: dq and dk [n, heads_k, dim_k] (summed over the
+ * value heads of a key head), dv as out, dgate and dbeta float32 [n, heads].
+ * dout: contiguous. The states are constants. scratch:
+ * bf_gated_delta_bwd_floats(p) floats. No atomics: results repeat bit for bit. */
+int64_t bf_gated_delta_bwd_floats(const bf_gated_delta* p);
+int bf_gated_delta_bwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, const void* dout,
+                       const float* kept, void* dq, void* dk, void* dv, float* dgate, float* dbeta, float* scratch, void* stream);
+/* One token of each of n sequences: p->init the states [n, heads, dim_k, dim_v],
+ * p->final_state the new ones (may be p->init); strides of any size; offsets,
+ * n_seq and longest are not read.                                           */
+int bf_gated_delta_step(const bf_gated_delta* p, const void* q, const void* k, const void* v, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -156,3 +156,81 @@ def linear_attention(q, k, v, log_decay, lens, scale, initial_state=None, dout=N
             res[f"{x}_bound"] = u * res[x].abs() + (up + c32) * size[x] + small * seen[x] + _tiny(dtype)
         res["state_bound"] = (up / 3 + c32) * size["state"] + _tiny(dtype) * max(list(lens) + [1]) * 8
     return res
+
+
+def gated_delta(q, k, v, log_gate, beta, lens, scale, initial_state=None, dout=None):
+    """S' = exp(g) S, e = v - S'^T k, S = S' + b k e^T, out = scale S^T q, a token at a time; q, k [n, Hk, dk], v [n, H, dv], log_gate
+    and beta [n, H] float64. Returns a dict: out, state [sequences, H, dk, dv], with dout dq, dk, dv, dlog_gate, dbeta (the
+    recurrence's own way back), and ``terms``: of each tensor how large the terms of its sums are, by sequence and head."""
+    H, group = v.shape[1], v.shape[1] // k.shape[1]
+    qh, kh = q.repeat_interleave(group, 1), k.repeat_interleave(group, 1)
+    dk, dv = q.shape[2], v.shape[2]
+    res = {"out": torch.zeros_like(v), "state": q.new_zeros(len(lens), H, dk, dv)}
+    if dout is not None:
+        res.update(dq=torch.zeros_like(qh), dk=torch.zeros_like(qh), dv=torch.zeros_like(v),
+                   dlog_gate=torch.zeros_like(log_gate), dbeta=torch.zeros_like(beta))
+    at = 0
+    for b, n in enumerate(lens):
+        s = q.new_zeros(H, dk, dv) if initial_state is None else initial_state[b].double().clone()
+        kept = []
+        for t in range(at, at + n):
+            before = s * log_gate[t].exp()[:, None, None]
+            e = v[t] - torch.einsum("hkv,hk->hv", before, kh[t])
+            s = before + kh[t][:, :, None] * (beta[t][:, None] * e)[:, None, :]
+            res["out"][t] = scale * torch.einsum("hkv,hk->hv", s, qh[t])
+            kept.append((before, e, s))
+        res["state"][b] = s
+        if dout is not None:
+            r = torch.zeros_like(s)
+            for t in range(at + n - 1, at - 1, -1):
+                before, e, s = kept.pop()
+                do = scale * dout[t]
+                r = r + qh[t][:, :, None] * do[:, None, :]
+                res["dq"][t] = torch.einsum("hkv,hv->hk", s, do)
+                du = torch.einsum("hkv,hk->hv", r, kh[t])
+                res["dbeta"][t] = (du * e).sum(-1)
+                res["dv"][t] = beta[t][:, None] * du
+                res["dk"][t] = torch.einsum("hkv,hv->hk", r, beta[t][:, None] * e)
+                r = r - kh[t][:, :, None] * res["dv"][t][:, None, :]
+                res["dk"][t] -= torch.einsum("hkv,hv->hk", before, res["dv"][t])
+                res["dlog_gate"][t] = (r * before).sum((1, 2))
+                r = r * log_gate[t].exp()[:, None, None]
+        at += n
+    # a gate's gradient is a sum over a chunk of products of q and k with their gradients, and of the states' with theirs
+    most = {x: torch.zeros(len(lens), y.shape[1], dtype=torch.float64) for x, y in res.items()}
+    at = 0
+    for b, n in enumerate(lens):
+        for x, y in res.items():
+            rows = y[b:b + 1] if x == "state" else y[at:at + n]
+            if rows.numel():
+                most[x][b] = rows.abs().movedim(1, 0).flatten(1).amax(1).cpu()
+        if dout is not None and n:
+            products = (qh[at:at + n] * res["dq"][at:at + n]).abs().sum(-1) + (kh[at:at + n] * res["dk"][at:at + n]).abs().sum(-1)
+            most["dlog_gate"][b] += 32 * products.amax(0).cpu()
+        at += n
+    if dout is not None:
+        for x in ("dq", "dk"):
+            res[x] = res[x].unflatten(1, (-1, group)).sum(2)
+            most[x] = most[x].unflatten(1, (-1, group)).sum(2)
+    res["terms"] = most
+    return res
+
+
+def gated_delta_bound(res, name, lens, dtype):
+    """How far a kernel's ``name`` may be off for keys of at most unit length and strengths of 0 to 2, whose chunk inverses have
+    entries of at most 2 and whose state transitions shrink what is off already. Operands in two bfloat16 parts are off by 2^-18
+    each, and their product leaves 2^-18 out: 2^-17 together at most (float32's three parts: 2^-25, less than the 2^-24 of each of
+    a sum's additions, of some sqrt(320) independent ones: 2^-20). Independent roundings of a chunk of 32 tokens and of a
+    sequence's chunks add up as a root; an inverse's row of 32 entries and three products in a row amplify by 16 at most. float16 and
+    bfloat16 results are rounded besides."""
+    y = res[name]
+    eta = 2.0 ** -20 if dtype == torch.float32 else 2.0 ** -17
+    u = 0.0 if name in ("state", "dlog_gate", "dbeta") else half_step(dtype)
+    size = torch.zeros_like(y)
+    at = 0
+    for b, n in enumerate(lens):
+        rows = slice(b, b + 1) if name == "state" else slice(at, at + n)
+        most = res["terms"][name][b].to(y.device)
+        size[rows] = most.view(1, -1, *([1] * (y.dim() - 2)))
+        at += n
+    return u * y.abs() + 16 * eta * math.sqrt(32 + max(list(lens) + [1])) * size + _tiny(dtype)
