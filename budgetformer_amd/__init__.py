@@ -16,12 +16,12 @@ from .attention import (CoreAttention, ExphormerCoreAttention, GPSCoreAttention,
 from .edges import EdgeTable, build_attention_edges
 from .graph import CSRGraph
 from .hip_ops import AttentionIndex
-from .sequences import (PackedSequences, RotaryFrequencies, gated_delta_rule, gated_delta_step, linear_attention,
+from .sequences import (PackedSequences, RelativeBuckets, RotaryFrequencies, gated_delta_rule, gated_delta_step, linear_attention,
                         linear_attention_step, packed_attention, rotary_embedding)
 
 __all__ = [
     "AttentionIndex", "CSRGraph", "CoreAttention", "EdgeTable", "ExphormerCoreAttention", "GPSCoreAttention",
-    "GTCoreAttention", "PackedSequences", "RotaryFrequencies",
+    "GTCoreAttention", "PackedSequences", "RelativeBuckets", "RotaryFrequencies",
     "build_attention_edges", "gated_delta_rule", "gated_delta_step", "linear_attention", "linear_attention_step", "packed_attention", "rotary_embedding",
     "sparse_edge_attention",
 ]

@@ -67,6 +67,11 @@ class LinearAttn(C.Structure):
     ]
 
 
+class PackedBias(C.Structure):
+    """Mirror of ``struct bf_packed_bias``."""
+    _fields_ = [("table", vp), ("map", vp), ("positions", vp), ("buckets", i32), ("reach", i32)]
+
+
 class GatedDelta(C.Structure):
     """Mirror of ``struct bf_gated_delta``."""
     _fields_ = [
@@ -179,6 +184,12 @@ _SIGS = {
     "bf_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, vp, P_f32, P_f32, vp]),
     "bf_packed_attn_bwd_floats": (i64, [C.POINTER(PackedAttn)]),
     "bf_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttn), vp, vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_packed_attn_bias_fwd_floats": (i64, [C.POINTER(PackedAttn), C.POINTER(PackedBias)]),
+    "bf_packed_attn_bias_rest": (C.c_int, [C.POINTER(PackedAttn), C.POINTER(PackedBias)]),
+    "bf_packed_attn_bias_fwd": (C.c_int, [C.POINTER(PackedAttn), C.POINTER(PackedBias), vp, vp, vp, vp, vp, P_f32, P_f32, vp]),
+    "bf_packed_attn_bias_bwd_floats": (i64, [C.POINTER(PackedAttn), C.POINTER(PackedBias)]),
+    "bf_packed_attn_bias_bwd": (C.c_int, [C.POINTER(PackedAttn), C.POINTER(PackedBias), vp, vp, vp, vp, vp, P_f32, vp, vp, vp, vp, P_f32,
+                                          P_f32, P_f32, vp]),
     "bf_rotary": (C.c_int, [vp, vp, i64, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64), vp, i32, vp, f32, i32,
                             i32, vp, vp, vp]),
     "bf_linear_attn_fwd_floats": (i64, [C.POINTER(LinearAttn)]),

@@ -34,7 +34,7 @@ import torch.nn as nn
 
 from . import hip_ops
 from .hip_ops import AttentionIndex
-from .sequences import PackedSequences, RotaryFrequencies, packed_attention, rotary_embedding
+from .sequences import PackedSequences, RelativeBuckets, RotaryFrequencies, packed_attention, rotary_embedding
 
 
 class _SparseEdgeAttention(torch.autograd.Function):
@@ -250,12 +250,18 @@ class CoreAttention(nn.Module):
     """Graphormer core attention (models/graphormer_dist_node_level.py:61-613), sparse and flash paths on HIP.
 
     ``rotary`` (a ``RotaryFrequencies``): q and k of the flash path are turned by their place in the sequence
-    first."""
+    first. ``buckets`` (a ``RelativeBuckets``): scores of the flash path get a learned bias, the parameter
+    ``relative_bias`` [heads, buckets], that begins at 0."""
+
+    buckets: Optional[RelativeBuckets] = None
 
     def __init__(self, hidden_size, attention_dropout_rate, num_heads, attn_bias_dim=None,
-                 rotary: Optional[RotaryFrequencies] = None):
+                 rotary: Optional[RotaryFrequencies] = None, buckets: Optional[RelativeBuckets] = None):
         super().__init__()
         self.rotary = rotary
+        if buckets is not None:
+            self.buckets = buckets
+            self.relative_bias = nn.Parameter(torch.zeros(num_heads, buckets.buckets))
         self._batches = _BatchSequences()
         self.hidden_size_per_attention_head = hidden_size // num_heads
         self.num_attention_heads_per_partition = num_heads
@@ -303,7 +309,7 @@ class CoreAttention(nn.Module):
         """softmax(q k^T / sqrt(hn)) v inside each of the batch's sequences
         (models/graphormer_dist_node_level.py:603-608): q [b, S, H, hn], k and v [b, S, heads, hn]. ``sequences`` (forward's
         edge_index): a ``PackedSequences`` over the b*S rows instead, for graphs packed along S; an edge set is ignored.
-        No bias and no attention dropout."""
+        No dense bias (``buckets`` gives a learned one) and no attention dropout."""
         if attn_bias is not None:
             raise NotImplementedError("attn_type='flash' takes no attention bias")
         if self.training and self.attention_dropout_rate > 0.0:
@@ -317,7 +323,11 @@ class CoreAttention(nn.Module):
             if seqs.n_q != seqs.n_k:
                 raise ValueError("rotary positions of the flash path need as many keys as rows")
             q, k = rotary_embedding(q, k, self.rotary, seqs=seqs)
-        return packed_attention(q, k, v, seqs).reshape(batch_size, s_len, width)
+        if self.buckets is None:
+            return packed_attention(q, k, v, seqs).reshape(batch_size, s_len, width)
+        if self.buckets.map.device != q.device:
+            self.buckets = self.buckets.to(q.device)
+        return packed_attention(q, k, v, seqs, bias=self.relative_bias, buckets=self.buckets).reshape(batch_size, s_len, width)
 
 
 class GTCoreAttention(nn.Module):

@@ -36,6 +36,16 @@
 // units of a power of 2 (kLift, kLiftBack). Delta is a difference's second part: a forward that trains keeps
 // what the rounding of out left (`rest`), for it.
 //
+// With a bias (BIAS) a score gets table[head, bucket(distance)], distance the key's place less the row's in their sequence. A
+// workgroup keeps its heads' tables by distance in LDS (log2 units); a block of 32 rows by 32 keys that lies farther than the
+// map's reach on one side has one value a row there, which goes into the exponent's addend: only the blocks near the diagonal
+// look up a value a score. The table's gradient, the sum of dS by bucket, is formed in the dQ pass: every lane has a column of its own in
+// LDS, a float a bucket (nothing is added by two lanes, so the order is fixed), far blocks add one sum of 16. A wave's columns
+// are summed by head at the end, and the waves' sums by packed_bias_sum, in order and in 64 bits. A row's dS add up to 0, and so
+// a bucket's sum is a small difference of large ones, which a Delta that is off by P's rounding would spoil (6e-4 of the
+// gradient in bfloat16): a forward that trains with a bias multiplies P's rounding's rest too, and out and its own rest are then good to
+// 2^-17 (1e-5 of the gradient).
+//
 // NaN and infinities in places a row does not see: a masked P is 0, but 0 * inf is not. Where a tile is masked its
 // staged operand is checked; one that holds such a value takes a path that multiplies the finite values only, and
 // finds by a second product of indicators which rows do see one.
@@ -46,6 +56,13 @@ namespace bf {
 namespace {
 
 // ---------------------------------------------------------------- arguments
+struct Bias {
+  const float* table;            // [hq, buckets]
+  const int32_t *map, *positions;
+  float* part;                   // sums of dS by a wave's rows: [32-row blocks, hq, buckets]
+  int32_t buckets, reach, width; // width: of a head's values by distance in LDS
+};
+
 struct Args {
   const void *q, *k, *v, *out, *dout;
   void *o, *rest, *dq, *dk, *dv;                   // rest: what the rounding of out left, or NULL
@@ -58,6 +75,7 @@ struct Args {
   float scale, c;                                  // c = scale * log2(e)
   Div by_group;
   int32_t xcd_groups;                              // of heads, dealt to the XCDs (place)
+  Bias bias;
 };
 
 struct Row {
@@ -119,6 +137,50 @@ __device__ __forceinline__ void store_cols(O* p, const F32x16 (&acc)[(DP + 31) /
   for (int n = 0; n < (DP + 31) / 32; ++n) store_block<O>(p, acc[n], by, n, dim, half);
 }
 
+// ---------------------------------------------------------------- bias by distance
+constexpr int kBiasPad = 3;       // four distances in a row are read together, from up to three before the reach's ends
+
+// The values (log2 units) of distances -reach - 3 .. reach + 3 of the key head's query heads.
+__device__ __forceinline__ int bucket_of(const Bias& b, int at) {        // at: distance + reach + 3
+  return min(max(b.map[min(max(at - kBiasPad, 0), 2 * b.reach)], 0), b.buckets - 1);
+}
+__device__ __forceinline__ void stage_bias(const Args& a, int h, float* lds, int tid, int nt) {
+  const Bias& b = a.bias;
+  for (int i = tid; i < b.width; i += nt) {
+    const float* t = b.table + int64_t(h) * a.group * b.buckets + bucket_of(b, i);
+    for (int g = 0; g < a.group; ++g) lds[g * b.width + i] = t[g * b.buckets] * kLog2e;
+  }
+}
+
+// The place among the keys that stands at a row, and of a wave's rows the first and the last one.
+__device__ __forceinline__ int row_place(const Args& a, int token, int lo) { return lo + a.bias.positions[token]; }
+__device__ __forceinline__ int2 wave_places(int place, bool any) {
+  int lo = any ? place : INT_MAX, hi = any ? place : INT_MIN;
+  for (int o = 32; o; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64)), hi = max(hi, __shfl_xor(hi, o, 64));
+  return make_int2(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
+}
+
+// Where keys [j0, j0 + n) lie to rows at places [p.x, p.y]: at least the reach before all of them (-1), behind all (1), or near.
+__device__ __forceinline__ int side_of(const Args& a, int j0, int n, int2 p) {
+  if (int64_t(j0) + n - 1 - p.x <= -int64_t(a.bias.reach)) return -1;
+  return int64_t(j0) - p.y >= a.bias.reach ? 1 : 0;
+}
+
+// Where distance x (and the three behind it) stand among a head's values.
+__device__ __forceinline__ int bias_at(const Args& a, int x) {
+  return min(max(x, -a.bias.reach - kBiasPad), a.bias.reach) + a.bias.reach + kBiasPad;
+}
+
+// A lane's row against the keys of a block's registers: x[r] = x[r] c + its value.
+__device__ __forceinline__ void add_bias(const Args& a, float (&x)[16], const float* head, int first, int half) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const float* t = head + bias_at(a, first + 8 * g + 4 * half);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * g + j] = fmaf(x[4 * g + j], a.c, t[j]);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 // A row's terms are taken relative to a maximum that is raised only when a score passes it by 2^kLazy: the sums, then
 // up to 2^kLazy times larger, lose nothing in float32, and most tiles skip the rescaling of the accumulators.
@@ -128,12 +190,13 @@ constexpr float kLazy = 6.f;
 // (half a step is 2^-34 below that). The factor is in the exponent (free) and in the sum, so the quotient does not see it.
 template <typename T> constexpr float kLift = std::is_same<T, _Float16>::value ? 9.f : 0.f;
 
-template <typename T, int DP, int NW, int BN, bool SPLIT>
+template <typename T, int DP, int NW, int BN, bool SPLIT, bool BIAS>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void packed_fwd(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BM = 32 * NW;
   __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
   __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
+  extern __shared__ __attribute__((aligned(16))) float bias_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   int tile, h, piece;
   if (!place(a, tile, h, piece)) return;
@@ -156,6 +219,19 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
   const int2 span = a.row_span[row.token];
   const int lo = span.x, hi = valid ? span.y : span.x;
 
+  int place_k = 0;
+  int2 places;
+  float end[2] = {0.f, 0.f};
+  const float* mine = nullptr;
+  if constexpr (BIAS) {
+    const int g = row.head - h * a.group;
+    place_k = row_place(a, row.token, lo);
+    places = wave_places(place_k, hi > lo);
+    mine = bias_lds + g * a.bias.width;
+    for (int e = 0; e < 2; ++e) end[e] = a.bias.table[int64_t(row.head) * a.bias.buckets + bucket_of(a.bias, e * a.bias.width)] * kLog2e;
+    // a piece that lies far from its rows reads none of them (the first tile's barriers come before they are read)
+    if (NW > 1 || side_of(a, kbeg, max(kend - kbeg, 0), places) == 0) stage_bias(a, h, bias_lds, tid, NT);
+  }
   Frag<T> qf[TL::kSteps];
   load_row<T, DP>(qf, valid ? static_cast<const T*>(a.q) + row.token * a.qs_t + row.head * a.qs_h : nullptr, a.dim, half);
   F32x16 o[TL::kBlocks];
@@ -197,6 +273,17 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
     }
     __builtin_amdgcn_s_setprio(0);
     const bool masked = j0 < wl.x || j0 + BN > wf.y || w_last < w_row0 + 31;
+    float by = a.c, add = 0.f;                       // a score is s by + add
+    if constexpr (BIAS) {
+      const int side = side_of(a, j0, BN, places);
+      if (side == 0) {
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) add_bias(a, s[b], mine, j0 + 32 * b - place_k, half);
+        by = 1.f;
+      } else {
+        add = side < 0 ? end[0] : end[1];
+      }
+    }
     if (masked) {
 #pragma unroll
       for (int b = 0; b < BN / 32; ++b) {
@@ -211,7 +298,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    float mc_new = fmaxf(mc, top * a.c);
+    float mc_new = fmaxf(mc, BIAS ? fmaf(top, by, add) : top * a.c);
     if (__any(mc_new > mc + kLazy)) {
       const float alpha = mc_new == -INFINITY ? 1.f : exp2_fast(mc - mc_new);
       l *= alpha;
@@ -221,12 +308,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
         for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
       mc = mc_new;
     }
-    const float base = mc == -INFINITY ? 0.f : mc - kLift<T>;
+    float base = mc == -INFINITY ? 0.f : mc - kLift<T>;
+    if constexpr (BIAS) base -= add;
 #pragma unroll
     for (int b = 0; b < BN / 32; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[b][r] = exp2_fast(fmaf(s[b][r], a.c, -base));
+        s[b][r] = exp2_fast(fmaf(s[b][r], BIAS ? by : a.c, -base));
         l += s[b][r];
       }
     if (masked && odd) {
@@ -248,6 +336,22 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && DP == 128) ? 1
         for (int n = 0; n < TL::kBlocks; ++n) o[n] = Mat<T>::mma(TL::col_frag(v_lds, t, n, lane), p, o[n]);
       }
       __builtin_amdgcn_s_setprio(0);
+    }
+    if constexpr (BIAS && sizeof(T) == 2) {
+      if (a.rest) {                                  // what the rounding of P left
+#pragma unroll
+        for (int t = 0; t < BN / 16; ++t) {
+          Frag<T> p;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = T(s[t / 2][8 * (t & 1) + j] - float(T(s[t / 2][8 * (t & 1) + j])));
+#pragma unroll
+          for (int n = 0; n < TL::kBlocks; ++n) {
+            Frag<T> vt = TL::col_frag(v_lds, t, n, lane);
+            if (masked && odd) vt = finite<T>(vt);
+            o[n] = Mat<T>::mma(vt, p, o[n]);
+          }
+        }
+      }
     }
   }
 
@@ -343,13 +447,19 @@ __device__ __forceinline__ bool shrink(float (&ds)[16], int& by) {
   return true;
 }
 
+// Adds to a place of LDS that only this lane adds to: no value comes back and nothing waits.
+__device__ __forceinline__ void add_own(float* p, float x) {
+  __hip_atomic_fetch_add(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
 // ---------------------------------------------------------------- backward: dQ (and Delta)
-template <typename T, int DP, int NW, int BN>
+template <typename T, int DP, int NW, int BN, bool BIAS>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_bwd_q(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BM = 32 * NW;
   __shared__ __attribute__((aligned(16))) char k_lds[TL::bytes(BN)];
   __shared__ __attribute__((aligned(16))) char v_lds[TL::bytes(BN)];
+  extern __shared__ __attribute__((aligned(16))) float bias_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   int tile, h, piece;
   if (!place(a, tile, h, piece)) return;
@@ -367,6 +477,27 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
   const int lo = span.x, hi = valid ? span.y : span.x;
   const int64_t at = int64_t(row.token) * a.hq + row.head;
 
+  int place_k = 0, end_bucket[2] = {0, 0};
+  int2 places;
+  float end[2] = {0.f, 0.f};
+  const float* mine = nullptr;
+  uint32_t* map_lds = nullptr;         // the buckets of four distances in a row, a byte each
+  float* cols = nullptr;               // the lane's sums by bucket, 64 apart
+  if constexpr (BIAS) {
+    place_k = row_place(a, row.token, lo);
+    places = wave_places(place_k, hi > lo);
+    mine = bias_lds + (row.head - h * a.group) * a.bias.width;
+    map_lds = reinterpret_cast<uint32_t*>(bias_lds + a.group * a.bias.width);
+    cols = bias_lds + (a.group + 1) * a.bias.width + wave * a.bias.buckets * 64 + lane;
+    for (int e = 0; e < 2; ++e) {
+      end_bucket[e] = bucket_of(a.bias, e * a.bias.width);
+      end[e] = a.bias.table[int64_t(row.head) * a.bias.buckets + end_bucket[e]] * kLog2e;
+    }
+    stage_bias(a, h, bias_lds, tid, NT);
+    for (int i = tid; i < a.bias.width; i += NT)
+      map_lds[i] = bucket_of(a.bias, i) | bucket_of(a.bias, i + 1) << 8 | bucket_of(a.bias, i + 2) << 16 | bucket_of(a.bias, i + 3) << 24;
+    for (int b = 0; b < a.bias.buckets; ++b) cols[64 * b] = 0.f;
+  }
   Frag<T> qf[TL::kSteps], gf[TL::kSteps];
   load_row<T, DP>(qf, valid ? static_cast<const T*>(a.q) + row.token * a.qs_t + row.head * a.qs_h : nullptr, a.dim, half);
   load_row<T, DP>(gf, valid ? static_cast<const T*>(a.dout) + at * a.dim : nullptr, a.dim, half);
@@ -393,6 +524,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
   if (lse == -INFINITY) lse = INFINITY;
   int lift = kLiftBack<T>;             // P, dS and the sums are times 2^lift
   lse -= float(lift);
+  float unit = kUnits<T> ? ldexpf(1.f, -lift) : 1.f;       // of P and dS
 
   F32x16 dq[TL::kBlocks];
 #pragma unroll
@@ -430,12 +562,43 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
       }
       __builtin_amdgcn_s_setprio(0);
       float ds[16];
+      float by = a.c, less = lse;
+      int side = 0;
+      if constexpr (BIAS) {
+        side = side_of(a, j0 + 32 * b, 32, places);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(fmaf(sa[r], a.c, -lse)) * (pa[r] - delta);
+        for (int r = 0; r < 16; ++r) ds[r] = sa[r];
+        if (side == 0) {
+          add_bias(a, ds, mine, j0 + 32 * b - place_k, half);
+          by = 1.f;
+        } else {
+          less -= side < 0 ? end[0] : end[1];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(fmaf(ds[r], by, -less)) * (pa[r] - delta);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(fmaf(sa[r], a.c, -lse)) * (pa[r] - delta);
+      }
       if (masked) {
         const uint32_t seen = seen_bits(lo - j0 - 32 * b, hi - j0 - 32 * b, half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = where_seen(seen, r, ds[r], 0.f);
+      }
+      if constexpr (BIAS) {
+        if (side == 0) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t four = map_lds[bias_at(a, j0 + 32 * b + 8 * g + 4 * half - place_k)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) add_own(cols + 64 * ((four >> (8 * j)) & 255u), ds[4 * g + j] * unit);
+          }
+        } else {
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += ds[r];
+          add_own(cols + 64 * (side < 0 ? end_bucket[0] : end_bucket[1]), sum * unit);
+        }
       }
       if constexpr (kUnits<T>) {
         int by;
@@ -446,6 +609,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
             for (int r = 0; r < 16; ++r) dq[n][r] = ldexpf(dq[n][r], by);
           lse -= float(by);                        // for the tiles that follow
           lift += by;
+          if constexpr (BIAS) unit = ldexpf(1.f, -lift);
         }
       }
       __builtin_amdgcn_s_setprio(1);
@@ -463,17 +627,57 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     }
   }
   if (valid) store_cols<DP>(static_cast<T*>(a.dq) + at * a.dim, dq, kUnits<T> ? ldexpf(a.scale, -lift) : a.scale, a.dim, half);
+  if constexpr (BIAS) {                // the wave's sums by head of the group and bucket: of the lanes whose row is the head's
+    __syncthreads();
+    float* part = a.bias.part + ((int64_t(tile) * NW + wave) * a.hk + h) * a.group * a.bias.buckets;
+    const int first = int(a.by_group(uint32_t(w_row0))) * a.group;            // a row of head 0
+    for (int i = lane; i < a.group * a.bias.buckets; i += 64) {
+      const int g = i / a.bias.buckets, b = i - g * a.bias.buckets;
+      int from = first + g - w_row0;
+      if (from < 0) from += a.group;
+      const int n = from < 32 ? (31 - from) / a.group + 1 : 0;
+      float sum = 0.f;
+      const float* c = cols - lane + 64 * b + from;
+      for (int k = 0, at = n ? b % n : 0; k < n; ++k) {                       // lanes of different buckets read different banks
+        sum += c[at * a.group] + c[at * a.group + 32];
+        if (++at == n) at = 0;
+      }
+      part[i] = sum;
+    }
+  }
+}
+
+// The sums of the waves' parts, `n` of `values` each: chunks of them first (double [chunks, values]), then the chunks.
+__global__ __launch_bounds__(256) void packed_bias_sum(const float* part, int64_t n, int64_t values, double* sums) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= values) return;
+  const int64_t each = (n + gridDim.y - 1) / gridDim.y, from = blockIdx.y * each, to = from + each < n ? from + each : n;
+  double s = 0.0;
+#pragma unroll 8
+  for (int64_t p = from; p < to; ++p) s += double(part[p * values + i]);
+  sums[blockIdx.y * values + i] = s;
+}
+__global__ __launch_bounds__(256) void packed_bias_last(const double* sums, int chunks, int64_t values, float* dtable) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= values) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (int p = 0; p < chunks; ++p) s += sums[p * values + i];
+  dtable[i] = float(s);
 }
 
 // ---------------------------------------------------------------- backward: dK and dV
 // A wave owns 32 keys (a lane one of them); Q and dO tiles of BR rows pass through LDS with their rows' lse and Delta.
-template <typename T, int DP, int NW, int BR>
+template <typename T, int DP, int NW, int BR, bool BIAS>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void packed_bwd_kv(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NT = 64 * NW, BK = 32 * NW;
   __shared__ __attribute__((aligned(16))) char q_lds[TL::bytes(BR)];
   __shared__ __attribute__((aligned(16))) char g_lds[TL::bytes(BR)];
-  __shared__ __attribute__((aligned(16))) float lse_lds[BR], delta_lds[BR];
+  // with a bias: lse; lse less the value of rows far behind the key, and far before it; the rows' places, and where their heads' values begin
+  __shared__ __attribute__((aligned(16))) float lse_lds[BIAS ? 3 : 1][BR], delta_lds[BR];
+  __shared__ __attribute__((aligned(16))) int place_lds[BIAS ? BR : 4], head_lds[BIAS ? BR : 4];
+  extern __shared__ __attribute__((aligned(16))) float bias_lds[];
   constexpr bool kVLds = sizeof(T) == 2 && DP == 128;
   __shared__ __attribute__((aligned(16))) char v_lds[kVLds ? TL::bytes(BK) : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
@@ -517,6 +721,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
   const T* gp = static_cast<const T*>(a.dout);
   Stage<T, DP, BR, NT> qs, gs;
   float stat = 0.f;
+  int place_q = 0, head_q = 0;
+  if constexpr (BIAS) {
+    stage_bias(a, h, bias_lds, tid, NT);
+    __syncthreads();
+  }
   auto fetch = [&](int i0) {
     qs.load(tid, rend - i0, a.dim, [&](int r) {
       const Row w = row_of(a, h, i0 + r);
@@ -529,6 +738,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
     if (tid < 2 * BR) {          // rows behind rend read the last one's: their P and dS are masked
       const Row w = row_of(a, h, min(i0 + (tid & (BR - 1)), rend - 1));
       stat = (tid < BR ? a.lse : a.delta)[int64_t(w.token) * a.hq + w.head];
+      if constexpr (BIAS) place_q = row_place(a, w.token, a.row_span[w.token].x), head_q = (w.head - h * a.group) * a.bias.width;
     }
   };
   static_assert(2 * BR <= NT, "one statistic a lane");
@@ -539,9 +749,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
     __syncthreads();
     qs.store(tid, q_lds);
     gs.store(tid, g_lds);
-    if (tid < BR)
-      lse_lds[tid] = stat == -INFINITY ? INFINITY : stat - float(kLiftBack<T>);       // as in the dQ pass; not looked at before: nothing waits in fetch
-    else if (tid < 2 * BR)
+    if (tid < BR) {
+      const float ls = stat == -INFINITY ? INFINITY : stat - float(kLiftBack<T>);       // as in the dQ pass; not looked at before: nothing waits in fetch
+      lse_lds[0][tid] = ls;
+      if constexpr (BIAS) {
+        lse_lds[1][tid] = ls - bias_lds[head_q];
+        lse_lds[2][tid] = ls - bias_lds[head_q + a.bias.width - 1];
+        place_lds[tid] = place_q, head_lds[tid] = head_q;
+      }
+    } else if (tid < 2 * BR)
       delta_lds[tid - BR] = stat;
     bool odd = false;
     if (i0 < last_span.x || i0 + BR > first_span.y) {
@@ -563,14 +779,32 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void p
                          kVLds ? TL::row_frag(v_lds, 32 * wave + col, st, half) : vf[st], pa);
       }
       float p[16], ds[16];
+      int side = 0;
+      float by = a.c;
+      if constexpr (BIAS) {
+        const int x = place_lds[32 * b + col];
+        if (__all(side_of(a, w_key0, 32, make_int2(x, x)) < 0)) side = 1;
+        else if (__all(side_of(a, w_key0, 32, make_int2(x, x)) > 0)) side = 2;
+        if (side == 0) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 pl = *reinterpret_cast<const int4*>(&place_lds[32 * b + 8 * g + 4 * half]);
+            const int4 hd = *reinterpret_cast<const int4*>(&head_lds[32 * b + 8 * g + 4 * half]);
+            const int pv[4] = {pl.x, pl.y, pl.z, pl.w}, hv[4] = {hd.x, hd.y, hd.z, hd.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sa[4 * g + j] = fmaf(sa[4 * g + j], a.c, bias_lds[hv[j] + bias_at(a, key - pv[j])]);
+          }
+          by = 1.f;
+        }
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 ls = *reinterpret_cast<const float4*>(&lse_lds[32 * b + 8 * g + 4 * half]);
+        const float4 ls = *reinterpret_cast<const float4*>(&lse_lds[BIAS ? side : 0][32 * b + 8 * g + 4 * half]);
         const float4 de = *reinterpret_cast<const float4*>(&delta_lds[32 * b + 8 * g + 4 * half]);
         const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          p[4 * g + j] = exp2_fast(fmaf(sa[4 * g + j], a.c, -lv[j]));
+          p[4 * g + j] = exp2_fast(fmaf(sa[4 * g + j], BIAS ? by : a.c, -lv[j]));
           ds[4 * g + j] = p[4 * g + j] * (pa[4 * g + j] - dl[j]);
         }
       }
@@ -881,6 +1115,199 @@ int order_tiles(Args& a, const bf_packed_attn* p, const int2* span, int group, i
   return BF_OK;
 }
 
+// ---------------------------------------------------------------- calls with and without a bias
+constexpr int kMaxReach = 1024, kMaxBuckets = 64;
+constexpr int64_t kMaxBiasFloats = 16384;        // of a key head's query heads by distance: 64 KB beside the largest kernel's 93
+
+int check_bias(const bf_packed_attn* p, const bf_packed_bias* b, const char* fn) {
+  BF_CHECK_ARG(b != nullptr, "%s: no bias", fn);
+  BF_CHECK_ARG(b->buckets >= 1 && b->buckets <= kMaxBuckets && b->reach >= 0 && b->reach <= kMaxReach,
+               "%s: %d buckets (1 to 64), distances up to %d (0 to 1024)", fn, b->buckets, b->reach);
+  BF_CHECK_ARG(b->table && b->map && (p->n_q == 0 || b->positions), "%s: no table, map or positions", fn);
+  const int64_t heads = p->heads_q / p->heads_k;
+  if (heads * (2 * b->reach + 1 + 2 * kBiasPad) > kMaxBiasFloats) {
+    set_error("%s: %lld query heads to a key head over distances up to %d (their product is at most some 8000)", fn, (long long)heads, b->reach);
+    return BF_ERR_UNSUPPORTED;
+  }
+  return BF_OK;
+}
+
+void set_bias(Args& a, const bf_packed_bias* b) {
+  a.bias.table = b->table, a.bias.map = b->map, a.bias.positions = b->positions;
+  a.bias.buckets = b->buckets, a.bias.reach = b->reach, a.bias.width = 2 * b->reach + 1 + 2 * kBiasPad;
+}
+
+bool is_short(const bf_packed_attn* p, const bf_packed_bias* b) { return !b && packed_is_short(p); }
+
+// Bytes of a workgroup's values by distance; in the dQ pass of the buckets by distance and of the lanes' sums too.
+unsigned bias_bytes(const Args& a, const bf_packed_bias* b, int dq_waves) {
+  if (!b) return 0;
+  return 4u * unsigned((a.group + (dq_waves ? 1 : 0)) * a.bias.width + dq_waves * a.bias.buckets * 64);
+}
+
+// A kernel may use more than the 64 KB that are a launch's own limit.
+template <typename K> int allow_lds(K kern, unsigned bytes) {
+  if (bytes > 0)
+    BF_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  return BF_OK;
+}
+
+template <typename F> int with_bias(const bf_packed_bias* b, F&& f) {
+  return b ? f(std::true_type()) : f(std::false_type());
+}
+
+int64_t fwd_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
+  if (p->n_q == 0 || is_short(p, b)) return 0;
+  const int n = pieces_of(p);
+  return n == 1 ? order_ints(p) : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
+}
+
+int forward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v, void* out, void* rest,
+            float* lse, float* scratch, void* stream) {
+  if (p->n_q == 0) return BF_OK;
+  BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
+  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_fwd: rest and scratch must be 16-byte aligned");
+  if (is_short(p, bias)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
+  Args a = make_args(p, q, k, v);
+  if (bias) set_bias(a, bias);
+  a.o = out, a.rest = rest, a.lse = lse;
+  a.pieces = pieces_of(p);
+  const hipStream_t st = as_stream(stream);
+  const unsigned lds = bias_bytes(a, bias, 0);
+  if (a.pieces == 1) {
+    return with_type(p->dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      return with_dim(a.dim, [&](auto dp) -> int {
+        return with_bias(bias, [&](auto biased) -> int {
+          constexpr int DP = decltype(dp)::value, BN = tile_keys<T>(), NW = fwd_waves(sizeof(T), DP);
+          a.tiles = int(ceil_div(a.rows, 32 * NW));
+          BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
+          auto kern = packed_fwd<T, DP, NW, BN, false, decltype(biased)::value>;
+          BF_CHECK_OK(allow_lds(kern, lds));
+          BF_LAUNCH("packed_attn_fwd", kern, grid_of(a), dim3(64 * NW), lds, st, a);
+          BF_CHECK_LAUNCH();
+          return BF_OK;
+        });
+      });
+    });
+  }
+  BF_CHECK_ARG(scratch != nullptr, "packed_attn_fwd: no scratch (bf_packed_attn_fwd_floats)");
+  const int64_t n_rows = p->n_q * p->heads_q;
+  a.part = scratch;
+  a.stat = scratch + n_rows * a.pieces * a.dim;
+  a.tiles = int(ceil_div(a.rows, 32));
+  return with_type(p->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_dim(a.dim, [&](auto dp) -> int {
+      return with_bias(bias, [&](auto biased) -> int {
+        constexpr int DP = decltype(dp)::value;
+        auto kern = packed_fwd<T, DP, 1, 32, true, decltype(biased)::value>;
+        BF_CHECK_OK(allow_lds(kern, lds));
+        BF_LAUNCH("packed_attn_fwd_pieces", kern, grid_of(a), dim3(64), lds, st, a);
+        BF_CHECK_LAUNCH();
+        BF_LAUNCH("packed_attn_join", (packed_join<T>), dim3(unsigned(ceil_div(n_rows, 4))), dim3(256), 0, st, a.part, a.stat,
+                  n_rows, a.pieces, a.dim, static_cast<T*>(out), static_cast<T*>(rest), lse);
+        BF_CHECK_LAUNCH();
+        return BF_OK;
+      });
+    });
+  });
+}
+
+// The parts of the table's gradient: a wave's of 32 rows of a key head each, and the chunks that they are summed in.
+int dq_waves_of(const bf_packed_attn* p) {
+  const int elem = p->dtype == BF_DTYPE_F32 ? 4 : 2;
+  return dq_waves(elem, p->head_dim > 64 ? 128 : 64);
+}
+int64_t bias_parts(const bf_packed_attn* p) {
+  const int waves = dq_waves_of(p);
+  return ceil_div(p->n_q * (p->heads_q / p->heads_k), int64_t(32 * waves)) * waves;
+}
+int bias_chunks(int64_t parts) { return int(parts < 64 ? 1 : parts < 64 * 64 ? parts / 64 : 64); }
+int64_t bias_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
+  if (!b) return 0;
+  const int64_t values = int64_t(p->heads_q) * b->buckets, parts = bias_parts(p);
+  return 2 * bias_chunks(parts) * values + ceil_div(parts * values, int64_t(4)) * 4;
+}
+
+int64_t bwd_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
+  if (is_short(p, b)) return 0;
+  const int n = kv_pieces_of(p);
+  return bias_floats(p, b) + order_ints(p) + (n == 1 ? 0 : 2 * p->n_k * p->heads_k * p->head_dim * n);
+}
+
+int backward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v, const void* out,
+             const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* dtable, float* delta,
+             float* scratch, void* stream) {
+  BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
+               "packed_attn_bwd: bad arguments");
+  BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
+  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_bwd: rest and scratch must be 16-byte aligned");
+  if (is_short(p, bias)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, delta, as_stream(stream));
+  BF_CHECK_ARG(!bias || (scratch && dtable), "packed_attn_bias_bwd: no scratch (bf_packed_attn_bias_bwd_floats) or no dtable");
+  Args a = make_args(p, q, k, v);
+  double* sums = nullptr;
+  const int64_t parts = bias_parts(p), values = bias ? int64_t(p->heads_q) * bias->buckets : 0;
+  const int chunks = bias_chunks(parts);
+  if (bias) {
+    set_bias(a, bias);
+    sums = reinterpret_cast<double*>(scratch);
+    a.bias.part = scratch + 2 * chunks * values;
+    scratch += bias_floats(p, bias);
+  }
+  a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
+  a.lse = const_cast<float*>(lse);
+  const hipStream_t st = as_stream(stream);
+  BF_CHECK_OK(with_type(p->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return with_dim(a.dim, [&](auto dp) -> int {
+      return with_bias(bias, [&](auto biased) -> int {
+        constexpr int DP = decltype(dp)::value;
+        constexpr bool BIAS = decltype(biased)::value;
+        if (a.rows > 0) {
+          constexpr int NW = dq_waves(sizeof(T), DP);
+          a.tiles = int(ceil_div(a.rows, 32 * NW));
+          BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
+          auto kern = packed_bwd_q<T, DP, NW, dq_keys(sizeof(T), DP), BIAS>;
+          const unsigned lds = bias_bytes(a, bias, NW);
+          BF_CHECK_OK(allow_lds(kern, lds));
+          BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * NW), lds, st, a);
+          BF_CHECK_LAUNCH();
+        }
+        if (a.n_k > 0) {
+          constexpr int NWK = kv_waves(sizeof(T), DP);
+          a.tiles = int(ceil_div(a.n_k, 32 * NWK));
+          a.pieces = kv_pieces_of(p);
+          BF_CHECK_OK(order_tiles(a, p, a.key_span, 1, 32 * NWK, a.n_k, scratch, st));
+          BF_CHECK_ARG(a.pieces == 1 || scratch, "packed_attn_bwd: no scratch (bf_packed_attn_bwd_floats)");
+          a.part = scratch + order_ints(p);
+          auto kern = packed_bwd_kv<T, DP, NWK, DP == 128 ? 32 : tile_rows<T>(), BIAS>;
+          const unsigned lds = bias_bytes(a, bias, 0);
+          BF_CHECK_OK(allow_lds(kern, lds));
+          BF_LAUNCH("packed_attn_bwd_kv", kern, grid_of(a), dim3(64 * NWK), lds, st, a);
+          BF_CHECK_LAUNCH();
+          if (a.pieces > 1) {
+            const int64_t all = p->n_k * p->heads_k * p->head_dim;
+            BF_LAUNCH("packed_attn_join_kv", (packed_join_kv<T>), dim3(unsigned(ceil_div(2 * all, 1024))), dim3(256), 0, st,
+                      a.part, all, a.pieces, static_cast<T*>(dk), static_cast<T*>(dv));
+            BF_CHECK_LAUNCH();
+          }
+        }
+        return BF_OK;
+      });
+    });
+  }));
+  if (bias) {
+    BF_LAUNCH("packed_bias_sum", packed_bias_sum, dim3(unsigned(ceil_div(values, 256)), unsigned(chunks)), dim3(256), 0, st, a.bias.part, parts,
+              values, sums);
+    BF_CHECK_LAUNCH();
+    BF_LAUNCH("packed_bias_last", packed_bias_last, dim3(unsigned(ceil_div(values, 256))), dim3(256), 0, st, sums, chunks, values, dtable);
+    BF_CHECK_LAUNCH();
+  }
+  return BF_OK;
+}
+
 }  // namespace
 }  // namespace bf
 
@@ -902,10 +1329,7 @@ extern "C" int bf_packed_spans(const int32_t* q_offsets, const int32_t* k_offset
 }
 
 extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
-  if (check(p, "packed_attn_fwd_floats", false) != BF_OK) return -1;
-  if (p->n_q == 0 || packed_is_short(p)) return 0;
-  const int n = pieces_of(p);
-  return n == 1 ? order_ints(p) : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
+  return check(p, "packed_attn_fwd_floats", false) == BF_OK ? fwd_floats(p, nullptr) : -1;
 }
 
 extern "C" int bf_packed_attn_rest(const bf_packed_attn* p) {
@@ -915,99 +1339,46 @@ extern "C" int bf_packed_attn_rest(const bf_packed_attn* p) {
 extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
                                   float* lse, float* scratch, void* stream) {
   BF_CHECK_OK(check(p, "packed_attn_fwd", false));
-  if (p->n_q == 0) return BF_OK;
-  BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
-  BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
-  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_fwd: rest and scratch must be 16-byte aligned");
-  if (packed_is_short(p)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
-  Args a = make_args(p, q, k, v);
-  a.o = out, a.rest = rest, a.lse = lse;
-  a.pieces = pieces_of(p);
-  const hipStream_t st = as_stream(stream);
-  if (a.pieces == 1) {
-    return with_type(p->dtype, [&](auto t) -> int {
-      using T = decltype(t);
-      return with_dim(a.dim, [&](auto dp) -> int {
-        constexpr int DP = decltype(dp)::value, BN = tile_keys<T>(), NW = fwd_waves(sizeof(T), DP);
-        a.tiles = int(ceil_div(a.rows, 32 * NW));
-        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
-        auto kern = packed_fwd<T, DP, NW, BN, false>;
-        BF_LAUNCH("packed_attn_fwd", kern, grid_of(a), dim3(64 * NW), 0, st, a);
-        BF_CHECK_LAUNCH();
-        return BF_OK;
-      });
-    });
-  }
-  BF_CHECK_ARG(scratch != nullptr, "packed_attn_fwd: no scratch (bf_packed_attn_fwd_floats)");
-  const int64_t n_rows = p->n_q * p->heads_q;
-  a.part = scratch;
-  a.stat = scratch + n_rows * a.pieces * a.dim;
-  a.tiles = int(ceil_div(a.rows, 32));
-  return with_type(p->dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    return with_dim(a.dim, [&](auto dp) -> int {
-      constexpr int DP = decltype(dp)::value;
-      auto kern = packed_fwd<T, DP, 1, 32, true>;
-      BF_LAUNCH("packed_attn_fwd_pieces", kern, grid_of(a), dim3(64), 0, st, a);
-      BF_CHECK_LAUNCH();
-      BF_LAUNCH("packed_attn_join", (packed_join<T>), dim3(unsigned(ceil_div(n_rows, 4))), dim3(256), 0, st, a.part, a.stat,
-                n_rows, a.pieces, a.dim, static_cast<T*>(out), static_cast<T*>(rest), lse);
-      BF_CHECK_LAUNCH();
-      return BF_OK;
-    });
-  });
+  return forward(p, nullptr, q, k, v, out, rest, lse, scratch, stream);
 }
 
 extern "C" int64_t bf_packed_attn_bwd_floats(const bf_packed_attn* p) {
-  if (check(p, "packed_attn_bwd_floats", true) != BF_OK) return -1;
-  if (packed_is_short(p)) return 0;
-  const int n = kv_pieces_of(p);
-  return order_ints(p) + (n == 1 ? 0 : 2 * p->n_k * p->heads_k * p->head_dim * n);
+  return check(p, "packed_attn_bwd_floats", true) == BF_OK ? bwd_floats(p, nullptr) : -1;
 }
 
 extern "C" int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, const void* out,
                                   const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta,
                                   float* scratch, void* stream) {
   BF_CHECK_OK(check(p, "packed_attn_bwd", true));
-  BF_CHECK_ARG((p->n_q == 0 || (q && out && lse && dout && dq && delta)) && (p->n_k == 0 || (k && v && dk && dv)),
-               "packed_attn_bwd: bad arguments");
-  BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
-  BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_bwd: rest and scratch must be 16-byte aligned");
-  if (packed_is_short(p)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, delta, as_stream(stream));
-  Args a = make_args(p, q, k, v);
-  a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
-  a.lse = const_cast<float*>(lse);
-  const hipStream_t st = as_stream(stream);
-  return with_type(p->dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    return with_dim(a.dim, [&](auto dp) -> int {
-      constexpr int DP = decltype(dp)::value;
-      if (a.rows > 0) {
-        constexpr int NW = dq_waves(sizeof(T), DP);
-        a.tiles = int(ceil_div(a.rows, 32 * NW));
-        BF_CHECK_OK(order_tiles(a, p, a.row_span, a.group, 32 * NW, a.rows, scratch, st));
-        auto kern = packed_bwd_q<T, DP, NW, dq_keys(sizeof(T), DP)>;
-        BF_LAUNCH("packed_attn_bwd_q", kern, grid_of(a), dim3(64 * NW), 0, st, a);
-        BF_CHECK_LAUNCH();
-      }
-      if (a.n_k > 0) {
-        constexpr int NWK = kv_waves(sizeof(T), DP);
-        a.tiles = int(ceil_div(a.n_k, 32 * NWK));
-        a.pieces = kv_pieces_of(p);
-        BF_CHECK_OK(order_tiles(a, p, a.key_span, 1, 32 * NWK, a.n_k, scratch, st));
-        BF_CHECK_ARG(a.pieces == 1 || scratch, "packed_attn_bwd: no scratch (bf_packed_attn_bwd_floats)");
-        a.part = scratch + order_ints(p);
-        auto kern = packed_bwd_kv<T, DP, NWK, DP == 128 ? 32 : tile_rows<T>()>;
-        BF_LAUNCH("packed_attn_bwd_kv", kern, grid_of(a), dim3(64 * NWK), 0, st, a);
-        BF_CHECK_LAUNCH();
-        if (a.pieces > 1) {
-          const int64_t all = p->n_k * p->heads_k * p->head_dim;
-          BF_LAUNCH("packed_attn_join_kv", (packed_join_kv<T>), dim3(unsigned(ceil_div(2 * all, 1024))), dim3(256), 0, st,
-                    a.part, all, a.pieces, static_cast<T*>(dk), static_cast<T*>(dv));
-          BF_CHECK_LAUNCH();
-        }
-      }
-      return BF_OK;
-    });
-  });
+  return backward(p, nullptr, q, k, v, out, rest, lse, dout, dq, dk, dv, nullptr, delta, scratch, stream);
+}
+
+extern "C" int64_t bf_packed_attn_bias_fwd_floats(const bf_packed_attn* p, const bf_packed_bias* bias) {
+  if (check(p, "packed_attn_bias_fwd_floats", false) != BF_OK || check_bias(p, bias, "packed_attn_bias_fwd_floats") != BF_OK) return -1;
+  return fwd_floats(p, bias);
+}
+
+extern "C" int bf_packed_attn_bias_rest(const bf_packed_attn* p, const bf_packed_bias* bias) {
+  return check(p, "packed_attn_bias_rest", false) == BF_OK && check_bias(p, bias, "packed_attn_bias_rest") == BF_OK &&
+         p->dtype != BF_DTYPE_F32 && !is_short(p, bias);
+}
+
+extern "C" int bf_packed_attn_bias_fwd(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v,
+                                       void* out, void* rest, float* lse, float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "packed_attn_bias_fwd", false));
+  BF_CHECK_OK(check_bias(p, bias, "packed_attn_bias_fwd"));
+  return forward(p, bias, q, k, v, out, rest, lse, scratch, stream);
+}
+
+extern "C" int64_t bf_packed_attn_bias_bwd_floats(const bf_packed_attn* p, const bf_packed_bias* bias) {
+  if (check(p, "packed_attn_bias_bwd_floats", true) != BF_OK || check_bias(p, bias, "packed_attn_bias_bwd_floats") != BF_OK) return -1;
+  return bwd_floats(p, bias);
+}
+
+extern "C" int bf_packed_attn_bias_bwd(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v,
+                                       const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
+                                       void* dv, float* dtable, float* delta, float* scratch, void* stream) {
+  BF_CHECK_OK(check(p, "packed_attn_bias_bwd", true));
+  BF_CHECK_OK(check_bias(p, bias, "packed_attn_bias_bwd"));
+  return backward(p, bias, q, k, v, out, rest, lse, dout, dq, dk, dv, dtable, delta, scratch, stream);
 }

@@ -579,10 +579,31 @@ bf_packed_attn packed_args(const at::Tensor& q, const at::Tensor& k, const at::T
   return p;
 }
 
-// Forward (bf_packed_attn_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2, rest). With `train`,
-// rest is what the backward reads beside out (empty where it needs nothing).
-std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-                                                   const at::Tensor& row_span, double scale, int64_t longest, bool train) {
+// A learned bias by buckets of the relative position: table float32 [heads_q, buckets], map int32 [2 reach + 1], the rows' positions.
+struct BiasIn {
+  at::Tensor table, map, positions;
+};
+
+bf_packed_bias bias_args(const BiasIn& b, const bf_packed_attn& p, const at::Device& dev) {
+  bf_packed_bias r{};
+  require(b.table, "bias", at::kFloat, dev);
+  TORCH_CHECK_VALUE(b.table.dim() == 2 && b.table.size(0) == p.heads_q && b.table.size(1) < (int64_t(1) << 30), "bias must be [", p.heads_q,
+                    ", buckets] (got ", b.table.sizes(), ")");
+  require(b.map, "map", at::kInt, dev);
+  TORCH_CHECK_VALUE(b.map.dim() == 1 && b.map.size(0) % 2 == 1 && b.map.size(0) < (int64_t(1) << 30), "map must be [2 reach + 1] (got ",
+                    b.map.sizes(), ")");
+  require(b.positions, "positions", at::kInt, dev);
+  TORCH_CHECK_VALUE(b.positions.dim() == 1 && b.positions.size(0) == p.n_q, "positions must be [", p.n_q, "] (got ", b.positions.sizes(), ")");
+  r.table = b.table.data_ptr<float>(), r.map = b.map.data_ptr<int32_t>(), r.positions = b.positions.data_ptr<int32_t>();
+  r.buckets = int32_t(b.table.size(1)), r.reach = int32_t(b.map.size(0) / 2);
+  return r;
+}
+
+// Forward (bf_packed_attn_fwd, bf_packed_attn_bias_fwd): (out [n_q, heads_q, head_dim], lse float32 [n_q, heads_q], in log2,
+// rest). With `train`, rest is what the backward reads beside out (empty where it needs nothing).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attn_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                                        const at::Tensor& row_span, double scale, int64_t longest, bool train,
+                                                        const BiasIn* bias_in) {
   TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = as_rows(q_in, "q");
@@ -591,23 +612,43 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor&
   const bf_packed_attn p = packed_args(q, k, v, row_span, scale, longest);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
-  const int64_t floats = bf_packed_attn_fwd_floats(&p);
-  const bool keeps = train && bf_packed_attn_rest(&p);
+  bf_packed_bias bias{};
+  if (bias_in) bias = bias_args(*bias_in, p, q.device());
+  const int64_t floats = bias_in ? bf_packed_attn_bias_fwd_floats(&p, &bias) : bf_packed_attn_fwd_floats(&p);
+  const bool keeps = train && (bias_in ? bf_packed_attn_bias_rest(&p, &bias) : bf_packed_attn_rest(&p));
   at::Tensor scratch, rest = keeps ? at::empty_like(out) : at::empty({0}, out.options());
   if (floats > 0) scratch = at::empty({floats}, lse.options());
-  check_rc(bf_packed_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                              keeps ? rest.data_ptr() : nullptr, lse.data_ptr<float>(),
-                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
-           "bf::packed_attn_fwd");
+  void* rp = keeps ? rest.data_ptr() : nullptr;
+  float* sp = floats > 0 ? scratch.data_ptr<float>() : nullptr;
+  if (bias_in)
+    check_rc(bf_packed_attn_bias_fwd(&p, &bias, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(), sp,
+                                     stream_of(q)),
+             "bf::packed_attn_bias_fwd");
+  else
+    check_rc(bf_packed_attn_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(), sp, stream_of(q)),
+             "bf::packed_attn_fwd");
   return {out, lse, rest};
 }
 
-// Backward (bf_packed_attn_bwd): (dq, dk, dv), contiguous.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-                                                               const at::Tensor& row_span, const at::Tensor& key_span,
-                                                               const at::Tensor& out, const at::Tensor& lse,
-                                                               const at::Tensor& dout_in, double scale, int64_t longest,
-                                                               const std::optional<at::Tensor>& rest) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                               const at::Tensor& row_span, double scale, int64_t longest, bool train) {
+  return attn_fwd(q, k, v, row_span, scale, longest, train, nullptr);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bias_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                                    const at::Tensor& bias, const at::Tensor& map,
+                                                                    const at::Tensor& positions, const at::Tensor& row_span, double scale,
+                                                                    int64_t longest, bool train) {
+  const BiasIn b{bias, map, positions};
+  return attn_fwd(q, k, v, row_span, scale, longest, train, &b);
+}
+
+// Backward (bf_packed_attn_bwd, bf_packed_attn_bias_bwd): (dq, dk, dv, dbias or undefined), contiguous.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> attn_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                                                    const at::Tensor& row_span, const at::Tensor& key_span,
+                                                                    const at::Tensor& out, const at::Tensor& lse,
+                                                                    const at::Tensor& dout_in, double scale, int64_t longest,
+                                                                    const std::optional<at::Tensor>& rest, const BiasIn* bias_in) {
   TORCH_CHECK_VALUE(q_in.is_cuda(), "q must be a device tensor (got ", q_in.device(), ")");
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = as_rows(q_in, "q");
@@ -631,14 +672,41 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor&
   }
   const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
   at::Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
-  at::Tensor delta = at::empty_like(lse), scratch;
-  const int64_t floats = bf_packed_attn_bwd_floats(&p);
+  at::Tensor delta = at::empty_like(lse), scratch, dbias;
+  bf_packed_bias bias{};
+  if (bias_in) {
+    bias = bias_args(*bias_in, p, dev);
+    dbias = at::empty_like(bias_in->table);
+  }
+  const int64_t floats = bias_in ? bf_packed_attn_bias_bwd_floats(&p, &bias) : bf_packed_attn_bwd_floats(&p);
   if (floats > 0) scratch = at::empty({floats}, lse.options());
-  check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(),
-                              dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(),
-                              floats > 0 ? scratch.data_ptr<float>() : nullptr, stream_of(q)),
-           "bf::packed_attn_bwd");
+  float* sp = floats > 0 ? scratch.data_ptr<float>() : nullptr;
+  if (bias_in)
+    check_rc(bf_packed_attn_bias_bwd(&p, &bias, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(),
+                                     dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dbias.data_ptr<float>(),
+                                     delta.data_ptr<float>(), sp, stream_of(q)),
+             "bf::packed_attn_bias_bwd");
+  else
+    check_rc(bf_packed_attn_bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rp, lse.data_ptr<float>(), dout.data_ptr(),
+                                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(), sp, stream_of(q)),
+             "bf::packed_attn_bwd");
+  return {dq, dk, dv, dbias};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                               const at::Tensor& row_span, const at::Tensor& key_span,
+                                                               const at::Tensor& out, const at::Tensor& lse, const at::Tensor& dout,
+                                                               double scale, int64_t longest, const std::optional<at::Tensor>& rest) {
+  auto [dq, dk, dv, dbias] = attn_bwd(q, k, v, row_span, key_span, out, lse, dout, scale, longest, rest, nullptr);
   return {dq, dk, dv};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> packed_attn_bias_bwd(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bias, const at::Tensor& map,
+    const at::Tensor& positions, const at::Tensor& row_span, const at::Tensor& key_span, const at::Tensor& out, const at::Tensor& lse,
+    const at::Tensor& dout, double scale, int64_t longest, const std::optional<at::Tensor>& rest) {
+  const BiasIn b{bias, map, positions};
+  return attn_bwd(q, k, v, row_span, key_span, out, lse, dout, scale, longest, rest, &b);
 }
 
 // Rotary positions (bf_rotary) of x and, if given, y: new contiguous tensors.
@@ -1021,6 +1089,48 @@ std::tuple<at::Tensor, at::Tensor> packed_attention(const at::Tensor& q, const a
   return {out, lse};
 }
 
+struct PackedBiasAttention : torch::autograd::Function<PackedBiasAttention> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& bias, const at::Tensor& map, const at::Tensor& positions, const at::Tensor& row_span,
+                               const at::Tensor& key_span, double scale, int64_t longest) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, lse, rest] = packed_attn_bias_fwd(q, k, v, bias, map, positions, row_span, scale, longest, true);
+    ctx->save_for_backward({q, k, v, bias, map, positions, row_span, key_span, out, lse, rest});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["longest"] = longest;
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    return {out, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(10);
+    if (!grads[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1], out[2], out[3]) =
+          packed_attn_bias_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], grads[0], ctx->saved_data["scale"].toDouble(),
+                               ctx->saved_data["longest"].toInt(), s[10]);
+    }
+    return once(std::move(out));
+  }
+};
+
+// packed_attn_bias_fwd's out and lse, with gradients for q, k, v and the bias.
+std::tuple<at::Tensor, at::Tensor> packed_bias_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                         const at::Tensor& bias, const at::Tensor& map, const at::Tensor& positions,
+                                                         const at::Tensor& row_span, const at::Tensor& key_span, double scale,
+                                                         int64_t longest) {
+  refuse_tangents({&q, &k, &v, &bias}, "packed_attention");
+  if (trains({&q, &k, &v, &bias})) {
+    variable_list r = PackedBiasAttention::apply(q, k, v, bias, map, positions, row_span, key_span, scale, longest);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [out, lse, rest] = packed_attn_bias_fwd(q, k, v, bias, map, positions, row_span, scale, longest, false);
+  return {out, lse};
+}
+
 struct Rotary : torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& y,
                                const at::Tensor& positions, const at::Tensor& turns, double amplitude, bool interleaved) {
@@ -1183,6 +1293,12 @@ TORCH_LIBRARY(bf, m) {
         "bool train=False) -> (Tensor, Tensor, Tensor)");
   m.def("packed_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor row_span, Tensor key_span, Tensor out, Tensor lse, "
         "Tensor dout, float scale, int longest=0, Tensor? rest=None) -> (Tensor, Tensor, Tensor)");
+  m.def("packed_attn_bias_fwd(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor map, Tensor positions, Tensor row_span, float scale, "
+        "int longest=0, bool train=False) -> (Tensor, Tensor, Tensor)");
+  m.def("packed_attn_bias_bwd(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor map, Tensor positions, Tensor row_span, Tensor key_span, "
+        "Tensor out, Tensor lse, Tensor dout, float scale, int longest=0, Tensor? rest=None) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("packed_bias_attention(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor map, Tensor positions, Tensor row_span, "
+        "Tensor key_span, float scale, int longest=0) -> (Tensor, Tensor)");
   m.def("rotary(Tensor x, Tensor? y, Tensor positions, Tensor turns, float amplitude=1.0, bool interleaved=False, "
         "bool inverse=False) -> (Tensor, Tensor)");
   m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor row_span, Tensor key_span, Tensor offsets, "
@@ -1222,11 +1338,14 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
   m.impl("packed_spans", &packed_spans);
   m.impl("packed_attn_fwd", &packed_attn_fwd);
   m.impl("packed_attn_bwd", &packed_attn_bwd);
+  m.impl("packed_attn_bias_fwd", &packed_attn_bias_fwd);
+  m.impl("packed_attn_bias_bwd", &packed_attn_bias_bwd);
   m.impl("rotary", &rotary);
   m.impl("linear_attn_fwd", &linear_attn_fwd);
   m.impl("linear_attn_bwd", &linear_attn_bwd);
   m.impl("linear_attn_step", &linear_attn_step);
   m.impl("packed_attention", &packed_attention);
+  m.impl("packed_bias_attention", &packed_bias_attention);
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("linear_attention", &linear_attention);
   m.impl("gated_delta_fwd", &gated_delta_fwd);
@@ -1237,6 +1356,7 @@ TORCH_LIBRARY_IMPL(bf, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(bf, AutogradCUDA, m) {
   m.impl("packed_attention", &packed_attention);
+  m.impl("packed_bias_attention", &packed_bias_attention);
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("linear_attention", &linear_attention);
   m.impl("gated_delta_rule", &gated_delta_rule);

@@ -5,7 +5,8 @@ sequences of a batch of graphs, random walks (a walk is the sequence of its node
 lengths. ``PackedSequences`` holds what a batch's layers share: where each sequence starts and what each
 row sees, built on the GPU once per batch as an ``AttentionIndex`` is once per edge set.
 
-  packed_attention       dense softmax attention inside each sequence (grouped heads, causal or not)
+  packed_attention       dense softmax attention inside each sequence (grouped heads, causal or not), with a learned bias
+                         by buckets of the relative position (``RelativeBuckets``)
   rotary_embedding       rotary positions of q and k
   linear_attention       linear attention with a decay for each head, chunked; linear_attention_step: its
                          recurrent form for single tokens
@@ -200,17 +201,105 @@ def _check_seqs(seqs, q: torch.Tensor, k: torch.Tensor) -> None:
 
 
 # ------------------------------------------------------------------ softmax attention
-def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = None, with_lse: bool = False):
-    """softmax(scale q k^T) v inside each sequence of a packed batch.
+class RelativeBuckets:
+    """Which bucket of a learned bias a relative position falls in: the key's place less the row's in their sequence.
+
+    Of ``buckets`` buckets (with ``bidirectional`` half for keys behind the row, at positive distances, the second half of them;
+    else keys behind it are taken as at its place) the first half hold one distance each, 0, 1, 2, ..; the others distances that grow by one
+    factor up to ``far``: with e exact buckets of n, distance x is in bucket e + floor((n - e) log(x / e) / log(far / e)), formed in whole
+    numbers. From ``far`` on all are in the last. ``from_map``: any map. Up to 64 buckets, over distances up to 1024 (a bucket that
+    holds all that is farther begins there at the latest)."""
+
+    _MOST_REACH, _MOST_BUCKETS = 1024, 64
+
+    def __init__(self, buckets: int = 32, far: int = 128, *, bidirectional: bool = True, device="cuda"):
+        buckets, far = int(buckets), int(far)
+        n = buckets // 2 if bidirectional else buckets
+        if buckets < 2 or (bidirectional and (buckets % 2 or buckets < 4)):
+            raise ValueError(f"{buckets} buckets (2 at least; bidirectional: an even number of 4 at least)")
+        if far <= n // 2 or far >= 2 ** 31:
+            raise ValueError(f"far {far} must lie behind the {n // 2} distances with a bucket of their own")
+        away = self._directed(n, far)
+        ahead = [n + b for b in away[1:]] if bidirectional else [0] * (len(away) - 1)
+        self._set(away[:0:-1] + [away[0]] + ahead, buckets, device)
+
+    @staticmethod
+    def _directed(n: int, far: int) -> list:
+        """The buckets of distances from 0 to where the last one begins, in one direction."""
+        exact = n // 2
+        steps, got = n - exact, list(range(exact))
+        while got[-1] < n - 1:
+            x, k = len(got), max(got[-1] - exact, 0)
+            while k + 1 < steps and (x >= far or x ** steps * exact ** (k + 1) >= far ** (k + 1) * exact ** steps):
+                k += 1
+            got.append(exact + k)
+            if x > RelativeBuckets._MOST_REACH:
+                raise NotImplementedError(f"the last of {n} buckets up to {far} begins behind distance {x - 1}")
+        return got
+
+    @classmethod
+    def from_map(cls, buckets_by_distance: Sequence[int], device="cuda") -> "RelativeBuckets":
+        """From the buckets of distances -reach .. reach (an odd number of them, on the host); farther ones are as the ends."""
+        got = [int(b) for b in buckets_by_distance]
+        if len(got) % 2 == 0:
+            raise ValueError(f"{len(got)} distances (an odd number, -reach to reach)")
+        if min(got) < 0:
+            raise ValueError("a bucket is negative")
+        self = object.__new__(cls)
+        self._set(got, max(got) + 1, device)
+        return self
+
+    def _set(self, by_distance: list, buckets: int, device) -> None:
+        device = PackedSequences._device(device)
+        while len(by_distance) > 1 and by_distance[0] == by_distance[1] and by_distance[-1] == by_distance[-2]:
+            by_distance = by_distance[1:-1]              # as the next nearer ones
+        if buckets > self._MOST_BUCKETS or len(by_distance) // 2 > self._MOST_REACH:
+            raise NotImplementedError(f"{buckets} buckets over distances up to {len(by_distance) // 2} ({self._MOST_BUCKETS} over "
+                                      f"{self._MOST_REACH} are supported)")
+        self.buckets, self.reach = buckets, len(by_distance) // 2
+        self.by_distance = tuple(by_distance)
+        with torch.inference_mode(False):                # a plain tensor: training saves it
+            self.map = torch.tensor(by_distance, dtype=torch.int32).to(device)
+
+    def of(self, distance: int) -> int:
+        """The bucket of one distance."""
+        return self.by_distance[min(max(int(distance), -self.reach), self.reach) + self.reach]
+
+    @torch.inference_mode(False)
+    def to(self, device) -> "RelativeBuckets":
+        got = object.__new__(RelativeBuckets)
+        got.buckets, got.reach, got.by_distance = self.buckets, self.reach, self.by_distance
+        got.map = self.map.to(PackedSequences._device(device))
+        return got
+
+
+def packed_attention(q, k, v, seqs: PackedSequences, scale: Optional[float] = None, with_lse: bool = False,
+                     bias: Optional[torch.Tensor] = None, buckets: Optional[RelativeBuckets] = None):
+    """softmax(scale q k^T + bias) v inside each sequence of a packed batch.
 
     q [n_q, heads, hn], k and v [n_k, kv_heads, hn] of one dtype (k and v are cast to q's), heads a multiple of
     kv_heads (query head h reads key head h // (heads // kv_heads)), hn a multiple of 8 up to 128. Rows and heads
     may have any strides. ``scale`` (positive, up to 2e38): 1 / sqrt(hn) by default. Returns out [n_q, heads, hn], or (out,
     lse) with ``with_lse``: lse float32 [n_q, heads], the log of the row's sum of exponentials, -inf for a row
-    that sees no key (its out is 0); lse is not differentiable. Gradients repeat bit for bit."""
+    that sees no key (its out is 0); lse is not differentiable. Gradients repeat bit for bit.
+
+    ``bias`` [heads, buckets] with ``buckets`` (a ``RelativeBuckets``): a learned value that a score gets by its head and the bucket
+    of the key's place less the row's (rows stand behind their sequence's earlier keys), taken in float32 (not scaled; -inf: keys there are not
+    seen); its gradient is the sum of its scores' gradients. The heads of a group times the distances (2 reach + 7) are
+    16384 at most."""
     _check_seqs(seqs, q, k)
     k, v = _as(q, k), _as(q, v)
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
+    if (bias is None) != (buckets is None):
+        raise ValueError("bias and buckets come together")
+    if buckets is not None:
+        if not isinstance(buckets, RelativeBuckets):
+            raise TypeError(f"buckets must be a RelativeBuckets (got {type(buckets)})")
+        if tuple(bias.shape) != (q.size(1), buckets.buckets):
+            raise ValueError(f"bias must be [{q.size(1)}, {buckets.buckets}] (got {list(bias.shape)})")
+        out, lse = _op("packed_bias_attention")(q, k, v, bias.float().contiguous(), buckets.map, seqs.positions(), seqs.row_span,
+                                                seqs.key_span, scale, seqs.longest)
+        return (out, lse * math.log(2.0)) if with_lse else out
     out, lse = _op("packed_attention")(q, k, v, seqs.row_span, seqs.key_span, scale, seqs.longest)
     return (out, lse * math.log(2.0)) if with_lse else out
 

@@ -843,6 +843,29 @@ int bf_packed_attn_bwd(const bf_packed_attn* p, const void* q, const void* k, co
                        const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* delta, float* scratch,
                        void* stream);
 
+/* The same with a learned bias by buckets of the relative position: a score is
+ * scale q.k + table[head, map[clamp(distance, -reach, reach) + reach]], distance
+ * the key's place less the row's in their sequence. table: float32 [heads_q,
+ * buckets]; map: int32 [2 reach + 1], values of 0 to buckets - 1; positions:
+ * bf_packed_spans' of the rows. buckets: up to 64; reach: up to 1024, times the
+ * query heads of a key head up to some 8000. dtable: float32 like table, the
+ * sums of the scores' gradients by bucket; they repeat bit for bit. The
+ * workspaces are as those of the calls without a bias, from the *_bias_* sizes. */
+typedef struct bf_packed_bias {
+  const float* table;
+  const int32_t* map;
+  const int32_t* positions;
+  int32_t buckets, reach;
+} bf_packed_bias;
+int64_t bf_packed_attn_bias_fwd_floats(const bf_packed_attn* p, const bf_packed_bias* bias);
+int bf_packed_attn_bias_rest(const bf_packed_attn* p, const bf_packed_bias* bias);
+int bf_packed_attn_bias_fwd(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v,
+                            void* out, void* rest, float* lse, float* scratch, void* stream);
+int64_t bf_packed_attn_bias_bwd_floats(const bf_packed_attn* p, const bf_packed_bias* bias);
+int bf_packed_attn_bias_bwd(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v,
+                            const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
+                            void* dv, float* dtable, float* delta, float* scratch, void* stream);
+
 /* Rotary positions: the first `rot` values of every head of x and y (rows of
  * `dim` values; y may be NULL with heads_y 0) turned pair by pair by the angle
  * 2 pi positions[row] * turns[pair] and scaled by amplitude; the rest is

@@ -30,17 +30,24 @@ def visible(m: int, n: int, causal: bool, device=None):
 
 
 def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, operand_tiny=None,
-              rounds=True):
+              rounds=True, table=None, bucket=None):
     """q [n_q, H, d], k, v [n_k, Hk, d] float64 packed. Returns a dict: out, lse (natural log) and with dout dq, dk, dv;
     with dtype also each one's bound (``out_bound``, ...). Rows that see no key: out 0, lse -inf. operand_tiny: half a step
     of a subnormal P or dS, where that is finer than the type's own. rounds: whether P and dS are operands of the type and
-    Delta comes from the rounded out (False: neither; Delta as good as from out and its rounding's rest, rounded itself)."""
+    Delta comes from the rounded out (False: neither; Delta as good as from out and its rounding's rest, rounded itself).
+    table [H, buckets] float64 and bucket, a function of distances (a key's place less the row's): scores get table[h, bucket],
+    and with dout there is dtable. Its bound takes a Delta from out and its rounding's rest, with P in two parts: a row's dS add
+    up to 0, and a sum over a bucket shows what is off in it."""
     H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
     g = H // Hk
     names = ["out"] + (["dq", "dk", "dv"] if dout is not None else [])
+    if table is not None and dout is not None:
+        names.append("dtable")
     res = {"out": torch.zeros_like(q), "dq": torch.zeros_like(q), "dk": torch.zeros_like(k), "dv": torch.zeros_like(v),
            "lse": q.new_full(q.shape[:2], -math.inf)}
     bnd = {x: torch.zeros_like(res[x]) for x in ("out", "dq", "dk", "dv")}
+    if table is not None:
+        res["dtable"], bnd["dtable"] = torch.zeros_like(table), torch.zeros_like(table)
     u = half_step(dtype) if dtype is not None else 0.0
     up = 0.0 if dtype == torch.float32 or not rounds else u      # P and dS as operands: rounded to the type
     tiny = _tiny(dtype)
@@ -52,9 +59,14 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
         if m == 0 or n == 0:
             continue
         see = visible(m, n, causal, q.device)
+        if table is not None:
+            at = bucket(torch.arange(n, device=q.device) - torch.arange(n - m, n, device=q.device)[:, None])
         for h in range(H):
             a, b, w = q[rows, h], k[keys, h // g], v[keys, h // g]
-            s = (a @ b.T * scale).masked_fill(~see, -math.inf)
+            s = a @ b.T * scale
+            if table is not None:
+                s = s + table[h][at]
+            s = s.masked_fill(~see, -math.inf)
             top = s.amax(1, keepdim=True).clamp(min=-1e300)
             p = (s - top).exp()
             z = p.sum(1, keepdim=True)
@@ -66,6 +78,8 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
             if dtype is None and dout is None:
                 continue
             big = scale * (a.abs() @ b.abs().T).masked_fill(~see, 0).amax() if see.any() else 0.0
+            if table is not None and see.any():
+                big = big + table[h][at].masked_fill(~see | ~torch.isfinite(table[h][at]), 0).abs().amax()
             # scores: sums of d products, each step off by 2^-24, scaled; their exponentials' relative error, the sums over n
             c32 = 2.0 ** -24 * (2 * (d + 8) * (1 + float(big)) + n + m * g + 32)
             ob = u * out.abs() + (up + c32) * (p @ w.abs()) + small * (see.double() @ w.abs()) + tiny
@@ -75,6 +89,12 @@ def attention(q, k, v, q_lens, k_lens, causal, scale, dout=None, dtype=None, ope
             do = dout[rows, h]
             dp = do @ w.T
             ds = p * (dp - (do * out).sum(1, keepdim=True))
+            if table is not None:
+                ob2 = (0.0 if dtype == torch.float32 else 2 * u * u) * (out.abs() + p @ w.abs()) + c32 * (p @ w.abs()) + tiny
+                off = c32 * ds.abs() + p * ((do.abs() * ob2).sum(1, keepdim=True) + 2 * c32 * (do.abs() @ w.abs().T))
+                for x in range(table.shape[1]):
+                    res["dtable"][h, x] += ds[at == x].sum()
+                    bnd["dtable"][h, x] += off[at == x].sum() + 2.0 ** -20 * ds[at == x].abs().sum()     # a column's up to some 300 additions
             res["dq"][rows, h] = scale * ds @ b
             res["dk"][keys, h // g] += scale * ds.T @ a
             res["dv"][keys, h // g] += p.T @ do
