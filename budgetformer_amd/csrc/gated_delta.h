@@ -43,8 +43,7 @@ struct DeltaArgs {
   const int32_t* offsets;
   float *g2, *gin, *gout;                      // [n, heads]: log2 of the gates up to the token in its chunk; exp(G), exp(G_C - G)
   uint4 *inv, *score, *inv_t, *score_t;        // operands of each (chunk, head); the transposed ones for the backward, or NULL
-  uint4* map_b;                                // M^T of each (segment, head) as an operand
-  __bf16* map_f;                               // M, row-major, a part behind the other
+  uint4 *map_f, *map_b;                        // M and M^T of each (segment, head), operands (the latter for the backward, or NULL)
   float *state, *dstate;                       // [segments, heads, dk, dv]: before each segment; the gradient behind it
   const float* init;
   float* final_state;
@@ -89,17 +88,26 @@ using BFrag = Frag<__bf16>;
 
 template <int N> struct Split { BFrag p[N]; };
 
+// Two values' parts, a word each (one conversion instruction for both).
+template <int N> __device__ __forceinline__ void split_two(float a, float b, uint32_t (&w)[N]) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const F2 f = {a, b};
+    w[n] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, B2));
+    a -= __uint_as_float(w[n] << 16);
+    b -= __uint_as_float(w[n] & 0xffff0000u);
+  }
+}
+
 template <int N> __device__ __forceinline__ Split<N> split(const float (&x)[8]) {
+  uint32_t w[4][N];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split_two<N>(x[2 * j], x[2 * j + 1], w[j]);
   Split<N> s;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float r = x[j];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      s.p[n][j] = __bf16(r);
-      r -= float(s.p[n][j]);
-    }
-  }
+  for (int n = 0; n < N; ++n) s.p[n] = __builtin_bit_cast(BFrag, make_uint4(w[0][n], w[1][n], w[2][n], w[3][n]));
   return s;
 }
 
@@ -181,18 +189,16 @@ __device__ __forceinline__ void store_parts(const Stage<T, D, C, NT>& st, int ti
     char* p = lds + row * PT::TL::kPitch + (c % S::kChunks) * int(sizeof(Out));
     const In v = __builtin_bit_cast(In, st.r[i]);
     const float w = by(row);
-    float x[S::kPer];
+    uint32_t o[S::kPer / 2][N];
 #pragma unroll
-    for (int j = 0; j < S::kPer; ++j) x[j] = float(v[j]) * w;
+    for (int j = 0; j < S::kPer / 2; ++j) split_two<N>(float(v[2 * j]) * w, float(v[2 * j + 1]) * w, o[j]);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      Out o;
+      typedef uint32_t Words __attribute__((ext_vector_type(S::kPer / 2)));
+      Words q;
 #pragma unroll
-      for (int j = 0; j < S::kPer; ++j) {
-        o[j] = __bf16(x[j]);
-        x[j] -= float(o[j]);
-      }
-      *reinterpret_cast<Out*>(p + n * PT::kPart) = o;
+      for (int j = 0; j < S::kPer / 2; ++j) q[j] = o[j][n];
+      *reinterpret_cast<Words*>(p + n * PT::kPart) = q;
     }
   }
 }
@@ -227,9 +233,10 @@ __device__ __forceinline__ Place find(const DeltaArgs& a, int64_t x, int per) {
     hi = lo + step < hi ? lo + step : hi;
   }
   Place p;
-  const int from = clamped(a, lo);
+  lo = __builtin_amdgcn_readfirstlane(int(lo));
+  const int from = __builtin_amdgcn_readfirstlane(clamped(a, lo));
   p.seq = int(lo);
-  p.seq_end = lo < a.n_seq ? max(clamped(a, lo + 1), from) : a.n;
+  p.seq_end = __builtin_amdgcn_readfirstlane(lo < a.n_seq ? max(clamped(a, lo + 1), from) : a.n);
   const int64_t idx = x - (from / per + lo), at = from + idx * per;
   p.none = idx < 0 || (idx > 0 && at >= p.seq_end);
   p.idx = int(idx);
@@ -248,6 +255,43 @@ template <typename O> __device__ __forceinline__ void clear_rows(O* p, const Pla
   if (p == nullptr) return;
   for (int r = at.begin; r < at.end; ++r)
     for (int d = tid; d < dim; d += nt) p[r * row + head + d] = O(0.f);
+}
+
+// A chunk's rows of a result, as a buffer: stores need no branch, since what lies behind the last row, or at kNowhere, is dropped.
+// (Behind a branch around a store the next wait for loads that are on their way waits for the stores as well: a pass over 17,900
+// tokens, 8 heads of 64, took 69 us so.)
+struct Rows {
+  __amdgpu_buffer_rsrc_t r;
+  int stride;                  // of a row, in values
+};
+constexpr int kNowhere = 0x7ffffff0;
+template <typename O> __device__ __forceinline__ Rows rows_at(O* p, int len, int stride, int dim) {
+  return Rows{__builtin_amdgcn_make_buffer_rsrc(p, 0, len > 0 ? ((len - 1) * stride + dim) * int(sizeof(O)) : 0, 0x20000), stride};
+}
+template <typename O> __device__ __forceinline__ void put(const Rows& w, int row, int at, bool in, float x) {
+  const int off = in ? (row * w.stride + at) * int(sizeof(O)) : kNowhere;
+  if constexpr (sizeof(O) == 2)
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, O(x)), w.r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), w.r, off, 0, 0);
+}
+template <typename O> __device__ __forceinline__ void put4(const Rows& w, int row, int at, bool in, float a, float b, float c, float d) {
+  typedef O V4 __attribute__((ext_vector_type(4)));
+  typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  const int off = in ? (row * w.stride + at) * int(sizeof(O)) : kNowhere;
+  const V4 v = {O(a), O(b), O(c), O(d)};
+  if constexpr (sizeof(O) == 2)
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(U2, v), w.r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(U4, v), w.r, off, 0, 0);
+}
+
+// Stores that are dropped, as many as follow a loop's loads each time round: the first wait for loads then counts what the others do.
+template <int N> __device__ __forceinline__ void no_stores(void* p) {
+  const Rows none = rows_at(static_cast<float*>(p), 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) put<float>(none, 0, 0, false, 0.f);
 }
 
 // ---------------------------------------------------------------- inverses and scores of the chunks
@@ -371,19 +415,30 @@ __global__ __launch_bounds__(64) void delta_prep(const DeltaArgs a) {
   }
 }
 
-// A chunk's operand of two steps, from memory.
-template <int N> struct ChunkFrag {
-  uint4 r[2][N];
-  __device__ __forceinline__ void load(const uint4* p) {
+// A chunk's operand of two steps on its way from memory to LDS; all waves read it there. (A workgroup of one wave has it in its
+// registers as it stands.)
+template <int N, int NT> struct ChunkFrag {
+  static constexpr int kAll = 2 * N * 64, kN = (kAll + NT - 1) / NT;
+  uint4 r[kN];
+  __device__ __forceinline__ void load(const uint4* p, int tid) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int n = 0; n < N; ++n) r[u][n] = p[(u * N + n) * 64];
+    for (int i = 0; i < kN; ++i) r[i] = p[min(i * NT + tid, kAll - 1)];
   }
-  __device__ __forceinline__ Split<N> get(int u) const {
+  __device__ __forceinline__ void store(uint4* lds, int tid) const {
+    if constexpr (NT == 64) return;
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (kAll % NT == 0 || i * NT + tid < kAll) lds[i * NT + tid] = r[i];
+  }
+  __device__ __forceinline__ Split<N> get(const uint4* lds, int u, int lane) const {
     Split<N> s;
 #pragma unroll
-    for (int n = 0; n < N; ++n) s.p[n] = __builtin_bit_cast(BFrag, r[u][n]);
+    for (int n = 0; n < N; ++n) {
+      if constexpr (NT == 64)
+        s.p[n] = __builtin_bit_cast(BFrag, r[u * N + n]);
+      else
+        s.p[n] = __builtin_bit_cast(BFrag, lds[(u * N + n) * 64 + lane]);
+    }
     return s;
   }
 };
@@ -406,19 +461,27 @@ __device__ __forceinline__ void by_token(float (&x)[16], const float* lds, int h
 }
 
 // A state's block of 32 rows, row-major [dk, dv] float32 in memory: register r row 32 b + acc_row(r, half), lane the column.
+// (A state has at most 2^14 values. `fresh`: the addresses are formed where they are used, and not kept through a loop.)
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ void load_state(F32x16& m, const float* s, int b, int z, int half, int dk, int dv) {
+  const int x0 = fresh(32 * b + 4 * half), zc = min(z, dv - 1);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int x = 32 * b + acc_row(r, half);
-    const float v = s ? s[int64_t(min(x, dk - 1)) * dv + min(z, dv - 1)] : 0.f;
+    const int x = x0 + acc_row(r, 0);
+    const float v = s ? s[min(x, dk - 1) * dv + zc] : 0.f;
     m[r] = x < dk && z < dv ? v : 0.f;
   }
 }
 __device__ __forceinline__ void store_state(const F32x16& m, float* s, int b, int z, int half, int dk, int dv) {
+  const int x0 = fresh(32 * b + 4 * half);
+  if (z >= dv) return;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int x = 32 * b + acc_row(r, half);
-    if (x < dk && z < dv) s[int64_t(x) * dv + z] = m[r];
+    const int x = x0 + acc_row(r, 0);
+    if (x < dk) s[x * dv + z] = m[r];
   }
 }
 
@@ -453,7 +516,7 @@ template <int N> __device__ __forceinline__ Marked<N> marked(const float (&x)[16
 // A wave owns 32 columns of the state (a lane one, its rows in registers). kMaps: the waves behind those of the values' columns
 // own M's.
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 128 ? 2 : 1) void delta_pass(const DeltaArgs a) {
+__global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, sizeof(T) == 2 || (MODE == kMaps && D == 128) ? 2 : 1) void delta_pass(const DeltaArgs a) {
   constexpr int NW = D / 32 * (MODE == kMaps ? 2 : 1), NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
   constexpr bool OUT = MODE != kMaps;
@@ -462,9 +525,10 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
   __shared__ __attribute__((aligned(16))) char k_lds[PX::kBytes];
   __shared__ __attribute__((aligned(16))) char q_lds[OUT ? PX::kBytes : 16];
   __shared__ __attribute__((aligned(16))) char v_lds[TZ::bytes(C)];
+  __shared__ uint4 inv_lds[NT > 64 ? 2 * kMid * 64 : 1], sc_lds[OUT && NT > 64 ? 2 * kMid * 64 : 1];
   __shared__ __attribute__((aligned(16))) float gin_lds[C], gout_lds[C], beta_lds[C];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x), x = slot / a.heads;
+  const int64_t slot = blockIdx.x, x = slot / a.heads;
   const int h = int(slot % a.heads);
   const Place at = find(a, x, C * a.seg_chunks);
   if (at.none) return;
@@ -495,22 +559,21 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
   const T* vp = static_cast<const T*>(a.v) + h * a.vs_h;
   const int64_t c0 = chunk_place(a, at, at.begin);
   Stage<T, D, C, NT> ks, qs, vs;
-  ChunkFrag<kMid> inv, sc;
+  ChunkFrag<kMid, NT> inv, sc;
   float gi = 0.f, go = 0.f, be = 0.f;
   auto fetch = [&](int t0) {
     const int n = min(C, at.end - t0);
     ks.load(tid, n, a.dim_k, [&](int r) { return kp + int64_t(t0 + r) * a.ks_t; });
     if constexpr (OUT) qs.load(tid, n, a.dim_k, [&](int r) { return qp + int64_t(t0 + r) * a.qs_t; });
     vs.load(tid, n, a.dim_v, [&](int r) { return vp + int64_t(t0 + r) * a.vs_t; });
-    if (tid < C) {
-      const int64_t i = int64_t(t0 + min(tid, n - 1)) * a.heads + h;
-      gi = a.gin[i], go = a.gout[i], be = a.beta[i];
-    }
-    const int64_t c = ((c0 + (t0 - at.begin) / C) * a.heads + h) * (2 * kMid * 64) + lane;
-    inv.load(a.inv + c);
-    if constexpr (OUT) sc.load(a.score + c);
+    const int64_t i = int64_t(t0 + min(tid & (C - 1), n - 1)) * a.heads + h;      // all waves: no branch between loads
+    gi = a.gin[i], go = a.gout[i], be = a.beta[i];
+    const int64_t c = ((c0 + (t0 - at.begin) / C) * a.heads + h) * (2 * kMid * 64);
+    inv.load(a.inv + c, tid);
+    if constexpr (OUT) sc.load(a.score + c, tid);
   };
   if (at.begin < at.end) fetch(at.begin);
+  if constexpr (OUT) no_stores<MODE == kTrain ? 20 : 4>(a.out);
   for (int t0 = at.begin; t0 < at.end; t0 += C) {
     const int len = min(C, at.end - t0);
     ks.clip(tid, len, a.dim_k);
@@ -520,8 +583,10 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
     store_parts<kIn>(ks, tid, k_lds);
     if constexpr (OUT) store_parts<kIn>(qs, tid, q_lds);
     vs.store(tid, v_lds);
+    inv.store(inv_lds, tid);
+    if constexpr (OUT) sc.store(sc_lds, tid);
+    const ChunkFrag<kMid, NT> now = inv, scn = sc;
     if (tid < C) gin_lds[tid] = gi, gout_lds[tid] = go, beta_lds[tid] = tid < len ? be : 0.f;
-    const ChunkFrag<kMid> now = inv, scn = sc;
     __syncthreads();
     if (t0 + C < at.end) fetch(t0 + C);
 
@@ -548,13 +613,13 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
     F32x16 e = zero16();
     if (!odd_values(w)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) e = mul(now.get(t), split_regs<kMid>(w, t), e);
+      for (int t = 0; t < 2; ++t) e = mul(now.get(inv_lds, t, lane), split_regs<kMid>(w, t), e);
     } else {
       F32x16 seen = zero16();
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Marked<kMid> y = marked<kMid>(w, t, half, col);
-        e = mul(now.get(t), y.finite, e);
+        e = mul(now.get(inv_lds, t, lane), y.finite, e);
         seen = Mat<__bf16>::mma(y.up, y.odd, seen);
       }
 #pragma unroll
@@ -564,12 +629,10 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
     float u[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) u[r] = e[r];
-    if (MODE == kTrain && z < a.dim_v) {
+    if constexpr (MODE == kTrain) {
+      const Rows to = rows_at(a.e + (int64_t(t0) * a.heads + h) * a.dim_v, len, a.heads * a.dim_v, a.dim_v);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = acc_row(r, half);
-        if (i < len) a.e[(int64_t(t0 + i) * a.heads + h) * a.dim_v + z] = e[r];
-      }
+      for (int r = 0; r < 16; ++r) put<float>(to, acc_row(r, half), z, z < a.dim_v, e[r]);
     }
     by_token(u, beta_lds, half);
     if constexpr (OUT) {
@@ -578,21 +641,25 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
       for (int r = 0; r < 16; ++r) o[r] *= f;
       if (!odd_values(u)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) o = mul(split_regs<kMid>(u, t), scn.get(t), o);
+        for (int t = 0; t < 2; ++t) o = mul(split_regs<kMid>(u, t), scn.get(sc_lds, t, lane), o);
       } else {
         F32x16 seen = zero16();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const Marked<kMid> y = marked<kMid>(u, t, half, col);
-          o = mul(y.finite, scn.get(t), o);
+          o = mul(y.finite, scn.get(sc_lds, t, lane), o);
           seen = Mat<__bf16>::mma(y.odd, y.up, seen);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (seen[r] > 0.f) o[r] = NAN;
       }
-      if (col < len)
-        store_block<T>(static_cast<T*>(a.out) + (int64_t(t0 + col) * a.heads + h) * a.dim_v, o, 1.f, wave, a.dim_v, half);
+      const Rows to = rows_at(static_cast<T*>(a.out) + (int64_t(t0) * a.heads + h) * a.dim_v, len, a.heads * a.dim_v, a.dim_v);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * wave + 8 * g + 4 * half;
+        put4<T>(to, col, d, d < a.dim_v, o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+      }
     }
     by_token(u, gout_lds, half);
 #pragma unroll
@@ -610,22 +677,38 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
     if (own) {
 #pragma unroll
       for (int b = 0; b < XB; ++b) store_state(m[b], a.state + sx * per, b, z, half, a.dim_k, a.dim_v);
-    } else {                                     // M, as the carries' operands: row-major, and transposed as the registers stand
-      __bf16* mf = a.map_f + sx * (kMid * D * D);
-      uint4* mb = a.map_b ? a.map_b + sx * (kMid * D * D / 8) : nullptr;
+    }
+    __syncthreads();                             // the tile of keys is no longer read
+    if (!own) {                                  // M as the carries' operands, by blocks of its rows and steps over its columns
+      const int w = wave % XB;
+      uint4* mf = a.map_f + sx * (kMid * D * D / 8) + lane;
+      uint4* mb = a.map_b ? a.map_b + sx * (kMid * D * D / 8) + lane : nullptr;
+      __bf16* mine = reinterpret_cast<__bf16*>(k_lds) + w * 1024;          // a 32 x 32 block, the wave's own
 #pragma unroll
-      for (int b = 0; b < XB; ++b)
+      for (int b = 0; b < XB; ++b) {
+        Split<kMid> s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const Split<kMid> s = split_regs<kMid>(m[b], t);
+          s[t] = split_regs<kMid>(m[b], t);
+          if (mb) {                              // M^T's rows are the lanes' columns: as the registers stand
 #pragma unroll
-          for (int n = 0; n < kMid; ++n) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mf[(n * D + 32 * b + 16 * t + acc_row(j, half)) * D + z] = s.p[n][j];
-            // of the block of M^T's rows `z`: steps over M's rows
-            if (mb) mb[(((wave % XB) * 2 * XB + 2 * b + t) * kMid + n) * 64 + lane] = __builtin_bit_cast(uint4, s.p[n]);
+            for (int n = 0; n < kMid; ++n) mb[((w * 2 * XB + 2 * b + t) * kMid + n) * 64] = __builtin_bit_cast(uint4, s[t].p[n]);
           }
         }
+#pragma unroll
+        for (int n = 0; n < kMid; ++n) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mine[acc_row(r, half) * 32 + col] = s[r / 8].p[n][r % 8];
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint2 lo = *reinterpret_cast<const uint2*>(mine + col * 32 + 16 * t + 4 * half);
+            const uint2 hi = *reinterpret_cast<const uint2*>(mine + col * 32 + 16 * t + 8 + 4 * half);
+            mf[((b * 2 * XB + 2 * w + t) * kMid + n) * 64] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
     }
   } else if (last && a.final_state) {
     float* fs = a.final_state + (int64_t(at.seq) * a.heads + h) * per;
@@ -635,74 +718,80 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, MODE == kMaps && D == 
 }
 
 // ---------------------------------------------------------------- states from segment to segment
-// A workgroup a (sequence, head): wave (b, w) forms block (rows 32 b, columns 32 w) of M S + B, with its rows of M on their
-// way a segment ahead; the blocks of S pass through LDS as operands. BACK: from the last segment, with M^T.
+// A workgroup 32 columns of a (sequence, head)'s state: wave b forms rows 32 b of M S + B. Its rows of M and of B are on their way
+// two segments ahead; the blocks of S pass through LDS as operands. BACK: from the last segment, with M^T.
 template <typename T, int D, bool BACK>
-__global__ __launch_bounds__(D * D / 16) void delta_carry(const DeltaArgs a) {
+__global__ __launch_bounds__(2 * D) void delta_carry(const DeltaArgs a) {
   constexpr int XB = D / 32, kMid = DeltaParts<T>::kMid, kSteps = 2 * XB;
-  __shared__ __attribute__((aligned(16))) uint4 s_lds[XB][kSteps][kMid][64];        // by columns' block, step
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int b = wave / XB, w = wave % XB, z = 32 * w + col;
-  const int h = int(blockIdx.x % a.heads);
+  __shared__ uint4 s_lds[2][kSteps][kMid][64];
+  const int tid = threadIdx.x, lane = tid & 63, b = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int z = 32 * int(blockIdx.x % XB) + col;
+  const int64_t unit = blockIdx.x / XB, units = gridDim.x / XB;
+  const int h = int(unit % a.heads);
   const int64_t per = int64_t(a.dim_k) * a.dim_v;
   const int seg = C * a.seg_chunks;
-  for (int64_t seq = blockIdx.x / a.heads; seq < a.n_seq; seq += gridDim.x / a.heads) {
+  for (int64_t seq = unit / a.heads; seq < a.n_seq; seq += units / a.heads) {
     const int from = clamped(a, seq), to = max(clamped(a, seq + 1), from);
     const int64_t x0 = from / seg + seq;
     const int n = max((to - from + seg - 1) / seg, 1);
-    F32x16 m;
-    load_state(m, !BACK && a.init ? a.init + (seq * a.heads + h) * per : nullptr, b, z, half, a.dim_k, a.dim_v);
-    BFrag mp[kSteps][kMid];
-    auto fetch = [&](int i) {
-      const int64_t sx = (x0 + i) * a.heads + h;
+    auto place_of = [&](int k) { return (x0 + (BACK ? n - 1 - k : k)) * a.heads + h; };
+    float* states = BACK ? a.dstate : a.state;
+    const uint4* maps = (BACK ? a.map_b : a.map_f) + b * kSteps * kMid * 64 + lane;
+    // the last segment visited hands nothing on; backwards the first one visited is begun from 0 and has no map
+    struct Ahead {
+      uint4 map[kSteps][kMid];
+      F32x16 part;
+    } ahead[2];
+    auto fetch = [&](int k, Ahead& to) {
+      if (k + 1 >= n) return;
+      const int64_t sx = place_of(k);
+      load_state(to.part, states + sx * per, b, z, half, a.dim_k, a.dim_v);
+      if (BACK && k == 0) return;
+      const uint4* p = maps + sx * (kMid * D * D / 8);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-        for (int p = 0; p < kMid; ++p) {
-          if constexpr (BACK) {
-            mp[s][p] = __builtin_bit_cast(BFrag, a.map_b[sx * (kMid * D * D / 8) + ((b * kSteps + s) * kMid + p) * 64 + lane]);
-          } else {
-            typedef __bf16 V4 __attribute__((ext_vector_type(4)));
-            const __bf16* r = a.map_f + sx * (kMid * D * D) + (p * D + 32 * b + col) * D + 16 * s + 4 * half;
-            const V4 lo = *reinterpret_cast<const V4*>(r), hi = *reinterpret_cast<const V4*>(r + 8);
-            mp[s][p] = BFrag{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          }
-        }
+        for (int x = 0; x < kMid; ++x) to.map[s][x] = p[(s * kMid + x) * 64];
     };
-    // the last segment visited hands nothing on; backwards the first one visited begins from 0
-    for (int k = 0; k < n; ++k) {
-      const int i = BACK ? n - 1 - k : k;
-      float* own = (BACK ? a.dstate : a.state) + ((x0 + i) * a.heads + h) * per;
-      const bool on = k + 1 < n, mapped = on && !(BACK && k == 0);
-      F32x16 next = zero16();
-      if (on) load_state(next, own, b, z, half, a.dim_k, a.dim_v);
-      if (mapped) fetch(i);
-      store_state(m, own, b, z, half, a.dim_k, a.dim_v);
-      if (mapped) {
+    F32x16 m;
+    load_state(m, !BACK && a.init ? a.init + (seq * a.heads + h) * per : nullptr, b, z, half, a.dim_k, a.dim_v);
+    auto step = [&](int k, Ahead& mine) {
+      store_state(m, states + place_of(k) * per, b, z, half, a.dim_k, a.dim_v);
+      if (k + 1 >= n) return;
+      F32x16 sum = mine.part;
+      if (!(BACK && k == 0)) {
+        uint4(*lds)[kMid][64] = s_lds[k & 1];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const Split<kMid> s = split_regs<kMid>(m, t);
 #pragma unroll
-          for (int p = 0; p < kMid; ++p) s_lds[w][2 * b + t][p][lane] = __builtin_bit_cast(uint4, s.p[p]);
+          for (int p = 0; p < kMid; ++p) lds[2 * b + t][p][lane] = __builtin_bit_cast(uint4, s.p[p]);
         }
-        __syncthreads();
+        __syncthreads();                         // one a segment: the other half of s_lds is written next
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
           Split<kMid> f, g;
 #pragma unroll
-          for (int p = 0; p < kMid; ++p) f.p[p] = mp[s][p], g.p[p] = __builtin_bit_cast(BFrag, s_lds[w][s][p][lane]);
-          next = mul(f, g, next);
+          for (int p = 0; p < kMid; ++p) f.p[p] = __builtin_bit_cast(BFrag, mine.map[s][p]), g.p[p] = __builtin_bit_cast(BFrag, lds[s][p][lane]);
+          sum = mul(f, g, sum);
         }
-        __syncthreads();
       }
-      m = next;
+      m = sum;
+      fetch(k + 2, mine);
+    };
+    fetch(0, ahead[0]);
+    fetch(1, ahead[1]);
+    for (int k = 0; k < n; k += 2) {
+      step(k, ahead[0]);
+      if (k + 1 < n) step(k + 1, ahead[1]);
     }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------- the backward pass over a segment: z, dv
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
+__global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_back(const DeltaArgs a) {
   constexpr int NW = D / 32, NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
   using PX = PartTile<kIn, D>;
@@ -710,9 +799,10 @@ __global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
   __shared__ __attribute__((aligned(16))) char k_lds[PX::kBytes];
   __shared__ __attribute__((aligned(16))) char q_lds[PX::kBytes];
   __shared__ __attribute__((aligned(16))) char g_lds[TZ::bytes(C)];
+  __shared__ uint4 inv_lds[NT > 64 ? 2 * kMid * 64 : 1], sc_lds[NT > 64 ? 2 * kMid * 64 : 1];
   __shared__ __attribute__((aligned(16))) float gin_lds[C], gout_lds[C], beta_lds[C];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x), x = slot / a.heads;
+  const int64_t slot = blockIdx.x, x = slot / a.heads;
   const int h = int(slot % a.heads);
   const Place at = find(a, x, C * a.seg_chunks);
   if (at.none) return;
@@ -733,23 +823,22 @@ __global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
   const T* gp = static_cast<const T*>(a.dout) + int64_t(h) * a.dim_v;
   const int64_t c0 = chunk_place(a, at, at.begin), gs_t = int64_t(a.heads) * a.dim_v;
   Stage<T, D, C, NT> ks, qs, gs;
-  ChunkFrag<kMid> inv, sc;
+  ChunkFrag<kMid, NT> inv, sc;
   float gi = 0.f, go = 0.f, be = 0.f;
   auto fetch = [&](int t0) {
     const int n = min(C, at.end - t0);
     ks.load(tid, n, a.dim_k, [&](int r) { return kp + int64_t(t0 + r) * a.ks_t; });
     qs.load(tid, n, a.dim_k, [&](int r) { return qp + int64_t(t0 + r) * a.qs_t; });
     gs.load(tid, n, a.dim_v, [&](int r) { return gp + int64_t(t0 + r) * gs_t; });
-    if (tid < C) {
-      const int64_t i = int64_t(t0 + min(tid, n - 1)) * a.heads + h;
-      gi = a.gin[i], go = a.gout[i], be = a.beta[i];
-    }
-    const int64_t c = ((c0 + (t0 - at.begin) / C) * a.heads + h) * (2 * kMid * 64) + lane;
-    inv.load(a.inv_t + c);
-    sc.load(a.score_t + c);
+    const int64_t i = int64_t(t0 + min(tid & (C - 1), n - 1)) * a.heads + h;      // all waves: no branch between loads
+    gi = a.gin[i], go = a.gout[i], be = a.beta[i];
+    const int64_t c = ((c0 + (t0 - at.begin) / C) * a.heads + h) * (2 * kMid * 64);
+    inv.load(a.inv_t + c, tid);
+    sc.load(a.score_t + c, tid);
   };
   const int chunks = (at.end - at.begin + C - 1) / C;
   if (chunks > 0) fetch(at.begin + (chunks - 1) * C);
+  if constexpr (MODE == kBack) no_stores<32>(a.dv);
   for (int c = chunks - 1; c >= 0; --c) {
     const int t0 = at.begin + c * C, len = min(C, at.end - t0);
     ks.clip(tid, len, a.dim_k);
@@ -759,8 +848,10 @@ __global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
     store_parts<kIn>(ks, tid, k_lds);
     store_parts<kIn>(qs, tid, q_lds);
     gs.store(tid, g_lds);
+    inv.store(inv_lds, tid);
+    sc.store(sc_lds, tid);
+    const ChunkFrag<kMid, NT> now = inv, scn = sc;
     if (tid < C) gin_lds[tid] = gi, gout_lds[tid] = go, beta_lds[tid] = tid < len ? be : 0.f;
-    const ChunkFrag<kMid> now = inv, scn = sc;
     __syncthreads();
     if (c > 0) fetch(t0 - C);
 
@@ -783,23 +874,22 @@ __global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[8 * t + j] = y[j] = float(f[j]);
-      du = mul(scn.get(t), split<kIn>(y), du);
+      du = mul(scn.get(sc_lds, t, lane), split<kIn>(y), du);
     }
     F32x16 zz = zero16();
 #pragma unroll
-    for (int t = 0; t < 2; ++t) zz = mul(now.get(t), split_regs<kMid>(du, t), zz);
+    for (int t = 0; t < 2; ++t) zz = mul(now.get(inv_lds, t, lane), split_regs<kMid>(du, t), zz);
 #pragma unroll
     for (int r = 0; r < 16; ++r) w[r] = zz[r];
     by_token(w, beta_lds, half);
-    if (MODE == kBack && z < a.dim_v) {
+    if constexpr (MODE == kBack) {
+      const int64_t o = (int64_t(t0) * a.heads + h) * a.dim_v;
+      const Rows to_z = rows_at(a.z + o, len, a.heads * a.dim_v, a.dim_v);
+      const Rows to_v = rows_at(static_cast<T*>(a.dv) + o, len, a.heads * a.dim_v, a.dim_v);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int i = acc_row(r, half);
-        const int64_t o = (int64_t(t0 + i) * a.heads + h) * a.dim_v + z;
-        if (i < len) {
-          a.z[o] = zz[r];
-          static_cast<T*>(a.dv)[o] = T(w[r]);
-        }
+        put<float>(to_z, acc_row(r, half), z, z < a.dim_v, zz[r]);
+        put<T>(to_v, acc_row(r, half), z, z < a.dim_v, w[r]);
       }
     }
     if (MODE == kBack && c == 0) break;            // nobody reads the state's gradient before the segment
@@ -832,7 +922,7 @@ __global__ __launch_bounds__(2 * D, 1) void delta_back(const DeltaArgs a) {
 // its columns are the values' values. BACK false: dq, dk' and db from the state before the segment on; true: dk", and from all of
 // them the gates', from the gradient behind the segment back.
 template <typename T, int D, bool BACK>
-__global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
+__global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(const DeltaArgs a) {
   constexpr int NW = D / 32, NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
   using PX = PartTile<kIn, D>;
@@ -845,7 +935,7 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
   __shared__ __attribute__((aligned(16))) float gin_lds[C], gout_lds[C], beta_lds[C], g2_lds[C];
   __shared__ float sum_lds[NW][C];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int64_t slot = xcd_slot(blockIdx.x, gridDim.x), x = slot / a.heads;
+  const int64_t slot = blockIdx.x, x = slot / a.heads;
   const int h = int(slot % a.heads);
   const Place at = find(a, x, C * a.seg_chunks);
   if (at.none) return;
@@ -909,10 +999,8 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
     gs.load(tid, n, a.dim_v, [&](int r) { return gp + int64_t(t0 + r) * row_v; });
     es.load(tid, n, a.dim_v, [&](int r) { return ep + int64_t(t0 + r) * row_v; });
     zs.load(tid, n, a.dim_v, [&](int r) { return zp + int64_t(t0 + r) * row_v; });
-    if (tid < C) {
-      const int64_t i = int64_t(t0 + min(tid, n - 1)) * a.heads + h;
-      gi = a.gin[i], go = a.gout[i], be = a.beta[i], g2 = a.g2[i];
-    }
+    const int64_t i = int64_t(t0 + min(tid & (C - 1), n - 1)) * a.heads + h;
+    gi = a.gin[i], go = a.gout[i], be = a.beta[i], g2 = a.g2[i];
   };
   const int chunks = (at.end - at.begin + C - 1) / C;
   auto begin_of = [&](int c) { return at.begin + (BACK ? chunks - 1 - c : c) * C; };
@@ -932,13 +1020,14 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
     store_parts<kMid>(zs, tid, z_lds);
     if constexpr (!BACK) {                       // db: a row's chunks are neighbouring lanes
       using S = Stage<float, D, C, NT>;
+      const Rows to = rows_at(a.dbeta + int64_t(t0) * a.heads + h, len, a.heads, 1);
 #pragma unroll
       for (int i = 0; i < S::kN; ++i) {
         const float4 y = __builtin_bit_cast(float4, es.r[i]), w = __builtin_bit_cast(float4, zs.r[i]);
         float s = y.x * w.x + y.y * w.y + y.z * w.z + y.w * w.w;
         for (int o = 1; o < S::kChunks; o <<= 1) s += __shfl_xor(s, o, 64);
-        const int n = i * NT + tid, r = n / S::kChunks;
-        if (n % S::kChunks == 0 && r < len) a.dbeta[int64_t(t0 + r) * a.heads + h] = s;
+        const int n = i * NT + tid;
+        put<float>(to, n / S::kChunks, 0, n % S::kChunks == 0, s);
       }
     }
     __syncthreads();
@@ -1007,7 +1096,12 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
       }
     }
     // results: a lane has a token's values 32 wave + 8 g + 4 half + (0 .. 3)
-    const int64_t row = int64_t(t0 + min(col, len - 1)) * row_k + int64_t(h) * a.dim_k;
+    const int64_t at0 = int64_t(t0) * row_k + int64_t(h) * a.dim_k;
+    // with value heads that share a key head the sums over them follow
+    const Rows wide = rows_at((BACK || !a.dq32 ? a.dk32 : a.dq32) + at0, a.dq32 ? len : 0, int(row_k), a.dq32 ? a.dim_k : 0);
+    const Rows narrow = rows_at((BACK ? static_cast<T*>(a.dk) : static_cast<T*>(a.dq)) + (a.dq32 ? 0 : at0), a.dq32 ? 0 : len, int(row_k),
+                                a.dq32 ? 0 : a.dim_k);
+    const Rows reader = rows_at(a.dk32 + at0, len, int(row_k), a.dim_k);
     float dot = 0.f;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -1018,22 +1112,19 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         dot += BACK ? -kv[j] * o1[4 * g + j] : qv[j] * o1[4 * g + j] + kv[j] * o2[4 * g + j];
-      if (col >= len || d >= a.dim_k) continue;
+      const bool in = d < a.dim_k;
+      float x[4] = {o1[4 * g], o1[4 * g + 1], o1[4 * g + 2], o1[4 * g + 3]};
       if constexpr (!BACK) {
-        *reinterpret_cast<float4*>(a.dk32 + row + d) = make_float4(o2[4 * g], o2[4 * g + 1], o2[4 * g + 2], o2[4 * g + 3]);
-        if (a.dq32)
-          *reinterpret_cast<float4*>(a.dq32 + row + d) = make_float4(o1[4 * g], o1[4 * g + 1], o1[4 * g + 2], o1[4 * g + 3]);
-        else
-          store4<T>(dq_out + row + d, o1[4 * g], o1[4 * g + 1], o1[4 * g + 2], o1[4 * g + 3]);
+        put4<float>(reader, col, d, in, o2[4 * g], o2[4 * g + 1], o2[4 * g + 2], o2[4 * g + 3]);
       } else {
-        const float4 y = *reinterpret_cast<const float4*>(a.dk32 + row + d);
-        const float4 s = make_float4(y.x + o1[4 * g], y.y + o1[4 * g + 1], y.z + o1[4 * g + 2], y.w + o1[4 * g + 3]);
-        if (a.dq32)
-          *reinterpret_cast<float4*>(a.dk32 + row + d) = s;
-        else
-          store4<T>(dk_out + row + d, s.x, s.y, s.z, s.w);
+        const float4 y = *reinterpret_cast<const float4*>(a.dk32 + at0 + min(col, len - 1) * row_k + min(d, a.dim_k - 4));
+        x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
       }
+      put4<float>(wide, col, d, in, x[0], x[1], x[2], x[3]);
+      put4<T>(narrow, col, d, in, x[0], x[1], x[2], x[3]);
     }
+    float before = 0.f;                          // what the other pass found of the gate's
+    if constexpr (BACK) before = a.dgate[int64_t(t0 + min(col, len - 1)) * a.heads + h];
     dot += __shfl_xor(dot, 32, 64);
     if (half == 0) sum_lds[wave][col] = dot;
     // the state
@@ -1075,23 +1166,20 @@ __global__ __launch_bounds__(2 * D, 1) void delta_grad(const DeltaArgs a) {
       }
     }
     __syncthreads();
-    if (wave == 0) {
-      float s = 0.f;
-      for (int w = 0; w < NW; ++w) s += sum_lds[w][col];
-      const int64_t o = int64_t(t0 + min(col, len - 1)) * a.heads + h;
-      if constexpr (!BACK) {
-        if (half == 0 && col < len) a.dgate[o] = s;
-      } else {                                   // the sum from the token to the chunk's end, and behind it
-        s = col < len ? s + a.dgate[o] : 0.f;
-        for (int n = 1; n < C; n <<= 1) {
-          const float y = __shfl_down(s, n, 32);
-          if (col + n < C) s += y;
-        }
-        s += running;
-        if (half == 0 && col < len) a.dgate[o] = s;
-        running = __shfl(s, 0, 64);
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s += sum_lds[w][col];
+    if constexpr (BACK) {                        // the sum from the token to the chunk's end, and behind it
+      s = col < len ? s + before : 0.f;
+#pragma unroll
+      for (int n = 1; n < C; n <<= 1) {
+        const float y = __shfl_down(s, n, 32);
+        if (col + n < C) s += y;
       }
+      s += running;
+      running = __shfl(s, 0, 64);
     }
+    put<float>(rows_at(a.dgate + int64_t(t0) * a.heads + h, len, a.heads, 1), col, 0, tid < C, s);
   }
 }
 
@@ -1190,7 +1278,7 @@ template <typename F> int with_delta_pad(const DeltaArgs& a, F&& f) {
 dim3 carry_grid(const DeltaArgs& a) {
   int64_t seqs = 1 + 2048 / a.heads;
   if (seqs > a.n_seq) seqs = a.n_seq;
-  return dim3(unsigned(seqs * a.heads));
+  return dim3(unsigned(seqs * a.heads * (delta_pad(a.dim_k, a.dim_v) / 32)));
 }
 
 }  // namespace
@@ -1211,7 +1299,7 @@ template <typename T> int DeltaLaunch<T>::forward(const DeltaArgs& a, hipStream_
     if (a.carried) {
       BF_LAUNCH("delta_maps", (delta_pass<T, D, kMaps>), grid, dim3(4 * D), 0, st, a);
       BF_CHECK_LAUNCH();
-      BF_LAUNCH("delta_carry", (delta_carry<T, D, false>), carry_grid(a), dim3(D * D / 16), 0, st, a);
+      BF_LAUNCH("delta_carry", (delta_carry<T, D, false>), carry_grid(a), dim3(2 * D), 0, st, a);
       BF_CHECK_LAUNCH();
     }
     auto pass = a.e ? delta_pass<T, D, kTrain> : delta_pass<T, D, kForward>;
@@ -1228,7 +1316,7 @@ template <typename T> int DeltaLaunch<T>::backward(const DeltaArgs& a, hipStream
     if (a.carried) {
       BF_LAUNCH("delta_back_maps", (delta_back<T, D, kBackMaps>), grid, dim3(2 * D), 0, st, a);
       BF_CHECK_LAUNCH();
-      BF_LAUNCH("delta_back_carry", (delta_carry<T, D, true>), carry_grid(a), dim3(D * D / 16), 0, st, a);
+      BF_LAUNCH("delta_back_carry", (delta_carry<T, D, true>), carry_grid(a), dim3(2 * D), 0, st, a);
       BF_CHECK_LAUNCH();
     }
     BF_LAUNCH("delta_back", (delta_back<T, D, kBack>), grid, dim3(2 * D), 0, st, a);

@@ -13,8 +13,8 @@ int check(const bf_gated_delta* p, const char* fn, bool step) {
       set_error("%s: head dims (%d, %d) (multiples of 8 up to 128 are supported)", fn, p->dim_k, p->dim_v);
       return BF_ERR_UNSUPPORTED;
     }
-  BF_CHECK_ARG(p->heads >= 1 && p->heads <= (1 << 20) && p->heads_k >= 1 && p->heads % p->heads_k == 0,
-               "%s: %d value heads over %d key heads (a multiple expected, up to 2^20)", fn, p->heads, p->heads_k);
+  BF_CHECK_ARG(p->heads >= 1 && p->heads <= (1 << 16) && p->heads_k >= 1 && p->heads % p->heads_k == 0,
+               "%s: %d value heads over %d key heads (a multiple expected, up to 2^16)", fn, p->heads, p->heads_k);
   BF_CHECK_ARG(p->n >= 0 && p->n < kMaxRows && p->n_seq >= 0 && p->n_seq < kMaxRows, "%s: bad sizes (%lld rows, %lld sequences)", fn,
                (long long)p->n, (long long)p->n_seq);
   BF_CHECK_ARG(p->scale == p->scale && p->scale <= 3e38f && p->scale >= -3e38f, "%s: scale %g", fn, double(p->scale));
@@ -33,15 +33,32 @@ int check(const bf_gated_delta* p, const char* fn, bool step) {
   return BF_OK;
 }
 
-// Chunks of a segment: so many that some 512 workgroups share a call, at least 4 (a segment's own contribution and its
-// map are as much work as its tokens) and at most 64.
-int seg_chunks(const bf_gated_delta* p) {
-  const int64_t n = ceil_div(p->n * p->heads, int64_t(512) * kDeltaChunk);
-  return int(n < 4 ? 4 : n > 64 ? 64 : n);
+// Chunks of a segment (4 to 64), by what a call with them takes: its passes (two with maps, eight that train: six and one of
+// them maps) cost a workgroup's chunks and some two more for its start, of all workgroups by 256 CUs, and the wait of its own
+// chunks one behind the other; the carry a step a segment of the longest sequence. Measured, in us: a pass of 512 workgroups of 8
+// chunks of 16 heads of 128 takes 54.7, 256 of 16 62.4, 1024 of 4 61; of 8 heads of 64 over 17,900 tokens 68.7, 100 and 74.7 of as
+// many chunks; a step of the carry 2.7. Sequences that fit a segment each need no maps and no carry.
+int seg_chunks(const bf_gated_delta* p, bool train) {
+  const int d = delta_pad(p->dim_k, p->dim_v);
+  const double work = d == 128 ? 2.1 : 1.5, wait = d == 128 ? 1.5 : 4.0;
+  const double chunks = double(p->n) / kDeltaChunk, longest = double(p->longest > 0 ? p->longest : p->n) / kDeltaChunk;
+  int best = 4;
+  double least = 1e30;
+  for (int len = 4; len <= 64; ++len) {
+    const double segs = chunks / len + 0.5 * double(p->n_seq), groups = (segs > double(p->n_seq) ? segs : double(p->n_seq)) * p->heads;
+    const bool whole = longest <= len;
+    const double own = whole && longest < len ? (longest > 1 ? longest : 1) : len;
+    const double pass = work * groups * (own + 2) / 256 + wait * own;
+    const double steps = whole ? 0 : longest / len;
+    const double cost = pass * (train ? (whole ? 5 : 7) : (whole ? 1 : 2.2)) + steps * 2.7 * (train ? 2 : 1);
+    if (cost < least) least = cost, best = len;
+    if (whole) break;
+  }
+  return best;
 }
 
-bool carries(const bf_gated_delta* p) {
-  const int64_t seg = int64_t(seg_chunks(p)) * kDeltaChunk;
+bool carries(const bf_gated_delta* p, bool train) {
+  const int64_t seg = int64_t(seg_chunks(p, train)) * kDeltaChunk;
   return p->n > seg && !(p->longest > 0 && p->longest <= seg);
 }
 
@@ -49,35 +66,36 @@ bool carries(const bf_gated_delta* p) {
 struct Sizes {
   int64_t chunks, segs;            // places
   int64_t rows, frags, map, state;
-  explicit Sizes(const bf_gated_delta* p) {
-    const int64_t seg = int64_t(seg_chunks(p)) * kDeltaChunk, d = delta_pad(p->dim_k, p->dim_v), parts = delta_mid_parts(p->dtype);
+  int seg_len;                     // chunks
+  bool carried;
+  Sizes(const bf_gated_delta* p, bool train) : seg_len(seg_chunks(p, train)), carried(carries(p, train)) {
+    const int64_t seg = int64_t(seg_len) * kDeltaChunk, d = delta_pad(p->dim_k, p->dim_v), parts = delta_mid_parts(p->dtype);
     chunks = p->n / kDeltaChunk + p->n_seq + 1;
     segs = p->n / seg + p->n_seq + 1;
     rows = ceil_div(p->n * p->heads, int64_t(4)) * 4;
     frags = chunks * p->heads * (2 * parts * 64 * 4);
-    map = carries(p) ? segs * p->heads * (parts * d * d / 2) : 0;
-    state = carries(p) ? segs * p->heads * int64_t(p->dim_k) * p->dim_v : 0;
+    map = carried ? segs * p->heads * (parts * d * d / 2) : 0;
+    state = carried ? segs * p->heads * int64_t(p->dim_k) * p->dim_v : 0;
   }
 };
 
 int64_t kept_floats(const bf_gated_delta* p) {
-  const Sizes s(p);
+  const Sizes s(p, true);
   return 3 * s.rows + 2 * s.frags + s.map + s.state + p->n * p->heads * p->dim_v;
 }
 
 int64_t fwd_floats(const bf_gated_delta* p, bool train) {
-  const Sizes s(p);
+  const Sizes s(p, train);
   return 2 * s.frags + s.map + (train ? 0 : 3 * s.rows + s.state);
 }
 
 int64_t bwd_floats(const bf_gated_delta* p) {
-  const Sizes s(p);
+  const Sizes s(p, true);
   const int64_t keys = p->n * p->heads * p->dim_k;
   return s.state + p->n * p->heads * p->dim_v + keys * (p->heads > p->heads_k ? 2 : 1);
 }
 
-DeltaArgs make_args(const bf_gated_delta* p, const void* q, const void* k, const void* v) {
-  const Sizes s(p);
+DeltaArgs make_args(const bf_gated_delta* p, const Sizes& s, const void* q, const void* k, const void* v) {
   DeltaArgs a{};
   a.q = q, a.k = k, a.v = v;
   a.qs_t = p->q_stride[0], a.qs_h = p->q_stride[1];
@@ -87,14 +105,13 @@ DeltaArgs make_args(const bf_gated_delta* p, const void* q, const void* k, const
   a.init = p->init, a.final_state = p->final_state;
   a.n = int32_t(p->n), a.n_seq = int32_t(p->n_seq), a.heads = p->heads, a.heads_k = p->heads_k, a.group = p->heads / p->heads_k;
   a.dim_k = p->dim_k, a.dim_v = p->dim_v;
-  a.seg_chunks = seg_chunks(p), a.n_chunk = s.chunks, a.n_seg = s.segs;
+  a.seg_chunks = s.seg_len, a.n_chunk = s.chunks, a.n_seg = s.segs;
   a.scale = p->scale;
-  a.carried = carries(p);
+  a.carried = s.carried;
   return a;
 }
 
-void take_kept(DeltaArgs& a, const bf_gated_delta* p, float* f) {
-  const Sizes s(p);
+void take_kept(DeltaArgs& a, const Sizes& s, float* f) {
   a.inv_t = reinterpret_cast<uint4*>(f), f += s.frags;
   a.score_t = reinterpret_cast<uint4*>(f), f += s.frags;
   a.map_b = s.map ? reinterpret_cast<uint4*>(f) : nullptr, f += s.map;
@@ -129,15 +146,15 @@ extern "C" int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const 
   BF_CHECK_ARG(aligned16({q, k, v, out, kept, scratch}), "gated_delta_fwd: tensors and workspaces must be 16-byte aligned");
   if (p->n == 0 && !(p->final_state && p->n_seq > 0)) return BF_OK;
   BF_CHECK_ARG(scratch != nullptr, "gated_delta_fwd: no scratch (bf_gated_delta_fwd_floats)");
-  DeltaArgs a = make_args(p, q, k, v);
-  const Sizes s(p);
+  const Sizes s(p, kept != nullptr);
+  DeltaArgs a = make_args(p, s, q, k, v);
   a.out = out;
   float* f = scratch;
   a.inv = reinterpret_cast<uint4*>(f), f += s.frags;
   a.score = reinterpret_cast<uint4*>(f), f += s.frags;
-  a.map_f = reinterpret_cast<__bf16*>(f), f += s.map;
+  a.map_f = reinterpret_cast<uint4*>(f), f += s.map;
   if (kept) {
-    take_kept(a, p, kept);
+    take_kept(a, s, kept);
   } else {
     a.state = f, f += s.state;
     a.g2 = f, f += s.rows;
@@ -162,11 +179,12 @@ extern "C" int bf_gated_delta_bwd(const bf_gated_delta* p, const void* q, const 
   if (p->n == 0) return BF_OK;
   BF_CHECK_ARG(q && k && v && dout && kept && dq && dk && dv && dgate && dbeta && scratch, "gated_delta_bwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, dout, kept, dq, dk, dv, scratch}), "gated_delta_bwd: tensors and workspaces must be 16-byte aligned");
-  DeltaArgs a = make_args(p, q, k, v);
-  take_kept(a, p, const_cast<float*>(kept));
+  const Sizes s(p, true);
+  DeltaArgs a = make_args(p, s, q, k, v);
+  take_kept(a, s, const_cast<float*>(kept));
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.dgate = dgate, a.dbeta = dbeta;
   float* f = scratch;
-  a.dstate = f, f += Sizes(p).state;
+  a.dstate = f, f += s.state;
   a.z = f, f += p->n * p->heads * p->dim_v;
   a.dk32 = f, f += p->n * p->heads * p->dim_k;
   a.dq32 = a.group > 1 ? f : nullptr;
