@@ -993,7 +993,7 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
   Stage<float, D, C, NT> es, zs;
   float gi = 0.f, go = 0.f, be = 0.f, g2 = 0.f;
   auto fetch = [&](int t0) {
-    const int n = min(C, at.end - t0);
+    const int n = min(C, at.end - t0), tid = D > 32 ? fresh(threadIdx.x) : threadIdx.x;
     ks.load(tid, n, a.dim_k, [&](int r) { return kp + int64_t(t0 + r) * a.ks_t; });
     qs.load(tid, n, a.dim_k, [&](int r) { return qp + int64_t(t0 + r) * a.qs_t; });
     gs.load(tid, n, a.dim_v, [&](int r) { return gp + int64_t(t0 + r) * row_v; });
@@ -1007,6 +1007,8 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
   if (chunks > 0) fetch(begin_of(0));
   for (int c = 0; c < chunks; ++c) {
     const int t0 = begin_of(c), len = min(C, at.end - t0);
+    // formed anew each time round for wide heads: the addresses of all tiles, kept through the loop, do not fit the registers
+    const int tid = D > 32 ? fresh(threadIdx.x) : threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     ks.clip(tid, len, a.dim_k);
     qs.clip(tid, len, a.dim_k);
     gs.clip(tid, len, a.dim_v);
@@ -1033,7 +1035,6 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
     __syncthreads();
     store_parts<kMid>(es, tid, u_lds, [&](int r) { return beta_lds[r]; });
     __syncthreads();
-    if (c + 1 < chunks) fetch(begin_of(c + 1));
 
     const float whole = gin_lds[C - 1];
     // products of the chunk's rows with each other: the lane's token against the registers'
@@ -1127,6 +1128,7 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
     if constexpr (BACK) before = a.dgate[int64_t(t0 + min(col, len - 1)) * a.heads + h];
     dot += __shfl_xor(dot, 32, 64);
     if (half == 0) sum_lds[wave][col] = dot;
+    if (c + 1 < chunks) fetch(begin_of(c + 1));      // not before: the registers were the chunk's products'
     // the state
 #pragma unroll
     for (int b = 0; b < XB; ++b)
