@@ -40,7 +40,7 @@
 // workgroup keeps its heads' tables by distance in LDS (log2 units); a block of 32 rows by 32 keys that lies farther than the
 // map's reach on one side has one value a row there, which goes into the exponent's addend: only the blocks near the diagonal
 // look up a value a score. The table's gradient, the sum of dS by bucket, is formed in the dQ pass: every lane has a column of its own in
-// LDS, a float a bucket (nothing is added by two lanes, so the order is fixed), far blocks add one sum of 16. A wave's columns
+// LDS, a float a bucket (nothing is added by two lanes, so the order is fixed); far blocks' sums stay in registers. A wave's columns
 // are summed by head at the end, and the waves' sums by packed_bias_sum, in order and in 64 bits. A row's dS add up to 0, and so
 // a bucket's sum is a small difference of large ones, which a Delta that is off by P's rounding would spoil (6e-4 of the
 // gradient in bfloat16): a forward that trains with a bias multiplies P's rounding's rest too, and out and its own rest are then good to
@@ -447,9 +447,20 @@ __device__ __forceinline__ bool shrink(float (&ds)[16], int& by) {
   return true;
 }
 
-// Adds to a place of LDS that only this lane adds to: no value comes back and nothing waits.
-__device__ __forceinline__ void add_own(float* p, float x) {
-  __hip_atomic_fetch_add(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// Adds four values to a lane's own places of LDS, 64 apart by bucket: read together, written in order, and where a bucket repeats
+// the later sum goes on from the earlier one. (LDS's float atomics take some 260 cycles a wave: dQ of 256 graphs of 9 to 250
+// nodes, 8 heads of 32, 341 us with them.)
+__device__ __forceinline__ void add_four(float* cols, uint32_t buckets, float a, float b, float c, float d) {
+  float* p0 = cols + 64 * (buckets & 255u);
+  float* p1 = cols + 64 * (buckets >> 8 & 255u);
+  float* p2 = cols + 64 * (buckets >> 16 & 255u);
+  float* p3 = cols + 64 * (buckets >> 24);
+  const float r0 = *p0, r1 = *p1, r2 = *p2, r3 = *p3;
+  const float s0 = r0 + a;
+  const float s1 = (p1 == p0 ? s0 : r1) + b;
+  const float s2 = (p2 == p1 ? s1 : p2 == p0 ? s0 : r2) + c;
+  const float s3 = (p3 == p2 ? s2 : p3 == p1 ? s1 : p3 == p0 ? s0 : r3) + d;
+  *p0 = s0, *p1 = s1, *p2 = s2, *p3 = s3;
 }
 
 // ---------------------------------------------------------------- backward: dQ (and Delta)
@@ -479,7 +490,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
   int place_k = 0, end_bucket[2] = {0, 0};
   int2 places;
-  float end[2] = {0.f, 0.f};
+  float end[2] = {0.f, 0.f}, far_sum[2] = {0.f, 0.f};
   const float* mine = nullptr;
   uint32_t* map_lds = nullptr;         // the buckets of four distances in a row, a byte each
   float* cols = nullptr;               // the lane's sums by bucket, 64 apart
@@ -589,15 +600,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
         if (side == 0) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const uint32_t four = map_lds[bias_at(a, j0 + 32 * b + 8 * g + 4 * half - place_k)];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) add_own(cols + 64 * ((four >> (8 * j)) & 255u), ds[4 * g + j] * unit);
+            add_four(cols, map_lds[bias_at(a, j0 + 32 * b + 8 * g + 4 * half - place_k)], ds[4 * g] * unit, ds[4 * g + 1] * unit,
+                     ds[4 * g + 2] * unit, ds[4 * g + 3] * unit);
           }
         } else {
           float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum += ds[r];
-          add_own(cols + 64 * (side < 0 ? end_bucket[0] : end_bucket[1]), sum * unit);
+          (side < 0 ? far_sum[0] : far_sum[1]) += sum * unit;
         }
       }
       if constexpr (kUnits<T>) {
@@ -628,34 +638,41 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
   }
   if (valid) store_cols<DP>(static_cast<T*>(a.dq) + at * a.dim, dq, kUnits<T> ? ldexpf(a.scale, -lift) : a.scale, a.dim, half);
   if constexpr (BIAS) {                // the wave's sums by head of the group and bucket: of the lanes whose row is the head's
+    for (int e = 0; e < 2; ++e) cols[64 * end_bucket[e]] += far_sum[e];
     __syncthreads();
     float* part = a.bias.part + ((int64_t(tile) * NW + wave) * a.hk + h) * a.group * a.bias.buckets;
     const int first = int(a.by_group(uint32_t(w_row0))) * a.group;            // a row of head 0
-    for (int i = lane; i < a.group * a.bias.buckets; i += 64) {
-      const int g = i / a.bias.buckets, b = i - g * a.bias.buckets;
+    for (int i = lane; i < 2 * a.group * a.bias.buckets; i += 64) {           // a lane's half each
+      const int o = i >> 1, g = o / a.bias.buckets, b = o - g * a.bias.buckets;
       int from = first + g - w_row0;
       if (from < 0) from += a.group;
       const int n = from < 32 ? (31 - from) / a.group + 1 : 0;
       float sum = 0.f;
-      const float* c = cols - lane + 64 * b + from;
-      for (int k = 0, at = n ? b % n : 0; k < n; ++k) {                       // lanes of different buckets read different banks
-        sum += c[at * a.group] + c[at * a.group + 32];
-        if (++at == n) at = 0;
+      const float* c = cols - lane + 64 * b + from + 32 * (i & 1);
+      int at = n ? b % n : 0;                                                 // lanes of different buckets read different banks
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        sum += c[at * a.group];
+        at = at + 1 == n ? 0 : at + 1;
       }
-      part[i] = sum;
+      sum += __shfl_xor(sum, 1, 64);
+      if ((i & 1) == 0) part[o] = sum;
     }
   }
 }
 
-// The sums of the waves' parts, `n` of `values` each: chunks of them first (double [chunks, values]), then the chunks.
-__global__ __launch_bounds__(256) void packed_bias_sum(const float* part, int64_t n, int64_t values, double* sums) {
+// The sums of the waves' parts, `n` of `values` each: chunks of them first (double [chunks, values]), then the chunks; one chunk is all.
+__global__ __launch_bounds__(256) void packed_bias_sum(const float* part, int64_t n, int64_t values, double* sums, float* dtable) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= values) return;
   const int64_t each = (n + gridDim.y - 1) / gridDim.y, from = blockIdx.y * each, to = from + each < n ? from + each : n;
   double s = 0.0;
 #pragma unroll 8
   for (int64_t p = from; p < to; ++p) s += double(part[p * values + i]);
-  sums[blockIdx.y * values + i] = s;
+  if (gridDim.y == 1)
+    dtable[i] = float(s);
+  else
+    sums[blockIdx.y * values + i] = s;
 }
 __global__ __launch_bounds__(256) void packed_bias_last(const double* sums, int chunks, int64_t values, float* dtable) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
@@ -1300,8 +1317,9 @@ int backward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q,
   }));
   if (bias) {
     BF_LAUNCH("packed_bias_sum", packed_bias_sum, dim3(unsigned(ceil_div(values, 256)), unsigned(chunks)), dim3(256), 0, st, a.bias.part, parts,
-              values, sums);
+              values, sums, dtable);
     BF_CHECK_LAUNCH();
+    if (chunks == 1) return BF_OK;
     BF_LAUNCH("packed_bias_last", packed_bias_last, dim3(unsigned(ceil_div(values, 256))), dim3(256), 0, st, sums, chunks, values, dtable);
     BF_CHECK_LAUNCH();
   }
