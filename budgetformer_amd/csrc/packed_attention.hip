@@ -1154,8 +1154,6 @@ void set_bias(Args& a, const bf_packed_bias* b) {
   a.bias.buckets = b->buckets, a.bias.reach = b->reach, a.bias.width = 2 * b->reach + 1 + 2 * kBiasPad;
 }
 
-bool is_short(const bf_packed_attn* p, const bf_packed_bias* b) { return !b && packed_is_short(p); }
-
 // Bytes of a workgroup's values by distance; in the dQ pass of the buckets by distance and of the lanes' sums too.
 unsigned bias_bytes(const Args& a, const bf_packed_bias* b, int dq_waves) {
   if (!b) return 0;
@@ -1174,7 +1172,7 @@ template <typename F> int with_bias(const bf_packed_bias* b, F&& f) {
 }
 
 int64_t fwd_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
-  if (p->n_q == 0 || is_short(p, b)) return 0;
+  if (p->n_q == 0 || packed_is_short(p, b)) return 0;
   const int n = pieces_of(p);
   return n == 1 ? order_ints(p) : p->n_q * p->heads_q * n * (int64_t(p->head_dim) + 2);
 }
@@ -1185,7 +1183,7 @@ int forward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, 
   BF_CHECK_ARG(q && out && lse && (p->n_k == 0 || (k && v)), "packed_attn_fwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out}), "packed_attn_fwd: q, k, v and out must be 16-byte aligned");
   BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_fwd: rest and scratch must be 16-byte aligned");
-  if (is_short(p, bias)) return packed_short_fwd(p, q, k, v, out, lse, as_stream(stream));
+  if (packed_is_short(p, bias)) return packed_short_fwd(p, bias, q, k, v, out, lse, as_stream(stream));
   Args a = make_args(p, q, k, v);
   if (bias) set_bias(a, bias);
   a.o = out, a.rest = rest, a.lse = lse;
@@ -1237,19 +1235,20 @@ int dq_waves_of(const bf_packed_attn* p) {
   const int elem = p->dtype == BF_DTYPE_F32 ? 4 : 2;
   return dq_waves(elem, p->head_dim > 64 ? 128 : 64);
 }
-int64_t bias_parts(const bf_packed_attn* p) {
+int64_t bias_parts(const bf_packed_attn* p, const bf_packed_bias* b) {
+  if (packed_is_short(p, b)) return packed_short_parts(p);
   const int waves = dq_waves_of(p);
   return ceil_div(p->n_q * (p->heads_q / p->heads_k), int64_t(32 * waves)) * waves;
 }
 int bias_chunks(int64_t parts) { return int(parts < 64 ? 1 : parts < 64 * 64 ? parts / 64 : 64); }
 int64_t bias_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
   if (!b) return 0;
-  const int64_t values = int64_t(p->heads_q) * b->buckets, parts = bias_parts(p);
+  const int64_t values = int64_t(p->heads_q) * b->buckets, parts = bias_parts(p, b);
   return 2 * bias_chunks(parts) * values + ceil_div(parts * values, int64_t(4)) * 4;
 }
 
 int64_t bwd_floats(const bf_packed_attn* p, const bf_packed_bias* b) {
-  if (is_short(p, b)) return 0;
+  if (packed_is_short(p, b)) return bias_floats(p, b);
   const int n = kv_pieces_of(p);
   return bias_floats(p, b) + order_ints(p) + (n == 1 ? 0 : 2 * p->n_k * p->heads_k * p->head_dim * n);
 }
@@ -1261,11 +1260,10 @@ int backward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q,
                "packed_attn_bwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, out, dout, dq, dk, dv}), "packed_attn_bwd: tensors must be 16-byte aligned");
   BF_CHECK_ARG(aligned16({rest, scratch}), "packed_attn_bwd: rest and scratch must be 16-byte aligned");
-  if (is_short(p, bias)) return packed_short_bwd(p, q, k, v, out, lse, dout, dq, dk, dv, delta, as_stream(stream));
   BF_CHECK_ARG(!bias || (scratch && dtable), "packed_attn_bias_bwd: no scratch (bf_packed_attn_bias_bwd_floats) or no dtable");
   Args a = make_args(p, q, k, v);
   double* sums = nullptr;
-  const int64_t parts = bias_parts(p), values = bias ? int64_t(p->heads_q) * bias->buckets : 0;
+  const int64_t parts = bias ? bias_parts(p, bias) : 0, values = bias ? int64_t(p->heads_q) * bias->buckets : 0;
   const int chunks = bias_chunks(parts);
   if (bias) {
     set_bias(a, bias);
@@ -1276,7 +1274,9 @@ int backward(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q,
   a.out = out, a.rest = const_cast<void*>(rest), a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.delta = delta;
   a.lse = const_cast<float*>(lse);
   const hipStream_t st = as_stream(stream);
-  BF_CHECK_OK(with_type(p->dtype, [&](auto t) -> int {
+  const bool is_short = packed_is_short(p, bias);
+  if (is_short) BF_CHECK_OK(packed_short_bwd(p, bias, q, k, v, out, lse, dout, dq, dk, dv, delta, a.bias.part, st));
+  if (!is_short) BF_CHECK_OK(with_type(p->dtype, [&](auto t) -> int {
     using T = decltype(t);
     return with_dim(a.dim, [&](auto dp) -> int {
       return with_bias(bias, [&](auto biased) -> int {
@@ -1351,7 +1351,7 @@ extern "C" int64_t bf_packed_attn_fwd_floats(const bf_packed_attn* p) {
 }
 
 extern "C" int bf_packed_attn_rest(const bf_packed_attn* p) {
-  return check(p, "packed_attn_rest", false) == BF_OK && p->dtype != BF_DTYPE_F32 && !packed_is_short(p);
+  return check(p, "packed_attn_rest", false) == BF_OK && p->dtype != BF_DTYPE_F32 && !packed_is_short(p, nullptr);
 }
 
 extern "C" int bf_packed_attn_fwd(const bf_packed_attn* p, const void* q, const void* k, const void* v, void* out, void* rest,
@@ -1378,7 +1378,7 @@ extern "C" int64_t bf_packed_attn_bias_fwd_floats(const bf_packed_attn* p, const
 
 extern "C" int bf_packed_attn_bias_rest(const bf_packed_attn* p, const bf_packed_bias* bias) {
   return check(p, "packed_attn_bias_rest", false) == BF_OK && check_bias(p, bias, "packed_attn_bias_rest") == BF_OK &&
-         p->dtype != BF_DTYPE_F32 && !is_short(p, bias);
+         p->dtype != BF_DTYPE_F32 && !packed_is_short(p, bias);
 }
 
 extern "C" int bf_packed_attn_bias_fwd(const bf_packed_attn* p, const bf_packed_bias* bias, const void* q, const void* k, const void* v,

@@ -102,6 +102,74 @@ def test_long_sequences_in_whole_rows(hip_device, lens, causal, d, dtype):
     _case(hip_device, lens, lens, 32, 16, d, causal, dtype, seed=37)
 
 
+def _is_short(lens, k_lens, H, Hk, d, dtype, buckets):
+    """Whether the call's rows are walked by a few lanes each (16-bit types then keep no rest for the backward)."""
+    import ctypes as C
+    from budgetformer_amd import _native as N
+    code = {torch.bfloat16: N.BF_DTYPE_BF16, torch.float16: N.BF_DTYPE_F16}[dtype]
+    a = N.PackedAttn(n_q=sum(lens), n_k=sum(k_lens), heads_q=H, heads_k=Hk, head_dim=d, dtype=code, row_span=64, key_span=64, scale=1.0,
+                     longest=max(list(lens) + list(k_lens)))
+    b = N.PackedBias(table=64, map=64, positions=64, buckets=buckets.buckets, reach=buckets.reach)
+    return not N.load().bf_packed_attn_bias_rest(C.byref(a), C.byref(b))
+
+
+SHORT = [5, 1, 24, 0, 17, 8, 23, 2, 13, 7, 24, 3]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("H,Hk,d", [(8, 8, 16), (3, 3, 8), (4, 2, 24), (6, 1, 32), (2, 2, 128)])
+def test_short_sequences(hip_device, H, Hk, d, causal, dtype):
+    bf = _bf()
+    lens = [min(n, 40 * Hk // H) for n in SHORT]          # the heads of a group share a row's lanes' time
+    for buckets in (bf.RelativeBuckets(8, 16, device=hip_device), bf.RelativeBuckets.from_map([1, 0, 2], device=hip_device),
+                    bf.RelativeBuckets.from_map([(7 * x) % 13 for x in range(101)], device=hip_device)):
+        if dtype != torch.float32:
+            assert _is_short(lens, lens, H, Hk, d, dtype, buckets)
+        _case(hip_device, lens, lens, H, Hk, d, causal, dtype, buckets=buckets, seed=23)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_short_rows_and_keys_of_different_lengths(hip_device, causal, dtype):
+    _case(hip_device, [3, 9, 0, 20, 1, 12], [11, 4, 6, 0, 24, 12], 4, 4, 16, causal, dtype, seed=29)
+
+
+def test_short_tables_that_leave_no_room(hip_device):
+    """Groups times buckets past what a workgroup keeps of short sequences: whole tiles."""
+    bf = _bf()
+    buckets = bf.RelativeBuckets(64, 200, device=hip_device)
+    lens = [min(n, 2) for n in SHORT]
+    assert _is_short(lens, lens, 4, 4, 16, torch.bfloat16, buckets) and not _is_short(lens, lens, 16, 1, 16, torch.bfloat16, buckets)
+    _case(hip_device, lens, lens, 16, 1, 16, True, torch.bfloat16, buckets=buckets, seed=31)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d", [(8, 8, 16), (6, 3, 16)])
+def test_short_sequences_in_many_ranges(hip_device, H, Hk, d, dtype):
+    """More rows than the workgroups take at once: every repeat of a batch gives its rows' results, and the table's gradient is the
+    sum of theirs (a column's additions are up to some thousand, each off by 2^-24 of a sum that stays below their absolute one)."""
+    bf, times = _bf(), 600
+    lens, n = SHORT, sum(SHORT)
+    buckets = bf.RelativeBuckets(16, 40, device=hip_device)
+    q, do = (_randn(61 + i, n, H, d, dtype=dtype, dev=hip_device) for i in range(2))
+    k, v = (_randn(63 + i, n, Hk, d, dtype=dtype, dev=hip_device) for i in range(2))
+    table = _randn(65, H, 16, dev=hip_device)
+
+    def run(m):
+        seqs = bf.PackedSequences.from_lengths(lens * m, device=hip_device)
+        leaves = [x.repeat(m, 1, 1).requires_grad_(True) for x in (q, k, v)] + [table.clone().requires_grad_(True)]
+        out = bf.packed_attention(*leaves[:3], seqs, bias=leaves[3], buckets=buckets)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do.repeat(m, 1, 1))]
+
+    one, many = run(1), run(times)
+    for a, b in zip(one[:4], many[:4]):
+        assert torch.equal(b.view(times, n, *b.shape[1:]), a.expand(times, *a.shape))
+    # sums of at most 24 * 24 pairs of each sequence and repeat: of absolute values a few times the largest entry
+    size = times * float(one[4].abs().max()) + times * 12.0
+    assert float((many[4].double() - times * one[4].double()).abs().max()) <= 2.0 ** -24 * 2000 * size / 10
+
+
 def _maps():
     bf = _bf()
     return {"none": lambda dev: bf.RelativeBuckets.from_map([0], device=dev), "one": lambda dev: bf.RelativeBuckets.from_map([2, 0, 1], device=dev),
