@@ -258,8 +258,6 @@ template <typename O> __device__ __forceinline__ void clear_rows(O* p, const Pla
 }
 
 // A chunk's rows of a result, as a buffer: stores need no branch, since what lies behind the last row, or at kNowhere, is dropped.
-// (Behind a branch around a store the next wait for loads that are on their way waits for the stores as well: a pass over 17,900
-// tokens, 8 heads of 64, took 69 us so.)
 struct Rows {
   __amdgpu_buffer_rsrc_t r;
   int stride;                  // of a row, in values
@@ -925,6 +923,10 @@ template <typename T, int D, bool BACK>
 __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(const DeltaArgs a) {
   constexpr int NW = D / 32, NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
+  // The gates' gradient is a sum of differences that nearly cancel, of what follows from these operands, so they keep a part more than
+  // elsewhere; they are registers only. 17.9K tokens, 8 heads of 64, bfloat16: dlog_gate 6e-6 off instead of 3e-5, both passes 162 us
+  // instead of 147 (heads of 128: 260 instead of 226). With u and z in three parts too: 5e-6, and 212 (371), by their LDS.
+  constexpr int kFine = 3;
   using PX = PartTile<kIn, D>;
   using PM = PartTile<kMid, D>;
   __shared__ __attribute__((aligned(16))) char k_lds[PX::kBytes];
@@ -1072,7 +1074,7 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
     for (int b = 0; b < XB; ++b)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const Split<kMid> s = split_regs<kMid>(m[b], t);
+        const Split<kFine> s = split_regs<kFine>(m[b], t);
         if constexpr (BACK) {
           o1 = mul(s, PM::rows_regs(u_lds, col, 2 * b + t, half), o1);
         } else {
@@ -1089,11 +1091,11 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
       kc[t] = PX::cols(k_lds, t, wave, lane);
       if constexpr (BACK) {
         qc[t] = PX::cols(q_lds, t, wave, lane);
-        o1 = mul(qc[t], split_regs<kMid>(f, t), o1);
-        o1 = mul(kc[t], split_regs<kMid>(ee, t), o1);
+        o1 = mul(qc[t], split_regs<kFine>(f, t), o1);
+        o1 = mul(kc[t], split_regs<kFine>(ee, t), o1);
       } else {
-        o1 = mul(kc[t], split_regs<kMid>(f, t), o1);
-        o2 = mul(kc[t], split_regs<kMid>(ee, t), o2);
+        o1 = mul(kc[t], split_regs<kFine>(f, t), o1);
+        o2 = mul(kc[t], split_regs<kFine>(ee, t), o2);
       }
     }
     // results: a lane has a token's values 32 wave + 8 g + 4 half + (0 .. 3)
@@ -1154,9 +1156,9 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
           }
         }
       }
-      const Split<kMid> ksp = split<kMid>(kx);
-      Split<kMid> qsp;
-      if constexpr (BACK) qsp = split<kMid>(qx);
+      const Split<kFine> ksp = split<kFine>(kx);
+      Split<kFine> qsp;
+      if constexpr (BACK) qsp = split<kFine>(qx);
 #pragma unroll
       for (int b = 0; b < XB; ++b) {
         if constexpr (BACK) {
