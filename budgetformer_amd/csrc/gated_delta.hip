@@ -59,7 +59,7 @@ int seg_chunks(const bf_gated_delta* p, bool train) {
 
 bool carries(const bf_gated_delta* p, bool train) {
   const int64_t seg = int64_t(seg_chunks(p, train)) * kDeltaChunk;
-  return p->n > seg && !(p->longest > 0 && p->longest <= seg);
+  return p->n > seg && p->n_seq > 0 && !(p->longest > 0 && p->longest <= seg);
 }
 
 // A call's workspaces, in floats: what the backward reads (kept), what only the forward needs, what only the backward does.
@@ -78,6 +78,16 @@ struct Sizes {
     state = carried ? segs * p->heads * int64_t(p->dim_k) * p->dim_v : 0;
   }
 };
+
+// A launch's threads are counted in 32 bits.
+int check_grids(const bf_gated_delta* p, const Sizes& s, const char* fn) {
+  const int64_t most = (int64_t(1) << 32) - 1, d = delta_pad(p->dim_k, p->dim_v);
+  if (s.chunks * p->heads > most / 64 || s.segs * p->heads > most / (s.carried ? 4 * d : 2 * d) || p->n * p->heads_k * p->dim_k > 2 * (most - 1024)) {
+    set_error("%s: %lld rows in %lld sequences of %d heads are more than a launch holds", fn, (long long)p->n, (long long)p->n_seq, p->heads);
+    return BF_ERR_UNSUPPORTED;
+  }
+  return BF_OK;
+}
 
 int64_t kept_floats(const bf_gated_delta* p) {
   const Sizes s(p, true);
@@ -132,11 +142,13 @@ template <typename F> int with_launch(int32_t dtype, F&& f) {
 using namespace bf;
 
 extern "C" int64_t bf_gated_delta_kept_floats(const bf_gated_delta* p) {
-  return check(p, "gated_delta_kept_floats", false) == BF_OK ? kept_floats(p) : -1;
+  if (check(p, "gated_delta_kept_floats", false) != BF_OK) return -1;
+  return check_grids(p, Sizes(p, true), "gated_delta_kept_floats") == BF_OK ? kept_floats(p) : -1;
 }
 
 extern "C" int64_t bf_gated_delta_fwd_floats(const bf_gated_delta* p, int32_t train) {
-  return check(p, "gated_delta_fwd_floats", false) == BF_OK ? fwd_floats(p, train != 0) : -1;
+  if (check(p, "gated_delta_fwd_floats", false) != BF_OK) return -1;
+  return check_grids(p, Sizes(p, train != 0), "gated_delta_fwd_floats") == BF_OK ? fwd_floats(p, train != 0) : -1;
 }
 
 extern "C" int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, void* out, float* kept,
@@ -147,6 +159,7 @@ extern "C" int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const 
   if (p->n == 0 && !(p->final_state && p->n_seq > 0)) return BF_OK;
   BF_CHECK_ARG(scratch != nullptr, "gated_delta_fwd: no scratch (bf_gated_delta_fwd_floats)");
   const Sizes s(p, kept != nullptr);
+  BF_CHECK_OK(check_grids(p, s, "gated_delta_fwd"));
   DeltaArgs a = make_args(p, s, q, k, v);
   a.out = out;
   float* f = scratch;
@@ -169,7 +182,8 @@ extern "C" int bf_gated_delta_fwd(const bf_gated_delta* p, const void* q, const 
 }
 
 extern "C" int64_t bf_gated_delta_bwd_floats(const bf_gated_delta* p) {
-  return check(p, "gated_delta_bwd_floats", false) == BF_OK ? bwd_floats(p) : -1;
+  if (check(p, "gated_delta_bwd_floats", false) != BF_OK) return -1;
+  return check_grids(p, Sizes(p, true), "gated_delta_bwd_floats") == BF_OK ? bwd_floats(p) : -1;
 }
 
 extern "C" int bf_gated_delta_bwd(const bf_gated_delta* p, const void* q, const void* k, const void* v, const void* dout,
@@ -180,6 +194,7 @@ extern "C" int bf_gated_delta_bwd(const bf_gated_delta* p, const void* q, const 
   BF_CHECK_ARG(q && k && v && dout && kept && dq && dk && dv && dgate && dbeta && scratch, "gated_delta_bwd: bad arguments");
   BF_CHECK_ARG(aligned16({q, k, v, dout, kept, dq, dk, dv, scratch}), "gated_delta_bwd: tensors and workspaces must be 16-byte aligned");
   const Sizes s(p, true);
+  BF_CHECK_OK(check_grids(p, s, "gated_delta_bwd"));
   DeltaArgs a = make_args(p, s, q, k, v);
   take_kept(a, s, const_cast<float*>(kept));
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.dgate = dgate, a.dbeta = dbeta;

@@ -937,7 +937,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_delta_fwd(const at::Tensor&
   at::Tensor out = at::empty(v.sizes(), v.options().memory_format(at::MemoryFormat::Contiguous)), scratch;
   at::Tensor state = return_state ? at::empty({p.n_seq, p.heads, p.dim_k, p.dim_v}, log_gate.options()) : at::empty({0}, log_gate.options());
   if (return_state) p.final_state = state.data_ptr<float>();
-  const int64_t floats = bf_gated_delta_fwd_floats(&p, train ? 1 : 0), keeps = train ? bf_gated_delta_kept_floats(&p) : 0;
+  const int64_t floats = bf_gated_delta_fwd_floats(&p, train ? 1 : 0), keeps = train && floats >= 0 ? bf_gated_delta_kept_floats(&p) : 0;
   at::Tensor kept = at::empty({std::max<int64_t>(keeps, 0)}, log_gate.options());
   if (floats > 0) scratch = at::empty({floats}, log_gate.options());
   check_rc(bf_gated_delta_fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), keeps > 0 ? kept.data_ptr<float>() : nullptr,

@@ -78,6 +78,17 @@ def test_addresses_and_workspaces():
         N.call("bf_gated_delta_step", C.byref(_args()), P, P, P, P, None)               # no states
 
 
+@pytest.mark.parametrize("kw", [dict(n_seq=2 ** 27), dict(n=2 ** 30, n_seq=2 ** 30), dict(n=2 ** 30, heads=2 ** 12, heads_k=2 ** 10)])
+def test_more_than_a_launch_holds(kw):
+    lib, a = N.load(), _args(**kw)
+    with pytest.raises(NotImplementedError, match="a launch holds"):
+        _fwd(a)
+    with pytest.raises(NotImplementedError, match="a launch holds"):
+        _bwd(a)
+    assert lib.bf_gated_delta_fwd_floats(C.byref(a), 1) == lib.bf_gated_delta_kept_floats(C.byref(a)) == -1
+    assert lib.bf_gated_delta_bwd_floats(C.byref(a)) == -1
+
+
 def test_no_rows_is_no_work():
     _fwd(_args(n=0), scratch=None)
     _bwd(_args(n=0), q=None, kept=None, scratch=None)

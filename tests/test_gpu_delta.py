@@ -329,3 +329,17 @@ def test_no_tokens(hip_device):
     none = bf.PackedSequences.from_lengths([], causal=True, device=hip_device)
     out, after = bf.gated_delta_rule(*args, none, return_state=True)
     assert out.numel() == 0 and after.shape == (0, 2, 16, 16)
+
+
+@pytest.mark.parametrize("check", [True, False])
+def test_rows_of_no_sequence(hip_device, check):
+    bf = _bf()
+    *args, do = _inputs(hip_device, 2500, 2, 2, 16, 16, torch.float32, 107)
+    offsets = torch.zeros(1, dtype=torch.int32, device=hip_device)
+    seqs = bf.PackedSequences.from_offsets(offsets, n_q=2500, causal=True, check=check)
+    leaves = [x.requires_grad_(True) for x in args]
+    out, after = bf.gated_delta_rule(*leaves, seqs, return_state=True)
+    assert after.shape == (0, 2, 16, 16)
+    assert not any(bool(x.any()) for x in (out, *torch.autograd.grad(out, leaves, do)))
+    with torch.no_grad():
+        assert not bool(bf.gated_delta_rule(*args, seqs).any())
