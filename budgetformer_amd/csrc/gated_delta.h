@@ -262,7 +262,7 @@ struct Rows {
   __amdgpu_buffer_rsrc_t r;
   int stride;                  // of a row, in values
 };
-constexpr int kNowhere = 0x7ffffff0;
+constexpr int kNowhere = 0x7ffe0000;          // also with a state's bytes added
 template <typename O> __device__ __forceinline__ Rows rows_at(O* p, int len, int stride, int dim) {
   return Rows{__builtin_amdgcn_make_buffer_rsrc(p, 0, len > 0 ? ((len - 1) * stride + dim) * int(sizeof(O)) : 0, 0x20000), stride};
 }
@@ -464,23 +464,19 @@ __device__ __forceinline__ int fresh(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+// Rows 32 b .. 32 b + 31 of a state, a lane column z: as a buffer without branches, since what lies outside of it (of NULL all) reads 0 and
+// is not written. The state's address is one for the workgroup.
 __device__ __forceinline__ void load_state(F32x16& m, const float* s, int b, int z, int half, int dk, int dv) {
-  const int x0 = fresh(32 * b + 4 * half), zc = min(z, dv - 1);
+  const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(s), 0, s ? dk * dv * 4 : 0, 0x20000);
+  const int at = fresh(z < dv ? ((32 * b + 4 * half) * dv + z) * 4 : kNowhere);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int x = x0 + acc_row(r, 0);
-    const float v = s ? s[min(x, dk - 1) * dv + zc] : 0.f;
-    m[r] = x < dk && z < dv ? v : 0.f;
-  }
+  for (int r = 0; r < 16; ++r) m[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, at + acc_row(r, 0) * dv * 4, 0, 0));
 }
 __device__ __forceinline__ void store_state(const F32x16& m, float* s, int b, int z, int half, int dk, int dv) {
-  const int x0 = fresh(32 * b + 4 * half);
-  if (z >= dv) return;
+  const auto to = __builtin_amdgcn_make_buffer_rsrc(s, 0, dk * dv * 4, 0x20000);
+  const int at = fresh(z < dv ? ((32 * b + 4 * half) * dv + z) * 4 : kNowhere);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int x = x0 + acc_row(r, 0);
-    if (x < dk) s[x * dv + z] = m[r];
-  }
+  for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m[r]), to, at + acc_row(r, 0) * dv * 4, 0, 0);
 }
 
 // An infinity or NaN among a wave's values by token is the tokens' from its own on, not the ones before, which a product with the
@@ -735,16 +731,15 @@ __global__ __launch_bounds__(2 * D) void delta_carry(const DeltaArgs a) {
     auto place_of = [&](int k) { return (x0 + (BACK ? n - 1 - k : k)) * a.heads + h; };
     float* states = BACK ? a.dstate : a.state;
     const uint4* maps = (BACK ? a.map_b : a.map_f) + b * kSteps * kMid * 64 + lane;
-    // the last segment visited hands nothing on; backwards the first one visited is begun from 0 and has no map
+    // The last segment visited hands nothing on. What is on its way is counted by the waits only without branches around loads and stores,
+    // so those behind the last segment read it again.
     struct Ahead {
       uint4 map[kSteps][kMid];
       F32x16 part;
     } ahead[2];
     auto fetch = [&](int k, Ahead& to) {
-      if (k + 1 >= n) return;
-      const int64_t sx = place_of(k);
+      const int64_t sx = place_of(k < n ? k : n - 1);
       load_state(to.part, states + sx * per, b, z, half, a.dim_k, a.dim_v);
-      if (BACK && k == 0) return;
       const uint4* p = maps + sx * (kMid * D * D / 8);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
@@ -755,34 +750,46 @@ __global__ __launch_bounds__(2 * D) void delta_carry(const DeltaArgs a) {
     load_state(m, !BACK && a.init ? a.init + (seq * a.heads + h) * per : nullptr, b, z, half, a.dim_k, a.dim_v);
     auto step = [&](int k, Ahead& mine) {
       store_state(m, states + place_of(k) * per, b, z, half, a.dim_k, a.dim_v);
-      if (k + 1 >= n) return;
-      F32x16 sum = mine.part;
-      if (!(BACK && k == 0)) {
-        uint4(*lds)[kMid][64] = s_lds[k & 1];
+      F32x16 sum = zero16();
+      uint4(*lds)[kMid][64] = s_lds[k & 1];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const Split<kMid> s = split_regs<kMid>(m, t);
+      for (int t = 0; t < 2; ++t) {
+        const Split<kMid> s = split_regs<kMid>(m, t);
 #pragma unroll
-          for (int p = 0; p < kMid; ++p) lds[2 * b + t][p][lane] = __builtin_bit_cast(uint4, s.p[p]);
-        }
-        __syncthreads();                         // one a segment: the other half of s_lds is written next
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          Split<kMid> f, g;
-#pragma unroll
-          for (int p = 0; p < kMid; ++p) f.p[p] = __builtin_bit_cast(BFrag, mine.map[s][p]), g.p[p] = __builtin_bit_cast(BFrag, lds[s][p][lane]);
-          sum = mul(f, g, sum);
-        }
+        for (int p = 0; p < kMid; ++p) lds[2 * b + t][p][lane] = __builtin_bit_cast(uint4, s.p[p]);
       }
-      m = sum;
+      __syncthreads();                           // one a segment: the other half of s_lds is written next
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        Split<kMid> f, g;
+#pragma unroll
+        for (int p = 0; p < kMid; ++p) f.p[p] = __builtin_bit_cast(BFrag, mine.map[s][p]), g.p[p] = __builtin_bit_cast(BFrag, lds[s][p][lane]);
+        sum = mul(f, g, sum);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m[r] = sum[r] + mine.part[r];       // not as what is added to: the registers would change their roles
       fetch(k + 2, mine);
+      __builtin_amdgcn_sched_barrier(0);
     };
-    fetch(0, ahead[0]);
-    fetch(1, ahead[1]);
-    for (int k = 0; k < n; k += 2) {
-      step(k, ahead[0]);
-      if (k + 1 < n) step(k + 1, ahead[1]);
+    int k = 0;
+    if (BACK && n > 1) {                         // the last segment begins from 0: no map
+      F32x16 part;
+      load_state(part, states + place_of(0) * per, b, z, half, a.dim_k, a.dim_v);
+      store_state(m, states + place_of(0) * per, b, z, half, a.dim_k, a.dim_v);
+      m = part;
+      k = 1;
     }
+    if (k + 1 < n) {
+      fetch(k, ahead[0]);
+      fetch(k + 1, ahead[1]);
+      for (;;) {
+        step(k, ahead[0]);
+        if (++k + 1 >= n) break;
+        step(k, ahead[1]);
+        if (++k + 1 >= n) break;
+      }
+    }
+    store_state(m, states + place_of(k) * per, b, z, half, a.dim_k, a.dim_v);
     __syncthreads();
   }
 }
