@@ -711,20 +711,28 @@ __global__ __launch_bounds__((MODE == kMaps ? 4 : 2) * D, sizeof(T) == 2 || (MOD
   }
 }
 
+// Sequences that the carry takes at once: of some thousand workgroups at most, which take several each.
+__host__ __device__ inline int carry_seqs(const DeltaArgs& a) {
+  const int seqs = 1 + 2048 / a.heads;
+  return seqs < a.n_seq ? seqs : a.n_seq;
+}
+
 // ---------------------------------------------------------------- states from segment to segment
 // A workgroup 32 columns of a (sequence, head)'s state: wave b forms rows 32 b of M S + B. Its rows of M and of B are on their way
-// two segments ahead; the blocks of S pass through LDS as operands. BACK: from the last segment, with M^T.
+// two segments ahead; the blocks of S pass through LDS as operands. BACK: from the last segment, with M^T. The workgroups of one
+// state are 8 apart: on one XCD, whose L2 then holds M for all of them.
 template <typename T, int D, bool BACK>
 __global__ __launch_bounds__(2 * D) void delta_carry(const DeltaArgs a) {
   constexpr int XB = D / 32, kMid = DeltaParts<T>::kMid, kSteps = 2 * XB;
   __shared__ uint4 s_lds[2][kSteps][kMid][64];
   const int tid = threadIdx.x, lane = tid & 63, b = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int z = 32 * int(blockIdx.x % XB) + col;
-  const int64_t unit = blockIdx.x / XB, units = gridDim.x / XB;
-  const int h = int(unit % a.heads);
+  const int z = 32 * int(blockIdx.x / 8 % XB) + col;
+  const int64_t unit = int64_t(blockIdx.x / (8 * XB)) * 8 + blockIdx.x % 8;
+  const int step_seqs = carry_seqs(a), h = int(unit % a.heads);
+  if (unit >= int64_t(step_seqs) * a.heads) return;
   const int64_t per = int64_t(a.dim_k) * a.dim_v;
   const int seg = C * a.seg_chunks;
-  for (int64_t seq = unit / a.heads; seq < a.n_seq; seq += units / a.heads) {
+  for (int64_t seq = unit / a.heads; seq < a.n_seq; seq += step_seqs) {
     const int from = clamped(a, seq), to = max(clamped(a, seq + 1), from);
     const int64_t x0 = from / seg + seq;
     const int n = max((to - from + seg - 1) / seg, 1);
@@ -1285,11 +1293,9 @@ template <typename F> int with_delta_pad(const DeltaArgs& a, F&& f) {
   }
 }
 
-// Workgroups that hand the states on: at most some thousand, which take several sequences each.
 dim3 carry_grid(const DeltaArgs& a) {
-  int64_t seqs = 1 + 2048 / a.heads;
-  if (seqs > a.n_seq) seqs = a.n_seq;
-  return dim3(unsigned(seqs * a.heads * (delta_pad(a.dim_k, a.dim_v) / 32)));
+  const int64_t units = int64_t(carry_seqs(a)) * a.heads;
+  return dim3(unsigned(ceil_div(units, int64_t(8)) * 8 * (delta_pad(a.dim_k, a.dim_v) / 32)));
 }
 
 }  // namespace

@@ -1,4 +1,6 @@
 // The gated delta rule over packed sequences: checks, how a call is cut, workspaces (the kernels: gated_delta.h).
+#include <cmath>
+
 #include "gated_delta.h"
 
 namespace bf {
@@ -33,24 +35,42 @@ int check(const bf_gated_delta* p, const char* fn, bool step) {
   return BF_OK;
 }
 
-// Chunks of a segment (4 to 64), by what a call with them takes: its passes (two with maps, eight that train: six and one of
-// them maps) cost a workgroup's chunks and some two more for its start, of all workgroups by 256 CUs, and the wait of its own
-// chunks one behind the other; the carry a step a segment of the longest sequence. Measured, in us: a pass of 512 workgroups of 8
-// chunks of 16 heads of 128 takes 54.7, 256 of 16 62.4, 1024 of 4 61; of 8 heads of 64 over 17,900 tokens 68.7, 100 and 74.7 of as
-// many chunks; a step of the carry 2.7. Sequences that fit a segment each need no maps and no carry.
+// Workgroups of a pass that a CU holds at once, by their registers and LDS.
+int slots(int32_t dtype, int d, bool train) {
+  if (dtype == BF_DTYPE_F32) return 128 / d;
+  if (d == 32) return 8;
+  if (d == 128) return train && dtype == BF_DTYPE_F16 ? 1 : 2;
+  return train && dtype == BF_DTYPE_F16 ? 3 : 4;
+}
+
+// Chunks of a segment (2 to 64), by what a call with them takes. A pass (two with maps, six that train) takes the chunks of a workgroup
+// one behind the other; a chunk takes longer the more workgroups a CU holds, but not in proportion while they mostly wait: with
+// heads of 128 a chunk of the forward pass 3.5 us alone and 6 of two, of a pass of gradients 8.5 and 14; with heads of 64 4.7, 6, 7.6
+// and 10.4 of one to four, of gradients 8.1, 8.8 and 9.7. So what fills the chip once is best, and a workgroup more than that costs a whole
+// round; the carry takes 1.7 us (0.9) a segment of the longest sequence. In us, all passes: one sequence of 8192, 16 heads of 128,
+// bfloat16, segments of 8, 12 and 16 chunks 203, 218 and 180; nine sequences of 17.5K tokens, 8 heads of 64, float16, training, of 4, 6, 7, 8 and
+// 12 468, 426, 411, 441 and 520. Sequences that fit a segment each need no maps and no carry.
 int seg_chunks(const bf_gated_delta* p, bool train) {
-  const int d = delta_pad(p->dim_k, p->dim_v);
-  const double work = d == 128 ? 2.1 : 1.5, wait = d == 128 ? 1.5 : 4.0;
+  const int d = delta_pad(p->dim_k, p->dim_v), most = slots(p->dtype, d, train);
+  const bool equal = p->longest > 0 && p->n == p->n_seq * int64_t(p->longest);
   const double chunks = double(p->n) / kDeltaChunk, longest = double(p->longest > 0 ? p->longest : p->n) / kDeltaChunk;
-  int best = 4;
+  const double seqs = double(p->n_seq), carry = d == 128 ? 1.7 : 0.9;
+  int best = 2;
   double least = 1e30;
-  for (int len = 4; len <= 64; ++len) {
-    const double segs = chunks / len + 0.5 * double(p->n_seq), groups = (segs > double(p->n_seq) ? segs : double(p->n_seq)) * p->heads;
+  for (int len = 2; len <= 64; ++len) {
     const bool whole = longest <= len;
+    // of sequences of unknown lengths the last segments are half full, more or less
+    double segs = equal ? seqs * ceil(longest / len) : chunks / len + 0.5 * seqs;
+    if (whole || segs < seqs) segs = seqs;
+    const double groups = segs * p->heads, full = floor(groups / (256 * most));
+    const double rest = ceil((groups - full * 256 * most) / 256 - 0.1);          // a few more find room: last segments are short
+    const auto slower = [&](double at_once) {
+      return d == 128 ? 0.32 + 0.68 * at_once : d == 32 ? 0.9 + 0.1 * at_once : at_once > 3 ? 1.9 : 0.8 + 0.2 * at_once;
+    };
+    const double rounds = full * slower(most) + (rest > 0 ? slower(rest) : 0);
     const double own = whole && longest < len ? (longest > 1 ? longest : 1) : len;
-    const double pass = work * groups * (own + 2) / 256 + wait * own;
-    const double steps = whole ? 0 : longest / len;
-    const double cost = pass * (train ? (whole ? 5 : 7) : (whole ? 1 : 2.2)) + steps * 2.7 * (train ? 2 : 1);
+    const double chunk = train ? (whole ? 25 : 32) : (whole ? 4 : 7.4), start = train ? 18 : 6;
+    const double cost = rounds * own * chunk + (full + (rest > 0)) * start + (whole ? 0 : longest / len * carry * (train ? 2 : 1));
     if (cost < least) least = cost, best = len;
     if (whole) break;
   }
