@@ -295,27 +295,26 @@ template <int N> __device__ __forceinline__ void no_stores(void* p) {
 // ---------------------------------------------------------------- inverses and scores of the chunks
 __device__ __forceinline__ float finite_gate2(float g) { return (g < -150.f ? -150.f : g) * kLog2e; }      // -inf too; NaN stays
 
-template <typename T, int D> __device__ __forceinline__ Split<DeltaParts<T>::kIn> row_parts(const T* p, int at, int dim) {
-  float x[8];
-  if (p && at < dim) {
-    const Frag<T> f = *reinterpret_cast<const Frag<T>*>(p + at);
-    if constexpr (std::is_same<T, __bf16>::value) {
-      Split<1> s;
-      s.p[0] = f;
-      return s;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = float(f[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+// Eight values of a row as an operand; `in`: else zeros.
+template <typename T> __device__ __forceinline__ Split<DeltaParts<T>::kIn> row_parts(Frag<T> f, bool in) {
+  if constexpr (sizeof(T) == 2) {
+    uint4 w = __builtin_bit_cast(uint4, f);
+    f = __builtin_bit_cast(Frag<T>, in ? w : make_uint4(0, 0, 0, 0));
   }
+  if constexpr (std::is_same<T, __bf16>::value) {
+    Split<1> s;
+    s.p[0] = f;
+    return s;
+  }
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = sizeof(T) == 2 || in ? float(f[j]) : 0.f;
   return split<DeltaParts<T>::kIn>(x);
 }
 
 // A wave a (chunk, head). Lanes 0 .. 31 solve for the columns of (1 + L)^-1, the others for those of (1 + L')^-1.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void delta_prep(const DeltaArgs a) {
+__global__ __launch_bounds__(64, 4) void delta_prep(const DeltaArgs a) {
   constexpr int kMid = DeltaParts<T>::kMid, kPitch = C + 4;
   __shared__ __attribute__((aligned(16))) float l_lds[2][C][kPitch];       // L and L' by columns, then the inverses by rows
   __shared__ __attribute__((aligned(16))) double g_lds[C];
@@ -328,14 +327,28 @@ __global__ __launch_bounds__(64) void delta_prep(const DeltaArgs a) {
   const int len = at.end - at.begin;
   const bool row_in = col < len;
   const int64_t row = at.begin + min(col, len - 1);
+  // all loads at once, and without branches, which would wait for each by itself
+  const T* kp = static_cast<const T*>(a.k) + row * a.ks_t + (h / a.group) * a.ks_h;
+  const T* qp = static_cast<const T*>(a.q) + row * a.qs_t + (h / a.group) * a.qs_h;
+  constexpr int kMost = std::is_same<T, __bf16>::value ? 8 : sizeof(T) == 2 ? 4 : 2, kAhead = D / 16 < kMost ? D / 16 : kMost;
+  Frag<T> ks[kAhead], qs[kAhead];
+  auto fetch = [&](int s) {
+    const int from = min(16 * s + 8 * half, a.dim_k - 8);
+    ks[s % kAhead] = *reinterpret_cast<const Frag<T>*>(kp + from);
+    qs[s % kAhead] = *reinterpret_cast<const Frag<T>*>(qp + from);
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) fetch(s);
 
-  double g = row_in ? double(finite_gate2(a.log_gate[row * a.heads + h])) : 0.0;
+  const float gate = a.log_gate[row * a.heads + h], strength = a.beta[row * a.heads + h];
+
+  double g = row_in ? double(finite_gate2(gate)) : 0.0;
   for (int o = 1; o < C; o <<= 1) {
     const double up = __shfl_up(g, o, 32);
     if (col >= o) g += up;
   }
   const double all = __shfl(g, C - 1, 32);
-  const float beta = row_in ? a.beta[row * a.heads + h] : 0.f;
+  const float beta = row_in ? strength : 0.f;
   if (half == 0) {
     g_lds[col] = g;
     beta_lds[col] = beta;
@@ -345,13 +358,12 @@ __global__ __launch_bounds__(64) void delta_prep(const DeltaArgs a) {
       a.gout[row * a.heads + h] = exp2_fast(float(all - g));
     }
   }
-  const T* kp = row_in ? static_cast<const T*>(a.k) + row * a.ks_t + (h / a.group) * a.ks_h : nullptr;
-  const T* qp = row_in ? static_cast<const T*>(a.q) + row * a.qs_t + (h / a.group) * a.qs_h : nullptr;
   F32x16 kk = zero16(), kq = zero16(), qk = zero16();
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
-    const auto k = row_parts<T, D>(kp, 16 * s + 8 * half, a.dim_k);
-    const auto q = row_parts<T, D>(qp, 16 * s + 8 * half, a.dim_k);
+    const bool in = row_in && 16 * s + 8 * half < a.dim_k;
+    const auto k = row_parts<T>(ks[s % kAhead], in), q = row_parts<T>(qs[s % kAhead], in);
+    if (s + kAhead < D / 16) fetch(s + kAhead);
     kk = mul(k, k, kk);
     kq = mul(k, q, kq);                          // lane: the row i, registers: the columns j
     if (a.score_t) qk = mul(q, k, qk);
@@ -930,6 +942,20 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_back(cons
   }
 }
 
+template <int CTRL> __device__ __forceinline__ float add_lane(float x) {
+  return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// The sum of N lanes beside each other (8, 16 or 32), in all of them: by rows of 16 without LDS.
+template <int N> __device__ __forceinline__ float add_neighbours(float x) {
+  static_assert(N == 8 || N == 16 || N == 32, "lanes");
+  x = add_lane<0xb1>(x);                         // the other of a pair
+  x = add_lane<0x4e>(x);                         // the other pair of four
+  x = add_lane<0x141>(x);                        // the other four of eight, mirrored
+  if constexpr (N > 8) x = add_lane<0x140>(x);   // the other eight of a row
+  if constexpr (N > 16) x += __shfl_xor(x, 16, 64);
+  return x;
+}
+
 // ---------------------------------------------------------------- gradients of q and k, of gates and strengths
 // Passes of linear attention over a segment, with the state transposed: a wave owns 32 of the keys' values (a lane one), the rows of
 // its columns are the values' values. BACK false: dq, dk' and db from the state before the segment on; true: dk", and from all of
@@ -1044,7 +1070,7 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
       for (int i = 0; i < S::kN; ++i) {
         const float4 y = __builtin_bit_cast(float4, es.r[i]), w = __builtin_bit_cast(float4, zs.r[i]);
         float s = y.x * w.x + y.y * w.y + y.z * w.z + y.w * w.w;
-        for (int o = 1; o < S::kChunks; o <<= 1) s += __shfl_xor(s, o, 64);
+        s = add_neighbours<S::kChunks>(s);
         const int n = i * NT + tid;
         put<float>(to, n / S::kChunks, 0, n % S::kChunks == 0, s);
       }
@@ -1097,6 +1123,16 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
           o2 = mul(s, PM::rows_regs(z_lds, col, 2 * b + t, half), o2);
         }
       }
+    // what the other pass found, on its way while the products are formed
+    float before = 0.f;
+    float4 other_k[4];
+    if constexpr (BACK) {
+      const int64_t row = t0 + min(col, len - 1);
+      before = a.dgate[row * a.heads + h];
+      const float* from = a.dk32 + (row * a.heads + h) * a.dim_k;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) other_k[g] = *reinterpret_cast<const float4*>(from + min(32 * wave + 8 * g + 4 * half, a.dim_k - 4));
+    }
     const float by1 = BACK ? gout_lds[col] : a.scale * gin_lds[col], by2 = -beta * gin_lds[col];
 #pragma unroll
     for (int r = 0; r < 16; ++r) o1[r] *= by1, o2[r] *= by2;
@@ -1135,14 +1171,11 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(cons
       if constexpr (!BACK) {
         put4<float>(reader, col, d, in, o2[4 * g], o2[4 * g + 1], o2[4 * g + 2], o2[4 * g + 3]);
       } else {
-        const float4 y = *reinterpret_cast<const float4*>(a.dk32 + at0 + min(col, len - 1) * row_k + min(d, a.dim_k - 4));
-        x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+        x[0] += other_k[g].x, x[1] += other_k[g].y, x[2] += other_k[g].z, x[3] += other_k[g].w;
       }
       put4<float>(wide, col, d, in, x[0], x[1], x[2], x[3]);
       put4<T>(narrow, col, d, in, x[0], x[1], x[2], x[3]);
     }
-    float before = 0.f;                          // what the other pass found of the gate's
-    if constexpr (BACK) before = a.dgate[int64_t(t0 + min(col, len - 1)) * a.heads + h];
     dot += __shfl_xor(dot, 32, 64);
     if (half == 0) sum_lds[wave][col] = dot;
     if (c + 1 < chunks) fetch(begin_of(c + 1));      // not before: the registers were the chunk's products'
