@@ -130,9 +130,10 @@ template <int NA, int NB> __device__ __forceinline__ F32x16 mul(const Split<NA>&
   return acc;
 }
 
-// A tile of C rows in N parts, a bfloat16 tile each.
+// A tile of C rows in N parts, a bfloat16 tile each. (Of 32 values in parts with half the padding: a CU then holds four of float32's
+// gradient passes instead of three.)
 template <int N, int D> struct PartTile {
-  using TL = Tile<__bf16, D>;
+  using TL = Tile<__bf16, D, (D == 32 && N > 1 ? 16 : 32)>;
   static constexpr int kPart = (TL::bytes(C) + 15) / 16 * 16, kBytes = N * kPart;
   static __device__ __forceinline__ Split<N> rows(const char* lds, int row, int s, int half) {
     Split<N> f;
@@ -961,7 +962,7 @@ template <int N> __device__ __forceinline__ float add_neighbours(float x) {
 // its columns are the values' values. BACK false: dq, dk' and db from the state before the segment on; true: dk", and from all of
 // them the gates', from the gradient behind the segment back.
 template <typename T, int D, bool BACK>
-__global__ __launch_bounds__(2 * D, sizeof(T) == 2 ? 2 : 1) void delta_grad(const DeltaArgs a) {
+__global__ __launch_bounds__(2 * D, sizeof(T) == 2 && (DeltaParts<T>::kIn == 1 || D < 128) ? 2 : 1) void delta_grad(const DeltaArgs a) {
   constexpr int NW = D / 32, NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
   // The gates' gradient is a sum of differences that nearly cancel, of what follows from these operands, so they keep a part more than

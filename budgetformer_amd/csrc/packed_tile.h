@@ -149,8 +149,8 @@ template <int STEPS, typename F> __device__ __forceinline__ void add_infinite(F3
 
 // A tile of rows of DP values in LDS. Rows are padded by 32 bytes: the 4 rows of a transposing read, and the 8 rows that
 // a cycle of 16-byte reads touches, then fall on different banks.
-template <typename T, int DP> struct Tile {
-  static constexpr int kPitch = DP * int(sizeof(T)) + 32;       // bytes of a row
+template <typename T, int DP, int PAD = 32> struct Tile {
+  static constexpr int kPitch = DP * int(sizeof(T)) + PAD;      // bytes of a row
   static constexpr int kSteps = DP / 16;                        // contractions of 16 over the row
   static constexpr int kBlocks = (DP + 31) / 32;                // blocks of 32 values of the row
   // DP 16 reads columns 16 .. 31 too (values that only reach product rows nobody stores): in bounds up to this slack
