@@ -966,8 +966,9 @@ __global__ __launch_bounds__(2 * D, sizeof(T) == 2 && (DeltaParts<T>::kIn == 1 |
   constexpr int NW = D / 32, NT = 64 * NW, XB = D / 32;
   constexpr int kIn = DeltaParts<T>::kIn, kMid = DeltaParts<T>::kMid;
   // The gates' gradient is a sum of differences that nearly cancel, of what follows from these operands, so they keep a part more than
-  // elsewhere; they are registers only. 17.9K tokens, 8 heads of 64, bfloat16: dlog_gate 6e-6 off instead of 3e-5, both passes 162 us
-  // instead of 147 (heads of 128: 260 instead of 226). With u and z in three parts too: 5e-6, and 212 (371), by their LDS.
+  // elsewhere; they are registers only. 17.5K tokens, 8 heads of 64, float16, in segments of 6: dlog_gate 6e-6 off instead of 3e-5, both
+  // passes 162 us instead of 147 (5.9K tokens, 16 heads of 128, bfloat16, segments of 8: 260 instead of 226). With u and z in three parts
+  // too: 5e-6, and 212 (371), by their LDS.
   constexpr int kFine = 3;
   using PX = PartTile<kIn, D>;
   using PM = PartTile<kMid, D>;
