@@ -46,15 +46,19 @@ int slots(int32_t dtype, int d, bool train) {
 // Chunks of a segment (2 to 64), by what a call with them takes. A pass (two with maps, six that train) takes the chunks of a workgroup
 // one behind the other; a chunk takes longer the more workgroups a CU holds, but not in proportion while they mostly wait: with
 // heads of 128 a chunk of the forward pass 3.5 us alone and 6 of two, of a pass of gradients 8.5 and 14; with heads of 64 4.7, 6, 7.6
-// and 10.4 of one to four, of gradients 8.1, 8.8 and 9.7. So what fills the chip once is best, and a workgroup more than that costs a whole
-// round; the carry takes 1.7 us (0.9) a segment of the longest sequence. In us, all passes: one sequence of 8192, 16 heads of 128,
-// bfloat16, segments of 8, 12 and 16 chunks 203, 218 and 180; nine sequences of 17.5K tokens, 8 heads of 64, float16, training, of 4, 6, 7, 8 and
-// 12 468, 426, 411, 441 and 520. Sequences that fit a segment each need no maps and no carry.
+// and 10.4 of one to four, of gradients 8.1, 8.8 and 9.7. So what fills the chip once is best, and some more workgroups cost a whole
+// round; the carry takes 2 us (0.9, 0.7) a segment of the longest sequence. A call in us by segments of 2, 4, 8, 16 and 32 chunks: 8192 tokens,
+// 16 heads of 128, bfloat16 467, 249, 184, 158, 227, training 1224, 794, 624, 591, 920; 1024 of 8 heads, training 153, 170, 247, 423,
+// 614; 8192 of 8 heads of 64, training 346, 260, 246, 353, 619; 16 sequences of 21K tokens, 4 heads of 32, training 181, 154, 174, 258, 457.
+// Sequences that fit a segment each need no maps and no carry.
 int seg_chunks(const bf_gated_delta* p, bool train) {
   const int d = delta_pad(p->dim_k, p->dim_v), most = slots(p->dtype, d, train);
   const bool equal = p->longest > 0 && p->n == p->n_seq * int64_t(p->longest);
   const double chunks = double(p->n) / kDeltaChunk, longest = double(p->longest > 0 ? p->longest : p->n) / kDeltaChunk;
-  const double seqs = double(p->n_seq), carry = d == 128 ? 1.7 : 0.9;
+  const double seqs = double(p->n_seq), carry = d == 128 ? 2.0 : d == 64 ? 0.9 : 0.7;
+  // of a chunk alone, of all passes and of those that a call without a carry has; of a pass's start
+  const double all = train ? (d == 128 ? 22 : d == 64 ? 17 : 12) : (d == 128 ? 4.8 : d == 64 ? 3.7 : 2.9), few = all * (train ? 0.78 : 0.55);
+  const double start = train ? 35 : 8;
   int best = 2;
   double least = 1e30;
   for (int len = 2; len <= 64; ++len) {
@@ -63,14 +67,14 @@ int seg_chunks(const bf_gated_delta* p, bool train) {
     double segs = equal ? seqs * ceil(longest / len) : chunks / len + 0.5 * seqs;
     if (whole || segs < seqs) segs = seqs;
     const double groups = segs * p->heads, full = floor(groups / (256 * most));
-    const double rest = ceil((groups - full * 256 * most) / 256 - 0.1);          // a few more find room: last segments are short
+    // a few more than fill it find room: last segments are short
+    const double rest = full > 0 ? ceil((groups - full * 256 * most) / 256 - 0.1) : ceil(groups / 256 - (groups > 256 ? 0.1 : 0.0));
     const auto slower = [&](double at_once) {
       return d == 128 ? 0.32 + 0.68 * at_once : d == 32 ? 0.9 + 0.1 * at_once : at_once > 3 ? 1.9 : 0.8 + 0.2 * at_once;
     };
     const double rounds = full * slower(most) + (rest > 0 ? slower(rest) : 0);
     const double own = whole && longest < len ? (longest > 1 ? longest : 1) : len;
-    const double chunk = train ? (whole ? 25 : 32) : (whole ? 4 : 7.4), start = train ? 18 : 6;
-    const double cost = rounds * own * chunk + (full + (rest > 0)) * start + (whole ? 0 : longest / len * carry * (train ? 2 : 1));
+    const double cost = rounds * own * (whole ? few : all) + (full + (rest > 0)) * start + (whole ? 0 : longest / len * carry * (train ? 2 : 1));
     if (cost < least) least = cost, best = len;
     if (whole) break;
   }
