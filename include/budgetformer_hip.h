@@ -933,7 +933,8 @@ int bf_linear_attn_step(const void* q, const void* k, const void* v, const float
  * 128. Sequence s is rows [offsets[s], offsets[s + 1]); rows behind the last one
  * have out 0. init (or NULL), final_state (or NULL): float32 [n_seq, heads,
  * dim_k, dim_v], the states before each sequence's first token and behind its
- * last. Gates below exp(-150) are taken as that. A value that is not finite
+ * last. Up to 2^16 value heads; calls whose launches would hold 2^32 threads are
+ * refused. Gates below exp(-150) are taken as that. A value that is not finite
  * makes what follows of its own sequence NaN (one of v: its column), of q its own
  * row.                                                                      */
 typedef struct bf_gated_delta {
